@@ -1,5 +1,6 @@
 """The C ABI of ``libhsn_amd.so`` (``include/hsn_window.h``, ``include/hsn_ops.h``,
-``include/hsn_trainer.h``, ``include/hsn_sweep.h``, ``include/hsn_round.h``) via ctypes.
+``include/hsn_trainer.h``, ``include/hsn_sweep.h``, ``include/hsn_round.h``,
+``include/hsn_scan.h``) via ctypes.
 
 The library is the product: every operator in :mod:`hsn_amd` reaches the GPU through these
 entry points, and nothing here falls back to another implementation. :func:`library` raises a
@@ -88,6 +89,10 @@ SIGNATURES: dict[str, list] = {
     "hsn_win_cell_round_check": [P],
     "hsn_win_cell_round_workspace": [P, P],
     "hsn_win_cell_round": [P, P],
+    "hsn_scan_workspace": [I, I, I, I, I, P],
+    "hsn_scan_forward": [P, L, L, P, L, L, I, I, P, P, P, P, P, I, I, I, P, L, P],
+    "hsn_scan_backward": [P, L, L, P, L, L, I, I, P, P, P, L, L, P, P, P, P, I, I, I, P, L, P],
+    "hsn_scan_step": [P, L, P, L, I, I, P, P, P, P, I, I, I, P],
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,383 @@
+"""The gated linear recurrence on the GPU against the float64 oracle: forward, backward, the
+autograd node, the single position, and what they refuse.
+
+Tolerances. A gate's share is right to a few ulps (3e-7), and an error made at one position stays in
+the state for about 1/b positions, so fp32 states are within 3e-7 / b of the exact ones, relative
+to the largest |h| and |c| on the way; with the gates below (b above 0.005 but for a few positions)
+that is 6e-5. The cotangents run through the same shares. A 16-bit output adds half a unit in its
+last place."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import language as L
+
+pytestmark = pytest.mark.gpu
+
+IO = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+HALF_ULP = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+STATE = 6e-5
+
+
+def _close(got, want, what=""):
+    got = got.double().cpu()
+    assert got.shape == want.shape, what
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    got, want = got.nan_to_num(), want.nan_to_num()
+    scale = max(1.0, float(want.abs().max())) if want.numel() else 1.0
+    return got, want, scale
+
+
+def _check(got, want, io=torch.float32, what=""):
+    a, b, scale = _close(got, want, what)
+    # 2^-24: the half unit of an fp16 value below its normal range
+    room = STATE * scale + HALF_ULP[io] * b.abs() * (1 + 1e-3) + (2.0 ** -24 if io == torch.float16 else 0)
+    off = (a - b).abs()
+    assert bool((off <= room).all()), f"{what}: off by {float((off - room).max()):.3g} over the bound"
+
+
+def _problem(B, T, D, io, dev, reset_p=0.05, h0=True, seed=0, layout="dense"):
+    g = torch.Generator().manual_seed(seed)
+
+    def rnd(*shape, mean=0.0, scale=1.0, dtype=torch.float32):
+        return (torch.randn(*shape, generator=g) * scale + mean).to(dtype)
+
+    if layout == "dense":
+        y, gate = rnd(B, T, D, dtype=io).to(dev), rnd(B, T, D, mean=-1.0, dtype=io).to(dev)
+    elif layout == "fused":  # both in one product's rows
+        z = torch.cat([rnd(B, T, D), rnd(B, T, D, mean=-1.0)], 2).to(io).to(dev)
+        y, gate = z[..., :D], z[..., D:]
+    elif layout == "positions_first":
+        y = rnd(T, B, D, dtype=io).to(dev).transpose(0, 1)
+        gate = rnd(T, B, D, mean=-1.0, dtype=io).to(dev).transpose(0, 1)
+    else:  # one element past an aligned start: no wide loads
+        y = rnd(B * T * D + 1, dtype=io).to(dev)[1:].view(B, T, D)
+        gate = rnd(B * T * D + 1, mean=-1.0, dtype=io).to(dev)[1:].view(B, T, D)
+    reset = (torch.rand(B, T, generator=g) < reset_p).to(dev) if reset_p else None
+    start = rnd(B, D).to(dev) if h0 else None
+    d_h, d_h_T = rnd(B, T, D, dtype=io).to(dev), rnd(B, D).to(dev)
+    return y, gate, reset, start, d_h, d_h_T
+
+
+def _cpu(*ts):
+    return [None if t is None else t.cpu() for t in ts]
+
+
+def _both_ways(p, candidate="tanh"):
+    from hsn_amd import scan
+
+    y, gate, reset, h0, d_h, d_h_T = p
+    io = y.dtype
+    out = scan.forward(y, gate, reset, h0, candidate=candidate)
+    d_y, d_gate, d_h0 = scan.backward(y, gate, out["marks"], reset, d_h, d_h_T,
+                                      candidate=candidate)
+    bare = scan.forward(y, gate, reset, h0, candidate=candidate, save=False)
+    assert bare["marks"] is None and torch.equal(bare["h"], out["h"])
+    c = _cpu(*p)
+    h, h_T = L.scan_forward(*c[:4], candidate)
+    want = L.scan_backward(*c, candidate)
+    assert out["h"].dtype == d_y.dtype == d_gate.dtype == io
+    _check(out["h"], h, io, "h")
+    _check(out["h_T"], h_T, what="h_T")
+    _check(d_y, want[0], io, "d_y")
+    _check(d_gate, want[1], io, "d_gate")
+    _check(d_h0, want[2], what="d_h0")
+    return out, (d_y, d_gate, d_h0)
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,T,D", [(1, 1, 1), (2, 7, 64), (3, 130, 100), (1, 257, 72), (2, 129, 8),
+                                   (5, 16, 33), (1, 1000, 130), (4, 256, 512), (1, 2049, 20)])
+def test_sizes(cuda_device, io, B, T, D):
+    _both_ways(_problem(B, T, D, IO[io], cuda_device, seed=T + D))
+
+
+@pytest.mark.parametrize("layout", ["fused", "positions_first", "odd_start"])
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 104, 37])
+def test_layouts(cuda_device, io, layout, D):
+    _both_ways(_problem(3, 300, D, IO[io], cuda_device, layout=layout, seed=D), "linear")
+
+
+@pytest.mark.parametrize("candidate", ["tanh", "linear"])
+@pytest.mark.parametrize("reset_p", [0.0, 0.5, 1.0])
+@pytest.mark.parametrize("h0", [False, True])
+def test_resets_and_start(cuda_device, candidate, reset_p, h0):
+    _both_ways(_problem(2, 300, 96, torch.float32, cuda_device, reset_p, h0, seed=4), candidate)
+
+
+@pytest.mark.parametrize("B,T,D", [(1, 5000, 64), (2, 9001, 24), (1, 4097, 200)])
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+def test_long_axis_in_few_rows(cuda_device, B, T, D, io):
+    """Time is split over workgroups; the same bits come back every time."""
+    p = _problem(B, T, D, IO[io], cuda_device, 1 / 700, seed=T)
+    first = _both_ways(p)
+    for _ in range(3):
+        again = _both_ways(p)
+        for a, b in zip((first[0]["h"], first[0]["h_T"], *first[1]),
+                        (again[0]["h"], again[0]["h_T"], *again[1])):
+            assert torch.equal(a, b)
+
+
+def test_saturated_and_infinite_gates(cuda_device):
+    """A gate of +inf writes the candidate, of -inf keeps the state; a share of 1e-30 is itself."""
+    y, gate, reset, h0, d_h, d_h_T = _problem(1, 300, 64, torch.float32, cuda_device, 0.0, seed=9)
+    gate[:, 10:40] = float("inf")
+    gate[:, 100:200] = float("-inf")
+    gate[:, 200:220] = -69.0
+    gate[:, 230:240] = 200.0
+    out, _ = _both_ways((y, gate, reset, h0, d_h, d_h_T))
+    assert torch.equal(out["h"][:, 100], out["h"][:, 199])
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("T", [40, 3000])
+def test_what_a_reset_drops_does_not_come_back(cuda_device, bad, T):
+    """A state that is not finite stays in its own row and channel, and ends at the next reset,
+    whatever lies between the two; without a reset a NaN stays to the end."""
+    y, gate, _, h0, d_h, d_h_T = _problem(2, T, 64, torch.float32, cuda_device, 0.0, seed=2)
+    reset = torch.zeros(2, T, dtype=torch.bool, device=cuda_device)
+    reset[0, T - 7] = True
+    h0[:, 5] = bad
+    from hsn_amd import scan
+
+    out = scan.forward(y, gate, reset, h0)
+    finite = torch.isfinite(out["h"])
+    assert bool(finite[0, T - 7:].all()) and not bool(finite[1, 0, 5])
+    assert bool(torch.isfinite(out["h_T"][0]).all())
+    rest = [c for c in range(64) if c != 5]
+    assert bool(finite[:, :, rest].all())
+    if bad != bad:
+        assert not bool(finite[0, :T - 7, 5].any()) and not bool(finite[1, :, 5].any())
+    want, _ = L.scan_forward(*_cpu(y, gate, reset, h0))
+    _check(out["h"][0, T - 7:], want[0, T - 7:])
+    # backward: the cotangent that the reset drops is exactly absent before it
+    d_h[0, T - 7:, 9] = bad
+    d_y, d_gate, _ = scan.backward(y, gate, out["marks"], reset, d_h, None)
+    assert bool(torch.isfinite(d_y[0, :T - 7, 9]).all())
+    assert not bool(torch.isfinite(d_y[0, T - 7, 9]))
+
+
+def test_a_nan_candidate_reaches_later_positions_until_the_reset(cuda_device):
+    y, gate, _, h0, _, _ = _problem(1, 600, 16, torch.float32, cuda_device, 0.0, seed=3)
+    y[0, 100, 3] = float("nan")
+    gate[0, 150, 7] = float("nan")
+    reset = torch.zeros(1, 600, dtype=torch.bool, device=cuda_device)
+    reset[0, 500] = True
+    from hsn_amd import scan
+
+    got = scan.forward(y, gate, reset, h0)["h"]
+    nan = torch.isnan(got[0]).cpu()
+    want = torch.zeros(600, 16, dtype=torch.bool)
+    want[100:500, 3] = True
+    want[150:500, 7] = True
+    assert torch.equal(nan, want)
+
+
+def test_empty(cuda_device):
+    from hsn_amd import scan
+
+    h0 = torch.randn(3, 10, device=cuda_device)
+    y = torch.empty(3, 0, 10, device=cuda_device)
+    out = scan.forward(y, y, None, h0)
+    assert out["h"].shape == (3, 0, 10) and torch.equal(out["h_T"], h0)
+    assert torch.equal(scan.forward(y, y)["h_T"], torch.zeros_like(h0))
+    d_y, d_gate, d_h0 = scan.backward(y, y, out["marks"], None, None, h0)
+    assert d_y.numel() == d_gate.numel() == 0 and torch.equal(d_h0, h0)
+    none = torch.empty(0, 5, 10, device=cuda_device)
+    out = scan.forward(none, none)
+    assert out["h"].shape == (0, 5, 10) and out["h_T"].shape == (0, 10)
+    assert scan.backward(none, none, out["marks"], None, none)[2].shape == (0, 10)
+    assert scan.step(none[:, 0], none[:, 0], h0).shape == (0, 10)
+
+
+def test_absent_cotangents(cuda_device):
+    from hsn_amd import scan
+
+    y, gate, reset, h0, d_h, d_h_T = _problem(2, 150, 48, torch.float32, cuda_device, seed=6)
+    marks = scan.forward(y, gate, reset, h0)["marks"]
+    for a, b in ((None, d_h_T), (d_h, None), (None, None)):
+        got = scan.backward(y, gate, marks, reset, a, b)
+        want = L.scan_backward(*_cpu(y, gate, reset, h0, a, b))
+        for g, w in zip(got, want):
+            _check(g, w)
+
+
+@pytest.mark.parametrize("candidate", ["tanh", "linear"])
+def test_autograd(cuda_device, candidate):
+    """The node's gradients against float64 autograd, with an expanded cotangent (a sum's), a
+    broadcast gate, and a second window that carries the state."""
+    from hsn_amd import scan
+
+    y, gate, reset, h0, _, _ = _problem(2, 200, 24, torch.float32, cuda_device, seed=8)
+    gate = gate[:, :, :1].clone()  # one gate for all channels: its gradient is the channels' sum
+
+    def loss(y, gate, h0, run):
+        gates = gate.expand(-1, -1, y.shape[2])
+        gates = gates if run is None else gates.contiguous()
+        cut = 120
+        parts = []
+        for lo, hi in ((0, cut), (cut, 200)):
+            r = reset[:, lo:hi].contiguous()
+            if run is None:
+                h, now = [], h0
+                c = torch.tanh(y) if candidate == "tanh" else y
+                b = torch.sigmoid(gates)
+                for t in range(lo, hi):
+                    now = torch.where(reset[:, t, None].to(y.device), torch.zeros_like(now), now)
+                    now = now + b[:, t] * (c[:, t] - now)
+                    h.append(now)
+                h = torch.stack(h, 1)
+            else:
+                h, now = run(y[:, lo:hi], gates[:, lo:hi], r, h0, candidate=candidate)
+            h0 = now
+            parts.append(h.sum())
+        return parts[0] + 2 * parts[1] + (now * now).sum()
+
+    got_in = [t.clone().requires_grad_() for t in (y, gate, h0)]
+    got = torch.autograd.grad(loss(*got_in, scan.gated_scan), got_in)
+    want_in = [t.double().cpu().requires_grad_() for t in (y, gate, h0)]
+    reset = reset.cpu()
+    want = torch.autograd.grad(loss(*want_in, None), want_in)
+    for g, w in zip(got, want):
+        _check(g, w)
+
+
+def test_the_state_alone_carries_a_gradient(cuda_device):
+    from hsn_amd import scan
+
+    y, gate, reset, h0, _, d = _problem(2, 30, 12, torch.float32, cuda_device, seed=5)
+    h0.requires_grad_()
+    _, h_T = scan.gated_scan(y, gate, reset, h0)
+    (got,) = torch.autograd.grad((h_T * d).sum(), [h0])
+    want = L.scan_backward(*_cpu(y, gate, reset, h0.detach(), None, d))[2]
+    _check(got, want)
+
+
+def test_offsets_past_31_bits(cuda_device):
+    """Rows and positions whose offsets in elements and bytes pass 2^31."""
+    from hsn_amd import scan
+
+    B, T, D = 2, 3, 64
+    far = 2 ** 31 + 64
+    room = torch.empty(far + 2 * 2 ** 20 + T * D, dtype=torch.bfloat16, device=cuda_device)
+    y = room.as_strided((B, T, D), (far, D, 1))
+    src, gate, reset, h0, d_h, d_h_T = _problem(B, T, D, torch.bfloat16, cuda_device, seed=1)
+    y.copy_(src)
+    a, b = scan.forward(y, gate, reset, h0), scan.forward(src, gate, reset, h0)
+    assert torch.equal(a["h"], b["h"])
+    wide = room.as_strided((1, 3, D), (0, 2 ** 30 + 64, 1))  # the last position past 2^31
+    wide.copy_(src[:1])
+    a = scan.forward(wide, gate[:1], None, h0[:1].contiguous())
+    b = scan.forward(src[:1], gate[:1], None, h0[:1].contiguous())
+    assert torch.equal(a["h"], b["h"])
+    ga = scan.backward(wide, gate[:1], a["marks"], None, wide)
+    gb = scan.backward(src[:1], gate[:1], b["marks"], None, src[:1])
+    assert all(torch.equal(x, z) for x, z in zip(ga, gb))
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,S,D", [(1, 1, 1), (5, 9, 33), (32, 256, 512), (3, 3, 100), (17, 40, 72)])
+@pytest.mark.parametrize("candidate", ["tanh", "linear"])
+def test_step(cuda_device, io, n, S, D, candidate):
+    from hsn_amd import scan
+
+    g = torch.Generator().manual_seed(n + D)
+    z = torch.randn(n, 2 * D, generator=g).to(IO[io]).to(cuda_device)
+    y, gate = z[:, :D], z[:, D:]
+    state = torch.randn(S, D, generator=g)
+    rows = torch.randperm(S, generator=g)[:n].to(torch.int32)
+    rows[n // 2] = [-1, S, -7][n % 3] if n > 1 else rows[0]
+    reset = torch.rand(n, generator=g) < 0.3
+    for r, f in ((rows, reset), (None, None)):
+        pool = state.to(cuda_device)
+        h = scan.step(y, gate, pool, rows=None if r is None else r.to(cuda_device),
+                      reset=None if f is None else f.to(cuda_device), candidate=candidate)
+        want, after = L.scan_step(*_cpu(y, gate), state, r, f, candidate)
+        _check(h, want, IO[io], "h")
+        _check(pool, after, what="state")
+        touched = set(range(n)) if r is None else set(r.tolist())
+        for row in set(range(S)) - touched:
+            assert torch.equal(pool[row].cpu(), state[row])
+
+
+def test_step_by_step_is_the_scan(cuda_device):
+    """Decoding position by position gives the window's states (the same arithmetic; the scan joins
+    spans, so the last bits may differ)."""
+    from hsn_amd import scan
+
+    y, gate, reset, h0, _, _ = _problem(3, 40, 64, torch.float32, cuda_device, seed=12)
+    want = scan.forward(y, gate, reset, h0)
+    state = h0.clone()
+    for t in range(40):
+        h = scan.step(y[:, t], gate[:, t], state, reset=reset[:, t].contiguous())
+        _check(h, want["h"][:, t].double().cpu())
+    _check(state, want["h_T"].double().cpu())
+
+
+def test_on_another_stream_and_in_a_graph(cuda_device):
+    """The calls run on the current stream and may be captured; every replay equals the eager
+    result."""
+    from hsn_amd import scan
+
+    p = _problem(1, 3000, 64, torch.float32, cuda_device, seed=21)
+    y, gate, reset, h0, d_h, d_h_T = p
+
+    def both():
+        out = scan.forward(y, gate, reset, h0)
+        return out["h"], out["h_T"], *scan.backward(y, gate, out["marks"], reset, d_h, d_h_T)
+
+    want = [t.clone() for t in both()]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = both()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    for k in range(3):
+        y.copy_(torch.randn(y.shape, generator=torch.Generator().manual_seed(k)))
+        graph.replay()
+        torch.cuda.synchronize()
+        now = both()
+        assert all(torch.equal(a, b) for a, b in zip(held, now))
+
+
+def test_refusals(cuda_device):
+    from hsn_amd import scan
+
+    y, gate, reset, h0, d_h, d_h_T = _problem(2, 20, 8, torch.float32, cuda_device)
+    marks = scan.forward(y, gate, reset, h0)["marks"]
+    state = torch.zeros(4, 8, device=cuda_device)
+    bad = [
+        lambda: scan.forward(y, gate[:, :-1]),
+        lambda: scan.forward(y, gate.bfloat16()),
+        lambda: scan.forward(y.double(), gate.double()),
+        lambda: scan.forward(y.transpose(1, 2), gate.transpose(1, 2)),
+        lambda: scan.forward(y[0], gate[0]),
+        lambda: scan.forward(y.cpu(), gate.cpu()),
+        lambda: scan.forward(y, gate.cpu()),
+        lambda: scan.forward(y, gate, reset.int()),
+        lambda: scan.forward(y, gate, reset[:, :-1]),
+        lambda: scan.forward(y, gate, reset, h0.bfloat16()),
+        lambda: scan.forward(y, gate, reset, h0[:1]),
+        lambda: scan.forward(y, gate, reset, h0, candidate="relu"),
+        lambda: scan.forward(y[..., :0], gate[..., :0]),
+        lambda: scan.backward(y, gate, marks[:, :, :4], reset, d_h),
+        lambda: scan.backward(y, gate, marks, reset, d_h.bfloat16()),
+        lambda: scan.backward(y, gate, marks, reset, d_h, d_h_T.double()),
+        lambda: scan.step(y[:, 0], gate[:, 0], state.bfloat16()),
+        lambda: scan.step(y[:, 0], gate[:, 0], state, rows=torch.zeros(2, dtype=torch.int64,
+                                                                       device=cuda_device)),
+        lambda: scan.step(y[:, 0], gate[:, 0], state[:, :4]),
+        lambda: scan.step(y[:, 0], gate[:, 0], state, reset=reset[:, :1].expand(2, 2)),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(RuntimeError):  # more sequences than states, and no rows
+        scan.step(y[:, 0], gate[:, 0], state[:1])
