@@ -1,6 +1,6 @@
 """The C ABI of ``libhsn_amd.so`` (``include/hsn_window.h``, ``include/hsn_ops.h``,
 ``include/hsn_trainer.h``, ``include/hsn_sweep.h``, ``include/hsn_round.h``,
-``include/hsn_scan.h``, ``include/hsn_sample.h``) via ctypes.
+``include/hsn_scan.h``, ``include/hsn_units_layer.h``, ``include/hsn_sample.h``) via ctypes.
 
 The library is the product: every operator in :mod:`hsn_amd` reaches the GPU through these
 entry points, and nothing here falls back to another implementation. :func:`library` raises a
@@ -93,6 +93,8 @@ SIGNATURES: dict[str, list] = {
     "hsn_scan_forward": [P, L, L, P, L, L, I, I, P, P, P, P, P, I, I, I, P, L, P],
     "hsn_scan_backward": [P, L, L, P, L, L, I, I, P, P, P, L, L, P, P, P, P, I, I, I, P, L, P],
     "hsn_scan_step": [P, L, P, L, I, I, P, P, P, P, I, I, I, P],
+    "hsn_units_layer_workspace": [I, I, I, I, I, I, I, I, P],
+    "hsn_units_layer": [P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P, L, P],
     "hsn_sample": [P, L, I, P, P, P, P, P, P, P, I, I, P],
 }
 
