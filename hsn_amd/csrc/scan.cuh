@@ -1,5 +1,22 @@
-// What the gated linear recurrence's kernels share: a position's share kept, share written and
-// candidate, in fp32.
+// The gated linear recurrence's kernels over tiles of positions (include/hsn_scan.h).
+//
+// A position is a map of the state, h -> a h + x with a = sigmoid(-g), x = sigmoid(g) c; maps join
+// (first (A1, H1), then (A2, H2)) to (A1 A2, A2 H1 + H2), so a span of positions is one pair, and
+// the time axis splits anywhere. A reset makes the map constant; it is marked by a negative A, so
+// that joins select the later value instead of multiplying the earlier one by zero (0 * inf).
+//
+// Tile: a workgroup of 512 threads takes 64 channels of one row (128 bytes of 16-bit storage) and
+// kTile positions. A thread has V neighbouring channels (one 16-byte load a position where the
+// layout allows) and the tile's positions in segments of S, kept in registers from the one load to
+// the one store: it folds its segment, the segments of a wave join by lane shuffles, the waves by
+// LDS, and the thread walks its segment again from the state before it.
+//
+// Time axis: where rows and channels alone fill the GPU, a workgroup walks its 64 channels' tiles
+// one after the other, the next tile's loads in flight. Else every tile is a workgroup of its own
+// (kSplit): it publishes its pair and takes the pairs before it from device memory. Tiles are
+// numbered by a ticket, so that whatever a workgroup waits for belongs to one that already runs
+// and publishes without waiting for a later one: every wait ends. Pairs are folded in groups of 16
+// tiles in a fixed order, so the bits do not depend on who arrives first.
 #pragma once
 
 #include "../../include/hsn_scan.h"
@@ -8,6 +25,23 @@
 
 namespace hsn {
 namespace scan {
+
+constexpr int kSpan = HSN_SCAN_SPAN;
+constexpr int kThreads = 512, kWaves = kThreads / kWave;
+constexpr int kChannels = 64;  // of a tile
+constexpr int kGroup = 16;     // tiles whose pairs are folded one by one
+
+struct Args {
+    const void *y, *gate, *d_h;
+    int64_t y_row, y_pos, gate_row, gate_pos, d_row, d_pos;
+    const uint8_t* reset;
+    const float *h0, *d_h_T;
+    float *h_T, *marks, *d_h0;
+    void *h, *d_y, *d_gate;
+    int T, D, candidate;
+    int strips_a_row, strips, tiles;
+    uint64_t* box;  // kSplit: the ticket's 64 words, [tiles][strips][64] pairs, [groups][strips][64]
+};
 
 // a = sigmoid(-g) (the share of the old state kept) and b = sigmoid(g) (the share written), each
 // to a few ulps of itself: e = exp(-|g|) never overflows, and of 1/(1+e) and e/(1+e) neither is a
@@ -34,6 +68,449 @@ __device__ __forceinline__ float tanh_exact(float y) {
 __device__ __forceinline__ float candidate(float y, int kind) {
     return kind == HSN_SCAN_TANH ? tanh_exact(y) : y;
 }
+
+struct Pair {
+    float A, H;
+};
+
+__device__ __forceinline__ bool constant(float A) { return __float_as_int(A) < 0; }
+__device__ __forceinline__ float apply(Pair m, float h) {
+    return constant(m.A) ? m.H : __builtin_fmaf(m.A, h, m.H);
+}
+// `first`, then `then`.
+__device__ __forceinline__ Pair join(Pair first, Pair then) {
+    return constant(then.A) ? then
+                            : Pair{first.A * then.A, __builtin_fmaf(then.A, first.H, then.H)};
+}
+
+template <typename E, int V>
+struct alignas(sizeof(E) * V) Pack {
+    E e[V];
+};
+
+// --------------------------------------------------------------------------------------------
+// The exchange of pairs between a row's tiles.
+// --------------------------------------------------------------------------------------------
+
+// A pair as one word that is never 0 (A's bits are below 0x7f800000 or negative, plus one; a NaN A
+// has a NaN H, and 0 says the same of such a map).
+__device__ __forceinline__ uint64_t pair_word(Pair m) {
+    const uint32_t a = m.A != m.A ? 0u : __float_as_uint(m.A);
+    return uint64_t(a + 1) << 32 | __float_as_uint(m.H);
+}
+__device__ __forceinline__ Pair word_pair(uint64_t w) {
+    return {__uint_as_float(uint32_t(w >> 32) - 1), __uint_as_float(uint32_t(w))};
+}
+
+// One relaxed agent-scope word: it is complete by itself, so the reader needs no fence.
+__device__ __forceinline__ void publish(uint64_t* at, uint64_t w) {
+    __hip_atomic_store(at, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Waits for a wave's 64 words. Each belongs to a workgroup with a lower ticket; the bound (seconds)
+// is there so that no fault elsewhere can hang the grid, and what it gives up on becomes NaN.
+__device__ __forceinline__ Pair await(const uint64_t* at) {
+    for (int spin = 0; spin < (1 << 21); ++spin) {
+        const uint64_t w = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (ballot(w == 0) == 0) return word_pair(w);
+        __builtin_amdgcn_s_sleep(1);
+    }
+    return {-1.0f, __int_as_float(0x7fc00000)};
+}
+
+struct ExchangeLds {
+    Pair item[kGroup][kChannels];
+};
+
+// The state before tile k of the strip (k counts in the order of processing), for each channel of
+// the first wave's lanes, from this tile's pair and `start`, the state before tile 0.
+__device__ __forceinline__ float exchange(const Args& p, ExchangeLds& lds, int k, int strip,
+                                          Pair total, float start) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    uint64_t* pairs = p.box + 64 + strip * kChannels + lane;
+    const int64_t line = int64_t(p.strips) * kChannels;
+    uint64_t* prefix = pairs + p.tiles * line;
+    if (wave == 0) publish(pairs + k * line, pair_word(total));
+    // item 0: the state before the group; item i: the pair of the group's tile i - 1
+    const int group = k / kGroup, before = k % kGroup;
+    for (int i = wave; i <= before; i += kWaves)
+        if (i)
+            lds.item[i][lane] = await(pairs + (group * kGroup + i - 1) * line);
+        else if (group)
+            lds.item[0][lane] = await(prefix + (group - 1) * line);
+    __syncthreads();
+    float h = start;
+    if (wave == 0) {
+        if (group) h = lds.item[0][lane].H;
+        for (int i = 1; i <= before; ++i) h = apply(lds.item[i][lane], h);
+        if (before == kGroup - 1 && k + 1 < p.tiles)
+            publish(prefix + group * line, pair_word({-1.0f, apply(total, h)}));
+    }
+    return h;
+}
+static_assert(kGroup <= 16, "a group's items: its prefix and up to 15 pairs");
+
+// --------------------------------------------------------------------------------------------
+// Forward.
+// --------------------------------------------------------------------------------------------
+
+template <typename E, int V, int S>
+struct Tile {
+    static constexpr int kLanes = kChannels / V;           // threads side by side
+    static constexpr int kSegs = kThreads / kLanes;        // segments of S positions
+    static constexpr int kTile = kSegs * S;
+    static_assert(kSpan % S == 0 && kTile % kSpan == 0, "marks lie between segments");
+};
+
+// The thread's inclusive join over the wave's segments up to its own, from the first on (UP) or
+// from the last on.
+template <int LANES, bool UP, int V>
+__device__ __forceinline__ void wave_join(float (&A)[V], float (&H)[V]) {
+    const int lane = lane_id();
+#pragma unroll
+    for (int d = LANES; d < kWave; d *= 2) {
+        const bool has = UP ? lane >= d : lane < kWave - d;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const Pair o = UP ? Pair{__shfl_up(A[v], d, kWave), __shfl_up(H[v], d, kWave)}
+                              : Pair{__shfl_down(A[v], d, kWave), __shfl_down(H[v], d, kWave)};
+            const Pair m = join(o, {A[v], H[v]});
+            A[v] = has ? m.A : A[v];
+            H[v] = has ? m.H : H[v];
+        }
+    }
+}
+
+template <typename E, int V, int S, bool kSplit>
+__global__ __launch_bounds__(kThreads) void forward_tiles(Args p) {
+    using G = Tile<E, V, S>;
+    using P = Pack<E, V>;
+    __shared__ Pair wave_pair[2][kWaves][kChannels];
+    __shared__ float carry[2][kChannels];
+    __shared__ ExchangeLds lds;
+    __shared__ uint32_t ticket;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int cl = tid % G::kLanes, seg = tid / G::kLanes;
+    int strip = blockIdx.x, tile = 0, end = p.tiles;
+    if constexpr (kSplit) {
+        if (tid == 0) ticket = atomicAdd(reinterpret_cast<uint32_t*>(p.box), 1u);
+        __syncthreads();
+        strip = ticket % p.strips, tile = ticket / p.strips, end = tile + 1;
+    }
+    const int64_t r = strip / p.strips_a_row;
+    const int ch0 = (strip % p.strips_a_row) * kChannels, ch = ch0 + cl * V;
+    const bool on = ch < p.D;
+    const E* y = static_cast<const E*>(p.y) + r * p.y_row + ch;
+    const E* g = static_cast<const E*>(p.gate) + r * p.gate_row + ch;
+    E* out = static_cast<E*>(p.h) + r * p.T * p.D + ch;
+    const int64_t spans = (p.T + kSpan - 1) / kSpan;
+    float start = 0.0f;
+    if (tid < kChannels && ch0 + tid < p.D && p.h0) start = p.h0[r * p.D + ch0 + tid];
+    if (tid < kChannels) carry[0][tid] = start;
+
+    P ry[S], rg[S];
+    uint32_t resets;
+    auto load = [&](int at) {
+        const int t0 = at * G::kTile + seg * S;
+        resets = 0;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const bool in = t0 + i < p.T;
+            ry[i] = P{}, rg[i] = P{};
+            if (in && on) {
+                ry[i] = *reinterpret_cast<const P*>(y + (t0 + i) * p.y_pos);
+                rg[i] = *reinterpret_cast<const P*>(g + (t0 + i) * p.gate_pos);
+            }
+            if (in && p.reset) resets |= uint32_t(p.reset[r * p.T + t0 + i] != 0) << i;
+        }
+    };
+    load(tile);
+    for (int buf = 0; tile < end; ++tile, buf ^= 1) {
+        const int t0 = tile * G::kTile + seg * S;
+        float a[S][V], x[S][V], A[V], H[V];
+        const uint32_t drop = resets;
+#pragma unroll
+        for (int v = 0; v < V; ++v) A[v] = 1.0f, H[v] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            if (drop >> i & 1)
+#pragma unroll
+                for (int v = 0; v < V; ++v) A[v] = -1.0f, H[v] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float b;
+                gates(to_f32(rg[i].e[v]), a[i][v], b);
+                x[i][v] = b * candidate(to_f32(ry[i].e[v]), p.candidate);
+                if (t0 + i >= p.T) a[i][v] = 1.0f, x[i][v] = 0.0f;
+                A[v] *= a[i][v];
+                H[v] = __builtin_fmaf(a[i][v], H[v], x[i][v]);
+            }
+        }
+        if (!kSplit && tile + 1 < end) load(tile + 1);
+        wave_join<G::kLanes, true, V>(A, H);
+        if (lane >= kWave - G::kLanes)
+#pragma unroll
+            for (int v = 0; v < V; ++v) wave_pair[buf][wave][cl * V + v] = {A[v], H[v]};
+        __syncthreads();
+        Pair total{1.0f, 0.0f};
+        if (tid < kChannels)
+            for (int w = 0; w < kWaves; ++w) total = join(total, wave_pair[buf][w][tid]);
+        float before = 0.0f;
+        if constexpr (kSplit) before = exchange(p, lds, tile, strip, total, start);
+        if (tid < kChannels) {
+            if constexpr (kSplit)
+                carry[0][tid] = before;
+            else
+                before = carry[buf][tid];
+            const float after = apply(total, before);
+            carry[buf ^ 1][tid] = after;
+            if (tile == p.tiles - 1 && ch0 + tid < p.D) p.h_T[r * p.D + ch0 + tid] = after;
+        }
+        if constexpr (kSplit) __syncthreads();
+        // the state before the thread's segment: the waves before, then the lanes before
+        float h[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            h[v] = carry[buf][cl * V + v];
+            for (int w = 0; w < wave; ++w) h[v] = apply(wave_pair[buf][w][cl * V + v], h[v]);
+            if constexpr (G::kLanes < kWave) {
+                const Pair m{__shfl_up(A[v], G::kLanes, kWave), __shfl_up(H[v], G::kLanes, kWave)};
+                h[v] = lane >= G::kLanes ? apply(m, h[v]) : h[v];
+            }
+        }
+        if (p.marks && on && t0 < p.T && t0 % kSpan == 0)
+#pragma unroll
+            for (int v = 0; v < V; ++v) p.marks[(r * spans + t0 / kSpan) * p.D + ch + v] = h[v];
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            P o;
+            if (drop >> i & 1)
+#pragma unroll
+                for (int v = 0; v < V; ++v) h[v] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                h[v] = __builtin_fmaf(a[i][v], h[v], x[i][v]);
+                o.e[v] = from_f32<E>(h[v]);
+            }
+            if (t0 + i < p.T && on) *reinterpret_cast<P*>(out + int64_t(t0 + i) * p.D) = o;
+        }
+    }
+}
+
+// --------------------------------------------------------------------------------------------
+// Backward: from the last tile to the first. mu, the cotangent that a position hands to the one
+// before it, is a (d_h + mu of the one after): the same pairs from the other end, with x = a d_h.
+// A tile makes its states again from the mark before it; d_gate is l q with q = a b (c - m h[t-1]).
+// --------------------------------------------------------------------------------------------
+
+template <typename E, int V, int S, bool kSplit>
+__global__ __launch_bounds__(kThreads) void backward_tiles(Args p) {
+    using G = Tile<E, V, S>;
+    using P = Pack<E, V>;
+    __shared__ Pair wave_pair[2][kWaves][kChannels];
+    __shared__ float wave_mu[2][kWaves][kChannels];
+    __shared__ float carry[2][kChannels], mark[2][kChannels];
+    __shared__ ExchangeLds lds;
+    __shared__ uint32_t ticket;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int cl = tid % G::kLanes, seg = tid / G::kLanes;
+    int strip = blockIdx.x, turn = 0, end = p.tiles;  // turn 0 is the last tile
+    if constexpr (kSplit) {
+        if (tid == 0) ticket = atomicAdd(reinterpret_cast<uint32_t*>(p.box), 1u);
+        __syncthreads();
+        strip = ticket % p.strips, turn = ticket / p.strips, end = turn + 1;
+    }
+    const int64_t r = strip / p.strips_a_row;
+    const int ch0 = (strip % p.strips_a_row) * kChannels, ch = ch0 + cl * V;
+    const bool on = ch < p.D, owner = tid < kChannels && ch0 + tid < p.D;
+    const E* y = static_cast<const E*>(p.y) + r * p.y_row + ch;
+    const E* g = static_cast<const E*>(p.gate) + r * p.gate_row + ch;
+    const E* d = static_cast<const E*>(p.d_h) + r * p.d_row + ch;
+    E* dy = static_cast<E*>(p.d_y) + r * p.T * p.D + ch;
+    E* dg = static_cast<E*>(p.d_gate) + r * p.T * p.D + ch;
+    const int64_t spans = (p.T + kSpan - 1) / kSpan;
+    float start = 0.0f;
+    if (owner && p.d_h_T) start = p.d_h_T[r * p.D + ch0 + tid];
+    if (tid < kChannels) carry[0][tid] = start;
+
+    P ry[S], rg[S], rd[S];
+    uint32_t resets;
+    float next_mark = 0.0f;
+    auto load = [&](int at) {
+        const int t0 = at * G::kTile + seg * S;
+        resets = 0;
+        if (owner) next_mark = p.marks[(r * spans + at * (G::kTile / kSpan)) * p.D + ch0 + tid];
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const bool in = t0 + i < p.T;
+            ry[i] = P{}, rg[i] = P{}, rd[i] = P{};
+            if (in && on) {
+                ry[i] = *reinterpret_cast<const P*>(y + (t0 + i) * p.y_pos);
+                rg[i] = *reinterpret_cast<const P*>(g + (t0 + i) * p.gate_pos);
+                if (p.d_h) rd[i] = *reinterpret_cast<const P*>(d + (t0 + i) * p.d_pos);
+            }
+            if (in && p.reset) resets |= uint32_t(p.reset[r * p.T + t0 + i] != 0) << i;
+        }
+    };
+    load(p.tiles - 1 - turn);
+    for (int buf = 0; turn < end; ++turn, buf ^= 1) {
+        const int tile = p.tiles - 1 - turn, t0 = tile * G::kTile + seg * S;
+        float a[S][V], b[S][V], c[S][V], A[V], H[V], B[V], M[V];
+        P rl[S];
+        const uint32_t drop = resets;
+#pragma unroll
+        for (int v = 0; v < V; ++v) A[v] = 1.0f, H[v] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            rl[i] = rd[i];
+            if (drop >> i & 1)
+#pragma unroll
+                for (int v = 0; v < V; ++v) A[v] = -1.0f, H[v] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                gates(to_f32(rg[i].e[v]), a[i][v], b[i][v]);
+                c[i][v] = candidate(to_f32(ry[i].e[v]), p.candidate);
+                if (t0 + i >= p.T) a[i][v] = 1.0f, b[i][v] = 0.0f, c[i][v] = 0.0f;
+                A[v] *= a[i][v];
+                H[v] = __builtin_fmaf(a[i][v], H[v], b[i][v] * c[i][v]);
+            }
+        }
+        if (tid < kChannels) mark[buf][tid] = next_mark;
+#pragma unroll
+        for (int v = 0; v < V; ++v) B[v] = A[v], M[v] = 0.0f;
+#pragma unroll
+        for (int i = S - 1; i >= 0; --i) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) M[v] = a[i][v] * (to_f32(rl[i].e[v]) + M[v]);
+            if (drop >> i & 1)
+#pragma unroll
+                for (int v = 0; v < V; ++v) M[v] = 0.0f;
+        }
+        if (!kSplit && turn + 1 < end) load(tile - 1);
+        wave_join<G::kLanes, true, V>(A, H);
+        wave_join<G::kLanes, false, V>(B, M);
+        if (lane >= kWave - G::kLanes)
+#pragma unroll
+            for (int v = 0; v < V; ++v) wave_pair[buf][wave][cl * V + v] = {A[v], H[v]};
+        if (lane < G::kLanes)
+#pragma unroll
+            for (int v = 0; v < V; ++v) wave_mu[buf][wave][cl * V + v] = M[v];
+        __syncthreads();
+        Pair total{1.0f, 0.0f};
+        if (tid < kChannels)
+            for (int w = kWaves - 1; w >= 0; --w)
+                total = join(total, {wave_pair[buf][w][tid].A, wave_mu[buf][w][tid]});
+        float after = 0.0f;  // in time
+        if constexpr (kSplit) after = exchange(p, lds, turn, strip, total, start);
+        if (tid < kChannels) {
+            if constexpr (kSplit)
+                carry[0][tid] = after;
+            else
+                after = carry[buf][tid];
+            const float before = apply(total, after);
+            carry[buf ^ 1][tid] = before;
+            if (tile == 0 && owner) p.d_h0[r * p.D + ch0 + tid] = before;
+        }
+        if constexpr (kSplit) __syncthreads();
+        // q over c, and b c'(y) over b, on the way through the states
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float h = mark[buf][cl * V + v];
+            for (int w = 0; w < wave; ++w) h = apply(wave_pair[buf][w][cl * V + v], h);
+            if constexpr (G::kLanes < kWave) {
+                const Pair m{__shfl_up(A[v], G::kLanes, kWave), __shfl_up(H[v], G::kLanes, kWave)};
+                h = lane >= G::kLanes ? apply(m, h) : h;
+            }
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                if (drop >> i & 1) h = 0.0f;
+                const float old = h, cand = c[i][v], share = b[i][v];
+                h = __builtin_fmaf(a[i][v], old, share * cand);
+                c[i][v] = a[i][v] * share * (cand - old);
+                if (p.candidate == HSN_SCAN_TANH)
+                    b[i][v] = share * __builtin_fmaf(-cand, cand, 1.0f);
+            }
+        }
+        float mu[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            mu[v] = carry[buf][cl * V + v];
+            for (int w = kWaves - 1; w > wave; --w)
+                mu[v] = apply({wave_pair[buf][w][cl * V + v].A, wave_mu[buf][w][cl * V + v]}, mu[v]);
+            if constexpr (G::kLanes < kWave) {
+                const Pair m{__shfl_down(B[v], G::kLanes, kWave),
+                             __shfl_down(M[v], G::kLanes, kWave)};
+                mu[v] = lane < kWave - G::kLanes ? apply(m, mu[v]) : mu[v];
+            }
+        }
+#pragma unroll
+        for (int i = S - 1; i >= 0; --i) {
+            P oy, og;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float l = to_f32(rl[i].e[v]) + mu[v];
+                oy.e[v] = from_f32<E>(b[i][v] * l);
+                og.e[v] = from_f32<E>(c[i][v] * l);
+                mu[v] = a[i][v] * l;
+            }
+            if (drop >> i & 1)
+#pragma unroll
+                for (int v = 0; v < V; ++v) mu[v] = 0.0f;
+            if (t0 + i < p.T && on) {
+                *reinterpret_cast<P*>(dy + int64_t(t0 + i) * p.D) = oy;
+                *reinterpret_cast<P*>(dg + int64_t(t0 + i) * p.D) = og;
+            }
+        }
+    }
+}
+
+// vec: the elements of a load, a divisor of the row length, the strides and the addresses.
+template <typename E>
+void launch_forward(const Args& p, int vec, bool split, hipStream_t st);
+template <typename E>
+void launch_backward(const Args& p, int vec, bool split, hipStream_t st);
+
+// Positions of a tile, by the kernels' segments.
+constexpr int kForwardPer = 32, kBackwardPer = 16;  // elements of a thread
+constexpr int kForwardTile = kThreads * kForwardPer / kChannels;
+constexpr int kBackwardTile = kThreads * kBackwardPer / kChannels;
+
+#ifdef HSN_SCAN_INSTANTIATE
+template <typename E, int V>
+void launch_forward_as(const Args& p, bool split, hipStream_t st) {
+    if (split)
+        forward_tiles<E, V, kForwardPer / V, true><<<p.strips * p.tiles, kThreads, 0, st>>>(p);
+    else
+        forward_tiles<E, V, kForwardPer / V, false><<<p.strips, kThreads, 0, st>>>(p);
+}
+template <typename E, int V>
+void launch_backward_as(const Args& p, bool split, hipStream_t st) {
+    if (split)
+        backward_tiles<E, V, kBackwardPer / V, true><<<p.strips * p.tiles, kThreads, 0, st>>>(p);
+    else
+        backward_tiles<E, V, kBackwardPer / V, false><<<p.strips, kThreads, 0, st>>>(p);
+}
+template <typename E>
+void launch_forward(const Args& p, int vec, bool split, hipStream_t st) {
+    if constexpr (sizeof(E) == 2)
+        if (vec == 8) return launch_forward_as<E, 8>(p, split, st);
+    if constexpr (sizeof(E) == 2)
+        if (vec == 2) return launch_forward_as<E, 2>(p, split, st);
+    if constexpr (sizeof(E) == 4)
+        if (vec == 4) return launch_forward_as<E, 4>(p, split, st);
+    launch_forward_as<E, 1>(p, split, st);
+}
+template <typename E>
+void launch_backward(const Args& p, int vec, bool split, hipStream_t st) {
+    if constexpr (sizeof(E) == 2)
+        if (vec == 8) return launch_backward_as<E, 8>(p, split, st);
+    if constexpr (sizeof(E) == 2)
+        if (vec == 2) return launch_backward_as<E, 2>(p, split, st);
+    if constexpr (sizeof(E) == 4)
+        if (vec == 4) return launch_backward_as<E, 4>(p, split, st);
+    launch_backward_as<E, 1>(p, split, st);
+}
+#endif
 
 }  // namespace scan
 }  // namespace hsn

@@ -1,91 +1,11 @@
-// The gated linear recurrence over whole sequences (include/hsn_scan.h): forward, backward and
-// the single position.
-//
-// Forward and backward: a lane walks one channel of one row through the positions. The backward
-// makes a span's states again from the mark before it (the state itself is not read: 5 elements a
-// position and channel instead of 6, and no rounding of h to the storage type in the gradient).
+// The gated linear recurrence over whole sequences (include/hsn_scan.h): the entry points and the
+// single position. The kernels over tiles are in scan.cuh.
 #include "abi_util.h"
 #include "scan.cuh"
 
 namespace hsn {
 namespace scan {
 namespace {
-
-constexpr int kSpan = HSN_SCAN_SPAN;
-constexpr int kThreads = 64;
-
-struct Args {
-    const void *y, *gate, *d_h;
-    int64_t y_row, y_pos, gate_row, gate_pos, d_row, d_pos;
-    const uint8_t* reset;
-    const float *h0, *d_h_T;
-    float *h_T, *marks, *d_h0;
-    void *h, *d_y, *d_gate;
-    int B, T, D, candidate;
-};
-
-template <typename E>
-__global__ __launch_bounds__(kThreads) void walk_forward(Args p) {
-    const int ch = blockIdx.x * kThreads + threadIdx.x, r = blockIdx.y;
-    if (ch >= p.D) return;
-    const E* y = static_cast<const E*>(p.y) + r * p.y_row + ch;
-    const E* g = static_cast<const E*>(p.gate) + r * p.gate_row + ch;
-    E* out = static_cast<E*>(p.h) + int64_t(r) * p.T * p.D + ch;
-    float h = p.h0 ? p.h0[int64_t(r) * p.D + ch] : 0.0f;
-    const int spans = (p.T + kSpan - 1) / kSpan;
-    for (int t = 0; t < p.T; ++t) {
-        if (p.marks && t % kSpan == 0) p.marks[(int64_t(r) * spans + t / kSpan) * p.D + ch] = h;
-        if (p.reset && p.reset[int64_t(r) * p.T + t]) h = 0.0f;
-        float a, b;
-        gates(to_f32(g[t * p.gate_pos]), a, b);
-        h = __builtin_fmaf(a, h, b * candidate(to_f32(y[t * p.y_pos]), p.candidate));
-        out[int64_t(t) * p.D] = from_f32<E>(h);
-    }
-    p.h_T[int64_t(r) * p.D + ch] = h;
-}
-
-template <typename E>
-__global__ __launch_bounds__(kThreads) void walk_backward(Args p) {
-    const int ch = blockIdx.x * kThreads + threadIdx.x, r = blockIdx.y;
-    if (ch >= p.D) return;
-    const E* y = static_cast<const E*>(p.y) + r * p.y_row + ch;
-    const E* g = static_cast<const E*>(p.gate) + r * p.gate_row + ch;
-    const E* d = static_cast<const E*>(p.d_h) + r * p.d_row + ch;
-    E* dy = static_cast<E*>(p.d_y) + int64_t(r) * p.T * p.D + ch;
-    E* dg = static_cast<E*>(p.d_gate) + int64_t(r) * p.T * p.D + ch;
-    const int spans = (p.T + kSpan - 1) / kSpan;
-    float mu = p.d_h_T ? p.d_h_T[int64_t(r) * p.D + ch] : 0.0f;  // the cotangent from later on
-    for (int s = spans - 1; s >= 0; --s) {
-        float q[kSpan];  // d_gate is l q, with q = a b (c - m h[t-1])
-        float h = p.marks[(int64_t(r) * spans + s) * p.D + ch];
-#pragma unroll
-        for (int i = 0; i < kSpan; ++i) {
-            const int t = s * kSpan + i;
-            q[i] = 0.0f;
-            if (t >= p.T) continue;
-            if (p.reset && p.reset[int64_t(r) * p.T + t]) h = 0.0f;
-            float a, b;
-            gates(to_f32(g[t * p.gate_pos]), a, b);
-            const float c = candidate(to_f32(y[t * p.y_pos]), p.candidate);
-            q[i] = a * b * (c - h);
-            h = __builtin_fmaf(a, h, b * c);
-        }
-#pragma unroll
-        for (int i = kSpan - 1; i >= 0; --i) {
-            const int t = s * kSpan + i;
-            if (t >= p.T) continue;
-            float a, b;
-            gates(to_f32(g[t * p.gate_pos]), a, b);
-            const float c = candidate(to_f32(y[t * p.y_pos]), p.candidate);
-            const float l = (p.d_h ? to_f32(d[t * p.d_pos]) : 0.0f) + mu;
-            dy[int64_t(t) * p.D] =
-                from_f32<E>(l * b * (p.candidate == HSN_SCAN_TANH ? 1.0f - c * c : 1.0f));
-            dg[int64_t(t) * p.D] = from_f32<E>(l * q[i]);
-            mu = p.reset && p.reset[int64_t(r) * p.T + t] ? 0.0f : a * l;
-        }
-    }
-    p.d_h0[int64_t(r) * p.D + ch] = mu;
-}
 
 template <typename E>
 __global__ __launch_bounds__(256) void step(const E* y, int64_t y_row, const E* gate,
@@ -120,7 +40,75 @@ void check(int B, int T, int D, int dtype, int candidate_kind) {
     HSN_REQUIRE(candidate_kind == HSN_SCAN_TANH || candidate_kind == HSN_SCAN_LINEAR,
                 HSN_ERR_INVALID_ARGUMENT, "unknown candidate");
     HSN_REQUIRE(B >= 0 && T >= 0 && D >= 1, HSN_ERR_INVALID_ARGUMENT, "B, T >= 0 and D >= 1");
-    HSN_REQUIRE(B <= 65535, HSN_ERR_SIZE_OVERFLOW, "at most 65535 rows");
+}
+
+// Every word of the exchange starts at 0 (a kernel, so that the call may be captured).
+__global__ __launch_bounds__(256) void clear(uint4* box, int64_t n) {
+    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (i < n) box[i] = uint4{};
+}
+
+// No positions: the state is carried over.
+__global__ __launch_bounds__(256) void carry_over(const float* from, float* to, int64_t n) {
+    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (i < n) to[i] = from ? from[i] : 0.0f;
+}
+
+// How a pass runs: the tiles of a row, and whether each is a workgroup of its own.
+struct Plan {
+    int strips_a_row, tiles;
+    int64_t strips, words;
+    bool split;
+};
+
+Plan plan(int B, int T, int D, int tile) {
+    Plan q;
+    q.strips_a_row = (D + kChannels - 1) / kChannels;
+    q.strips = int64_t(B) * q.strips_a_row;
+    q.tiles = (T + tile - 1) / tile;
+    q.split = q.tiles > 1 && q.strips < 256;
+    const int64_t groups = (q.tiles + kGroup - 1) / kGroup;
+    q.words = q.split ? 64 + (q.tiles + groups) * q.strips * kChannels : 0;
+    HSN_REQUIRE(q.strips <= INT32_MAX && q.strips * (q.split ? q.tiles : 1) <= INT32_MAX,
+                HSN_ERR_SIZE_OVERFLOW, "too many rows and channels for one grid");
+    return q;
+}
+
+// The elements of one load that the row length, the strides and the addresses allow.
+int vector_of(int size, int D, std::initializer_list<const void*> at,
+              std::initializer_list<int64_t> strides) {
+    for (int vec : {16 / size, size == 2 ? 2 : 1}) {
+        bool fits = D % vec == 0;
+        for (const void* p : at) fits &= reinterpret_cast<uintptr_t>(p) % (vec * size) == 0;
+        for (int64_t s : strides) fits &= s % vec == 0;
+        if (fits) return vec;
+    }
+    return 1;
+}
+
+void run(Args& p, const Plan& q, int dtype, int vec, bool back, void* workspace,
+         int64_t workspace_bytes, hipStream_t st) {
+    p.strips_a_row = q.strips_a_row, p.strips = static_cast<int>(q.strips), p.tiles = q.tiles;
+    if (q.split) {
+        HSN_REQUIRE(workspace && workspace_bytes >= 8 * q.words, HSN_ERR_INVALID_ARGUMENT,
+                    "the workspace is too small");
+        HSN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, HSN_ERR_INVALID_ARGUMENT,
+                    "the workspace must be aligned to 16 bytes");
+        p.box = static_cast<uint64_t*>(workspace);
+        const int64_t n = q.words / 2;
+        clear<<<static_cast<uint32_t>((n + 255) / 256), 256, 0, st>>>(
+            reinterpret_cast<uint4*>(p.box), n);
+    }
+    by_dtype(dtype, [&](auto e) {
+        using E = decltype(e);
+        back ? launch_backward<E>(p, vec, q.split, st) : launch_forward<E>(p, vec, q.split, st);
+    });
+    HSN_HIP(hipGetLastError());
+}
+
+void run_empty(const float* from, float* to, int64_t n, hipStream_t st) {
+    carry_over<<<static_cast<uint32_t>((n + 255) / 256), 256, 0, st>>>(from, to, n);
+    HSN_HIP(hipGetLastError());
 }
 
 }  // namespace
@@ -132,10 +120,9 @@ using namespace hsn::scan;
 
 extern "C" int hsn_scan_workspace(int B, int T, int D, int dtype, int backward, int64_t* bytes) {
     HSN_ABI_BEGIN
-    (void)backward;
     check(B, T, D, dtype, HSN_SCAN_TANH);
     HSN_REQUIRE(bytes, HSN_ERR_INVALID_ARGUMENT, "bytes must not be NULL");
-    *bytes = 0;
+    *bytes = 8 * plan(B, T, D, backward ? kBackwardTile : kForwardTile).words;
     HSN_ABI_END
 }
 
@@ -145,19 +132,22 @@ extern "C" int hsn_scan_forward(const void* y, int64_t y_row, int64_t y_pos, con
                                 float* marks, int B, int T, int D, void* workspace,
                                 int64_t workspace_bytes, void* stream) {
     HSN_ABI_BEGIN
-    (void)workspace, (void)workspace_bytes;
     check(B, T, D, dtype, candidate_kind);
     if (B == 0) return HSN_OK;
     HSN_REQUIRE(h_T && (T == 0 || (y && gate && h)), HSN_ERR_INVALID_ARGUMENT,
                 "a required pointer is NULL");
+    if (T == 0) {
+        run_empty(h0, h_T, int64_t(B) * D, as_stream(stream));
+        return HSN_OK;
+    }
     Args p{};
     p.y = y, p.gate = gate, p.y_row = y_row, p.y_pos = y_pos, p.gate_row = gate_row;
     p.gate_pos = gate_pos, p.reset = reset, p.h0 = h0, p.h = h, p.h_T = h_T, p.marks = marks;
-    p.B = B, p.T = T, p.D = D, p.candidate = candidate_kind;
-    by_dtype(dtype, [&](auto e) {
-        walk_forward<decltype(e)><<<dim3((D + kThreads - 1) / kThreads, B), kThreads, 0, as_stream(stream)>>>(p);
-    });
-    HSN_HIP(hipGetLastError());
+    p.T = T, p.D = D, p.candidate = candidate_kind;
+    const int vec = vector_of(dtype == HSN_DTYPE_F32 ? 4 : 2, D, {y, gate, h},
+                              {y_row, y_pos, gate_row, gate_pos});
+    run(p, plan(B, T, D, kForwardTile), dtype, vec, false, workspace, workspace_bytes,
+        as_stream(stream));
     HSN_ABI_END
 }
 
@@ -168,20 +158,23 @@ extern "C" int hsn_scan_backward(const void* y, int64_t y_row, int64_t y_pos, co
                                  void* d_gate, float* d_h0, int B, int T, int D, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
     HSN_ABI_BEGIN
-    (void)workspace, (void)workspace_bytes;
     check(B, T, D, dtype, candidate_kind);
     if (B == 0) return HSN_OK;
     HSN_REQUIRE(d_h0 && (T == 0 || (y && gate && marks && d_y && d_gate)),
                 HSN_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
+    if (T == 0) {
+        run_empty(d_h_T, d_h0, int64_t(B) * D, as_stream(stream));
+        return HSN_OK;
+    }
     Args p{};
     p.y = y, p.gate = gate, p.d_h = d_h, p.y_row = y_row, p.y_pos = y_pos, p.gate_row = gate_row;
     p.gate_pos = gate_pos, p.d_row = d_row, p.d_pos = d_pos, p.reset = reset, p.d_h_T = d_h_T;
     p.marks = const_cast<float*>(marks), p.d_y = d_y, p.d_gate = d_gate, p.d_h0 = d_h0;
-    p.B = B, p.T = T, p.D = D, p.candidate = candidate_kind;
-    by_dtype(dtype, [&](auto e) {
-        walk_backward<decltype(e)><<<dim3((D + kThreads - 1) / kThreads, B), kThreads, 0, as_stream(stream)>>>(p);
-    });
-    HSN_HIP(hipGetLastError());
+    p.T = T, p.D = D, p.candidate = candidate_kind;
+    const int vec = vector_of(dtype == HSN_DTYPE_F32 ? 4 : 2, D, {y, gate, d_h, d_y, d_gate},
+                              {y_row, y_pos, gate_row, gate_pos, d_row, d_pos});
+    run(p, plan(B, T, D, kBackwardTile), dtype, vec, true, workspace, workspace_bytes,
+        as_stream(stream));
     HSN_ABI_END
 }
 

@@ -1,0 +1,11 @@
+// The gated linear recurrence's kernels in bf16 storage, in a translation unit of their own so that
+// they compile in parallel.
+#define HSN_SCAN_INSTANTIATE
+#include "scan.cuh"
+
+namespace hsn {
+namespace scan {
+template void launch_forward<bf16_t>(const Args&, int, bool, hipStream_t);
+template void launch_backward<bf16_t>(const Args&, int, bool, hipStream_t);
+}  // namespace scan
+}  // namespace hsn

@@ -28,7 +28,7 @@ from ._lib import call, ptr, stream_of
 __all__ = ["SPAN", "forward", "backward", "gated_scan", "GatedScan", "step", "available"]
 
 #: positions between two of the states that :func:`forward` keeps for :func:`backward`
-SPAN = 16
+SPAN = 128
 
 CANDIDATES = {"tanh": 0, "linear": 1}
 _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16,

@@ -28,7 +28,7 @@ extern "C" {
 
 /* Positions between two kept states: marks is [B, ceil(T / HSN_SCAN_SPAN), D], the state before
  * every position that is a multiple of it (before that position's own reset). */
-#define HSN_SCAN_SPAN 16
+#define HSN_SCAN_SPAN 128
 
 /* Bytes of device workspace hsn_scan_forward (backward = 0) or hsn_scan_backward (1) needs for
  * the shape; 0 where it needs none. Its contents do not matter before the call. */

@@ -129,7 +129,7 @@ def test_saturated_and_infinite_gates(cuda_device):
     gate[:, 200:220] = -69.0
     gate[:, 230:240] = 200.0
     out, _ = _both_ways((y, gate, reset, h0, d_h, d_h_T))
-    assert torch.equal(out["h"][:, 100], out["h"][:, 199])
+    _check(out["h"][:, 199], out["h"][:, 100].double().cpu())  # joined apart: not the same bits
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
