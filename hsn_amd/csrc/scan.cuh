@@ -6,17 +6,23 @@
 // that joins select the later value instead of multiplying the earlier one by zero (0 * inf).
 //
 // Tile: a workgroup of 512 threads takes 64 channels of one row (128 bytes of 16-bit storage) and
-// kTile positions. A thread has V neighbouring channels (one 16-byte load a position where the
-// layout allows) and the tile's positions in segments of S, kept in registers from the one load to
-// the one store: it folds its segment, the segments of a wave join by lane shuffles, the waves by
-// LDS, and the thread walks its segment again from the state before it.
+// kTile positions. A thread has V neighbouring channels (2 where the layout allows, else 1) and a
+// segment of S positions, kept in registers from the one load to the one store: it folds its segment,
+// the segments of a wave join by lane shuffles, the waves by LDS, and the thread walks its segment
+// again from the state before it. Wider packs halve the loads but double the segments of a wave and
+// with them the joins, and the kernel is bound by the instructions it issues before it is bound by
+// HBM: with V = 4 a walk over 8 x 4096 x 2048 in bf16 takes 130 us forward and 255 us backward, with
+// V = 2 98 and 187 us.
 //
-// Time axis: where rows and channels alone fill the GPU, a workgroup walks its 64 channels' tiles
-// one after the other, the next tile's loads in flight. Else every tile is a workgroup of its own
-// (kSplit): it publishes its pair and takes the pairs before it from device memory. Tiles are
-// numbered by a ticket, so that whatever a workgroup waits for belongs to one that already runs
-// and publishes without waiting for a later one: every wait ends. Pairs are folded in groups of 16
-// tiles in a fixed order, so the bits do not depend on who arrives first.
+// Time axis: a workgroup walks its 64 channels' tiles one after the other, the next tile's loads in
+// flight, where rows and channels alone fill the GPU and the tiles are few. Else every tile is a
+// workgroup of its own (kSplit): it publishes its pair and takes the pairs before it from device
+// memory. Tiles are numbered by a ticket, so that whatever a workgroup waits for belongs to one that
+// already runs and publishes without waiting for a later one: every wait ends. Pairs are folded in
+// groups of 16 tiles in a fixed order, so the bits do not depend on who arrives first. Split, the
+// same 8 x 4096 x 2048 take 97 and 170 us (4.2 and 3.9 TB/s of the 3 and 5 elements that have to move),
+// and one row of 32769 x 1024 60 us, which one walk a strip takes 1.0 ms for; at 32 x 256 x 512 in
+// fp32 the walk's 13.6 and 19.4 us are less than the split's 13.6 and 22.7 and the clearing of its words.
 #pragma once
 
 #include "../../include/hsn_scan.h"
@@ -40,33 +46,37 @@ struct Args {
     void *h, *d_y, *d_gate;
     int T, D, candidate;
     int strips_a_row, strips, tiles;
+    bool reset_words;  // every fourth flag of a row is aligned to four bytes
     uint64_t* box;  // kSplit: the ticket's 64 words, [tiles][strips][64] pairs, [groups][strips][64]
 };
 
 // a = sigmoid(-g) (the share of the old state kept) and b = sigmoid(g) (the share written), each
-// to a few ulps of itself: e = exp(-|g|) never overflows, and of 1/(1+e) and e/(1+e) neither is a
-// difference from 1 (1 - b would leave nothing of a small a).
+// to a few ulps of itself: 1/(1+e) and e/(1+e) with e = exp(-g), neither a difference from 1 (1 - b
+// would leave nothing of a small a). e stops at 2^126, so that a is 1 and b 2^-126 for every g below
+// -87 and not inf * 0; the minimum keeps a NaN.
 __device__ __forceinline__ void gates(float g, float& a, float& b) {
-    const float e = __builtin_amdgcn_exp2f(-kLog2e * __builtin_fabsf(g));
-    const float big = __builtin_amdgcn_rcpf(1.0f + e);
-    const float small = e * big;
-    a = g >= 0.0f ? small : big;
-    b = g >= 0.0f ? big : small;
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(-kLog2e * g, 126.0f));
+    b = __builtin_amdgcn_rcpf(1.0f + e);
+    a = e * b;
 }
 
-// tanh(y) to a few ulps of itself: (1 - e) / (1 + e) with e = exp(-2|y|), and the series
-// y - y^3/3 + 2 y^5/15 below |y| = 1/16, where 1 - e cancels (the next term, 17 y^7 / 315, is
-// under 4e-9 of y there).
-__device__ __forceinline__ float tanh_exact(float y) {
-    const float e = __builtin_amdgcn_exp2f(-2.0f * kLog2e * __builtin_fabsf(y));
-    const float t = __builtin_copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), y);
+// tanh(y) = 1 - 2 / (1 + exp(2y)), right to 1.2e-7 of 1, and for small |y|, where that is a
+// difference of equals, the series y - y^3/3 + 2 y^5/15 (fp32 storage: below 1/8 the next term,
+// 17 y^7 / 315, is under 2e-7 of y) or y alone (16-bit storage: below 1/128 it is right to 2e-5 of
+// itself, a hundredth of the storage's rounding).
+template <typename E>
+__device__ __forceinline__ float tanh_of(float y) {
+    const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * y);
+    const float t = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+    if constexpr (sizeof(E) == 2) return __builtin_fabsf(y) < 0.0078125f ? y : t;
     const float y2 = y * y;
     const float s = __builtin_fmaf(y2 * y, __builtin_fmaf(y2, 2.0f / 15.0f, -1.0f / 3.0f), y);
-    return __builtin_fabsf(y) < 0.0625f ? s : t;
+    return __builtin_fabsf(y) < 0.125f ? s : t;
 }
 
+template <typename E>
 __device__ __forceinline__ float candidate(float y, int kind) {
-    return kind == HSN_SCAN_TANH ? tanh_exact(y) : y;
+    return kind == HSN_SCAN_TANH ? tanh_of<E>(y) : y;
 }
 
 struct Pair {
@@ -87,6 +97,66 @@ template <typename E, int V>
 struct alignas(sizeof(E) * V) Pack {
     E e[V];
 };
+
+template <typename E, int V>
+__device__ __forceinline__ Pack<E, V> filled(float v) {
+    Pack<E, V> p;
+#pragma unroll
+    for (int i = 0; i < V; ++i) p.e[i] = from_f32<E>(v);
+    return p;
+}
+
+// The segment's values of one tensor: S positions from t0 on, `fill` after the last.
+template <typename E, int V, int S>
+__device__ __forceinline__ void load_segment(Pack<E, V> (&to)[S], const E* row, int64_t pos, int t0,
+                                             int T, bool whole, float fill) {
+    using P = Pack<E, V>;
+    const E* at = row + t0 * pos;
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < S; ++i, at += pos) to[i] = *reinterpret_cast<const P*>(at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i, at += pos) {
+            to[i] = filled<E, V>(fill);
+            if (t0 + i < T) to[i] = *reinterpret_cast<const P*>(at);
+        }
+    }
+}
+
+template <typename E, int V, int S>
+__device__ __forceinline__ void store_segment(const Pack<E, V> (&from)[S], E* row, int64_t pos,
+                                              int t0, int T) {
+    using P = Pack<E, V>;
+    E* at = row + t0 * pos;
+    if (t0 + S <= T) {
+#pragma unroll
+        for (int i = 0; i < S; ++i, at += pos) *reinterpret_cast<P*>(at) = from[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i, at += pos)
+            if (t0 + i < T) *reinterpret_cast<P*>(at) = from[i];
+    }
+}
+
+// Bit i: a reset before position t0 + i.
+template <int S>
+__device__ __forceinline__ uint32_t load_resets(const uint8_t* row, int t0, int T, bool words) {
+    uint32_t bits = 0;
+    if (!row) return 0;
+    if (words) {  // four flags a load: byte k (0 or 1) goes to bit 24 + k
+#pragma unroll
+        for (int i = 0; i < S; i += 4) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(row + t0 + i);
+            bits |= ((w & 0x01010101u) * 0x01020408u >> 24 & 15u) << i;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+            if (t0 + i < T) bits |= uint32_t(row[t0 + i] != 0) << i;
+    }
+    return bits;
+}
 
 // --------------------------------------------------------------------------------------------
 // The exchange of pairs between a row's tiles.
@@ -200,8 +270,11 @@ __global__ __launch_bounds__(kThreads) void forward_tiles(Args p) {
     const int64_t r = strip / p.strips_a_row;
     const int ch0 = (strip % p.strips_a_row) * kChannels, ch = ch0 + cl * V;
     const bool on = ch < p.D;
-    const E* y = static_cast<const E*>(p.y) + r * p.y_row + ch;
-    const E* g = static_cast<const E*>(p.gate) + r * p.gate_row + ch;
+    // lanes past the last channel load the last ones and store nothing
+    const int from = on ? ch : p.D - V;
+    const E* y = static_cast<const E*>(p.y) + r * p.y_row + from;
+    const E* g = static_cast<const E*>(p.gate) + r * p.gate_row + from;
+    const uint8_t* reset = p.reset ? p.reset + r * p.T : nullptr;
     E* out = static_cast<E*>(p.h) + r * p.T * p.D + ch;
     const int64_t spans = (p.T + kSpan - 1) / kSpan;
     float start = 0.0f;
@@ -210,25 +283,36 @@ __global__ __launch_bounds__(kThreads) void forward_tiles(Args p) {
 
     P ry[S], rg[S];
     uint32_t resets;
+    // after the last position: a gate of -inf, which keeps the state
     auto load = [&](int at) {
         const int t0 = at * G::kTile + seg * S;
-        resets = 0;
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const bool in = t0 + i < p.T;
-            ry[i] = P{}, rg[i] = P{};
-            if (in && on) {
-                ry[i] = *reinterpret_cast<const P*>(y + (t0 + i) * p.y_pos);
-                rg[i] = *reinterpret_cast<const P*>(g + (t0 + i) * p.gate_pos);
-            }
-            if (in && p.reset) resets |= uint32_t(p.reset[r * p.T + t0 + i] != 0) << i;
-        }
+        const bool whole = (at + 1) * G::kTile <= p.T;
+        load_segment<E, V, S>(ry, y, p.y_pos, t0, p.T, whole, 0.0f);
+        load_segment<E, V, S>(rg, g, p.gate_pos, t0, p.T, whole, -__builtin_inff());
+        resets = load_resets<S>(reset, t0, p.T, whole && p.reset_words);
     };
     load(tile);
     for (int buf = 0; tile < end; ++tile, buf ^= 1) {
         const int t0 = tile * G::kTile + seg * S;
         float a[S][V], x[S][V], A[V], H[V];
         const uint32_t drop = resets;
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                gates(to_f32(rg[i].e[v]), a[i][v], x[i][v]);
+            }
+        if (p.candidate == HSN_SCAN_TANH) {
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[i][v] *= tanh_of<E>(to_f32(ry[i].e[v]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[i][v] *= to_f32(ry[i].e[v]);
+        }
 #pragma unroll
         for (int v = 0; v < V; ++v) A[v] = 1.0f, H[v] = 0.0f;
 #pragma unroll
@@ -238,10 +322,6 @@ __global__ __launch_bounds__(kThreads) void forward_tiles(Args p) {
                 for (int v = 0; v < V; ++v) A[v] = -1.0f, H[v] = 0.0f;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                float b;
-                gates(to_f32(rg[i].e[v]), a[i][v], b);
-                x[i][v] = b * candidate(to_f32(ry[i].e[v]), p.candidate);
-                if (t0 + i >= p.T) a[i][v] = 1.0f, x[i][v] = 0.0f;
                 A[v] *= a[i][v];
                 H[v] = __builtin_fmaf(a[i][v], H[v], x[i][v]);
             }
@@ -281,19 +361,19 @@ __global__ __launch_bounds__(kThreads) void forward_tiles(Args p) {
         if (p.marks && on && t0 < p.T && t0 % kSpan == 0)
 #pragma unroll
             for (int v = 0; v < V; ++v) p.marks[(r * spans + t0 / kSpan) * p.D + ch + v] = h[v];
+        P o[S];
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            P o;
             if (drop >> i & 1)
 #pragma unroll
                 for (int v = 0; v < V; ++v) h[v] = 0.0f;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 h[v] = __builtin_fmaf(a[i][v], h[v], x[i][v]);
-                o.e[v] = from_f32<E>(h[v]);
+                o[i].e[v] = from_f32<E>(h[v]);
             }
-            if (t0 + i < p.T && on) *reinterpret_cast<P*>(out + int64_t(t0 + i) * p.D) = o;
         }
+        store_segment<E, V, S>(o, out, p.D, t0, on ? p.T : 0);
     }
 }
 
@@ -323,9 +403,11 @@ __global__ __launch_bounds__(kThreads) void backward_tiles(Args p) {
     const int64_t r = strip / p.strips_a_row;
     const int ch0 = (strip % p.strips_a_row) * kChannels, ch = ch0 + cl * V;
     const bool on = ch < p.D, owner = tid < kChannels && ch0 + tid < p.D;
-    const E* y = static_cast<const E*>(p.y) + r * p.y_row + ch;
-    const E* g = static_cast<const E*>(p.gate) + r * p.gate_row + ch;
-    const E* d = static_cast<const E*>(p.d_h) + r * p.d_row + ch;
+    const int from = on ? ch : p.D - V;
+    const E* y = static_cast<const E*>(p.y) + r * p.y_row + from;
+    const E* g = static_cast<const E*>(p.gate) + r * p.gate_row + from;
+    const E* d = static_cast<const E*>(p.d_h) + r * p.d_row + from;
+    const uint8_t* reset = p.reset ? p.reset + r * p.T : nullptr;
     E* dy = static_cast<E*>(p.d_y) + r * p.T * p.D + ch;
     E* dg = static_cast<E*>(p.d_gate) + r * p.T * p.D + ch;
     const int64_t spans = (p.T + kSpan - 1) / kSpan;
@@ -336,21 +418,17 @@ __global__ __launch_bounds__(kThreads) void backward_tiles(Args p) {
     P ry[S], rg[S], rd[S];
     uint32_t resets;
     float next_mark = 0.0f;
+    if (!p.d_h)
+#pragma unroll
+        for (int i = 0; i < S; ++i) rd[i] = P{};
     auto load = [&](int at) {
         const int t0 = at * G::kTile + seg * S;
-        resets = 0;
+        const bool whole = (at + 1) * G::kTile <= p.T;
+        load_segment<E, V, S>(ry, y, p.y_pos, t0, p.T, whole, 0.0f);
+        load_segment<E, V, S>(rg, g, p.gate_pos, t0, p.T, whole, -__builtin_inff());
+        if (p.d_h) load_segment<E, V, S>(rd, d, p.d_pos, t0, p.T, whole, 0.0f);
+        resets = load_resets<S>(reset, t0, p.T, whole && p.reset_words);
         if (owner) next_mark = p.marks[(r * spans + at * (G::kTile / kSpan)) * p.D + ch0 + tid];
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const bool in = t0 + i < p.T;
-            ry[i] = P{}, rg[i] = P{}, rd[i] = P{};
-            if (in && on) {
-                ry[i] = *reinterpret_cast<const P*>(y + (t0 + i) * p.y_pos);
-                rg[i] = *reinterpret_cast<const P*>(g + (t0 + i) * p.gate_pos);
-                if (p.d_h) rd[i] = *reinterpret_cast<const P*>(d + (t0 + i) * p.d_pos);
-            }
-            if (in && p.reset) resets |= uint32_t(p.reset[r * p.T + t0 + i] != 0) << i;
-        }
     };
     load(p.tiles - 1 - turn);
     for (int buf = 0; turn < end; ++turn, buf ^= 1) {
@@ -359,18 +437,28 @@ __global__ __launch_bounds__(kThreads) void backward_tiles(Args p) {
         P rl[S];
         const uint32_t drop = resets;
 #pragma unroll
+        for (int i = 0; i < S; ++i) {
+            rl[i] = rd[i];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                gates(to_f32(rg[i].e[v]), a[i][v], b[i][v]);
+                c[i][v] = to_f32(ry[i].e[v]);
+            }
+        }
+        if (p.candidate == HSN_SCAN_TANH)
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int v = 0; v < V; ++v) c[i][v] = tanh_of<E>(c[i][v]);
+#pragma unroll
         for (int v = 0; v < V; ++v) A[v] = 1.0f, H[v] = 0.0f;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            rl[i] = rd[i];
             if (drop >> i & 1)
 #pragma unroll
                 for (int v = 0; v < V; ++v) A[v] = -1.0f, H[v] = 0.0f;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                gates(to_f32(rg[i].e[v]), a[i][v], b[i][v]);
-                c[i][v] = candidate(to_f32(ry[i].e[v]), p.candidate);
-                if (t0 + i >= p.T) a[i][v] = 1.0f, b[i][v] = 0.0f, c[i][v] = 0.0f;
                 A[v] *= a[i][v];
                 H[v] = __builtin_fmaf(a[i][v], H[v], b[i][v] * c[i][v]);
             }
@@ -413,22 +501,28 @@ __global__ __launch_bounds__(kThreads) void backward_tiles(Args p) {
         }
         if constexpr (kSplit) __syncthreads();
         // q over c, and b c'(y) over b, on the way through the states
+        float h[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float h = mark[buf][cl * V + v];
-            for (int w = 0; w < wave; ++w) h = apply(wave_pair[buf][w][cl * V + v], h);
+            h[v] = mark[buf][cl * V + v];
+            for (int w = 0; w < wave; ++w) h[v] = apply(wave_pair[buf][w][cl * V + v], h[v]);
             if constexpr (G::kLanes < kWave) {
                 const Pair m{__shfl_up(A[v], G::kLanes, kWave), __shfl_up(H[v], G::kLanes, kWave)};
-                h = lane >= G::kLanes ? apply(m, h) : h;
+                h[v] = lane >= G::kLanes ? apply(m, h[v]) : h[v];
             }
+        }
+        const float slope = p.candidate == HSN_SCAN_TANH ? -1.0f : 0.0f;  // c' = 1 - c^2, or 1
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                if (drop >> i & 1) h = 0.0f;
-                const float old = h, cand = c[i][v], share = b[i][v];
-                h = __builtin_fmaf(a[i][v], old, share * cand);
-                c[i][v] = a[i][v] * share * (cand - old);
-                if (p.candidate == HSN_SCAN_TANH)
-                    b[i][v] = share * __builtin_fmaf(-cand, cand, 1.0f);
+        for (int i = 0; i < S; ++i) {
+            if (drop >> i & 1)
+#pragma unroll
+                for (int v = 0; v < V; ++v) h[v] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float cand = c[i][v], share = b[i][v];
+                c[i][v] = a[i][v] * share * (cand - h[v]);
+                h[v] = __builtin_fmaf(a[i][v], h[v], share * cand);
+                b[i][v] = share * __builtin_fmaf(slope * cand, cand, 1.0f);
             }
         }
         float mu[V];
@@ -443,24 +537,22 @@ __global__ __launch_bounds__(kThreads) void backward_tiles(Args p) {
                 mu[v] = lane < kWave - G::kLanes ? apply(m, mu[v]) : mu[v];
             }
         }
+        P oy[S], og[S];
 #pragma unroll
         for (int i = S - 1; i >= 0; --i) {
-            P oy, og;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float l = to_f32(rl[i].e[v]) + mu[v];
-                oy.e[v] = from_f32<E>(b[i][v] * l);
-                og.e[v] = from_f32<E>(c[i][v] * l);
+                oy[i].e[v] = from_f32<E>(b[i][v] * l);
+                og[i].e[v] = from_f32<E>(c[i][v] * l);
                 mu[v] = a[i][v] * l;
             }
             if (drop >> i & 1)
 #pragma unroll
                 for (int v = 0; v < V; ++v) mu[v] = 0.0f;
-            if (t0 + i < p.T && on) {
-                *reinterpret_cast<P*>(dy + int64_t(t0 + i) * p.D) = oy;
-                *reinterpret_cast<P*>(dg + int64_t(t0 + i) * p.D) = og;
-            }
         }
+        store_segment<E, V, S>(oy, dy, p.D, t0, on ? p.T : 0);
+        store_segment<E, V, S>(og, dg, p.D, t0, on ? p.T : 0);
     }
 }
 
@@ -492,23 +584,11 @@ void launch_backward_as(const Args& p, bool split, hipStream_t st) {
 }
 template <typename E>
 void launch_forward(const Args& p, int vec, bool split, hipStream_t st) {
-    if constexpr (sizeof(E) == 2)
-        if (vec == 8) return launch_forward_as<E, 8>(p, split, st);
-    if constexpr (sizeof(E) == 2)
-        if (vec == 2) return launch_forward_as<E, 2>(p, split, st);
-    if constexpr (sizeof(E) == 4)
-        if (vec == 4) return launch_forward_as<E, 4>(p, split, st);
-    launch_forward_as<E, 1>(p, split, st);
+    vec == 2 ? launch_forward_as<E, 2>(p, split, st) : launch_forward_as<E, 1>(p, split, st);
 }
 template <typename E>
 void launch_backward(const Args& p, int vec, bool split, hipStream_t st) {
-    if constexpr (sizeof(E) == 2)
-        if (vec == 8) return launch_backward_as<E, 8>(p, split, st);
-    if constexpr (sizeof(E) == 2)
-        if (vec == 2) return launch_backward_as<E, 2>(p, split, st);
-    if constexpr (sizeof(E) == 4)
-        if (vec == 4) return launch_backward_as<E, 4>(p, split, st);
-    launch_backward_as<E, 1>(p, split, st);
+    vec == 2 ? launch_backward_as<E, 2>(p, split, st) : launch_backward_as<E, 1>(p, split, st);
 }
 #endif
 
