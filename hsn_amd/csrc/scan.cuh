@@ -19,7 +19,7 @@
 // workgroup of its own (kSplit): it publishes its pair and takes the pairs before it from device
 // memory. Tiles are numbered by a ticket, so that whatever a workgroup waits for belongs to one that
 // already runs and publishes without waiting for a later one: every wait ends. Pairs are folded in
-// groups of 16 tiles in a fixed order, so the bits do not depend on who arrives first. Split, the
+// groups of 32 tiles in a fixed order, so the bits do not depend on who arrives first. Split, the
 // same 8 x 4096 x 2048 take 97 and 170 us (4.2 and 3.9 TB/s of the 3 and 5 elements that have to move),
 // and one row of 32769 x 1024 60 us, which one walk a strip takes 1.0 ms for; at 32 x 256 x 512 in
 // fp32 the walk's 13.6 and 19.4 us are less than the split's 13.6 and 22.7 and the clearing of its words.
@@ -35,7 +35,7 @@ namespace scan {
 constexpr int kSpan = HSN_SCAN_SPAN;
 constexpr int kThreads = 512, kWaves = kThreads / kWave;
 constexpr int kChannels = 64;  // of a tile
-constexpr int kGroup = 16;     // tiles whose pairs are folded one by one
+constexpr int kGroup = 32;     // tiles whose pairs are folded one by one
 
 struct Args {
     const void *y, *gate, *d_h;
@@ -177,15 +177,28 @@ __device__ __forceinline__ void publish(uint64_t* at, uint64_t w) {
     __hip_atomic_store(at, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Waits for a wave's 64 words. Each belongs to a workgroup with a lower ticket; the bound (seconds)
-// is there so that no fault elsewhere can hang the grid, and what it gives up on becomes NaN.
-__device__ __forceinline__ Pair await(const uint64_t* at) {
+// Waits for N times a wave's 64 words, N loads in flight. Each belongs to a workgroup with a lower
+// ticket; the bound (seconds) is there so that no fault elsewhere can hang the grid, and what it
+// gives up on becomes NaN. An absent item (NULL) is the identity.
+template <int N>
+__device__ __forceinline__ void await(const uint64_t* const (&at)[N], Pair (&pair)[N]) {
     for (int spin = 0; spin < (1 << 21); ++spin) {
-        const uint64_t w = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (ballot(w == 0) == 0) return word_pair(w);
+        uint64_t w[N];
+        bool missing = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            w[i] = at[i] ? __hip_atomic_load(at[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                         : pair_word({1.0f, 0.0f});
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            missing |= w[i] == 0;
+            pair[i] = word_pair(w[i]);
+        }
+        if (ballot(missing) == 0) return;
         __builtin_amdgcn_s_sleep(1);
     }
-    return {-1.0f, __int_as_float(0x7fc00000)};
+#pragma unroll
+    for (int i = 0; i < N; ++i) pair[i] = {-1.0f, __int_as_float(0x7fc00000)};
 }
 
 struct ExchangeLds {
@@ -203,11 +216,19 @@ __device__ __forceinline__ float exchange(const Args& p, ExchangeLds& lds, int k
     if (wave == 0) publish(pairs + k * line, pair_word(total));
     // item 0: the state before the group; item i: the pair of the group's tile i - 1
     const int group = k / kGroup, before = k % kGroup;
-    for (int i = wave; i <= before; i += kWaves)
-        if (i)
-            lds.item[i][lane] = await(pairs + (group * kGroup + i - 1) * line);
-        else if (group)
-            lds.item[0][lane] = await(prefix + (group - 1) * line);
+    constexpr int kItems = kGroup / kWaves;
+    const uint64_t* at[kItems];
+    Pair item[kItems];
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+        const int i = wave + j * kWaves;
+        at[j] = nullptr;
+        if (i == 0 && group) at[j] = prefix + (group - 1) * line;
+        if (i > 0 && i <= before) at[j] = pairs + (group * kGroup + i - 1) * line;
+    }
+    await<kItems>(at, item);
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) lds.item[wave + j * kWaves][lane] = item[j];
     __syncthreads();
     float h = start;
     if (wave == 0) {
@@ -218,7 +239,7 @@ __device__ __forceinline__ float exchange(const Args& p, ExchangeLds& lds, int k
     }
     return h;
 }
-static_assert(kGroup <= 16, "a group's items: its prefix and up to 15 pairs");
+static_assert(kGroup % kWaves == 0, "a group's items, its prefix and the pairs before, by waves");
 
 // --------------------------------------------------------------------------------------------
 // Forward.
@@ -562,18 +583,27 @@ void launch_forward(const Args& p, int vec, bool split, hipStream_t st);
 template <typename E>
 void launch_backward(const Args& p, int vec, bool split, hipStream_t st);
 
-// Positions of a tile, by the kernels' segments.
-constexpr int kForwardPer = 32, kBackwardPer = 16;  // elements of a thread
-constexpr int kForwardTile = kThreads * kForwardPer / kChannels;
-constexpr int kBackwardTile = kThreads * kBackwardPer / kChannels;
+// Elements of a thread's segments. Forward in fp32, 16: more workgroups fit a compute unit and the
+// loads overlap better (8 x 8192 x 1024 split: 165 us, with 32 184). In 16 bits the halves' joins
+// cost more than that gives (8 x 4096 x 2048 split: 100 us with 32, 119 with 16). The backward has
+// three values an element to keep and no room for 32.
+template <typename E>
+constexpr int kForwardPer = sizeof(E) == 4 ? 16 : 32;
+constexpr int kBackwardPer = 16;
+
+// Positions of a tile.
+inline int forward_tile(int element_size) {
+    return kThreads / kChannels * (element_size == 4 ? kForwardPer<float> : kForwardPer<bf16_t>);
+}
+inline int backward_tile() { return kThreads / kChannels * kBackwardPer; }
 
 #ifdef HSN_SCAN_INSTANTIATE
 template <typename E, int V>
 void launch_forward_as(const Args& p, bool split, hipStream_t st) {
     if (split)
-        forward_tiles<E, V, kForwardPer / V, true><<<p.strips * p.tiles, kThreads, 0, st>>>(p);
+        forward_tiles<E, V, kForwardPer<E> / V, true><<<p.strips * p.tiles, kThreads, 0, st>>>(p);
     else
-        forward_tiles<E, V, kForwardPer / V, false><<<p.strips, kThreads, 0, st>>>(p);
+        forward_tiles<E, V, kForwardPer<E> / V, false><<<p.strips, kThreads, 0, st>>>(p);
 }
 template <typename E, int V>
 void launch_backward_as(const Args& p, bool split, hipStream_t st) {

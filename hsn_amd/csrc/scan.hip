@@ -34,6 +34,8 @@ void by_dtype(int dtype, F&& f) {
     return f(bf16_t{});
 }
 
+int size_of(int dtype) { return dtype == HSN_DTYPE_F32 ? 4 : 2; }
+
 void check(int B, int T, int D, int dtype, int candidate_kind) {
     HSN_REQUIRE(dtype == HSN_DTYPE_F32 || dtype == HSN_DTYPE_F16 || dtype == HSN_DTYPE_BF16,
                 HSN_ERR_UNSUPPORTED_DTYPE, "dtype must be F32, F16 or BF16");
@@ -123,7 +125,7 @@ extern "C" int hsn_scan_workspace(int B, int T, int D, int dtype, int backward, 
     HSN_ABI_BEGIN
     check(B, T, D, dtype, HSN_SCAN_TANH);
     HSN_REQUIRE(bytes, HSN_ERR_INVALID_ARGUMENT, "bytes must not be NULL");
-    *bytes = 8 * plan(B, T, D, backward ? kBackwardTile : kForwardTile).words;
+    *bytes = 8 * plan(B, T, D, backward ? backward_tile() : forward_tile(size_of(dtype))).words;
     HSN_ABI_END
 }
 
@@ -145,9 +147,9 @@ extern "C" int hsn_scan_forward(const void* y, int64_t y_row, int64_t y_pos, con
     p.y = y, p.gate = gate, p.y_row = y_row, p.y_pos = y_pos, p.gate_row = gate_row;
     p.gate_pos = gate_pos, p.reset = reset, p.h0 = h0, p.h = h, p.h_T = h_T, p.marks = marks;
     p.T = T, p.D = D, p.candidate = candidate_kind;
-    const int vec = vector_of(dtype == HSN_DTYPE_F32 ? 4 : 2, D, {y, gate, h},
+    const int vec = vector_of(size_of(dtype), D, {y, gate, h},
                               {y_row, y_pos, gate_row, gate_pos});
-    run(p, plan(B, T, D, kForwardTile), dtype, vec, false, workspace, workspace_bytes,
+    run(p, plan(B, T, D, forward_tile(size_of(dtype))), dtype, vec, false, workspace, workspace_bytes,
         as_stream(stream));
     HSN_ABI_END
 }
@@ -172,9 +174,9 @@ extern "C" int hsn_scan_backward(const void* y, int64_t y_row, int64_t y_pos, co
     p.gate_pos = gate_pos, p.d_row = d_row, p.d_pos = d_pos, p.reset = reset, p.d_h_T = d_h_T;
     p.marks = const_cast<float*>(marks), p.d_y = d_y, p.d_gate = d_gate, p.d_h0 = d_h0;
     p.T = T, p.D = D, p.candidate = candidate_kind;
-    const int vec = vector_of(dtype == HSN_DTYPE_F32 ? 4 : 2, D, {y, gate, d_h, d_y, d_gate},
+    const int vec = vector_of(size_of(dtype), D, {y, gate, d_h, d_y, d_gate},
                               {y_row, y_pos, gate_row, gate_pos, d_row, d_pos});
-    run(p, plan(B, T, D, kBackwardTile), dtype, vec, true, workspace, workspace_bytes,
+    run(p, plan(B, T, D, backward_tile()), dtype, vec, true, workspace, workspace_bytes,
         as_stream(stream));
     HSN_ABI_END
 }
