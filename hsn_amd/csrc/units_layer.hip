@@ -1,6 +1,27 @@
-// A whole layer of routed units for a few tokens (include/hsn_units_layer.h), in three launches:
-// the router's products and the choice (a workgroup a token), the hidden units (a lane a column of
-// one chosen unit of one token), the outputs (a lane a column of one token, over its K units).
+// A whole layer of routed units for a few tokens (include/hsn_units_layer.h).
+//
+//   route    (token, chunk of units): the router's products, a wave a unit; the choice in the same
+//            launch where one chunk holds all units, else in `choose`.
+//   product  (column tile and split of the rows, slot): z = x W1[e] for the tokens that chose the
+//            slot's unit e, as fp32 sums of the split's rows.
+//   product  the same for v W2[e], where v is made from the first product's sums on the way.
+//   combine  (token, 256 columns): the weighted sum over the token's units, in a fixed order.
+//
+// What bounds it is one read of the chosen units' weights, so the products stream them from HBM into
+// registers once, 16 bytes a lane, as they lie ([in, out]), and give them to the matrix cores with up
+// to 16 tokens as the other operand. A wave takes 32 rows and 16 lanes' columns a step, lane group g =
+// lane / 16 the rows 8 g .. 8 g + 7: eight loads of one row each. In 16-bit storage a lane then
+// holds 8 columns of 8 consecutive rows; byte permutes pair neighbouring rows into the operands of 8
+// products 16x16x32, the m-th with the columns c0 + m of the lanes. Rows are split over a workgroup's
+// waves and, where units and column tiles are few, over workgroups, so that some 512 workgroups
+// keep the loads of two steps each in flight.
+//
+// x enters the first product exactly. v is fp32: with bf16 weights it goes to the matrix cores as the
+// sum of two bf16 (16 significant bits, 2^-17 of v at most is lost; one bf16 would lose 2^-9); fp16
+// weights are widened and multiply v in fp32, since fp16 has not the range of an unscaled v.
+#include <algorithm>
+#include <type_traits>
+
 #include "../../include/hsn_units_layer.h"
 #include "abi_util.h"
 #include "common.cuh"
@@ -11,85 +32,376 @@ namespace units_layer {
 namespace {
 
 constexpr int kMaxUnits = HSN_UNITS_MAX, kMaxChosen = HSN_UNITS_MAX_CHOSEN;
+constexpr int kMaxTokens = HSN_UNITS_MAX_TOKENS;
+constexpr int kRouteThreads = 1024, kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kRows = 32;    // rows of a step
+constexpr int kTokens = 16;  // tokens of a product
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+// One of the two products: [pairs, rows] times [M, rows, cols] by the pairs' units.
+struct Product {
+    const void* W;
+    float* sums;  // [splits, pairs, cols]
+    int rows, cols, tiles, splits, split_rows;
+};
 
 struct Args {
-    const void *x, *router, *W1, *b1, *W2, *b2;
+    const void *x, *router, *b1, *b2;
     void* y;
     int64_t x_row;
-    int* unit;      // [n, K] the choice
-    float* share;   // [n, K]
-    float* hidden;  // [n, K, H]
+    float* logit;  // [n, M]
+    int* unit;     // [n, K] the choice
+    float* share;  // [n, K]
+    Product up, down;
     int n, M, K, d_in, H, d_out, activation;
 };
 
+// 16 bytes from any element's address (one load; the GPU takes global addresses unaligned).
 template <typename E>
-__global__ __launch_bounds__(256) void route(Args a) {
-    __shared__ float logit[kMaxUnits];
-    const int i = blockIdx.x, lane = threadIdx.x % kWave;
-    const E* x = static_cast<const E*>(a.x) + i * a.x_row;
-    for (int m = threadIdx.x / kWave; m < a.M; m += 4) {
-        const E* w = static_cast<const E*>(a.router) + int64_t(m) * a.d_in;
-        float sum = 0.0f;
-        for (int k = lane; k < a.d_in; k += kWave) sum = __builtin_fmaf(to_f32(x[k]), to_f32(w[k]), sum);
-        for (int d = 1; d < kWave; d *= 2) sum += wave_shfl_xor(sum, d);
-        if (lane == 0) logit[m] = sum;
+__device__ __forceinline__ v4u load16(const E* p) {
+    v4u r;
+    __builtin_memcpy(&r, p, 16);
+    return r;
+}
+
+// --------------------------------------------------------------------------------------------
+// The router.
+// --------------------------------------------------------------------------------------------
+
+// The token's K units from its products in LDS: a unit's rank is the number of units before it
+// (larger, or equal and lower).
+__device__ void choose_from(const Args& a, int i, const float* logit, float* chosen) {
+    __syncthreads();
+    const int m = threadIdx.x;
+    if (m < a.M) {
+        const uint32_t key = score_key(logit[m]);
+        int rank = 0;
+        for (int j = 0; j < a.M; ++j) {
+            const uint32_t other = score_key(logit[j]);
+            rank += other > key || (other == key && j < m);
+        }
+        if (rank < a.K) {
+            a.unit[i * a.K + rank] = m;
+            chosen[rank] = logit[m];
+        }
     }
     __syncthreads();
-    if (threadIdx.x >= kWave) return;
-    // the K largest by (key, lowest unit), one a round
-    float top = 0.0f, sum = 0.0f, mine = 0.0f;
-    bool taken[kMaxUnits / kWave] = {};
-    for (int k = 0; k < a.K; ++k) {
-        uint64_t best = 0;
-        for (int j = 0; j < kMaxUnits / kWave; ++j) {
-            const int m = j * kWave + lane;
-            if (m < a.M && !taken[j])
-                best = max(best, uint64_t(score_key(logit[m])) << 32 | uint32_t(~m));
+    if (m < a.K) {
+        float sum = 0.0f;
+        for (int k = 0; k < a.K; ++k) sum += expf(chosen[k] - chosen[0]);
+        a.share[i * a.K + m] = expf(chosen[m] - chosen[0]) / sum;
+    }
+}
+
+template <typename E>
+__global__ __launch_bounds__(kRouteThreads) void route(Args a, int chunk) {
+    __shared__ float logit[kMaxUnits], chosen[kMaxChosen];
+    constexpr int kVec = 16 / sizeof(E), kStep = kWave * kVec;
+    const int i = blockIdx.x, lane = threadIdx.x % kWave;
+    const int first = blockIdx.y * chunk, last = min(a.M, first + chunk);
+    const E* x = static_cast<const E*>(a.x) + i * a.x_row;
+    for (int m = first + int(threadIdx.x) / kWave; m < last; m += kRouteThreads / kWave) {
+        const E* w = static_cast<const E*>(a.router) + int64_t(m) * a.d_in;
+        float sum = 0.0f;
+        int k = lane * kVec;
+#pragma unroll 4
+        for (; k + kVec <= a.d_in; k += kStep) {
+            const v4u xv = load16(x + k), wv = load16(w + k);
+            E xe[kVec], we[kVec];
+            __builtin_memcpy(xe, &xv, 16);
+            __builtin_memcpy(we, &wv, 16);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) sum = __builtin_fmaf(to_f32(xe[j]), to_f32(we[j]), sum);
         }
-        for (int d = 1; d < kWave; d *= 2)
-            best = max(best, uint64_t(__shfl_xor(static_cast<unsigned long long>(best), d, kWave)));
-        const int m = static_cast<int>(~static_cast<uint32_t>(best));
-        for (int j = 0; j < kMaxUnits / kWave; ++j) taken[j] |= m == j * kWave + lane;
-        if (k == 0) top = logit[m];
-        const float e = expf(logit[m] - top);
-        sum += e;
-        if (lane == k) mine = e;
-        if (lane == 0) a.unit[i * a.K + k] = m;
+        for (; k < a.d_in; ++k)  // the last, incomplete pack is one lane's
+            sum = __builtin_fmaf(to_f32(x[k]), to_f32(w[k]), sum);
+        for (int d = 1; d < kWave; d *= 2) sum += wave_shfl_xor(sum, d);
+        if (lane == 0) {
+            logit[m] = sum;
+            if (gridDim.y > 1) a.logit[i * a.M + m] = sum;
+        }
     }
-    if (lane < a.K) a.share[i * a.K + lane] = mine / sum;
+    if (gridDim.y == 1) choose_from(a, i, logit, chosen);
+}
+
+__global__ __launch_bounds__(kMaxUnits) void choose(Args a) {
+    __shared__ float logit[kMaxUnits], chosen[kMaxChosen];
+    const int i = blockIdx.x;
+    if (int(threadIdx.x) < a.M) logit[threadIdx.x] = a.logit[i * a.M + threadIdx.x];
+    choose_from(a, i, logit, chosen);
+}
+
+// --------------------------------------------------------------------------------------------
+// The products.
+// --------------------------------------------------------------------------------------------
+
+// Eight rows of the left operand: pair's rows k0 + 8 g .. + 7 (0 from `end` on).
+template <typename E>
+__device__ __forceinline__ void load_x(const Args& a, int pair, int k, int end, E (&to)[8]) {
+    const E* x = static_cast<const E*>(a.x) + (pair / a.K) * a.x_row + k;
+    if (k + 8 <= end) {
+        __builtin_memcpy(to, x, sizeof(to));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) to[j] = k + j < end ? x[j] : from_f32<E>(0.0f);
+    }
+}
+
+// Eight of a pair's first-product values: the splits' sums, then the bias.
+template <typename E>
+__device__ __forceinline__ void load_z(const Args& a, int pair, int unit, int col, int count,
+                                       float (&z)[8]) {
+    const int64_t stride = int64_t(a.n) * a.K * a.up.cols;
+    const float* at = a.up.sums + int64_t(pair) * a.up.cols + col;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[j] = 0.0f;
+    for (int s = 0; s < a.up.splits; ++s, at += stride)
+        if (count == 8) {
+            float v[8];
+            __builtin_memcpy(v, at, sizeof(v));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] += v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < count) z[j] += at[j];
+        }
+    if (a.b1) {
+        const E* b = static_cast<const E*>(a.b1) + int64_t(unit) * a.up.cols + col;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < count) z[j] += to_f32(b[j]);
+    }
 }
 
 template <typename E>
-__global__ __launch_bounds__(64) void up(Args a) {
-    const int col = blockIdx.x * 64 + threadIdx.x, pair = blockIdx.y;
-    if (col >= a.H) return;
-    const bool gated = a.activation == HSN_UNITS_SWIGLU;
-    const int H1 = gated ? 2 * a.H : a.H;
-    const int64_t unit = a.unit[pair];
-    const E* x = static_cast<const E*>(a.x) + (pair / a.K) * a.x_row;
-    const E* w = static_cast<const E*>(a.W1) + unit * a.d_in * H1 + col;
-    const E* b = static_cast<const E*>(a.b1) + unit * H1 + col;
-    float z = a.b1 ? to_f32(b[0]) : 0.0f, g = a.b1 && gated ? to_f32(b[a.H]) : 0.0f;
-    for (int k = 0; k < a.d_in; ++k) {
-        const float v = to_f32(x[k]);
-        z = __builtin_fmaf(v, to_f32(w[int64_t(k) * H1]), z);
-        if (gated) g = __builtin_fmaf(v, to_f32(w[int64_t(k) * H1 + a.H]), g);
+__device__ __forceinline__ void load_hidden(const Args& a, int pair, int unit, int k, int end,
+                                            float (&v)[8]) {
+    const int count = min(8, max(0, end - k));
+    float z[8];
+    load_z<E>(a, pair, unit, k, count, z);
+    if (a.activation == HSN_UNITS_SWIGLU) {
+        float g[8];
+        load_z<E>(a, pair, unit, a.H + k, count, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = z[j] * act_sigmoid(z[j]) * g[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = units::gelu(z[j]);
     }
-    a.hidden[int64_t(pair) * a.H + col] = gated ? z * act_sigmoid(z) * g : units::gelu(z);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? v[j] : 0.0f;
+}
+
+__device__ __forceinline__ v4f mfma(v8bf a, v8bf b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Column m of the lane's eight rows as the eight-row operand of a 16-bit product.
+template <typename V8>
+__device__ __forceinline__ V8 column(const v4u (&row)[8], int m) {
+    v4u r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r[i] = __builtin_amdgcn_perm(row[2 * i + 1][m / 2], row[2 * i][m / 2],
+                                     m % 2 ? 0x07060302u : 0x05040100u);
+    return __builtin_bit_cast(V8, r);
 }
 
 template <typename E>
-__global__ __launch_bounds__(64) void down(Args a) {
-    const int col = blockIdx.x * 64 + threadIdx.x, i = blockIdx.y;
+__device__ __forceinline__ float element(v4u row, int m) {
+    E e[16 / sizeof(E)];
+    __builtin_memcpy(e, &row, 16);
+    return to_f32(e[m]);
+}
+
+template <typename E, bool kDown>
+__global__ __launch_bounds__(kThreads, 2) void product(Args a) {
+    constexpr int kCols = 16 / sizeof(E);   // of a lane
+    constexpr int kTileCols = 16 * kCols;
+    constexpr bool kBf16 = __is_same(E, bf16_t), kF32 = __is_same(E, float);
+    __shared__ float red[kWaves][kTokens][kTileCols];
+    __shared__ uint32_t mask[kMaxUnits / 32];
+    __shared__ int list[kMaxTokens], listed;
+    const Product& p = kDown ? a.down : a.up;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int pairs = a.n * a.K, slot = blockIdx.y;
+    // the slot's unit, the slot-th of the chosen ones, and its pairs (at most one a token)
+    int unit, count = 1;
+    if (a.n == 1) {
+        unit = a.unit[slot];
+        if (tid == 0) list[0] = slot;
+        __syncthreads();
+    } else {
+        if (tid < kMaxUnits / 32) mask[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < pairs; i += kThreads)
+            atomicOr(&mask[a.unit[i] / 32], 1u << a.unit[i] % 32);
+        __syncthreads();
+        unit = -1;
+        for (int w = 0, seen = 0; w < kMaxUnits / 32; ++w) {
+            uint32_t bits = uniform(mask[w]);
+            const int here = __popc(bits);
+            if (unit < 0 && seen + here > slot) {
+                for (int k = seen; k < slot; ++k) bits &= bits - 1;
+                unit = w * 32 + __ffs(bits) - 1;
+            }
+            seen += here;
+        }
+        if (unit < 0) return;
+        if (wave == 0) {
+            int n = 0;
+            for (int base = 0; base < pairs; base += kWave) {
+                const bool hit = base + lane < pairs && a.unit[base + lane] == unit;
+                const uint64_t hits = ballot(hit);
+                if (hit) list[n + lanes_below(hits)] = base + lane;
+                n += __popcll(hits);
+            }
+            if (lane == 0) listed = n;
+        }
+        __syncthreads();
+        count = listed;
+    }
+    const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles;
+    const int begin = split * p.split_rows, end = min(p.rows, begin + p.split_rows);
+    const int group = lane / 16, col_lane = lane % 16;
+    // a lane's columns end with the row: the last lanes share the last columns
+    auto first_col = [&](int l) { return max(0, min(tile * kTileCols + l * kCols, p.cols - kCols)); };
+    const E* W = static_cast<const E*>(p.W) + int64_t(unit) * p.rows * p.cols + first_col(col_lane);
+    const bool narrow = p.cols < kCols;
+
+    auto load_rows = [&](int k0, v4u (&row)[8]) {
+        const int k = k0 + 8 * group;
+        const E* at = W + int64_t(k) * p.cols;
+        if (k0 + kRows <= end && !narrow) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) row[j] = load16(at + int64_t(j) * p.cols);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                E e[kCols];
+                row[j] = v4u{};
+                if (k + j >= end) continue;
+                if (!narrow) {
+                    row[j] = load16(at + int64_t(j) * p.cols);
+                    continue;
+                }
+#pragma unroll
+                for (int m = 0; m < kCols; ++m)
+                    e[m] = m < p.cols ? at[int64_t(j) * p.cols + m] : from_f32<E>(0.0f);
+                __builtin_memcpy(&row[j], e, 16);
+            }
+        }
+    };
+
+    for (int t0 = 0; t0 < count; t0 += kTokens) {
+        const int here = min(kTokens, count - t0);
+        const int pair = list[t0 + min(col_lane, here - 1)];
+        v4f acc[kCols];
+#pragma unroll
+        for (int m = 0; m < kCols; ++m) acc[m] = v4f{};
+        auto multiply = [&](int k0, const v4u (&row)[8]) {
+            const int k = k0 + 8 * group;
+            if constexpr (kDown) {
+                float v[8];
+                load_hidden<E>(a, pair, unit, k, end, v);
+                if constexpr (kBf16) {
+                    v8bf hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        hi[j] = static_cast<__bf16>(v[j]);
+                        const float rest = v[j] - static_cast<float>(hi[j]);
+                        // an infinite v is all in hi
+                        lo[j] = static_cast<__bf16>(__builtin_fabsf(v[j]) < 3e38f ? rest : 0.0f);
+                    }
+#pragma unroll
+                    for (int m = 0; m < kCols; ++m) {
+                        const v8bf w = column<v8bf>(row, m);
+                        acc[m] = mfma(lo, w, acc[m]);
+                        acc[m] = mfma(hi, w, acc[m]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int m = 0; m < kCols; ++m)
+                            acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                v[j], element<E>(row[j], m), acc[m], 0, 0, 0);
+                }
+            } else {
+                E x[8];
+                load_x<E>(a, pair, k, end, x);
+                if constexpr (kF32) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int m = 0; m < kCols; ++m)
+                            acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                x[j], element<E>(row[j], m), acc[m], 0, 0, 0);
+                } else {
+                    using V8 = typename std::conditional<kBf16, v8bf, v8h>::type;
+                    V8 left;
+                    __builtin_memcpy(&left, x, 16);
+#pragma unroll
+                    for (int m = 0; m < kCols; ++m) acc[m] = mfma(left, column<V8>(row, m), acc[m]);
+                }
+            }
+        };
+        // the next step's rows in flight
+        v4u even[8], odd[8];
+        constexpr int kStep = kWaves * kRows;
+        int k0 = begin + wave * kRows;
+        if (k0 < end) load_rows(k0, even);
+        while (k0 < end) {
+            if (k0 + kStep < end) load_rows(k0 + kStep, odd);
+            multiply(k0, even);
+            k0 += kStep;
+            if (k0 >= end) break;
+            if (k0 + kStep < end) load_rows(k0 + kStep, even);
+            multiply(k0, odd);
+            k0 += kStep;
+        }
+        // the waves' sums, in their order; a lane has the tokens 4 group + i
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (4 * group + i < here)
+#pragma unroll
+                for (int m = 0; m < kCols; ++m)
+                    red[wave][4 * group + i][col_lane * kCols + m] = acc[m][i];
+        __syncthreads();
+        for (int i = tid; i < here * kTileCols; i += kThreads) {
+            const int t = i / kTileCols, c = i % kTileCols;
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) sum += red[w][t][c];
+            const int col = first_col(c / kCols) + c % kCols;
+            if (col < p.cols)
+                p.sums[(int64_t(split) * pairs + list[t0 + t]) * p.cols + col] = sum;
+        }
+        __syncthreads();
+    }
+}
+
+template <typename E>
+__global__ __launch_bounds__(256) void combine(Args a) {
+    const int col = blockIdx.x * 256 + threadIdx.x, i = blockIdx.y;
     if (col >= a.d_out) return;
+    const int64_t stride = int64_t(a.n) * a.K * a.d_out;
     float y = 0.0f;
     for (int k = 0; k < a.K; ++k) {
         const int pair = i * a.K + k;
-        const int64_t unit = a.unit[pair];
-        const E* w = static_cast<const E*>(a.W2) + unit * a.H * a.d_out + col;
-        const float* v = a.hidden + int64_t(pair) * a.H;
-        float z = a.b2 ? to_f32(static_cast<const E*>(a.b2)[unit * a.d_out + col]) : 0.0f;
-        for (int j = 0; j < a.H; ++j) z = __builtin_fmaf(v[j], to_f32(w[int64_t(j) * a.d_out]), z);
+        const float* at = a.down.sums + int64_t(pair) * a.d_out + col;
+        float z = 0.0f;
+        for (int s = 0; s < a.down.splits; ++s) z += at[s * stride];
+        if (a.b2)
+            z += to_f32(static_cast<const E*>(a.b2)[int64_t(a.unit[pair]) * a.d_out + col]);
         y = __builtin_fmaf(a.share[pair], z, y);
     }
     static_cast<E*>(a.y)[int64_t(i) * a.d_out + col] = from_f32<E>(y);
@@ -109,29 +421,55 @@ void check(int n, int M, int K, int d_in, int H, int d_out, int dtype, int activ
                 "widths of at most 65536");
 }
 
-int64_t layout(Args* a, char* base, int n, int K, int H) {
+// How a product's rows are split: some 512 workgroups (two a compute unit), but at least two steps a
+// wave.
+Product plan(const void* W, int rows, int cols, int slots, int size) {
+    Product p{};
+    p.W = W, p.rows = rows, p.cols = cols;
+    p.tiles = (cols + 16 * (16 / size) - 1) / (16 * (16 / size));
+    const int most = std::max(1, rows / (2 * kWaves * kRows));
+    const int splits = std::min(most, std::max(1, 512 / (slots * p.tiles)));
+    p.split_rows = ((rows + splits - 1) / splits + kRows - 1) / kRows * kRows;
+    p.splits = (rows + p.split_rows - 1) / p.split_rows;
+    return p;
+}
+
+// Fills `a`'s products and its parts of the workspace; returns the workspace's bytes.
+int64_t layout(Args& a, const void* W1, const void* W2, char* base, int size) {
+    const int slots = std::min(a.n * a.K, a.M);
+    const int64_t pairs = int64_t(a.n) * a.K;
+    a.up = plan(W1, a.d_in, a.activation == HSN_UNITS_SWIGLU ? 2 * a.H : a.H, std::max(1, slots), size);
+    a.down = plan(W2, a.H, a.d_out, std::max(1, slots), size);
     int64_t at = 0;
-    auto take = [&](int64_t bytes) {
+    auto take = [&](int64_t count) {
         char* p = base + at;
-        at += (bytes + 255) / 256 * 256;
+        at += (4 * count + 255) / 256 * 256;
         return p;
     };
-    char* unit = take(4LL * n * K);
-    char* share = take(4LL * n * K);
-    char* hidden = take(4LL * n * K * H);
-    if (a) {
-        a->unit = reinterpret_cast<int*>(unit);
-        a->share = reinterpret_cast<float*>(share);
-        a->hidden = reinterpret_cast<float*>(hidden);
-    }
+    a.logit = reinterpret_cast<float*>(take(int64_t(a.n) * a.M));
+    a.unit = reinterpret_cast<int*>(take(pairs));
+    a.share = reinterpret_cast<float*>(take(pairs));
+    a.up.sums = reinterpret_cast<float*>(take(a.up.splits * pairs * a.up.cols));
+    a.down.sums = reinterpret_cast<float*>(take(a.down.splits * pairs * a.down.cols));
     return at;
 }
 
 template <typename E>
 void launch(const Args& a, hipStream_t st) {
-    route<E><<<a.n, 256, 0, st>>>(a);
-    up<E><<<dim3((a.H + 63) / 64, a.n * a.K), 64, 0, st>>>(a);
-    down<E><<<dim3((a.d_out + 63) / 64, a.n), 64, 0, st>>>(a);
+    // One workgroup reads the whole router for a token; above 256 KiB, and where the tokens are few,
+    // the units are chunked (and chosen in a launch of their own).
+    const int64_t router = int64_t(a.M) * a.d_in * sizeof(E);
+    int chunks = 1;
+    if (router > 256 * 1024 && a.n < 64)
+        chunks = static_cast<int>(std::min<int64_t>((a.M + 15) / 16, router / (128 * 1024)));
+    const int chunk = (a.M + chunks - 1) / chunks;
+    chunks = (a.M + chunk - 1) / chunk;
+    route<E><<<dim3(a.n, chunks), kRouteThreads, 0, st>>>(a, chunk);
+    if (chunks > 1) choose<<<a.n, kMaxUnits, 0, st>>>(a);
+    const int slots = std::min(a.n * a.K, a.M);
+    product<E, false><<<dim3(a.up.tiles * a.up.splits, slots), kThreads, 0, st>>>(a);
+    product<E, true><<<dim3(a.down.tiles * a.down.splits, slots), kThreads, 0, st>>>(a);
+    combine<E><<<dim3((a.d_out + 255) / 256, a.n), 256, 0, st>>>(a);
 }
 
 }  // namespace
@@ -146,7 +484,9 @@ extern "C" int hsn_units_layer_workspace(int n, int M, int K, int d_in, int H, i
     HSN_ABI_BEGIN
     check(n, M, K, d_in, H, d_out, dtype, activation);
     HSN_REQUIRE(bytes, HSN_ERR_INVALID_ARGUMENT, "bytes must not be NULL");
-    *bytes = layout(nullptr, nullptr, n, K, H);
+    Args a{};
+    a.n = n, a.M = M, a.K = K, a.d_in = d_in, a.H = H, a.d_out = d_out, a.activation = activation;
+    *bytes = layout(a, nullptr, nullptr, nullptr, dtype == HSN_DTYPE_F32 ? 4 : 2);
     HSN_ABI_END
 }
 
@@ -159,9 +499,13 @@ extern "C" int hsn_units_layer(const void* x, int64_t x_row, const void* router,
     if (n == 0) return HSN_OK;
     HSN_REQUIRE(x && router && W1 && W2 && y && workspace, HSN_ERR_INVALID_ARGUMENT,
                 "a required pointer is NULL");
-    Args a{x, router, W1, b1, W2, b2, y, x_row, nullptr, nullptr, nullptr, n, M, K, d_in, H, d_out,
-           activation};
-    HSN_REQUIRE(workspace_bytes >= layout(&a, static_cast<char*>(workspace), n, K, H),
+    HSN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, HSN_ERR_INVALID_ARGUMENT,
+                "the workspace must be aligned to 16 bytes");
+    Args a{};
+    a.x = x, a.x_row = x_row, a.router = router, a.b1 = b1, a.b2 = b2, a.y = y;
+    a.n = n, a.M = M, a.K = K, a.d_in = d_in, a.H = H, a.d_out = d_out, a.activation = activation;
+    HSN_REQUIRE(workspace_bytes >= layout(a, W1, W2, static_cast<char*>(workspace),
+                                          dtype == HSN_DTYPE_F32 ? 4 : 2),
                 HSN_ERR_INVALID_ARGUMENT, "the workspace is too small");
     if (dtype == HSN_DTYPE_F32)
         launch<float>(a, as_stream(stream));
