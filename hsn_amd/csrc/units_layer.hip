@@ -1,11 +1,11 @@
 // A whole layer of routed units for a few tokens (include/hsn_units_layer.h).
 //
-//   route    (token, chunk of units): the router's products, a wave a unit; the choice in the same
-//            launch where one chunk holds all units, else in `choose`.
+//   route    (token, four units): the router's products, a wave a unit.
+//   choose   (token): the K units; where the tokens are few, in the first product instead.
 //   product  (column tile and split of the rows, slot): z = x W1[e] for the tokens that chose the
 //            slot's unit e, as fp32 sums of the split's rows.
 //   product  the same for v W2[e], where v is made from the first product's sums on the way.
-//   combine  (token, 256 columns): the weighted sum over the token's units, in a fixed order.
+//   combine  (token, 64 columns): the weighted sum over the token's units, in a fixed order.
 //
 // What bounds it is one read of the chosen units' weights, so the products stream them from HBM into
 // registers once, 16 bytes a lane, as they lie ([in, out]), and give them to the matrix cores with up
@@ -16,9 +16,11 @@
 // waves and, where units and column tiles are few, over workgroups, so that some 512 workgroups
 // keep the loads of two steps each in flight.
 //
-// x enters the first product exactly. v is fp32: with bf16 weights it goes to the matrix cores as the
-// sum of two bf16 (16 significant bits, 2^-17 of v at most is lost; one bf16 would lose 2^-9); fp16
-// weights are widened and multiply v in fp32, since fp16 has not the range of an unscaled v.
+// x enters the first product exactly. v is fp32: 16-bit weights multiply it on the 16-bit matrix cores as
+// the sum of two bf16 (16 significant bits, 2^-17 of v at most is lost; one bf16 would lose 2^-9), fp16
+// weights as two bf16 themselves (8 and 3 of their 11 bits, nothing lost), since fp16 has not the range of
+// an unscaled v and fp32 products of widened weights take four times the matrix cores' time. A
+// workgroup makes v for its rows in LDS, 512 rows at a time, with the first weights in flight.
 #include <algorithm>
 #include <type_traits>
 
@@ -33,9 +35,10 @@ namespace {
 
 constexpr int kMaxUnits = HSN_UNITS_MAX, kMaxChosen = HSN_UNITS_MAX_CHOSEN;
 constexpr int kMaxTokens = HSN_UNITS_MAX_TOKENS;
-constexpr int kRouteThreads = 1024, kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kRows = 32;    // rows of a step
 constexpr int kTokens = 16;  // tokens of a product
+constexpr int kStage = 512;  // rows of v in LDS
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -58,6 +61,7 @@ struct Args {
     float* share;  // [n, K]
     Product up, down;
     int n, M, K, d_in, H, d_out, activation;
+    bool choose_inline;  // the first product chooses
 };
 
 // 16 bytes from any element's address (one load; the GPU takes global addresses unaligned).
@@ -72,67 +76,90 @@ __device__ __forceinline__ v4u load16(const E* p) {
 // The router.
 // --------------------------------------------------------------------------------------------
 
-// The token's K units from its products in LDS: a unit's rank is the number of units before it
-// (larger, or equal and lower).
-__device__ void choose_from(const Args& a, int i, const float* logit, float* chosen) {
+// The units of up to kThreads / M tokens from their products, a thread a unit of a token: a unit's rank
+// is the number of units before it (larger, or equal and lower), and the first K are chosen. Every
+// thread of the workgroup calls it; `units` and `shares` (LDS) get [tokens, K].
+struct ChoiceLds {
+    uint32_t key[kThreads + 4];
+    float logit[kThreads];
+    int unit[kThreads];
+    float share[kThreads];
+};
+static_assert(kThreads >= kMaxUnits && kMaxChosen <= 16, "a token's units, a thread each");
+
+__device__ __forceinline__ void choose_units(ChoiceLds& lds, int M, int K, int tokens, float logit) {
+    const int tid = threadIdx.x, i = tid / M, m = tid % M;
+    const uint32_t key = score_key(logit);
+    if (i < tokens) lds.key[tid] = key;
     __syncthreads();
-    const int m = threadIdx.x;
-    if (m < a.M) {
-        const uint32_t key = score_key(logit[m]);
-        int rank = 0;
-        for (int j = 0; j < a.M; ++j) {
-            const uint32_t other = score_key(logit[j]);
-            rank += other > key || (other == key && j < m);
+    int rank = 0;
+    if (i < tokens) {
+        const uint32_t* others = lds.key + i * M;
+        int j = 0;
+        for (; j + 8 <= M; j += 8) {
+            uint32_t other[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) other[k] = others[j + k];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) rank += other[k] > key || (other[k] == key && j + k < m);
         }
-        if (rank < a.K) {
-            a.unit[i * a.K + rank] = m;
-            chosen[rank] = logit[m];
-        }
+        for (; j < M; ++j) rank += others[j] > key || (others[j] == key && j < m);
     }
+    const bool chosen = i < tokens && rank < K;
+    if (chosen) lds.unit[i * K + rank] = m, lds.logit[i * K + rank] = logit;
     __syncthreads();
-    if (m < a.K) {
+    const int first = tid / K * K;
+    if (tid < tokens * K) lds.share[tid] = expf(lds.logit[tid] - lds.logit[first]);
+    __syncthreads();
+    if (tid < tokens * K) {
         float sum = 0.0f;
-        for (int k = 0; k < a.K; ++k) sum += expf(chosen[k] - chosen[0]);
-        a.share[i * a.K + m] = expf(chosen[m] - chosen[0]) / sum;
+        for (int k = 0; k < K; ++k) sum += lds.share[first + k];
+        lds.logit[tid] = lds.share[tid] / sum;
     }
+    __syncthreads();
+    if (tid < tokens * K) lds.share[tid] = lds.logit[tid];
+}
+
+// A thread writes what it wrote to LDS.
+__device__ __forceinline__ void write_choice(const Args& a, const ChoiceLds& lds, int first_token,
+                                             int tokens) {
+    const int tid = threadIdx.x;
+    if (tid >= tokens * a.K) return;
+    a.unit[first_token * a.K + tid] = lds.unit[tid];
+    a.share[first_token * a.K + tid] = lds.share[tid];
 }
 
 template <typename E>
-__global__ __launch_bounds__(kRouteThreads) void route(Args a, int chunk) {
-    __shared__ float logit[kMaxUnits], chosen[kMaxChosen];
+__global__ __launch_bounds__(kThreads) void route(Args a) {
     constexpr int kVec = 16 / sizeof(E), kStep = kWave * kVec;
     const int i = blockIdx.x, lane = threadIdx.x % kWave;
-    const int first = blockIdx.y * chunk, last = min(a.M, first + chunk);
+    const int m = blockIdx.y * kWaves + threadIdx.x / kWave;
+    if (m >= a.M) return;
     const E* x = static_cast<const E*>(a.x) + i * a.x_row;
-    for (int m = first + int(threadIdx.x) / kWave; m < last; m += kRouteThreads / kWave) {
-        const E* w = static_cast<const E*>(a.router) + int64_t(m) * a.d_in;
-        float sum = 0.0f;
-        int k = lane * kVec;
+    const E* w = static_cast<const E*>(a.router) + int64_t(m) * a.d_in;
+    float sum = 0.0f;
+    int k = lane * kVec;
 #pragma unroll 4
-        for (; k + kVec <= a.d_in; k += kStep) {
-            const v4u xv = load16(x + k), wv = load16(w + k);
-            E xe[kVec], we[kVec];
-            __builtin_memcpy(xe, &xv, 16);
-            __builtin_memcpy(we, &wv, 16);
+    for (; k + kVec <= a.d_in; k += kStep) {
+        const v4u xv = load16(x + k), wv = load16(w + k);
+        E xe[kVec], we[kVec];
+        __builtin_memcpy(xe, &xv, 16);
+        __builtin_memcpy(we, &wv, 16);
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) sum = __builtin_fmaf(to_f32(xe[j]), to_f32(we[j]), sum);
-        }
-        for (; k < a.d_in; ++k)  // the last, incomplete pack is one lane's
-            sum = __builtin_fmaf(to_f32(x[k]), to_f32(w[k]), sum);
-        for (int d = 1; d < kWave; d *= 2) sum += wave_shfl_xor(sum, d);
-        if (lane == 0) {
-            logit[m] = sum;
-            if (gridDim.y > 1) a.logit[i * a.M + m] = sum;
-        }
+        for (int j = 0; j < kVec; ++j) sum = __builtin_fmaf(to_f32(xe[j]), to_f32(we[j]), sum);
     }
-    if (gridDim.y == 1) choose_from(a, i, logit, chosen);
+    for (; k < a.d_in; ++k)  // the last, incomplete pack is one lane's
+        sum = __builtin_fmaf(to_f32(x[k]), to_f32(w[k]), sum);
+    for (int d = 1; d < kWave; d *= 2) sum += wave_shfl_xor(sum, d);
+    if (lane == 0) a.logit[i * a.M + m] = sum;
 }
 
-__global__ __launch_bounds__(kMaxUnits) void choose(Args a) {
-    __shared__ float logit[kMaxUnits], chosen[kMaxChosen];
+__global__ __launch_bounds__(kThreads) void choose(Args a) {
+    __shared__ ChoiceLds lds;
     const int i = blockIdx.x;
-    if (int(threadIdx.x) < a.M) logit[threadIdx.x] = a.logit[i * a.M + threadIdx.x];
-    choose_from(a, i, logit, chosen);
+    choose_units(lds, a.M, a.K, 1,
+                 int(threadIdx.x) < a.M ? a.logit[i * a.M + threadIdx.x] : 0.0f);
+    write_choice(a, lds, i, 1);
 }
 
 // --------------------------------------------------------------------------------------------
@@ -203,15 +230,27 @@ __device__ __forceinline__ v4f mfma(v8bf a, v8bf b, v4f c) {
 __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ v4f mfma(float a, float b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// The upper and the lower halves of two words, as one word.
+__device__ __forceinline__ uint32_t upper(uint32_t lo, uint32_t hi) {
+    return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+}
+__device__ __forceinline__ uint32_t lower(uint32_t lo, uint32_t hi) {
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
 
 // Column m of the lane's eight rows as the eight-row operand of a 16-bit product.
 template <typename V8>
 __device__ __forceinline__ V8 column(const v4u (&row)[8], int m) {
     v4u r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        r[i] = __builtin_amdgcn_perm(row[2 * i + 1][m / 2], row[2 * i][m / 2],
-                                     m % 2 ? 0x07060302u : 0x05040100u);
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t even = row[2 * i][m / 2], odd = row[2 * i + 1][m / 2];
+        r[i] = m % 2 ? upper(even, odd) : lower(even, odd);
+    }
     return __builtin_bit_cast(V8, r);
 }
 
@@ -222,28 +261,85 @@ __device__ __forceinline__ float element(v4u row, int m) {
     return to_f32(e[m]);
 }
 
+// Column m of fp16 rows as two bf16 operands: the upper 8 bits of each and the rest.
+__device__ __forceinline__ void column_halves(const v4u (&row)[8], int m, v8bf& hi, v8bf& lo) {
+    v4u h, l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t whole[2], rest[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            whole[k] = __float_as_uint(element<_Float16>(row[2 * i + k], m));
+            const float top = __uint_as_float(whole[k] & 0xffff0000u);
+            const float w = __uint_as_float(whole[k]);
+            // an infinite weight is all in `hi`; a NaN stays one
+            rest[k] = __builtin_fabsf(w) < __builtin_inff() ? __float_as_uint(w - top) : 0u;
+        }
+        h[i] = upper(whole[0], whole[1]);
+        l[i] = upper(rest[0], rest[1]);
+    }
+    hi = __builtin_bit_cast(v8bf, h);
+    lo = __builtin_bit_cast(v8bf, l);
+}
+
+// v in LDS: fp32, or two bf16. The rows are padded by 16 bytes, so that 16 tokens' packs lie in
+// different banks.
+template <bool kHalves>
+struct Hidden {
+    float v[kTokens][kStage + 4];
+    __device__ __forceinline__ void put(int t, int k, const float (&x)[8]) {
+        __builtin_memcpy(&v[t][k], x, sizeof(x));
+    }
+};
+template <>
+struct Hidden<true> {
+    uint16_t hi[kTokens][kStage + 8], lo[kTokens][kStage + 8];
+    __device__ __forceinline__ void put(int t, int k, const float (&x)[8]) {
+        v8bf h, l;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            h[j] = static_cast<__bf16>(x[j]);
+            const float rest = x[j] - static_cast<float>(h[j]);
+            // an infinite v is all in hi
+            l[j] = static_cast<__bf16>(__builtin_fabsf(x[j]) < 3e38f ? rest : 0.0f);
+        }
+        __builtin_memcpy(&hi[t][k], &h, 16);
+        __builtin_memcpy(&lo[t][k], &l, 16);
+    }
+};
+
 template <typename E, bool kDown>
 __global__ __launch_bounds__(kThreads, 2) void product(Args a) {
     constexpr int kCols = 16 / sizeof(E);   // of a lane
     constexpr int kTileCols = 16 * kCols;
     constexpr bool kBf16 = __is_same(E, bf16_t), kF32 = __is_same(E, float);
-    __shared__ float red[kWaves][kTokens][kTileCols];
+    __shared__ union {
+        float red[kWaves][kTokens][kTileCols];
+        Hidden<!kF32> hidden;
+        ChoiceLds choice;
+    } lds;
     __shared__ uint32_t mask[kMaxUnits / 32];
     __shared__ int list[kMaxTokens], listed;
     const Product& p = kDown ? a.down : a.up;
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int pairs = a.n * a.K, slot = blockIdx.y;
+    const int* units = a.unit;
+    if constexpr (!kDown)
+        if (a.choose_inline) {  // every workgroup chooses, the first writes the choice down
+            choose_units(lds.choice, a.M, a.K, a.n, tid < a.n * a.M ? a.logit[tid] : 0.0f);
+            if (blockIdx.x == 0 && slot == 0) write_choice(a, lds.choice, 0, a.n);
+            units = lds.choice.unit;
+        }
     // the slot's unit, the slot-th of the chosen ones, and its pairs (at most one a token)
     int unit, count = 1;
     if (a.n == 1) {
-        unit = a.unit[slot];
+        unit = uniform(units[slot]);
         if (tid == 0) list[0] = slot;
         __syncthreads();
     } else {
         if (tid < kMaxUnits / 32) mask[tid] = 0;
         __syncthreads();
-        for (int i = tid; i < pairs; i += kThreads)
-            atomicOr(&mask[a.unit[i] / 32], 1u << a.unit[i] % 32);
+        for (int i = tid; i < pairs; i += kThreads) atomicOr(&mask[units[i] / 32], 1u << units[i] % 32);
         __syncthreads();
         unit = -1;
         for (int w = 0, seen = 0; w < kMaxUnits / 32; ++w) {
@@ -259,7 +355,7 @@ __global__ __launch_bounds__(kThreads, 2) void product(Args a) {
         if (wave == 0) {
             int n = 0;
             for (int base = 0; base < pairs; base += kWave) {
-                const bool hit = base + lane < pairs && a.unit[base + lane] == unit;
+                const bool hit = base + lane < pairs && units[base + lane] == unit;
                 const uint64_t hits = ballot(hit);
                 if (hit) list[n + lanes_below(hits)] = base + lane;
                 n += __popcll(hits);
@@ -304,83 +400,96 @@ __global__ __launch_bounds__(kThreads, 2) void product(Args a) {
     for (int t0 = 0; t0 < count; t0 += kTokens) {
         const int here = min(kTokens, count - t0);
         const int pair = list[t0 + min(col_lane, here - 1)];
+        int stage = begin;
         v4f acc[kCols];
 #pragma unroll
         for (int m = 0; m < kCols; ++m) acc[m] = v4f{};
         auto multiply = [&](int k0, const v4u (&row)[8]) {
-            const int k = k0 + 8 * group;
-            if constexpr (kDown) {
-                float v[8];
-                load_hidden<E>(a, pair, unit, k, end, v);
-                if constexpr (kBf16) {
-                    v8bf hi, lo;
+            const int k = k0 + 8 * group, t = min(col_lane, here - 1);
+            if constexpr (kF32) {
+                float left[8];
+                if constexpr (kDown)
+                    __builtin_memcpy(left, &lds.hidden.v[t][k - stage], sizeof(left));
+                else
+                    load_x<E>(a, pair, k, end, left);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        hi[j] = static_cast<__bf16>(v[j]);
-                        const float rest = v[j] - static_cast<float>(hi[j]);
-                        // an infinite v is all in hi
-                        lo[j] = static_cast<__bf16>(__builtin_fabsf(v[j]) < 3e38f ? rest : 0.0f);
-                    }
+                for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int m = 0; m < kCols; ++m) {
+                    for (int m = 0; m < kCols; ++m)
+                        acc[m] = mfma(left[j], element<E>(row[j], m), acc[m]);
+            } else if constexpr (kDown) {
+                v8bf hi, lo;
+                __builtin_memcpy(&hi, &lds.hidden.hi[t][k - stage], 16);
+                __builtin_memcpy(&lo, &lds.hidden.lo[t][k - stage], 16);
+#pragma unroll
+                for (int m = 0; m < kCols; ++m) {
+                    if constexpr (kBf16) {
                         const v8bf w = column<v8bf>(row, m);
                         acc[m] = mfma(lo, w, acc[m]);
                         acc[m] = mfma(hi, w, acc[m]);
+                    } else {
+                        v8bf w, rest;
+                        column_halves(row, m, w, rest);
+                        acc[m] = mfma(lo, rest, acc[m]);
+                        acc[m] = mfma(lo, w, acc[m]);
+                        acc[m] = mfma(hi, rest, acc[m]);
+                        acc[m] = mfma(hi, w, acc[m]);
                     }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-#pragma unroll
-                        for (int m = 0; m < kCols; ++m)
-                            acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                v[j], element<E>(row[j], m), acc[m], 0, 0, 0);
                 }
             } else {
+                using V8 = typename std::conditional<kBf16, v8bf, v8h>::type;
                 E x[8];
                 load_x<E>(a, pair, k, end, x);
-                if constexpr (kF32) {
+                const V8 left = __builtin_bit_cast(V8, x);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-#pragma unroll
-                        for (int m = 0; m < kCols; ++m)
-                            acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                x[j], element<E>(row[j], m), acc[m], 0, 0, 0);
-                } else {
-                    using V8 = typename std::conditional<kBf16, v8bf, v8h>::type;
-                    V8 left;
-                    __builtin_memcpy(&left, x, 16);
-#pragma unroll
-                    for (int m = 0; m < kCols; ++m) acc[m] = mfma(left, column<V8>(row, m), acc[m]);
-                }
+                for (int m = 0; m < kCols; ++m) acc[m] = mfma(left, column<V8>(row, m), acc[m]);
             }
         };
         // the next step's rows in flight
         v4u even[8], odd[8];
         constexpr int kStep = kWaves * kRows;
+        static_assert(kStage % (2 * kStep) == 0, "a stage begins with an even step");
         int k0 = begin + wave * kRows;
         if (k0 < end) load_rows(k0, even);
-        while (k0 < end) {
-            if (k0 + kStep < end) load_rows(k0 + kStep, odd);
-            multiply(k0, even);
-            k0 += kStep;
-            if (k0 >= end) break;
-            if (k0 + kStep < end) load_rows(k0 + kStep, even);
-            multiply(k0, odd);
-            k0 += kStep;
+        for (stage = begin; stage < end; stage += kDown ? kStage : end) {
+            const int stage_end = kDown ? min(end, stage + kStage) : end;
+            if constexpr (kDown) {
+                __syncthreads();
+                // to the end of the last step; 0 after the last row
+                const int filled = stage + (stage_end - stage + kRows - 1) / kRows * kRows;
+                for (int i = tid; i < here * (kStage / 8); i += kThreads) {
+                    const int t = i / (kStage / 8), k = stage + i % (kStage / 8) * 8;
+                    if (k >= filled) continue;
+                    float v[8];
+                    load_hidden<E>(a, list[t0 + t], unit, k, end, v);
+                    lds.hidden.put(t, k - stage, v);
+                }
+                __syncthreads();
+            }
+            while (k0 < stage_end) {
+                if (k0 + kStep < end) load_rows(k0 + kStep, odd);
+                multiply(k0, even);
+                k0 += kStep;
+                if (k0 >= stage_end) break;  // only at the rows' end
+                if (k0 + kStep < end) load_rows(k0 + kStep, even);
+                multiply(k0, odd);
+                k0 += kStep;
+            }
         }
+        __syncthreads();
         // the waves' sums, in their order; a lane has the tokens 4 group + i
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (4 * group + i < here)
 #pragma unroll
                 for (int m = 0; m < kCols; ++m)
-                    red[wave][4 * group + i][col_lane * kCols + m] = acc[m][i];
+                    lds.red[wave][4 * group + i][col_lane * kCols + m] = acc[m][i];
         __syncthreads();
         for (int i = tid; i < here * kTileCols; i += kThreads) {
             const int t = i / kTileCols, c = i % kTileCols;
             float sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) sum += red[w][t][c];
+            for (int w = 0; w < kWaves; ++w) sum += lds.red[w][t][c];
             const int col = first_col(c / kCols) + c % kCols;
             if (col < p.cols)
                 p.sums[(int64_t(split) * pairs + list[t0 + t]) * p.cols + col] = sum;
@@ -389,21 +498,33 @@ __global__ __launch_bounds__(kThreads, 2) void product(Args a) {
     }
 }
 
+// Wave w takes the token's units w, w + 4, ..: their sums over the splits, four loads in flight.
 template <typename E>
-__global__ __launch_bounds__(256) void combine(Args a) {
-    const int col = blockIdx.x * 256 + threadIdx.x, i = blockIdx.y;
-    if (col >= a.d_out) return;
+__global__ __launch_bounds__(kThreads) void combine(Args a) {
+    __shared__ float part[kWaves][kWave];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, i = blockIdx.y;
+    const int col = blockIdx.x * kWave + lane, from = min(col, a.d_out - 1);
     const int64_t stride = int64_t(a.n) * a.K * a.d_out;
     float y = 0.0f;
-    for (int k = 0; k < a.K; ++k) {
+    for (int k = wave; k < a.K; k += kWaves) {
         const int pair = i * a.K + k;
-        const float* at = a.down.sums + int64_t(pair) * a.d_out + col;
+        const float* at = a.down.sums + int64_t(pair) * a.d_out + from;
         float z = 0.0f;
-        for (int s = 0; s < a.down.splits; ++s) z += at[s * stride];
+        for (int s = 0; s < a.down.splits; s += 4) {
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = s + j < a.down.splits ? at[(s + j) * stride] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z += v[j];
+        }
         if (a.b2)
-            z += to_f32(static_cast<const E*>(a.b2)[int64_t(a.unit[pair]) * a.d_out + col]);
+            z += to_f32(static_cast<const E*>(a.b2)[int64_t(a.unit[pair]) * a.d_out + from]);
         y = __builtin_fmaf(a.share[pair], z, y);
     }
+    part[wave][lane] = y;
+    __syncthreads();
+    if (wave != 0 || col >= a.d_out) return;
+    for (int w = 1; w < kWaves; ++w) y += part[w][lane];
     static_cast<E*>(a.y)[int64_t(i) * a.d_out + col] = from_f32<E>(y);
 }
 
@@ -455,21 +576,16 @@ int64_t layout(Args& a, const void* W1, const void* W2, char* base, int size) {
 }
 
 template <typename E>
-void launch(const Args& a, hipStream_t st) {
-    // One workgroup reads the whole router for a token; above 256 KiB, and where the tokens are few,
-    // the units are chunked (and chosen in a launch of their own).
-    const int64_t router = int64_t(a.M) * a.d_in * sizeof(E);
-    int chunks = 1;
-    if (router > 256 * 1024 && a.n < 64)
-        chunks = static_cast<int>(std::min<int64_t>((a.M + 15) / 16, router / (128 * 1024)));
-    const int chunk = (a.M + chunks - 1) / chunks;
-    chunks = (a.M + chunk - 1) / chunk;
-    route<E><<<dim3(a.n, chunks), kRouteThreads, 0, st>>>(a, chunk);
-    if (chunks > 1) choose<<<a.n, kMaxUnits, 0, st>>>(a);
+void launch(Args a, hipStream_t st) {
+    // The choice is the first product's where all tokens' units are a thread each, which saves a
+    // launch (of 4 us), else a launch of its own.
+    a.choose_inline = a.n * a.M <= kThreads;
+    route<E><<<dim3(a.n, (a.M + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
+    if (!a.choose_inline) choose<<<a.n, kThreads, 0, st>>>(a);
     const int slots = std::min(a.n * a.K, a.M);
     product<E, false><<<dim3(a.up.tiles * a.up.splits, slots), kThreads, 0, st>>>(a);
     product<E, true><<<dim3(a.down.tiles * a.down.splits, slots), kThreads, 0, st>>>(a);
-    combine<E><<<dim3((a.d_out + 255) / 256, a.n), 256, 0, st>>>(a);
+    combine<E><<<dim3((a.d_out + kWave - 1) / kWave, a.n), kThreads, 0, st>>>(a);
 }
 
 }  // namespace

@@ -6,12 +6,12 @@
  *   z = x[i] W1[e] + b1[e],  v = gelu(z) (HSN_UNITS_GELU: z/2 (1 + erf(z / sqrt 2)), H1 = H) or
  *   silu(z[:H]) z[H:] (HSN_UNITS_SWIGLU, H1 = 2 H);
  *   y[i] = sum over e in S of p[e] (v W2[e] + b2[e]).
- * x [n, d_in] with rows x_row elements apart, router [M, d_in], W1 [M, d_in, H1], b1 [M, H1], W2 [M, H, d_out], b2 [M,
- * d_out] and y [n, d_out] in `dtype` (HSN_DTYPE_F32, _F16 or _BF16), dense and row-major but for
- * x; b1 and b2 may be NULL. The weights have the unit bank's layout ([in, out], hsn_ops.h).
- * Products are summed in fp32 and nothing is rounded to 16 bits before y, but for bf16 weights v
- * enters its product with 16 significant bits (the sum of two bf16). 1 <= K <= min(M, HSN_UNITS_MAX_CHOSEN),
- * M <= HSN_UNITS_MAX, n <= HSN_UNITS_MAX_TOKENS.
+ * x [n, d_in], router [M, d_in], W1 [M, d_in, H1], b1 [M, H1], W2 [M, H, d_out], b2 [M, d_out] and
+ * y [n, d_out] are in `dtype` (HSN_DTYPE_F32, _F16 or _BF16), dense and row-major but for x, whose
+ * rows are x_row elements apart; b1 and b2 may be NULL. The weights have the unit bank's layout
+ * ([in, out], hsn_ops.h). Products are summed in fp32 and nothing is rounded to 16 bits before y, but
+ * v enters its product with 16-bit weights with 16 significant bits (the sum of two bf16).
+ * 1 <= K <= min(M, HSN_UNITS_MAX_CHOSEN), M <= HSN_UNITS_MAX, n <= HSN_UNITS_MAX_TOKENS.
  *
  * workspace: hsn_units_layer_workspace() bytes of device memory, 16-byte aligned; its contents do
  * not matter before the call. Nothing is allocated and nothing is kept between calls, so the call
