@@ -3,14 +3,22 @@
 // A token's weight is a whole number, so masses can be added in any order: by atomics into
 // histogram bins, by lanes, by waves. The order of tokens is the order of score_key(logit), then
 // of the token. A row takes these passes over its logits:
-//   1. the largest logit and its first token (all that a greedy row needs);
-//   2. with top_k or top_p: counts and masses in 2048 bins, linear in x over the range where a
-//      weight is not 0 (x > -27.73). They say in which bin each filter cuts. Where the tokens down
-//      to that bin are at most 1024 they are gathered into LDS and sorted there, and the row ends
-//      without another pass; otherwise the cut is found on the keys' digits (11, 11 and 10 bits),
-//      a pass over the row for each;
-//   3. the kept weights' sums in the order of tokens, 64 packs of 16 bytes at a time, then one
-//      wave's walk through the 64 packs that hold the answer.
+//   1. the largest logit and its first token (all that a greedy row needs).
+//   2. with top_k up to 512: the k-th largest of the 1024 threads' own largest keys is no larger than
+//      the k-th largest key of the row, so every token that top_k keeps is among those from it on,
+//      some k (1 + k / 2048) of them where the large ones lie anywhere. They are gathered
+//      into LDS and sorted there, the other filters and the choice follow on the list, and no other
+//      token's exponential is ever taken.
+//      Else, with a top_k or a top_p: counts and masses in 2048 bins, linear in x over the range where
+//      a weight is not 0 (x > -27.73). They say in which bin the filter cuts. Where the tokens down to
+//      that bin are at most 1024 they are gathered and sorted as above (a third pass); otherwise the
+//      cut is found on the keys' digits (11, 11 and 10 bits), a pass over the row for each.
+//   3. without a list: the kept weights' sums in the order of tokens, 64 packs of 16 bytes at a time,
+//      then one wave's walk through the 64 packs that hold the answer.
+// What bounds a row is the instructions of one compute unit: the passes over keys are short, an exact
+// exponential and its fixed point take some 30 instructions.
+#include <type_traits>
+
 #include "../../include/hsn_sample.h"
 #include "abi_util.h"
 #include "common.cuh"
@@ -22,7 +30,6 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / kWave;
 constexpr int kBins = 2048, kList = 1024;
 constexpr float kBinScale = kBins / 27.75f;  // 2^-40 = exp(-27.726)
-constexpr float kOne = 1099511627776.0f;     // 2^40
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // score_key(-inf)
 constexpr int kChunks = 2 * kThreads;        // sums of 64 packs: 2^18 / (64 * 4) + 1 at most
 
@@ -39,6 +46,7 @@ struct Args {
 struct Shared {
     uint64_t mass[kBins];   // bins; then the sums of 64 packs
     uint32_t count[kBins];
+    uint32_t least[kBins];  // the smallest key of a bin
     uint64_t list[kList];
     uint64_t wave64[kWaves];
     uint32_t wave32[kWaves];
@@ -86,18 +94,40 @@ struct Row {
 };
 
 // The weight of a logit by its key: e, and w as the fixed point of e.
+//
+// x = d / t, d = l - best, is the correctly rounded quotient. With r the rounded 1 / t, d r is within 2
+// ulps of it; q + (d - q t) r brings that within 1 ulp, and once more to the correctly rounded quotient
+// (Markstein, IBM J. Res. Dev. 34, 1990: the last step of a division by iteration), as long as nothing
+// leaves the normal range: t within 2^+-60 (`quick`), and a d so small that it does gives e = 1 either
+// way. A d of -inf gives a NaN, and no weight.
 struct Weigh {
     uint32_t best_key;
-    float best, t;
+    float best, t, r;
+    bool quick;
+    __device__ Weigh(uint32_t key, float temperature) : best_key(key), best(key_value(key)), t(temperature) {
+        r = 1.0f / t;
+        quick = t > 0x1p-60f && t < 0x1p60f && best < __builtin_inff();
+    }
     __device__ __forceinline__ float x(uint32_t k) const {
-        return k == best_key ? 0.0f : (key_value(k) - best) / t;
+        if (k == best_key) return 0.0f;
+        const float d = key_value(k) - best;
+        if (!quick) return d / t;
+        const float near = d * r;
+        const float q = __builtin_fmaf(__builtin_fmaf(-near, t, d), r, near);
+        return __builtin_fmaf(__builtin_fmaf(-q, t, d), r, q);
+    }
+    static __device__ __forceinline__ float e_of(float x) {
+        return x > -30.0f ? expf(x) : 0.0f;  // 2^40 e is below 1 from x = -27.73 on; NaN: none
     }
     __device__ __forceinline__ float e(uint32_t k) const {
-        const float v = k == kKeyNegInf ? 0.0f : expf(x(k));
-        return v > 0.0f ? v : 0.0f;  // +inf over an infinite temperature is no share
+        return k == kKeyNegInf ? 0.0f : e_of(x(k));
     }
+    // floor(2^40 e) for 0 <= e <= 1: the 24 bits of e, shifted
     static __device__ __forceinline__ uint64_t fixed(float e) {
-        return static_cast<uint64_t>(e * kOne);
+        const uint32_t bits = __float_as_uint(e);
+        const uint64_t m = uint64_t((bits & 0x7fffffu) | 0x800000u) << 17;  // 2^40 at exponent 0
+        const int down = 127 - static_cast<int>(bits >> 23);
+        return down < 64 ? m >> down : 0;
     }
     __device__ __forceinline__ uint64_t w(uint32_t k) const { return fixed(e(k)); }
 };
@@ -133,7 +163,7 @@ __device__ uint32_t block_max(uint32_t v, Shared& s) {
 
 __device__ void clear_bins(Shared& s) {
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0, s.least[i] = ~0u;
     __syncthreads();
 }
 
@@ -303,18 +333,21 @@ __device__ int walk(const Row<E>& row, Shared& s, F&& f, L&& limit) {
 }
 
 // Sorts the first `n` (a power of two up to kList) threads' values, the largest first.
-__device__ uint64_t sort_down(uint64_t v, int n, Shared& s) {
+template <typename T>
+__device__ T sort_down(T v, int n, Shared& s) {
+    using Wide = typename std::conditional<sizeof(T) == 8, unsigned long long, unsigned int>::type;
+    T* list = reinterpret_cast<T*>(s.list);
     const int i = threadIdx.x;
     for (int k = 2; k <= n; k *= 2)
         for (int j = k / 2; j > 0; j /= 2) {
-            uint64_t o;
+            T o;
             if (j < kWave) {
-                o = __shfl_xor(static_cast<unsigned long long>(v), j, kWave);
+                o = __shfl_xor(static_cast<Wide>(v), j, kWave);
             } else {
                 __syncthreads();
-                s.list[i] = v;
+                list[i] = v;
                 __syncthreads();
-                o = s.list[i ^ j];
+                o = list[i ^ j];
             }
             const bool keep_max = ((i & k) == 0) == ((i & j) == 0);
             if (i < n) v = keep_max ? max(v, o) : min(v, o);
@@ -327,6 +360,59 @@ __device__ __forceinline__ uint64_t at_share(float u, uint64_t total) {
     const double r = floor(static_cast<double>(u) * static_cast<double>(total));
     const uint64_t i = r > 0 ? static_cast<uint64_t>(r) : 0;
     return i < total ? i : total - 1;
+}
+
+// The rest of a row on its list of `n` tokens (in LDS, any order): every token that top_k keeps and
+// every one larger than some token of the list. by_count: top_k cuts; else `total` is the row's
+// whole mass, which top_p is a share of.
+__device__ void finish_list(Shared& s, const Weigh& weigh, int n, bool by_count, int top_k,
+                            float top_p, float min_p, float u, uint64_t total, int64_t* token) {
+    const int tid = threadIdx.x;
+    int size = 1;
+    while (size < n) size *= 2;
+    uint64_t v = tid < n ? s.list[tid] : 0;
+    v = sort_down(v, size, s);
+    uint32_t key = static_cast<uint32_t>(v >> 32);
+    const float e = tid < n ? weigh.e(key) : 0.0f;
+    uint64_t w = tid < n && (!by_count || tid < top_k) ? Weigh::fixed(e) : 0;
+    uint64_t sum;
+    const uint64_t run = block_scan(w, s, sum);
+    const double target = static_cast<double>(top_p) * static_cast<double>(by_count ? sum : total);
+    bool kept = w && (top_p >= 1.0f || static_cast<double>(run - w) < target) && e >= min_p;
+    kept |= tid == 0;
+    // the kept tokens in their order: the least token is the largest complement
+    v = kept ? (v << 32 | v >> 32) : 0;
+    v = sort_down(v, size, s);
+    key = static_cast<uint32_t>(v);
+    w = v && tid < n ? weigh.w(key) : 0;
+    const uint64_t end = block_scan(w, s, sum);
+    const uint64_t r = at_share(u, sum);
+    if (w && end > r && end - w <= r) *token = int64_t(uint32_t(~(v >> 32)));
+}
+
+// Every token with a key from `least` on into the list; how many there are (the list holds kList).
+template <typename E>
+__device__ int gather(const Row<E>& row, Shared& s, uint32_t least) {
+    __syncthreads();
+    if (threadIdx.x == 0) s.n_list = 0;
+    __syncthreads();
+    for (int p = threadIdx.x; p < row.packs; p += kThreads) {
+        uint32_t key[Row<E>::kVec];
+        const int first = row.keys(p, key);
+        uint32_t top = key[0];
+#pragma unroll
+        for (int j = 1; j < Row<E>::kVec; ++j) top = max(top, key[j]);
+        if (top < least) continue;
+        for (int j = 0; j < Row<E>::kVec; ++j) {
+            if (key[j] < least) continue;
+            const uint32_t place = atomicAdd(&s.n_list, 1u);
+            if (place < kList) s.list[place] = uint64_t(key[j]) << 32 | uint32_t(~(first + j));
+        }
+    }
+    __syncthreads();
+    const int n = static_cast<int>(s.n_list);
+    __syncthreads();
+    return n;
 }
 
 template <typename E>
@@ -357,8 +443,17 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
         if (tid == 0) a.tokens[i] = best <= kKeyNegInf ? -1 : first;
         return;
     }
-    const Weigh weigh{best, key_value(best), t};
+    const Weigh weigh(best, t);
 
+    if (top_k > 0 && top_k <= kList / 2 && top_k < a.V) {
+        const uint32_t sorted = sort_down(mine, kThreads, s);
+        if (tid == top_k - 1) s.found = sorted;
+        __syncthreads();
+        const uint32_t least = max(s.found, kKeyNegInf + 1);
+        const int n = gather(row, s, least);
+        if (n <= kList)
+            return finish_list(s, weigh, n, true, top_k, top_p, min_p, u, 0, a.tokens + i);
+    }
     Cut cut_k{0, 0}, cut_p{0, 0};
     if ((top_k > 0 && top_k < a.V) || !(top_p >= 1.0f)) {
         clear_bins(s);
@@ -366,11 +461,14 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
             uint32_t key[kVec];
             row.keys(p, key);
             for (int j = 0; j < kVec; ++j) {
-                const uint64_t w = weigh.w(key[j]);
+                if (key[j] == kKeyNegInf) continue;
+                const float x = weigh.x(key[j]);
+                const uint64_t w = Weigh::fixed(Weigh::e_of(x));
                 if (!w) continue;
-                const int bin = min(kBins - 1, static_cast<int>(-weigh.x(key[j]) * kBinScale));
+                const int bin = min(kBins - 1, static_cast<int>(-x * kBinScale));
                 atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[bin]), (unsigned long long)w);
                 atomicAdd(&s.count[bin], 1u);
+                atomicMin(&s.least[bin], key[j]);
             }
         }
         __syncthreads();
@@ -385,54 +483,11 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
         if (!by_count) {
             block_scan(s.mass[2 * tid] + s.mass[2 * tid + 1], s, total);
             target = static_cast<double>(top_p) * static_cast<double>(total);
-            if (!(top_p >= 1.0f)) {
-                at = find_bin(s, false, 0, target > 0 ? target : 1.0, 0);
-            } else {
-                at = Place{};
-                at.found = false;
-                at.count_before = kList + 1;  // nothing cuts
-            }
+            if (!(top_p >= 1.0f)) at = find_bin(s, false, 0, target > 0 ? target : 1.0, 0);
         }
-        const uint32_t n = at.count_before + at.count;
-        const bool cuts = by_count || !(top_p >= 1.0f);
-        if (cuts && n <= kList) {
-            // every token down to the cut's bin, sorted in LDS
-            if (tid == 0) s.n_list = 0;
-            s.list[tid] = 0;
-            __syncthreads();
-            const int last = at.found ? at.bin : kBins - 1;
-            for (int p = tid; p < row.packs; p += kThreads) {
-                uint32_t key[kVec];
-                const int at0 = row.keys(p, key);
-                for (int j = 0; j < kVec; ++j) {
-                    if (key[j] == kKeyNegInf || !weigh.w(key[j])) continue;
-                    if (min(kBins - 1, static_cast<int>(-weigh.x(key[j]) * kBinScale)) > last) continue;
-                    const uint32_t place = atomicAdd(&s.n_list, 1u);
-                    if (place < kList) s.list[place] = uint64_t(key[j]) << 32 | uint32_t(~(at0 + j));
-                }
-            }
-            __syncthreads();
-            int size = 1;
-            while (size < static_cast<int>(n)) size *= 2;
-            uint64_t v = s.list[tid];
-            v = sort_down(v, size, s);
-            uint32_t key = static_cast<uint32_t>(v >> 32);
-            float e = tid < int(n) ? weigh.e(key) : 0.0f;
-            uint64_t w = tid < int(n) && (!by_count || tid < top_k) ? Weigh::fixed(e) : 0;
-            uint64_t sum;
-            const uint64_t run = block_scan(w, s, sum);
-            if (by_count) target = static_cast<double>(top_p) * static_cast<double>(sum);
-            bool kept = w && (top_p >= 1.0f || static_cast<double>(run - w) < target) && e >= min_p;
-            kept |= tid == 0;
-            // the kept tokens in their order: the least token is the largest complement
-            v = kept ? (v << 32 | v >> 32) : 0;
-            v = sort_down(v, size, s);
-            key = static_cast<uint32_t>(v);
-            w = v && tid < int(n) ? weigh.w(key) : 0;
-            const uint64_t end = block_scan(w, s, sum);
-            const uint64_t r = at_share(u, sum);
-            if (w && end > r && end - w <= r) a.tokens[i] = int64_t(uint32_t(~(v >> 32)));
-            return;
+        if ((by_count || !(top_p >= 1.0f)) && at.found && at.count_before + at.count <= kList) {
+            const int n = gather(row, s, s.least[at.bin]);
+            return finish_list(s, weigh, n, by_count, top_k, top_p, min_p, u, total, a.tokens + i);
         }
         if (by_count) cut_k = descend(row, weigh, s, true, top_k, 0.0, total);
         if (!(top_p >= 1.0f)) {
