@@ -28,10 +28,15 @@ namespace sample {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / kWave;
+// Packs a thread has in flight where it only compares keys; where it takes exponentials the other
+// waves' instructions hide a load.
+constexpr int kBatch = 4;
 constexpr int kBins = 2048, kList = 1024;
 constexpr float kBinScale = kBins / 27.75f;  // 2^-40 = exp(-27.726)
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // score_key(-inf)
 constexpr int kChunks = 2 * kThreads;        // sums of 64 packs: 2^18 / (64 * 4) + 1 at most
+
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 struct Args {
     const void* logits;
@@ -60,36 +65,68 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k ^ (static_cast<int32_t>(k) < 0 ? 0x80000000u : 0xffffffffu));
 }
 
-// A row's logits as packs of 16 bytes from the last 16-byte boundary at or before its start.
+// A row's logits as packs of 16 bytes from the last 16-byte boundary at or before its start. Packs
+// [whole, whole_end) lie inside the row.
 template <typename E>
 struct Row {
     static constexpr int kVec = 16 / sizeof(E);
     const E* at;  // of pack 0's first element
-    int skip, V, packs;
+    int skip, V, packs, whole, whole_end;
     __device__ Row(const E* row, int v) : V(v) {
         skip = static_cast<int>((reinterpret_cast<uintptr_t>(row) / sizeof(E)) % kVec);
         at = row - skip;
         packs = (V + skip + kVec - 1) / kVec;
+        whole = skip ? 1 : 0;
+        whole_end = (V + skip) / kVec;
     }
-    // The keys of pack p's logits (-inf outside the row; NaN counts as -inf), first token p0.
-    __device__ __forceinline__ int keys(int p, uint32_t (&k)[kVec]) const {
-        const int first = p * kVec - skip;
+    __device__ __forceinline__ int first(int p) const { return p * kVec - skip; }
+    // Packs p, p + stride, ..: N loads in flight. A pack that is not whole is read element by element
+    // afterwards; outside the row there is -inf.
+    template <int N>
+    __device__ __forceinline__ void load(int p, int stride, v4u (&pack)[N]) const {
+        if (whole < whole_end)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int q = min(max(p + n * stride, whole), whole_end - 1);
+                pack[n] = *reinterpret_cast<const v4u*>(at + int64_t(q) * kVec);
+            }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int q = p + n * stride;
+            if (q >= whole && q < whole_end) continue;
+            E e[kVec];
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                const int t = first(q) + j;
+                e[j] = t >= 0 && t < V ? at[int64_t(q) * kVec + j] : from_f32<E>(-__builtin_inff());
+            }
+            __builtin_memcpy(&pack[n], e, 16);
+        }
+    }
+    // The keys of a pack's logits; NaN counts as -inf.
+    static __device__ __forceinline__ void keys(const v4u& pack, uint32_t (&k)[kVec]) {
         E e[kVec];
-        if (first >= 0 && first + kVec <= V) {
-            __builtin_memcpy(e, __builtin_assume_aligned(at + int64_t(p) * kVec, 16), 16);
+        __builtin_memcpy(e, &pack, 16);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) k[i] = key(to_f32(e[i]));
-        } else {
+        for (int j = 0; j < kVec; ++j) {
+            const float l = to_f32(e[j]);
+            k[j] = l != l ? kKeyNegInf : score_key(l);
+        }
+    }
+    // f(first token, keys) for every pack, the workgroup's threads side by side, N loads in flight.
+    template <int N, typename F>
+    __device__ __forceinline__ void each(F&& f) const {
+        for (int p = threadIdx.x; p < packs; p += N * kThreads) {
+            v4u pack[N];
+            load(p, kThreads, pack);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                const bool in = first + i >= 0 && first + i < V;
-                k[i] = in ? key(to_f32(at[int64_t(p) * kVec + i])) : kKeyNegInf;
+            for (int n = 0; n < N; ++n) {
+                if (p + n * kThreads >= packs) break;
+                uint32_t key[kVec];
+                keys(pack[n], key);
+                f(first(p + n * kThreads), key);
             }
         }
-        return first;
-    }
-    static __device__ __forceinline__ uint32_t key(float l) {
-        return l != l ? kKeyNegInf : score_key(l);
     }
 };
 
@@ -133,7 +170,7 @@ struct Weigh {
 };
 
 // Inclusive sum over the workgroup in thread order; `total` the whole. Ends with a barrier passed.
-__device__ uint64_t block_scan(uint64_t v, Shared& s, uint64_t& total) {
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, Shared& s, uint64_t& total) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     for (int d = 1; d < kWave; d *= 2) {
         const uint64_t o = __shfl_up(static_cast<unsigned long long>(v), d, kWave);
@@ -151,7 +188,7 @@ __device__ uint64_t block_scan(uint64_t v, Shared& s, uint64_t& total) {
     return before + v;
 }
 
-__device__ uint32_t block_max(uint32_t v, Shared& s) {
+__device__ __forceinline__ uint32_t block_max(uint32_t v, Shared& s) {
     for (int d = 1; d < kWave; d *= 2) v = max(v, wave_shfl_xor(v, d));
     __syncthreads();
     if (threadIdx.x % kWave == 0) s.wave32[threadIdx.x / kWave] = v;
@@ -161,7 +198,7 @@ __device__ uint32_t block_max(uint32_t v, Shared& s) {
     return m;
 }
 
-__device__ void clear_bins(Shared& s) {
+__device__ __forceinline__ void clear_bins(Shared& s) {
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0, s.least[i] = ~0u;
     __syncthreads();
@@ -182,7 +219,7 @@ struct Place {
     uint64_t mass_before, mass;
 };
 
-__device__ Place find_bin(Shared& s, bool by_count, uint64_t k, double target, uint64_t base) {
+__device__ __forceinline__ Place find_bin(Shared& s, bool by_count, uint64_t k, double target, uint64_t base) {
     const int b = 2 * threadIdx.x;
     const uint64_t m0 = s.mass[b], m1 = s.mass[b + 1];
     const uint32_t c0 = s.count[b], c1 = s.count[b + 1];
@@ -216,7 +253,7 @@ __device__ Place find_bin(Shared& s, bool by_count, uint64_t k, double target, u
 
 // How many of `n` equal weights w a mass filter keeps, `base` of mass before them: the j-th is kept
 // where the mass before it is under the target.
-__device__ uint64_t equal_under(uint64_t base, uint64_t w, uint64_t n, double target) {
+__device__ __forceinline__ uint64_t equal_under(uint64_t base, uint64_t w, uint64_t n, double target) {
     const double guess = (target - static_cast<double>(base)) / static_cast<double>(w);
     uint64_t c = guess > 0 ? (guess < double(n) ? static_cast<uint64_t>(guess) : n) : 0;
     while (c < n && static_cast<double>(base + c * w) < target) ++c;
@@ -226,7 +263,7 @@ __device__ uint64_t equal_under(uint64_t base, uint64_t w, uint64_t n, double ta
 
 // The cut of one filter, found digit by digit; mass_at: the mass of what it keeps.
 template <typename E>
-__device__ Cut descend(const Row<E>& row, const Weigh& weigh, Shared& s, bool by_count, uint64_t k,
+__device__ __forceinline__ Cut descend(const Row<E>& row, const Weigh& weigh, Shared& s, bool by_count, uint64_t k,
                        double target, uint64_t& mass_at) {
     uint32_t prefix = 0;
     uint64_t base_mass = 0, base_count = 0;
@@ -234,9 +271,7 @@ __device__ Cut descend(const Row<E>& row, const Weigh& weigh, Shared& s, bool by
     for (int level = 1; level <= 3; ++level) {
         const int up = shifts[level - 1], shift = shifts[level], bits = up - shift;
         clear_bins(s);
-        for (int p = threadIdx.x; p < row.packs; p += kThreads) {
-            uint32_t key[Row<E>::kVec];
-            row.keys(p, key);
+        row.template each<1>([&](int, const uint32_t (&key)[Row<E>::kVec]) {
             for (int i = 0; i < Row<E>::kVec; ++i) {
                 if (level > 1 && key[i] >> up != prefix) continue;
                 const uint64_t w = weigh.w(key[i]);
@@ -246,12 +281,12 @@ __device__ Cut descend(const Row<E>& row, const Weigh& weigh, Shared& s, bool by
                 atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[bin]), (unsigned long long)w);
                 atomicAdd(&s.count[bin], 1u);
             }
-        }
+        });
         __syncthreads();
         const Place at = find_bin(s, by_count, by_count ? k - base_count : 0, target, base_mass);
         if (!at.found) {  // the filter keeps everything
             mass_at = base_mass + at.mass_before;
-            return {0, 0};
+            return Cut{0, 0};
         }
         base_mass += at.mass_before;
         base_count += at.count_before;
@@ -270,24 +305,24 @@ __device__ Cut descend(const Row<E>& row, const Weigh& weigh, Shared& s, bool by
 // The first token, in order, at which the running sum of f(key, token) exceeds `limit(total)`;
 // V where none does.
 template <typename E, typename F, typename L>
-__device__ int walk(const Row<E>& row, Shared& s, F&& f, L&& limit) {
+__device__ __forceinline__ int walk(const Row<E>& row, Shared& s, F&& f, L&& limit) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int chunks = (row.packs + kWave - 1) / kWave;
     __syncthreads();
     for (int i = threadIdx.x; i < kChunks; i += kThreads) s.mass[i] = 0;
     if (threadIdx.x == 0) s.found = kChunks;
     __syncthreads();
-    auto pack_sum = [&](int p) {
+    auto pack_sum = [&](int p, const v4u& pack) {
         uint64_t sum = 0;
-        if (p < row.packs) {
-            uint32_t key[Row<E>::kVec];
-            const int first = row.keys(p, key);
-            for (int i = 0; i < Row<E>::kVec; ++i) sum += f(key[i], first + i);
-        }
-        return sum;
+        uint32_t key[Row<E>::kVec];
+        Row<E>::keys(pack, key);
+        for (int i = 0; i < Row<E>::kVec; ++i) sum += f(key[i], row.first(p) + i);
+        return p < row.packs ? sum : 0;
     };
     for (int c = wave; c < chunks; c += kWaves) {
-        uint64_t sum = pack_sum(c * kWave + lane);
+        v4u pack[1];
+        row.load(c * kWave + lane, 0, pack);
+        uint64_t sum = pack_sum(c * kWave + lane, pack[0]);
         for (int d = 1; d < kWave; d *= 2)
             sum += __shfl_xor(static_cast<unsigned long long>(sum), d, kWave);
         if (lane == 0) s.mass[c] = sum;
@@ -309,7 +344,9 @@ __device__ int walk(const Row<E>& row, Shared& s, F&& f, L&& limit) {
     if (c >= kChunks) return row.V;
     if (wave == 0) {
         const int p = c * kWave + lane;
-        const uint64_t sum = pack_sum(p);
+        v4u pack[1];
+        row.load(p, 0, pack);
+        const uint64_t sum = pack_sum(p, pack[0]);
         uint64_t run = sum;
         for (int d = 1; d < kWave; d *= 2) {
             const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), d, kWave);
@@ -318,11 +355,11 @@ __device__ int walk(const Row<E>& row, Shared& s, F&& f, L&& limit) {
         run += s.found_mass - sum;  // before this pack
         if (run <= r && run + sum > r) {
             uint32_t key[Row<E>::kVec];
-            const int first = row.keys(p, key);
+            Row<E>::keys(pack[0], key);
             for (int i = 0; i < Row<E>::kVec; ++i) {
-                run += f(key[i], first + i);
+                run += f(key[i], row.first(p) + i);
                 if (run > r) {
-                    s.found_below = first + i;
+                    s.found_below = row.first(p) + i;
                     break;
                 }
             }
@@ -334,7 +371,7 @@ __device__ int walk(const Row<E>& row, Shared& s, F&& f, L&& limit) {
 
 // Sorts the first `n` (a power of two up to kList) threads' values, the largest first.
 template <typename T>
-__device__ T sort_down(T v, int n, Shared& s) {
+__device__ __forceinline__ T sort_down(T v, int n, Shared& s) {
     using Wide = typename std::conditional<sizeof(T) == 8, unsigned long long, unsigned int>::type;
     T* list = reinterpret_cast<T*>(s.list);
     const int i = threadIdx.x;
@@ -365,7 +402,7 @@ __device__ __forceinline__ uint64_t at_share(float u, uint64_t total) {
 // The rest of a row on its list of `n` tokens (in LDS, any order): every token that top_k keeps and
 // every one larger than some token of the list. by_count: top_k cuts; else `total` is the row's
 // whole mass, which top_p is a share of.
-__device__ void finish_list(Shared& s, const Weigh& weigh, int n, bool by_count, int top_k,
+__device__ __forceinline__ void finish_list(Shared& s, const Weigh& weigh, int n, bool by_count, int top_k,
                             float top_p, float min_p, float u, uint64_t total, int64_t* token) {
     const int tid = threadIdx.x;
     int size = 1;
@@ -392,27 +429,31 @@ __device__ void finish_list(Shared& s, const Weigh& weigh, int n, bool by_count,
 
 // Every token with a key from `least` on into the list; how many there are (the list holds kList).
 template <typename E>
-__device__ int gather(const Row<E>& row, Shared& s, uint32_t least) {
+__device__ __forceinline__ int gather(const Row<E>& row, Shared& s, uint32_t least) {
     __syncthreads();
     if (threadIdx.x == 0) s.n_list = 0;
     __syncthreads();
-    for (int p = threadIdx.x; p < row.packs; p += kThreads) {
-        uint32_t key[Row<E>::kVec];
-        const int first = row.keys(p, key);
+    row.template each<kBatch>([&](int first, const uint32_t (&key)[Row<E>::kVec]) {
         uint32_t top = key[0];
 #pragma unroll
         for (int j = 1; j < Row<E>::kVec; ++j) top = max(top, key[j]);
-        if (top < least) continue;
+        if (top < least) return;
         for (int j = 0; j < Row<E>::kVec; ++j) {
             if (key[j] < least) continue;
             const uint32_t place = atomicAdd(&s.n_list, 1u);
             if (place < kList) s.list[place] = uint64_t(key[j]) << 32 | uint32_t(~(first + j));
         }
-    }
+    });
     __syncthreads();
     const int n = static_cast<int>(s.n_list);
     __syncthreads();
     return n;
+}
+
+// The mass that top_p asks for; a positive one, so that the first token is under it.
+__device__ __forceinline__ double mass_target(float top_p, uint64_t total) {
+    const double target = static_cast<double>(top_p) * static_cast<double>(total);
+    return target > 0 ? target : 1.0;
 }
 
 template <typename E>
@@ -429,12 +470,11 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
 
     uint32_t best = 0;
     int first = a.V;
-    for (int p = tid; p < row.packs; p += kThreads) {
-        uint32_t key[kVec];
-        const int at = row.keys(p, key);
+    row.template each<kBatch>([&](int at, const uint32_t (&key)[kVec]) {
+#pragma unroll
         for (int j = 0; j < kVec; ++j)
             if (key[j] > best) best = key[j], first = at + j;
-    }
+    });
     const uint32_t mine = best;
     best = block_max(best, s);
     // the least first token: the largest of its complement
@@ -445,21 +485,22 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
     }
     const Weigh weigh(best, t);
 
-    if (top_k > 0 && top_k <= kList / 2 && top_k < a.V) {
+    const bool cuts_k = top_k > 0 && top_k < a.V, cuts_p = !(top_p >= 1.0f);
+    if (cuts_k && top_k <= kList / 2) {
         const uint32_t sorted = sort_down(mine, kThreads, s);
         if (tid == top_k - 1) s.found = sorted;
         __syncthreads();
-        const uint32_t least = max(s.found, kKeyNegInf + 1);
-        const int n = gather(row, s, least);
-        if (n <= kList)
-            return finish_list(s, weigh, n, true, top_k, top_p, min_p, u, 0, a.tokens + i);
+        const int n = gather(row, s, max(s.found, kKeyNegInf + 1));
+        if (n <= kList) {
+            finish_list(s, weigh, n, true, top_k, top_p, min_p, u, 0, a.tokens + i);
+            return;
+        }
     }
-    Cut cut_k{0, 0}, cut_p{0, 0};
-    if ((top_k > 0 && top_k < a.V) || !(top_p >= 1.0f)) {
+    Cut cut{0, 0};
+    if (cuts_k || cuts_p) {
         clear_bins(s);
-        for (int p = tid; p < row.packs; p += kThreads) {
-            uint32_t key[kVec];
-            row.keys(p, key);
+        row.template each<1>([&](int, const uint32_t (&key)[kVec]) {
+#pragma unroll
             for (int j = 0; j < kVec; ++j) {
                 if (key[j] == kKeyNegInf) continue;
                 const float x = weigh.x(key[j]);
@@ -470,47 +511,39 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
                 atomicAdd(&s.count[bin], 1u);
                 atomicMin(&s.least[bin], key[j]);
             }
-        }
+        });
         __syncthreads();
-        bool by_count = top_k > 0 && top_k < a.V;
-        Place at{};
-        if (by_count) {
-            at = find_bin(s, true, top_k, 0.0, 0);
-            by_count = at.found;  // else fewer tokens than top_k have a weight
-        }
-        uint64_t total = 0;
-        double target = 0.0;
-        if (!by_count) {
-            block_scan(s.mass[2 * tid] + s.mass[2 * tid + 1], s, total);
-            target = static_cast<double>(top_p) * static_cast<double>(total);
-            if (!(top_p >= 1.0f)) at = find_bin(s, false, 0, target > 0 ? target : 1.0, 0);
-        }
-        if ((by_count || !(top_p >= 1.0f)) && at.found && at.count_before + at.count <= kList) {
+        uint64_t total;
+        block_scan(s.mass[2 * tid] + s.mass[2 * tid + 1], s, total);
+        Place at = find_bin(s, cuts_k, top_k, 0.0, 0);
+        const bool by_count = cuts_k && at.found;  // else fewer tokens than top_k have a weight
+        if (!by_count && cuts_p) at = find_bin(s, false, 0, mass_target(top_p, total), 0);
+        if ((by_count || cuts_p) && at.found && at.count_before + at.count <= kList) {
             const int n = gather(row, s, s.least[at.bin]);
-            return finish_list(s, weigh, n, by_count, top_k, top_p, min_p, u, total, a.tokens + i);
+            finish_list(s, weigh, n, by_count, top_k, top_p, min_p, u, total, a.tokens + i);
+            return;
         }
-        if (by_count) cut_k = descend(row, weigh, s, true, top_k, 0.0, total);
-        if (!(top_p >= 1.0f)) {
+        // the earlier of the two filters' cuts
+        if (by_count) cut = descend(row, weigh, s, true, top_k, 0.0, total);
+        if (cuts_p) {
             uint64_t unused;
-            target = static_cast<double>(top_p) * static_cast<double>(total);
-            cut_p = descend(row, weigh, s, false, 0, target > 0 ? target : 1.0, unused);
+            const Cut c = descend(row, weigh, s, false, 0, mass_target(top_p, total), unused);
+            if (c.key > cut.key || (c.key == cut.key && c.equal < cut.equal)) cut = c;
         }
     }
-    // the earlier of the two cuts
-    Cut cut = cut_k;
-    if (cut_p.key > cut.key || (cut_p.key == cut.key && cut_p.equal < cut.equal)) cut = cut_p;
+    // the last token kept among those equal to the cut's key
     int last_equal = a.V;
     if (cut.key)
         last_equal = walk(row, s, [&](uint32_t k, int) { return uint64_t(k == cut.key); },
-                          [&](uint64_t) { return cut.equal ? cut.equal - 1 : 0; });
+                          [&](uint64_t) { return cut.equal - 1; });
     const int token = walk(
         row, s,
         [&](uint32_t k, int j) {
-            if (k < cut.key || (k == cut.key && (!cut.equal || j > last_equal))) return uint64_t(0);
+            if (k < cut.key || (k == cut.key && j > last_equal)) return uint64_t(0);
             const float e = weigh.e(k);
             return e >= min_p || j == first ? Weigh::fixed(e) : 0;
         },
-        [&](uint64_t total) { return at_share(u, total); });
+        [&](uint64_t whole) { return at_share(u, whole); });
     if (tid == 0) a.tokens[i] = token;
 }
 
