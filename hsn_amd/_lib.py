@@ -95,7 +95,8 @@ SIGNATURES: dict[str, list] = {
     "hsn_scan_step": [P, L, P, L, I, I, P, P, P, P, I, I, I, P],
     "hsn_units_layer_workspace": [I, I, I, I, I, I, I, I, P],
     "hsn_units_layer": [P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P, L, P],
-    "hsn_sample": [P, L, I, P, P, P, P, P, P, P, I, I, P],
+    "hsn_sample_workspace": [I, I, I, P],
+    "hsn_sample": [P, L, I, P, P, P, P, P, P, P, I, I, P, L, P],
 }
 
 _lock = threading.Lock()

@@ -1,4 +1,5 @@
-// The choice of a token from logits (include/hsn_sample.h): one workgroup a row.
+// The choice of a token from logits (include/hsn_sample.h): one workgroup a row, or, where rows are few
+// and long, a workgroup a slice of one for the passes over the logits and then one a row.
 //
 // A token's weight is a whole number, so masses can be added in any order: by atomics into
 // histogram bins, by lanes, by waves. The order of tokens is the order of score_key(logit), then
@@ -17,6 +18,7 @@
 //      then one wave's walk through the 64 packs that hold the answer.
 // What bounds a row is the instructions of one compute unit: the passes over keys are short, an exact
 // exponential and its fixed point take some 30 instructions.
+#include <algorithm>
 #include <type_traits>
 
 #include "../../include/hsn_sample.h"
@@ -32,6 +34,8 @@ constexpr int kThreads = 1024, kWaves = kThreads / kWave;
 // waves' instructions hide a load.
 constexpr int kBatch = 4;
 constexpr int kBins = 2048, kList = 1024;
+constexpr int kListTop = kList / 2;  // the largest top_k that a list is tried for
+constexpr int kMostSlices = 16;
 constexpr float kBinScale = kBins / 27.75f;  // 2^-40 = exp(-27.726)
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // score_key(-inf)
 constexpr int kChunks = 2 * kThreads;        // sums of 64 packs: 2^18 / (64 * 4) + 1 at most
@@ -46,6 +50,32 @@ struct Args {
     hsn_sample_settings settings;
     int64_t* tokens;
     int V;
+    // a row in slices of slice_packs packs (0: whole rows), with [n, slices] each, and lists of kList
+    int slices, slice_packs;
+    uint32_t* best;    // the slice's largest key
+    int* first;        // its first token
+    uint32_t* listed;  // how many tokens the slice's list has; above kList: no list
+    uint64_t* lists;
+    uint64_t* sums;    // [n, kChunks] sums of 64 packs' weights
+};
+
+// A row's settings; NaN and 0 temperatures are greedy.
+struct Settings {
+    float t, top_p, min_p, u;
+    int top_k;
+    bool cuts_k, cuts_p;
+    __device__ Settings(const Args& a, int i) {
+        t = a.temperature ? a.temperature[i] : a.settings.temperature;
+        top_k = a.top_k ? a.top_k[i] : a.settings.top_k;
+        top_p = a.top_p ? a.top_p[i] : a.settings.top_p;
+        min_p = a.min_p ? a.min_p[i] : a.settings.min_p;
+        u = a.u[i];
+        cuts_k = top_k > 0 && top_k < a.V;
+        cuts_p = !(top_p >= 1.0f);
+    }
+    __device__ bool greedy() const { return !(t > 0); }
+    // the list of the tokens from the k-th largest of the threads' maxima on is tried
+    __device__ bool lists() const { return cuts_k && top_k <= kListTop; }
 };
 
 struct Shared {
@@ -113,15 +143,15 @@ struct Row {
             k[j] = l != l ? kKeyNegInf : score_key(l);
         }
     }
-    // f(first token, keys) for every pack, the workgroup's threads side by side, N loads in flight.
+    // f(first token, keys) for packs [from, to), the workgroup's threads side by side, N loads in flight.
     template <int N, typename F>
-    __device__ __forceinline__ void each(F&& f) const {
-        for (int p = threadIdx.x; p < packs; p += N * kThreads) {
+    __device__ __forceinline__ void each(int from, int to, F&& f) const {
+        for (int p = from + int(threadIdx.x); p < to; p += N * kThreads) {
             v4u pack[N];
             load(p, kThreads, pack);
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                if (p + n * kThreads >= packs) break;
+                if (p + n * kThreads >= to) break;
                 uint32_t key[kVec];
                 keys(pack[n], key);
                 f(first(p + n * kThreads), key);
@@ -271,7 +301,7 @@ __device__ __forceinline__ Cut descend(const Row<E>& row, const Weigh& weigh, Sh
     for (int level = 1; level <= 3; ++level) {
         const int up = shifts[level - 1], shift = shifts[level], bits = up - shift;
         clear_bins(s);
-        row.template each<1>([&](int, const uint32_t (&key)[Row<E>::kVec]) {
+        row.template each<1>(0, row.packs, [&](int, const uint32_t (&key)[Row<E>::kVec]) {
             for (int i = 0; i < Row<E>::kVec; ++i) {
                 if (level > 1 && key[i] >> up != prefix) continue;
                 const uint64_t w = weigh.w(key[i]);
@@ -302,31 +332,41 @@ __device__ __forceinline__ Cut descend(const Row<E>& row, const Weigh& weigh, Sh
     return {0, 0};
 }
 
+template <typename E, typename F>
+__device__ __forceinline__ uint64_t pack_sum(const Row<E>& row, int p, const v4u& pack, F&& f) {
+    uint64_t sum = 0;
+    uint32_t key[Row<E>::kVec];
+    Row<E>::keys(pack, key);
+#pragma unroll
+    for (int i = 0; i < Row<E>::kVec; ++i) sum += f(key[i], row.first(p) + i);
+    return p < row.packs ? sum : 0;
+}
+
+// The sums of f(key, token) over 64 packs each, from pack `from` up to `to`, a wave a sum.
+template <typename E, typename F>
+__device__ __forceinline__ void chunk_sums(const Row<E>& row, int from, int to, uint64_t* sums, F&& f) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    for (int c = from / kWave + wave; c * kWave < to; c += kWaves) {
+        v4u pack[1];
+        row.load(c * kWave + lane, 0, pack);
+        uint64_t sum = pack_sum(row, c * kWave + lane, pack[0], f);
+        for (int d = 1; d < kWave; d *= 2)
+            sum += __shfl_xor(static_cast<unsigned long long>(sum), d, kWave);
+        if (lane == 0) sums[c] = sum;
+    }
+}
+
 // The first token, in order, at which the running sum of f(key, token) exceeds `limit(total)`;
-// V where none does.
+// V where none does. `sums`: the sums of 64 packs where they are made already, else NULL.
 template <typename E, typename F, typename L>
-__device__ __forceinline__ int walk(const Row<E>& row, Shared& s, F&& f, L&& limit) {
+__device__ __forceinline__ int walk(const Row<E>& row, Shared& s, const uint64_t* sums, F&& f, L&& limit) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int chunks = (row.packs + kWave - 1) / kWave;
     __syncthreads();
-    for (int i = threadIdx.x; i < kChunks; i += kThreads) s.mass[i] = 0;
+    for (int i = threadIdx.x; i < kChunks; i += kThreads) s.mass[i] = sums && i < chunks ? sums[i] : 0;
     if (threadIdx.x == 0) s.found = kChunks;
     __syncthreads();
-    auto pack_sum = [&](int p, const v4u& pack) {
-        uint64_t sum = 0;
-        uint32_t key[Row<E>::kVec];
-        Row<E>::keys(pack, key);
-        for (int i = 0; i < Row<E>::kVec; ++i) sum += f(key[i], row.first(p) + i);
-        return p < row.packs ? sum : 0;
-    };
-    for (int c = wave; c < chunks; c += kWaves) {
-        v4u pack[1];
-        row.load(c * kWave + lane, 0, pack);
-        uint64_t sum = pack_sum(c * kWave + lane, pack[0]);
-        for (int d = 1; d < kWave; d *= 2)
-            sum += __shfl_xor(static_cast<unsigned long long>(sum), d, kWave);
-        if (lane == 0) s.mass[c] = sum;
-    }
+    if (!sums) chunk_sums(row, 0, row.packs, s.mass, f);
     __syncthreads();
     const uint64_t s0 = s.mass[2 * threadIdx.x], s1 = s.mass[2 * threadIdx.x + 1];
     uint64_t total;
@@ -346,7 +386,7 @@ __device__ __forceinline__ int walk(const Row<E>& row, Shared& s, F&& f, L&& lim
         const int p = c * kWave + lane;
         v4u pack[1];
         row.load(p, 0, pack);
-        const uint64_t sum = pack_sum(p, pack[0]);
+        const uint64_t sum = pack_sum(row, p, pack[0], f);
         uint64_t run = sum;
         for (int d = 1; d < kWave; d *= 2) {
             const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), d, kWave);
@@ -427,13 +467,14 @@ __device__ __forceinline__ void finish_list(Shared& s, const Weigh& weigh, int n
     if (w && end > r && end - w <= r) *token = int64_t(uint32_t(~(v >> 32)));
 }
 
-// Every token with a key from `least` on into the list; how many there are (the list holds kList).
+// Every token of packs [from, to) with a key from `least` on into the list; how many there are (the list
+// holds kList).
 template <typename E>
-__device__ __forceinline__ int gather(const Row<E>& row, Shared& s, uint32_t least) {
+__device__ __forceinline__ int gather(const Row<E>& row, int from, int to, Shared& s, uint32_t least) {
     __syncthreads();
     if (threadIdx.x == 0) s.n_list = 0;
     __syncthreads();
-    row.template each<kBatch>([&](int first, const uint32_t (&key)[Row<E>::kVec]) {
+    row.template each<kBatch>(from, to, [&](int first, const uint32_t (&key)[Row<E>::kVec]) {
         uint32_t top = key[0];
 #pragma unroll
         for (int j = 1; j < Row<E>::kVec; ++j) top = max(top, key[j]);
@@ -456,41 +497,140 @@ __device__ __forceinline__ double mass_target(float top_p, uint64_t total) {
     return target > 0 ? target : 1.0;
 }
 
+// A token's weight where no filter but min_p cuts; the row's first token always has one.
+struct Plain {
+    Weigh weigh;
+    float min_p;
+    int first;
+    __device__ __forceinline__ uint64_t operator()(uint32_t k, int token) const {
+        const float e = weigh.e(k);
+        return e >= min_p || token == first ? Weigh::fixed(e) : 0;
+    }
+};
+
+// The largest key of packs [from, to) and its first token; `mine`: the thread's largest.
 template <typename E>
+__device__ __forceinline__ void find_best(const Row<E>& row, int from, int to, Shared& s, uint32_t& mine,
+                                          uint32_t& best, int& first) {
+    mine = 0, first = row.V;
+    row.template each<kBatch>(from, to, [&](int at, const uint32_t (&key)[Row<E>::kVec]) {
+#pragma unroll
+        for (int j = 0; j < Row<E>::kVec; ++j)
+            if (key[j] > mine) mine = key[j], first = at + j;
+    });
+    best = block_max(mine, s);
+    // the least first token: the largest of its complement
+    first = ~block_max(mine == best ? ~static_cast<uint32_t>(first) : 0, s);
+}
+
+// The k-th largest of the threads' keys, or the least key above -inf.
+__device__ __forceinline__ uint32_t list_from(uint32_t mine, int k, Shared& s) {
+    const uint32_t sorted = sort_down(mine, kThreads, s);
+    if (int(threadIdx.x) == k - 1) s.found = sorted;
+    __syncthreads();
+    return max(s.found, kKeyNegInf + 1);
+}
+
+// One slice of a row: its largest key, and its list where top_k is tried by lists.
+template <typename E>
+__global__ __launch_bounds__(kThreads) void sample_slices(Args a) {
+    __shared__ Shared s;
+    const int i = blockIdx.y, at = i * a.slices + blockIdx.x, tid = threadIdx.x;
+    const Row<E> row(static_cast<const E*>(a.logits) + i * a.row, a.V);
+    const Settings set(a, i);
+    const int from = blockIdx.x * a.slice_packs, to = min(row.packs, from + a.slice_packs);
+    uint32_t mine, best;
+    int first;
+    find_best(row, from, to, s, mine, best, first);
+    if (tid == 0) a.best[at] = best, a.first[at] = first;
+    if (set.greedy() || !set.lists()) return;
+    const int n = best > kKeyNegInf ? gather(row, from, to, s, list_from(mine, set.top_k, s)) : 0;
+    if (tid == 0) a.listed[at] = n;
+    if (tid < n) a.lists[int64_t(at) * kList + tid] = s.list[tid];
+}
+
+// The largest key and its first token from the slices'.
+__device__ __forceinline__ void best_of_slices(const Args& a, int i, uint32_t& best, int& first) {
+    best = 0, first = a.V;
+    for (int k = 0; k < a.slices; ++k) best = max(best, a.best[i * a.slices + k]);
+    for (int k = 0; k < a.slices; ++k)
+        if (a.best[i * a.slices + k] == best) first = min(first, a.first[i * a.slices + k]);
+}
+
+// One slice's sums of 64 packs' weights, for rows that neither top_k nor top_p cuts.
+template <typename E>
+__global__ __launch_bounds__(kThreads) void sample_sums(Args a) {
+    const int i = blockIdx.y;
+    const Settings set(a, i);
+    if (set.greedy() || set.cuts_k || set.cuts_p) return;
+    const Row<E> row(static_cast<const E*>(a.logits) + i * a.row, a.V);
+    uint32_t best;
+    int first;
+    best_of_slices(a, i, best, first);
+    if (best <= kKeyNegInf) return;
+    const int from = blockIdx.x * a.slice_packs, to = min(row.packs, from + a.slice_packs);
+    chunk_sums(row, from, to, a.sums + int64_t(i) * kChunks, Plain{Weigh(best, set.t), set.min_p, first});
+}
+
+// The slices' lists as one: the tokens from the k-th largest of the threads' maxima over them on;
+// how many, or more than kList where there is no such list.
+__device__ __forceinline__ int merge_lists(const Args& a, int i, int k, Shared& s) {
+    const int tid = threadIdx.x;
+    uint64_t v[kMostSlices];
+    uint32_t mine = 0;
+    bool whole = true;
+#pragma unroll
+    for (int j = 0; j < kMostSlices; ++j) {
+        const int at = i * a.slices + min(j, a.slices - 1);
+        const uint32_t n = j < a.slices ? a.listed[at] : 0;
+        whole &= n <= kList;
+        v[j] = tid < int(n) && n <= kList ? a.lists[int64_t(at) * kList + tid] : 0;
+    }
+    if (!whole) return kList + 1;
+#pragma unroll
+    for (int j = 0; j < kMostSlices; ++j) mine = max(mine, static_cast<uint32_t>(v[j] >> 32));
+    const uint32_t least = list_from(mine, k, s);
+    if (tid == 0) s.n_list = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kMostSlices; ++j)
+        if (static_cast<uint32_t>(v[j] >> 32) >= least) {
+            const uint32_t place = atomicAdd(&s.n_list, 1u);
+            if (place < kList) s.list[place] = v[j];
+        }
+    __syncthreads();
+    return static_cast<int>(s.n_list);
+}
+
+// A row: from its logits, or (kSlices) from what its slices have left.
+template <typename E, bool kSlices>
 __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
     __shared__ Shared s;
     const int i = blockIdx.x, tid = threadIdx.x;
     const Row<E> row(static_cast<const E*>(a.logits) + i * a.row, a.V);
     constexpr int kVec = Row<E>::kVec;
-    const float t = a.temperature ? a.temperature[i] : a.settings.temperature;
-    const int top_k = a.top_k ? a.top_k[i] : a.settings.top_k;
-    const float top_p = a.top_p ? a.top_p[i] : a.settings.top_p;
-    const float min_p = a.min_p ? a.min_p[i] : a.settings.min_p;
-    const float u = a.u[i];
+    const Settings set(a, i);
+    const int top_k = set.top_k;
+    const float top_p = set.top_p, min_p = set.min_p, u = set.u;
+    const bool cuts_k = set.cuts_k, cuts_p = set.cuts_p;
 
-    uint32_t best = 0;
-    int first = a.V;
-    row.template each<kBatch>([&](int at, const uint32_t (&key)[kVec]) {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j)
-            if (key[j] > best) best = key[j], first = at + j;
-    });
-    const uint32_t mine = best;
-    best = block_max(best, s);
-    // the least first token: the largest of its complement
-    first = ~block_max(mine == best ? ~static_cast<uint32_t>(first) : 0, s);
-    if (best <= kKeyNegInf || !(t > 0)) {
+    uint32_t mine = 0, best;
+    int first;
+    if constexpr (kSlices)
+        best_of_slices(a, i, best, first);
+    else
+        find_best(row, 0, row.packs, s, mine, best, first);
+    if (best <= kKeyNegInf || set.greedy()) {
         if (tid == 0) a.tokens[i] = best <= kKeyNegInf ? -1 : first;
         return;
     }
-    const Weigh weigh(best, t);
-
-    const bool cuts_k = top_k > 0 && top_k < a.V, cuts_p = !(top_p >= 1.0f);
-    if (cuts_k && top_k <= kList / 2) {
-        const uint32_t sorted = sort_down(mine, kThreads, s);
-        if (tid == top_k - 1) s.found = sorted;
-        __syncthreads();
-        const int n = gather(row, s, max(s.found, kKeyNegInf + 1));
+    const Weigh weigh(best, set.t);
+    if (set.lists()) {
+        int n;
+        if constexpr (kSlices)
+            n = merge_lists(a, i, top_k, s);
+        else
+            n = gather(row, 0, row.packs, s, list_from(mine, top_k, s));
         if (n <= kList) {
             finish_list(s, weigh, n, true, top_k, top_p, min_p, u, 0, a.tokens + i);
             return;
@@ -499,7 +639,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
     Cut cut{0, 0};
     if (cuts_k || cuts_p) {
         clear_bins(s);
-        row.template each<1>([&](int, const uint32_t (&key)[kVec]) {
+        row.template each<1>(0, row.packs, [&](int, const uint32_t (&key)[kVec]) {
 #pragma unroll
             for (int j = 0; j < kVec; ++j) {
                 if (key[j] == kKeyNegInf) continue;
@@ -519,7 +659,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
         const bool by_count = cuts_k && at.found;  // else fewer tokens than top_k have a weight
         if (!by_count && cuts_p) at = find_bin(s, false, 0, mass_target(top_p, total), 0);
         if ((by_count || cuts_p) && at.found && at.count_before + at.count <= kList) {
-            const int n = gather(row, s, s.least[at.bin]);
+            const int n = gather(row, 0, row.packs, s, s.least[at.bin]);
             finish_list(s, weigh, n, by_count, top_k, top_p, min_p, u, total, a.tokens + i);
             return;
         }
@@ -534,14 +674,13 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
     // the last token kept among those equal to the cut's key
     int last_equal = a.V;
     if (cut.key)
-        last_equal = walk(row, s, [&](uint32_t k, int) { return uint64_t(k == cut.key); },
+        last_equal = walk(row, s, nullptr, [&](uint32_t k, int) { return uint64_t(k == cut.key); },
                           [&](uint64_t) { return cut.equal - 1; });
+    const Plain plain{weigh, min_p, first};
     const int token = walk(
-        row, s,
+        row, s, kSlices && !cuts_k && !cuts_p ? a.sums + int64_t(i) * kChunks : nullptr,
         [&](uint32_t k, int j) {
-            if (k < cut.key || (k == cut.key && j > last_equal)) return uint64_t(0);
-            const float e = weigh.e(k);
-            return e >= min_p || j == first ? Weigh::fixed(e) : 0;
+            return k < cut.key || (k == cut.key && j > last_equal) ? uint64_t(0) : plain(k, j);
         },
         [&](uint64_t whole) { return at_share(u, whole); });
     if (tid == 0) a.tokens[i] = token;
@@ -551,30 +690,101 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
 }  // namespace sample
 }  // namespace hsn
 
-using namespace hsn;
+namespace hsn {
+namespace sample {
+namespace {
 
-extern "C" int hsn_sample(const void* logits, int64_t row, int dtype, const float* u,
-                          const float* temperature, const int32_t* top_k, const float* top_p,
-                          const float* min_p, const hsn_sample_settings* settings, int64_t* tokens,
-                          int n, int V, void* stream) {
-    HSN_ABI_BEGIN
+// Rows in slices: some 512 workgroups, each with at least a pack a thread. Whole rows (0) where they
+// fill the GPU or are short.
+int slices_of(int n, int V, int size) {
+    const int packs = (V + 16 / size - 1) / (16 / size) + 1;
+    const int slices = std::min(kMostSlices, std::min(packs / kThreads, 512 / std::max(n, 1)));
+    return slices > 1 ? slices : 0;
+}
+
+int64_t layout(Args& a, char* base, int n, int size) {
+    a.slices = slices_of(n, a.V, size);
+    if (!a.slices) return 0;
+    const int packs = (a.V + 16 / size - 1) / (16 / size) + 1;  // of a row at any address
+    a.slice_packs = ((packs + a.slices - 1) / a.slices + kWave - 1) / kWave * kWave;
+    const int64_t parts = int64_t(n) * a.slices;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        char* p = base + at;
+        at += (bytes + 255) / 256 * 256;
+        return p;
+    };
+    a.lists = reinterpret_cast<uint64_t*>(take(8 * parts * kList));
+    a.sums = reinterpret_cast<uint64_t*>(take(8 * int64_t(n) * kChunks));
+    a.best = reinterpret_cast<uint32_t*>(take(4 * parts));
+    a.first = reinterpret_cast<int*>(take(4 * parts));
+    a.listed = reinterpret_cast<uint32_t*>(take(4 * parts));
+    return at;
+}
+
+template <typename E>
+void launch(const Args& a, int n, hipStream_t st) {
+    if (!a.slices) {
+        sample_rows<E, false><<<n, kThreads, 0, st>>>(a);
+        return;
+    }
+    sample_slices<E><<<dim3(a.slices, n), kThreads, 0, st>>>(a);
+    // where the settings are the same for all rows, whether any row needs the sums is known here
+    const hsn_sample_settings& f = a.settings;
+    const bool cut = (!a.top_k && f.top_k > 0 && f.top_k < a.V) || (!a.top_p && !(f.top_p >= 1.0f));
+    if (!cut) sample_sums<E><<<dim3(a.slices, n), kThreads, 0, st>>>(a);
+    sample_rows<E, true><<<n, kThreads, 0, st>>>(a);
+}
+
+void check(int n, int V, int dtype) {
     HSN_REQUIRE(dtype == HSN_DTYPE_F32 || dtype == HSN_DTYPE_F16 || dtype == HSN_DTYPE_BF16,
                 HSN_ERR_UNSUPPORTED_DTYPE, "logits must be F32, F16 or BF16");
     HSN_REQUIRE(n >= 0 && V >= 1, HSN_ERR_INVALID_ARGUMENT, "n >= 0 and V >= 1");
     HSN_REQUIRE(V <= HSN_SAMPLE_MAX_TOKENS, HSN_ERR_SIZE_OVERFLOW, "at most 2^18 tokens");
+}
+
+}  // namespace
+}  // namespace sample
+}  // namespace hsn
+
+using namespace hsn;
+using namespace hsn::sample;
+
+extern "C" int hsn_sample_workspace(int n, int V, int dtype, int64_t* bytes) {
+    HSN_ABI_BEGIN
+    check(n, V, dtype);
+    HSN_REQUIRE(bytes, HSN_ERR_INVALID_ARGUMENT, "bytes must not be NULL");
+    Args a{};
+    a.V = V;
+    *bytes = layout(a, nullptr, n, dtype == HSN_DTYPE_F32 ? 4 : 2);
+    HSN_ABI_END
+}
+
+extern "C" int hsn_sample(const void* logits, int64_t row, int dtype, const float* u,
+                          const float* temperature, const int32_t* top_k, const float* top_p,
+                          const float* min_p, const hsn_sample_settings* settings, int64_t* tokens,
+                          int n, int V, void* workspace, int64_t workspace_bytes, void* stream) {
+    HSN_ABI_BEGIN
+    check(n, V, dtype);
     if (n == 0) return HSN_OK;
     HSN_REQUIRE(logits && u && tokens, HSN_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
     HSN_REQUIRE(settings || (temperature && top_k && top_p && min_p), HSN_ERR_INVALID_ARGUMENT,
                 "a setting without an array needs settings");
-    sample::Args a{logits, row, u, temperature, top_p, min_p, top_k, {}, tokens, V};
+    Args a{};
+    a.logits = logits, a.row = row, a.u = u, a.temperature = temperature, a.top_p = top_p;
+    a.min_p = min_p, a.top_k = top_k, a.tokens = tokens, a.V = V;
     if (settings) a.settings = *settings;
-    hipStream_t st = as_stream(stream);
+    const int64_t bytes = layout(a, static_cast<char*>(workspace), n, dtype == HSN_DTYPE_F32 ? 4 : 2);
+    HSN_REQUIRE(!bytes || (workspace && workspace_bytes >= bytes), HSN_ERR_INVALID_ARGUMENT,
+                "the workspace is too small");
+    HSN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, HSN_ERR_INVALID_ARGUMENT,
+                "the workspace must be aligned to 16 bytes");
     if (dtype == HSN_DTYPE_F32)
-        sample::sample_rows<float><<<n, sample::kThreads, 0, st>>>(a);
+        launch<float>(a, n, as_stream(stream));
     else if (dtype == HSN_DTYPE_F16)
-        sample::sample_rows<_Float16><<<n, sample::kThreads, 0, st>>>(a);
+        launch<_Float16>(a, n, as_stream(stream));
     else
-        sample::sample_rows<bf16_t><<<n, sample::kThreads, 0, st>>>(a);
+        launch<bf16_t>(a, n, as_stream(stream));
     HSN_HIP(hipGetLastError());
     HSN_ABI_END
 }

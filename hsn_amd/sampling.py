@@ -81,8 +81,14 @@ def sample(logits: Tensor, u: Tensor, *, temperature: Union[float, Tensor] = 1.0
         raise ValueError(f"top_k must be in [0, 2^31), got {k}")
     settings = _Settings(t, k, p, m)
     tokens = torch.empty(n, dtype=torch.int64, device=logits.device)
-    call("hsn_sample", ptr(logits), logits.stride(0), _DTYPE[logits.dtype], ptr(u), t_at, k_at,
-         p_at, m_at, ctypes.byref(settings), ptr(tokens), n, V, stream_of(logits.device))
+    code = _DTYPE[logits.dtype]
+    size = ctypes.c_int64(0)
+    call("hsn_sample_workspace", n, V, code, ctypes.byref(size))
+    ws = None
+    if size.value:
+        ws = torch.empty(size.value, dtype=torch.uint8, device=logits.device)
+    call("hsn_sample", ptr(logits), logits.stride(0), code, ptr(u), t_at, k_at, p_at, m_at,
+         ctypes.byref(settings), ptr(tokens), n, V, ptr(ws), size.value, stream_of(logits.device))
     return tokens
 
 

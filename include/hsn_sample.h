@@ -39,10 +39,14 @@ typedef struct hsn_sample_settings {
     float min_p;
 } hsn_sample_settings;
 
+/* Bytes of device workspace hsn_sample needs, 16-byte aligned; 0 where it needs none. Its contents do
+ * not matter before the call. */
+int hsn_sample_workspace(int n, int V, int dtype, int64_t* bytes);
+
 int hsn_sample(const void* logits, int64_t row, int dtype, const float* u,
                const float* temperature, const int32_t* top_k, const float* top_p,
                const float* min_p, const hsn_sample_settings* settings, int64_t* tokens, int n,
-               int V, void* stream);
+               int V, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
