@@ -7,7 +7,8 @@
 //   1. the largest logit and its first token (all that a greedy row needs).
 //   2. with top_k up to 512: the k-th largest of the 1024 threads' own largest keys is no larger than
 //      the k-th largest key of the row, so every token that top_k keeps is among those from it on,
-//      some k (1 + k / 2048) of them where the large ones lie anywhere. They are gathered
+//      some k (1 + k / 2048) of them where the large ones lie anywhere. They (or those from a little
+//      below it on, found by one histogram of the 1024 keys) are gathered
 //      into LDS and sorted there, the other filters and the choice follow on the list, and no other
 //      token's exponential is ever taken.
 //      Else, with a top_k or a top_p: counts and masses in 2048 bins, linear in x over the range where
@@ -24,6 +25,7 @@
 #include "../../include/hsn_sample.h"
 #include "abi_util.h"
 #include "common.cuh"
+#include "dpp.cuh"
 
 namespace hsn {
 namespace sample {
@@ -85,8 +87,7 @@ struct Shared {
     uint64_t list[kList];
     uint64_t wave64[kWaves];
     uint32_t wave32[kWaves];
-    uint64_t total64;
-    uint32_t total32, n_list, found, found_below;
+    uint32_t n_list, found, found_below;
     uint64_t found_mass;
 };
 static_assert(kBins == 2 * kThreads && kChunks <= kBins, "two bins a thread");
@@ -409,26 +410,59 @@ __device__ __forceinline__ int walk(const Row<E>& row, Shared& s, const uint64_t
     return static_cast<int>(s.found_below);
 }
 
-// Sorts the first `n` (a power of two up to kList) threads' values, the largest first.
-template <typename T>
-__device__ __forceinline__ T sort_down(T v, int n, Shared& s) {
-    using Wide = typename std::conditional<sizeof(T) == 8, unsigned long long, unsigned int>::type;
-    T* list = reinterpret_cast<T*>(s.list);
+// The value of lane ^ J, without LDS: within 16 lanes by DPP, across rows by the permlane swaps.
+template <int J>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    if constexpr (J == 1) return dpp_u32<dpp::kXor1>(v);
+    if constexpr (J == 2) return dpp_u32<dpp::kXor2>(v);
+    if constexpr (J == 4) return dpp_u32<0x1B>(dpp_u32<dpp::kHalfMirror>(v));  // ^7, then ^3
+    if constexpr (J == 8) return dpp_u32<dpp::kRor8>(v);
+    if constexpr (J == 16) {
+        const RowPair r = pair16(v);
+        return lane_id() & 16 ? r.lo : r.hi;
+    }
+    if constexpr (J == 32) {
+        const RowPair r = pair32(v);
+        return lane_id() & 32 ? r.lo : r.hi;
+    }
+}
+template <int J>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+    return uint64_t(lane_xor<J>(static_cast<uint32_t>(v >> 32))) << 32 |
+           lane_xor<J>(static_cast<uint32_t>(v));
+}
+
+// The steps J, J / 2, .. 1 of a bitonic merge within a wave.
+template <int J>
+__device__ __forceinline__ void wave_merge(uint64_t& v, bool down) {
+    const uint64_t o = lane_xor<J>(v);
+    v = down == ((lane_id() & J) == 0) ? max(v, o) : min(v, o);
+    if constexpr (J > 1) wave_merge<J / 2>(v, down);
+}
+template <int K>
+__device__ __forceinline__ void wave_sort(uint64_t& v) {
+    if constexpr (K > 2) wave_sort<K / 2>(v);
+    wave_merge<K / 2>(v, (threadIdx.x & K) == 0);
+}
+
+// Sorts the first `n` threads' values (n <= kList), the largest first; the other threads up to the
+// next power of two hold 0. Waves beyond it only pass the barriers.
+__device__ __forceinline__ uint64_t sort_down(uint64_t v, int n, Shared& s) {
     const int i = threadIdx.x;
-    for (int k = 2; k <= n; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            T o;
-            if (j < kWave) {
-                o = __shfl_xor(static_cast<Wide>(v), j, kWave);
-            } else {
-                __syncthreads();
-                list[i] = v;
-                __syncthreads();
-                o = list[i ^ j];
-            }
-            const bool keep_max = ((i & k) == 0) == ((i & j) == 0);
-            if (i < n) v = keep_max ? max(v, o) : min(v, o);
+    int size = kWave;
+    while (size < n) size *= 2;
+    const bool in = i < size;
+    if (in) wave_sort<kWave>(v);
+    for (int k = 2 * kWave; k <= size; k *= 2) {
+        for (int j = k / 2; j >= kWave; j /= 2) {
+            __syncthreads();
+            s.list[i] = v;
+            __syncthreads();
+            const uint64_t o = s.list[i ^ j];
+            if (in) v = ((i & k) == 0) == ((i & j) == 0) ? max(v, o) : min(v, o);
         }
+        if (in) wave_merge<kWave / 2>(v, (i & k) == 0);
+    }
     __syncthreads();
     return v;
 }
@@ -445,10 +479,8 @@ __device__ __forceinline__ uint64_t at_share(float u, uint64_t total) {
 __device__ __forceinline__ void finish_list(Shared& s, const Weigh& weigh, int n, bool by_count, int top_k,
                             float top_p, float min_p, float u, uint64_t total, int64_t* token) {
     const int tid = threadIdx.x;
-    int size = 1;
-    while (size < n) size *= 2;
     uint64_t v = tid < n ? s.list[tid] : 0;
-    v = sort_down(v, size, s);
+    v = sort_down(v, n, s);
     uint32_t key = static_cast<uint32_t>(v >> 32);
     const float e = tid < n ? weigh.e(key) : 0.0f;
     uint64_t w = tid < n && (!by_count || tid < top_k) ? Weigh::fixed(e) : 0;
@@ -457,11 +489,17 @@ __device__ __forceinline__ void finish_list(Shared& s, const Weigh& weigh, int n
     const double target = static_cast<double>(top_p) * static_cast<double>(by_count ? sum : total);
     bool kept = w && (top_p >= 1.0f || static_cast<double>(run - w) < target) && e >= min_p;
     kept |= tid == 0;
-    // the kept tokens in their order: the least token is the largest complement
+    // the kept tokens, the list's first ones, in their order: the least token is the largest complement
+    if (tid == 0) s.n_list = 0;
+    __syncthreads();
+    if (const uint64_t lanes = ballot(kept); lanes && tid % kWave == 0)
+        atomicMax(&s.n_list, uint32_t(tid + kWave - __clzll(lanes)));
+    __syncthreads();
+    const int left = static_cast<int>(s.n_list);
     v = kept ? (v << 32 | v >> 32) : 0;
-    v = sort_down(v, size, s);
+    v = sort_down(v, left, s);
     key = static_cast<uint32_t>(v);
-    w = v && tid < n ? weigh.w(key) : 0;
+    w = v && tid < left ? weigh.w(key) : 0;
     const uint64_t end = block_scan(w, s, sum);
     const uint64_t r = at_share(u, sum);
     if (w && end > r && end - w <= r) *token = int64_t(uint32_t(~(v >> 32)));
@@ -523,12 +561,22 @@ __device__ __forceinline__ void find_best(const Row<E>& row, int from, int to, S
     first = ~block_max(mine == best ? ~static_cast<uint32_t>(first) : 0, s);
 }
 
-// The k-th largest of the threads' keys, or the least key above -inf.
-__device__ __forceinline__ uint32_t list_from(uint32_t mine, int k, Shared& s) {
-    const uint32_t sorted = sort_down(mine, kThreads, s);
-    if (int(threadIdx.x) == k - 1) s.found = sorted;
+// A key no larger than the k-th largest of the threads' keys `mine`, and above -inf: the end of the bin
+// that the k-th lies in, of 2048 bins from `best` down to the least of them or to three octaves below.
+__device__ __forceinline__ uint32_t list_from(uint32_t mine, uint32_t best, int k, Shared& s) {
+    constexpr uint32_t kFurthest = 3u << 23;
+    const uint32_t lowest = ~block_max(~max(mine, kKeyNegInf), s);
+    const uint32_t range = min(best - lowest, kFurthest);
+    const int shift = max(0, 32 - __clz(int(range)) - 11);  // range >> shift < 2048
+    clear_bins(s);
+    const uint32_t bin = min(best - max(mine, kKeyNegInf), range) >> shift;
+    if (mine > kKeyNegInf) atomicAdd(&s.count[bin], 1u);
     __syncthreads();
-    return max(s.found, kKeyNegInf + 1);
+    const Place at = find_bin(s, true, k, 0.0, 0);
+    if (!at.found) return kKeyNegInf + 1;  // fewer than k threads have a key
+    const uint32_t end = (uint32_t(at.bin) + 1) << shift;
+    if (end <= range) return best - end + 1;
+    return range < kFurthest ? max(lowest, kKeyNegInf + 1) : kKeyNegInf + 1;  // the last bin
 }
 
 // One slice of a row: its largest key, and its list where top_k is tried by lists.
@@ -544,7 +592,7 @@ __global__ __launch_bounds__(kThreads) void sample_slices(Args a) {
     find_best(row, from, to, s, mine, best, first);
     if (tid == 0) a.best[at] = best, a.first[at] = first;
     if (set.greedy() || !set.lists()) return;
-    const int n = best > kKeyNegInf ? gather(row, from, to, s, list_from(mine, set.top_k, s)) : 0;
+    const int n = best > kKeyNegInf ? gather(row, from, to, s, list_from(mine, best, set.top_k, s)) : 0;
     if (tid == 0) a.listed[at] = n;
     if (tid < n) a.lists[int64_t(at) * kList + tid] = s.list[tid];
 }
@@ -574,7 +622,7 @@ __global__ __launch_bounds__(kThreads) void sample_sums(Args a) {
 
 // The slices' lists as one: the tokens from the k-th largest of the threads' maxima over them on;
 // how many, or more than kList where there is no such list.
-__device__ __forceinline__ int merge_lists(const Args& a, int i, int k, Shared& s) {
+__device__ __forceinline__ int merge_lists(const Args& a, int i, int k, uint32_t best, Shared& s) {
     const int tid = threadIdx.x;
     uint64_t v[kMostSlices];
     uint32_t mine = 0;
@@ -589,7 +637,7 @@ __device__ __forceinline__ int merge_lists(const Args& a, int i, int k, Shared& 
     if (!whole) return kList + 1;
 #pragma unroll
     for (int j = 0; j < kMostSlices; ++j) mine = max(mine, static_cast<uint32_t>(v[j] >> 32));
-    const uint32_t least = list_from(mine, k, s);
+    const uint32_t least = list_from(mine, best, k, s);
     if (tid == 0) s.n_list = 0;
     __syncthreads();
 #pragma unroll
@@ -628,9 +676,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
     if (set.lists()) {
         int n;
         if constexpr (kSlices)
-            n = merge_lists(a, i, top_k, s);
+            n = merge_lists(a, i, top_k, best, s);
         else
-            n = gather(row, 0, row.packs, s, list_from(mine, top_k, s));
+            n = gather(row, 0, row.packs, s, list_from(mine, best, top_k, s));
         if (n <= kList) {
             finish_list(s, weigh, n, true, top_k, top_p, min_p, u, 0, a.tokens + i);
             return;
