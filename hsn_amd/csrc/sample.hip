@@ -200,33 +200,61 @@ struct Weigh {
     __device__ __forceinline__ uint64_t w(uint32_t k) const { return fixed(e(k)); }
 };
 
-// Inclusive sum over the workgroup in thread order; `total` the whole. Ends with a barrier passed.
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, Shared& s, uint64_t& total) {
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    for (int d = 1; d < kWave; d *= 2) {
-        const uint64_t o = __shfl_up(static_cast<unsigned long long>(v), d, kWave);
-        if (lane >= d) v += o;
-    }
-    __syncthreads();
-    if (lane == kWave - 1) s.wave64[wave] = v;
-    __syncthreads();
-    uint64_t before = 0;
-    total = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        if (w == wave) before = total;
-        total += s.wave64[w];
-    }
-    return before + v;
+// The value CTRL lanes below by DPP (0 where there is none), for the sums below.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_below(uint32_t v) {
+    return static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_below(uint64_t v) {
+    return uint64_t(dpp_below<CTRL, ROWS>(static_cast<uint32_t>(v >> 32))) << 32 |
+           dpp_below<CTRL, ROWS>(static_cast<uint32_t>(v));
 }
 
+// Inclusive sum over 16 lanes, or over the wave, in lane order.
+template <typename T>
+__device__ __forceinline__ T row_scan(T v) {
+    v += dpp_below<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += dpp_below<0x112, 0xf>(v);
+    v += dpp_below<0x114, 0xf>(v);
+    v += dpp_below<0x118, 0xf>(v);
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v = row_scan(v);
+    v += dpp_below<0x142, 0xa>(v);  // row_bcast:15 into the odd rows
+    v += dpp_below<0x143, 0xc>(v);  // row_bcast:31 into the upper half
+    return v;
+}
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
+    return uint64_t(readlane(static_cast<uint32_t>(v >> 32), lane)) << 32 |
+           readlane(static_cast<uint32_t>(v), lane);
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return readlane(v, lane); }
+
+// Inclusive sum over the workgroup in thread order; `total` the whole. Ends with a barrier passed.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, Shared& s, T& total) {
+    const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
+    T* waves = reinterpret_cast<T*>(s.wave64);
+    v = wave_scan(v);
+    __syncthreads();
+    if (lane == kWave - 1) waves[wave] = v;
+    __syncthreads();
+    const T run = row_scan(waves[lane % kWaves]);  // the waves' sums, in every row of lanes
+    total = lane_value(run, kWaves - 1);
+    return v + (wave ? lane_value(run, wave - 1) : T(0));
+}
+static_assert(kWaves == 16, "a row of lanes holds the waves' sums");
+
 __device__ __forceinline__ uint32_t block_max(uint32_t v, Shared& s) {
-    for (int d = 1; d < kWave; d *= 2) v = max(v, wave_shfl_xor(v, d));
+    v = group_max<kWave>(v);
     __syncthreads();
     if (threadIdx.x % kWave == 0) s.wave32[threadIdx.x / kWave] = v;
     __syncthreads();
-    uint32_t m = 0;
-    for (int w = 0; w < kWaves; ++w) m = max(m, s.wave32[w]);
-    return m;
+    return group_max<16>(s.wave32[threadIdx.x % kWaves]);
 }
 
 __device__ __forceinline__ void clear_bins(Shared& s) {
@@ -255,7 +283,7 @@ __device__ __forceinline__ Place find_bin(Shared& s, bool by_count, uint64_t k, 
     const uint64_t m0 = s.mass[b], m1 = s.mass[b + 1];
     const uint32_t c0 = s.count[b], c1 = s.count[b + 1];
     uint64_t mt, ct;
-    const uint64_t mi = block_scan(m0 + m1, s, mt), ci = block_scan(c0 + uint64_t(c1), s, ct);
+    const uint64_t mi = block_scan(m0 + m1, s, mt), ci = block_scan(uint64_t(c0) + c1, s, ct);
     if (threadIdx.x == 0) s.found = kBins;
     __syncthreads();
     const uint64_t m_at[3] = {mi - m1 - m0, mi - m1, mi};
@@ -350,10 +378,8 @@ __device__ __forceinline__ void chunk_sums(const Row<E>& row, int from, int to, 
     for (int c = from / kWave + wave; c * kWave < to; c += kWaves) {
         v4u pack[1];
         row.load(c * kWave + lane, 0, pack);
-        uint64_t sum = pack_sum(row, c * kWave + lane, pack[0], f);
-        for (int d = 1; d < kWave; d *= 2)
-            sum += __shfl_xor(static_cast<unsigned long long>(sum), d, kWave);
-        if (lane == 0) sums[c] = sum;
+        const uint64_t sum = wave_scan(pack_sum(row, c * kWave + lane, pack[0], f));
+        if (lane == kWave - 1) sums[c] = sum;
     }
 }
 
@@ -388,12 +414,7 @@ __device__ __forceinline__ int walk(const Row<E>& row, Shared& s, const uint64_t
         v4u pack[1];
         row.load(p, 0, pack);
         const uint64_t sum = pack_sum(row, p, pack[0], f);
-        uint64_t run = sum;
-        for (int d = 1; d < kWave; d *= 2) {
-            const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), d, kWave);
-            if (lane >= d) run += o;
-        }
-        run += s.found_mass - sum;  // before this pack
+        uint64_t run = wave_scan(sum) + s.found_mass - sum;  // before this pack
         if (run <= r && run + sum > r) {
             uint32_t key[Row<E>::kVec];
             Row<E>::keys(pack[0], key);
@@ -562,19 +583,26 @@ __device__ __forceinline__ void find_best(const Row<E>& row, int from, int to, S
 }
 
 // A key no larger than the k-th largest of the threads' keys `mine`, and above -inf: the end of the bin
-// that the k-th lies in, of 2048 bins from `best` down to the least of them or to three octaves below.
+// that the k-th lies in, of 1024 bins from `best` down to the least of them or to three octaves below.
 __device__ __forceinline__ uint32_t list_from(uint32_t mine, uint32_t best, int k, Shared& s) {
     constexpr uint32_t kFurthest = 3u << 23;
-    const uint32_t lowest = ~block_max(~max(mine, kKeyNegInf), s);
+    const int tid = threadIdx.x;
+    mine = max(mine, kKeyNegInf);
+    const uint32_t lowest = ~block_max(~mine, s);
     const uint32_t range = min(best - lowest, kFurthest);
-    const int shift = max(0, 32 - __clz(int(range)) - 11);  // range >> shift < 2048
-    clear_bins(s);
-    const uint32_t bin = min(best - max(mine, kKeyNegInf), range) >> shift;
-    if (mine > kKeyNegInf) atomicAdd(&s.count[bin], 1u);
+    const int shift = max(0, 32 - __clz(int(range)) - 10);  // range >> shift < 1024
+    s.count[tid] = 0;
+    if (tid == 0) s.found = kThreads;
     __syncthreads();
-    const Place at = find_bin(s, true, k, 0.0, 0);
-    if (!at.found) return kKeyNegInf + 1;  // fewer than k threads have a key
-    const uint32_t end = (uint32_t(at.bin) + 1) << shift;
+    if (mine > kKeyNegInf) atomicAdd(&s.count[min(best - mine, range) >> shift], 1u);
+    __syncthreads();
+    uint32_t all;
+    const uint32_t here = s.count[tid], run = block_scan(here, s, all);
+    if (run >= uint32_t(k) && run - here < uint32_t(k)) s.found = tid;
+    __syncthreads();
+    const uint32_t bin = s.found;
+    if (bin == kThreads) return kKeyNegInf + 1;  // fewer than k threads have a key
+    const uint32_t end = (bin + 1) << shift;
     if (end <= range) return best - end + 1;
     return range < kFurthest ? max(lowest, kKeyNegInf + 1) : kKeyNegInf + 1;  // the last bin
 }
@@ -597,13 +625,14 @@ __global__ __launch_bounds__(kThreads) void sample_slices(Args a) {
     if (tid < n) a.lists[int64_t(at) * kList + tid] = s.list[tid];
 }
 
-// The largest key and its first token from the slices'.
+// The largest key and its first token from the slices', a lane a slice.
 __device__ __forceinline__ void best_of_slices(const Args& a, int i, uint32_t& best, int& first) {
-    best = 0, first = a.V;
-    for (int k = 0; k < a.slices; ++k) best = max(best, a.best[i * a.slices + k]);
-    for (int k = 0; k < a.slices; ++k)
-        if (a.best[i * a.slices + k] == best) first = min(first, a.first[i * a.slices + k]);
+    const int k = threadIdx.x % kMostSlices, at = i * a.slices + min(k, a.slices - 1);
+    const uint32_t key = a.best[at], token = a.first[at];
+    best = group_max<kMostSlices>(key);
+    first = ~group_max<kMostSlices>(key == best ? ~token : 0);
 }
+static_assert(kMostSlices == 16, "a row of lanes holds the slices");
 
 // One slice's sums of 64 packs' weights, for rows that neither top_k nor top_p cuts.
 template <typename E>
