@@ -38,6 +38,7 @@ constexpr int kBatch = 4;
 constexpr int kBins = 2048, kList = 1024;
 constexpr int kListTop = kList / 2;  // the largest top_k that a list is tried for
 constexpr int kMostSlices = 16;
+constexpr int kSumThreads = 256, kSumChunks = 4 * kSumThreads / kWave;  // of sample_sums
 constexpr float kBinScale = kBins / 27.75f;  // 2^-40 = exp(-27.726)
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // score_key(-inf)
 constexpr int kChunks = 2 * kThreads;        // sums of 64 packs: 2^18 / (64 * 4) + 1 at most
@@ -371,11 +372,11 @@ __device__ __forceinline__ uint64_t pack_sum(const Row<E>& row, int p, const v4u
     return p < row.packs ? sum : 0;
 }
 
-// The sums of f(key, token) over 64 packs each, from pack `from` up to `to`, a wave a sum.
+// The sums of f(key, token) over 64 packs each, from chunk `from` up to `to`, a wave a sum.
 template <typename E, typename F>
 __device__ __forceinline__ void chunk_sums(const Row<E>& row, int from, int to, uint64_t* sums, F&& f) {
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    for (int c = from / kWave + wave; c * kWave < to; c += kWaves) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+    for (int c = from + wave; c < to; c += waves) {
         v4u pack[1];
         row.load(c * kWave + lane, 0, pack);
         const uint64_t sum = wave_scan(pack_sum(row, c * kWave + lane, pack[0], f));
@@ -393,7 +394,7 @@ __device__ __forceinline__ int walk(const Row<E>& row, Shared& s, const uint64_t
     for (int i = threadIdx.x; i < kChunks; i += kThreads) s.mass[i] = sums && i < chunks ? sums[i] : 0;
     if (threadIdx.x == 0) s.found = kChunks;
     __syncthreads();
-    if (!sums) chunk_sums(row, 0, row.packs, s.mass, f);
+    if (!sums) chunk_sums(row, 0, chunks, s.mass, f);
     __syncthreads();
     const uint64_t s0 = s.mass[2 * threadIdx.x], s1 = s.mass[2 * threadIdx.x + 1];
     uint64_t total;
@@ -634,9 +635,11 @@ __device__ __forceinline__ void best_of_slices(const Args& a, int i, uint32_t& b
 }
 static_assert(kMostSlices == 16, "a row of lanes holds the slices");
 
-// One slice's sums of 64 packs' weights, for rows that neither top_k nor top_p cuts.
+// A part of a row's sums of 64 packs' weights, for rows that neither top_k nor top_p cuts: a wave four
+// sums, so that a batch with few such rows still fills the GPU (64 rows of 131072 in bf16: 16 sums a wave
+// take 32 us).
 template <typename E>
-__global__ __launch_bounds__(kThreads) void sample_sums(Args a) {
+__global__ __launch_bounds__(kSumThreads) void sample_sums(Args a) {
     const int i = blockIdx.y;
     const Settings set(a, i);
     if (set.greedy() || set.cuts_k || set.cuts_p) return;
@@ -645,7 +648,8 @@ __global__ __launch_bounds__(kThreads) void sample_sums(Args a) {
     int first;
     best_of_slices(a, i, best, first);
     if (best <= kKeyNegInf) return;
-    const int from = blockIdx.x * a.slice_packs, to = min(row.packs, from + a.slice_packs);
+    const int from = blockIdx.x * kSumChunks;
+    const int to = min((row.packs + kWave - 1) / kWave, from + kSumChunks);
     chunk_sums(row, from, to, a.sums + int64_t(i) * kChunks, Plain{Weigh(best, set.t), set.min_p, first});
 }
 
@@ -775,7 +779,7 @@ namespace {
 // fill the GPU or are short.
 int slices_of(int n, int V, int size) {
     const int packs = (V + 16 / size - 1) / (16 / size) + 1;
-    const int slices = std::min(kMostSlices, std::min(packs / kThreads, 512 / std::max(n, 1)));
+    const int slices = std::min(kMostSlices, std::min(packs / (2 * kThreads), 512 / std::max(n, 1)));
     return slices > 1 ? slices : 0;
 }
 
@@ -809,7 +813,10 @@ void launch(const Args& a, int n, hipStream_t st) {
     // where the settings are the same for all rows, whether any row needs the sums is known here
     const hsn_sample_settings& f = a.settings;
     const bool cut = (!a.top_k && f.top_k > 0 && f.top_k < a.V) || (!a.top_p && !(f.top_p >= 1.0f));
-    if (!cut) sample_sums<E><<<dim3(a.slices, n), kThreads, 0, st>>>(a);
+    if (!cut) {
+        const int chunks = (a.slices * a.slice_packs + kWave - 1) / kWave;
+        sample_sums<E><<<dim3((chunks + kSumChunks - 1) / kSumChunks, n), kSumThreads, 0, st>>>(a);
+    }
     sample_rows<E, true><<<n, kThreads, 0, st>>>(a);
 }
 
