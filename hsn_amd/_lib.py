@@ -204,8 +204,16 @@ def ptr(t) -> int | None:
     return t.data_ptr()
 
 
+def addr(t) -> int | None:
+    """Device address of a tensor whose device the caller has checked (``None`` for an absent one)."""
+    return None if t is None else t.data_ptr()
+
+
 def stream_of(device) -> int:
     """The current torch stream of ``device`` as a hipStream_t handle."""
     import torch
 
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is not None and device.index is not None:  # without the stream object, 1 us less
+        return raw(device.index)
     return torch.cuda.current_stream(device).cuda_stream

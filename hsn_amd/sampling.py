@@ -11,13 +11,14 @@ CPU path here. Nothing is kept between calls.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Union
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import call, ptr, stream_of
+from ._lib import addr, call, stream_of
 
 __all__ = ["MAX_TOKENS", "sample", "available"]
 
@@ -33,16 +34,23 @@ class _Settings(ctypes.Structure):
                 ("top_p", ctypes.c_float), ("min_p", ctypes.c_float)]
 
 
-def _setting(v, name: str, dtype: torch.dtype, n: int, logits: Tensor):
+def _setting(v, name: str, dtype: torch.dtype, n: int, device):
     """``(the address of a setting's row values, its value for all rows)``."""
     if not isinstance(v, Tensor):
         return None, v
-    if tuple(v.shape) != (n,) or v.dtype != dtype or v.device != logits.device:
-        raise ValueError(f"{name} must be a number or ({n},) {dtype} on {logits.device}, got "
+    if v.shape != (n,) or v.dtype != dtype or v.device != device:
+        raise ValueError(f"{name} must be a number or ({n},) {dtype} on {device}, got "
                          f"{tuple(v.shape)} {v.dtype} on {v.device}")
     if not v.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return ptr(v), 0
+    return v.data_ptr(), 0
+
+
+@lru_cache(maxsize=1024)
+def _workspace_bytes(n: int, V: int, dtype: int) -> int:
+    out = ctypes.c_int64(0)
+    call("hsn_sample_workspace", n, V, dtype, ctypes.byref(out))
+    return out.value
 
 
 def sample(logits: Tensor, u: Tensor, *, temperature: Union[float, Tensor] = 1.0,
@@ -64,31 +72,30 @@ def sample(logits: Tensor, u: Tensor, *, temperature: Union[float, Tensor] = 1.0
         raise ValueError("logits must be [n, V] in float32, float16 or bfloat16, got "
                          f"{tuple(logits.shape)} {logits.dtype}")
     n, V = logits.shape
+    dev = logits.device
     if not 1 <= V <= MAX_TOKENS:
         raise ValueError(f"V must be in [1, {MAX_TOKENS}], got {V}")
-    if logits.stride(1) != 1 and V > 1:
+    row, last = logits.stride()
+    if last != 1 and V > 1:
         raise ValueError("a row of logits must be contiguous")
-    if tuple(u.shape) != (n,) or u.dtype != torch.float32 or u.device != logits.device:
-        raise ValueError(f"u must be ({n},) float32 on {logits.device}, got {tuple(u.shape)} "
-                         f"{u.dtype} on {u.device}")
+    if u.shape != (n,) or u.dtype != torch.float32 or u.device != dev:
+        raise ValueError(f"u must be ({n},) float32 on {dev}, got {tuple(u.shape)} {u.dtype} on "
+                         f"{u.device}")
     if not u.is_contiguous():
         raise ValueError("u must be contiguous")
-    t_at, t = _setting(temperature, "temperature", torch.float32, n, logits)
-    k_at, k = _setting(top_k, "top_k", torch.int32, n, logits)
-    p_at, p = _setting(top_p, "top_p", torch.float32, n, logits)
-    m_at, m = _setting(min_p, "min_p", torch.float32, n, logits)
+    t_at, t = _setting(temperature, "temperature", torch.float32, n, dev)
+    k_at, k = _setting(top_k, "top_k", torch.int32, n, dev)
+    p_at, p = _setting(top_p, "top_p", torch.float32, n, dev)
+    m_at, m = _setting(min_p, "min_p", torch.float32, n, dev)
     if not 0 <= k < 2 ** 31:
         raise ValueError(f"top_k must be in [0, 2^31), got {k}")
-    settings = _Settings(t, k, p, m)
-    tokens = torch.empty(n, dtype=torch.int64, device=logits.device)
     code = _DTYPE[logits.dtype]
-    size = ctypes.c_int64(0)
-    call("hsn_sample_workspace", n, V, code, ctypes.byref(size))
-    ws = None
-    if size.value:
-        ws = torch.empty(size.value, dtype=torch.uint8, device=logits.device)
-    call("hsn_sample", ptr(logits), logits.stride(0), code, ptr(u), t_at, k_at, p_at, m_at,
-         ctypes.byref(settings), ptr(tokens), n, V, ptr(ws), size.value, stream_of(logits.device))
+    size = _workspace_bytes(n, V, code)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    tokens = torch.empty(n, dtype=torch.int64, device=dev)
+    call("hsn_sample", logits.data_ptr(), row, code, u.data_ptr(), t_at, k_at, p_at, m_at,
+         ctypes.byref(_Settings(t, k, p, m)), tokens.data_ptr(), n, V, addr(ws), size,
+         stream_of(dev))
     return tokens
 
 

@@ -17,13 +17,14 @@ no CPU path here. Nothing is kept between calls.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import call, ptr, stream_of
+from ._lib import addr, call, stream_of
 
 __all__ = ["SPAN", "forward", "backward", "gated_scan", "GatedScan", "step", "available"]
 
@@ -41,44 +42,52 @@ def _candidate(name: str) -> int:
     return CANDIDATES[name]
 
 
-def _dtype(t: Tensor, name: str) -> int:
-    if t.dtype not in _DTYPE:
-        raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
-    return _DTYPE[t.dtype]
+def _first(y: Tensor, dims: int) -> tuple:
+    """The checks of ``y``: ``(its shape, dtype code, dtype, device)``, which the others must have."""
+    if not y.is_cuda:
+        raise ValueError(f"y is on {y.device}: the kernels take ROCm device tensors")
+    shape, dtype = y.shape, y.dtype
+    if len(shape) != dims or shape[-1] == 0:
+        raise ValueError(f"y must have {dims} dimensions and at least one channel, got "
+                         f"{tuple(shape)}")
+    if dtype not in _DTYPE:
+        raise ValueError(f"y must be float32, float16 or bfloat16, got {dtype}")
+    return shape, _DTYPE[dtype], dtype, y.device
 
 
-def _strided(t: Tensor, name: str, like: Tensor) -> None:
-    """A tensor of the inputs' shape, type and device whose last dimension is contiguous."""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype} on {like.device}, got "
-                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+def _strides(t: Tensor, name: str, shape, dtype, device) -> tuple:
+    """The strides of a tensor of the inputs' shape, type and device whose last dimension is
+    contiguous."""
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {device}, got {tuple(t.shape)} "
+                         f"{t.dtype} on {t.device}")
+    strides = t.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
+    return strides
 
 
-def _dense(t: Optional[Tensor], name: str, shape: tuple, dtype: torch.dtype, like: Tensor) -> None:
+def _dense(t: Optional[Tensor], name: str, shape: tuple, dtype: torch.dtype, device) -> Optional[int]:
+    """The address of a contiguous tensor of this shape and type (``None`` for an absent one)."""
     if t is None:
-        return
-    if tuple(t.shape) != shape or t.dtype != dtype or t.device != like.device:
-        raise ValueError(f"{name} must be {shape} {dtype} on {like.device}, got {tuple(t.shape)} "
+        return None
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {device}, got {tuple(t.shape)} "
                          f"{t.dtype} on {t.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
 
 
-def _shape(y: Tensor, dims: int) -> tuple:
-    if not y.is_cuda:
-        raise ValueError(f"y is on {y.device}: the kernels take ROCm device tensors")
-    if y.dim() != dims or y.shape[-1] == 0:
-        raise ValueError(f"y must have {dims} dimensions and at least one channel, got "
-                         f"{tuple(y.shape)}")
-    return tuple(y.shape)
+@lru_cache(maxsize=1024)
+def _workspace_bytes(B: int, T: int, D: int, dtype: int, backward: int) -> int:
+    out = ctypes.c_int64(0)
+    call("hsn_scan_workspace", B, T, D, dtype, backward, ctypes.byref(out))
+    return out.value
 
 
 def _workspace(B: int, T: int, D: int, dtype: int, backward: int, device):
-    out = ctypes.c_int64(0)
-    call("hsn_scan_workspace", B, T, D, dtype, backward, ctypes.byref(out))
-    n = out.value
+    n = _workspace_bytes(B, T, D, dtype, backward)
     return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
 
 
@@ -87,21 +96,20 @@ def forward(y: Tensor, gate: Tensor, reset: Optional[Tensor] = None, h0: Optiona
     """The recurrence over a window: ``h [B, T, D]`` in ``y``'s dtype, the end state ``h_T [B, D]``
     (fp32) and, with ``save``, ``marks``: the states :func:`backward` starts from. ``reset [B, T]``
     is bool, ``h0 [B, D]`` fp32 (``None``: no resets, zero)."""
-    B, T, D = _shape(y, 3)
-    code, dev = _dtype(y, "y"), y.device
-    _strided(y, "y", y)
-    _strided(gate, "gate", y)
-    _dense(reset, "reset", (B, T), torch.bool, y)
-    _dense(h0, "h0", (B, D), torch.float32, y)
-    h = torch.empty(B, T, D, dtype=y.dtype, device=dev)
-    h_T = torch.empty(B, D, dtype=torch.float32, device=dev)
+    shape, code, io, dev = _first(y, 3)
+    B, T, D = shape
+    ys, gs = _strides(y, "y", shape, io, dev), _strides(gate, "gate", shape, io, dev)
+    reset_at = _dense(reset, "reset", (B, T), torch.bool, dev)
+    h0_at = _dense(h0, "h0", (B, D), torch.float32, dev)
+    h = torch.empty(shape, dtype=io, device=dev)
+    h_T = torch.empty((B, D), dtype=torch.float32, device=dev)
     marks = None
     if save:
-        marks = torch.empty(B, -(-T // SPAN), D, dtype=torch.float32, device=dev)
+        marks = torch.empty((B, -(-T // SPAN), D), dtype=torch.float32, device=dev)
     ws, ws_bytes = _workspace(B, T, D, code, 0, dev)
-    call("hsn_scan_forward", ptr(y), y.stride(0), y.stride(1), ptr(gate), gate.stride(0),
-         gate.stride(1), code, _candidate(candidate), ptr(reset), ptr(h0), ptr(h), ptr(h_T),
-         ptr(marks), B, T, D, ptr(ws), ws_bytes, stream_of(dev))
+    call("hsn_scan_forward", y.data_ptr(), ys[0], ys[1], gate.data_ptr(), gs[0], gs[1], code,
+         _candidate(candidate), reset_at, h0_at, h.data_ptr(), h_T.data_ptr(), addr(marks), B, T, D,
+         addr(ws), ws_bytes, stream_of(dev))
     return {"h": h, "h_T": h_T, "marks": marks}
 
 
@@ -111,24 +119,21 @@ def backward(y: Tensor, gate: Tensor, marks: Tensor, reset: Optional[Tensor],
     """``(d_y, d_gate, d_h0)`` from :func:`forward`'s inputs and ``marks`` and the cotangents
     ``d_h [B, T, D]`` (``y``'s dtype) and ``d_h_T [B, D]`` (fp32), either ``None`` where absent.
     The cotangent of the state is fp32; ``d_y`` and ``d_gate`` have ``y``'s dtype."""
-    B, T, D = _shape(y, 3)
-    code, dev = _dtype(y, "y"), y.device
-    _strided(y, "y", y)
-    _strided(gate, "gate", y)
-    _dense(marks, "marks", (B, -(-T // SPAN), D), torch.float32, y)
-    _dense(reset, "reset", (B, T), torch.bool, y)
-    _dense(d_h_T, "d_h_T", (B, D), torch.float32, y)
-    row = pos = 0
-    if d_h is not None:
-        _strided(d_h, "d_h", y)
-        row, pos = d_h.stride(0), d_h.stride(1)
-    d_y = torch.empty(B, T, D, dtype=y.dtype, device=dev)
-    d_gate = torch.empty_like(d_y)
-    d_h0 = torch.empty(B, D, dtype=torch.float32, device=dev)
+    shape, code, io, dev = _first(y, 3)
+    B, T, D = shape
+    ys, gs = _strides(y, "y", shape, io, dev), _strides(gate, "gate", shape, io, dev)
+    marks_at = _dense(marks, "marks", (B, -(-T // SPAN), D), torch.float32, dev)
+    reset_at = _dense(reset, "reset", (B, T), torch.bool, dev)
+    d_h_T_at = _dense(d_h_T, "d_h_T", (B, D), torch.float32, dev)
+    ds = (0, 0) if d_h is None else _strides(d_h, "d_h", shape, io, dev)
+    d_y = torch.empty(shape, dtype=io, device=dev)
+    d_gate = torch.empty(shape, dtype=io, device=dev)
+    d_h0 = torch.empty((B, D), dtype=torch.float32, device=dev)
     ws, ws_bytes = _workspace(B, T, D, code, 1, dev)
-    call("hsn_scan_backward", ptr(y), y.stride(0), y.stride(1), ptr(gate), gate.stride(0),
-         gate.stride(1), code, _candidate(candidate), ptr(reset), ptr(marks), ptr(d_h), row, pos,
-         ptr(d_h_T), ptr(d_y), ptr(d_gate), ptr(d_h0), B, T, D, ptr(ws), ws_bytes, stream_of(dev))
+    call("hsn_scan_backward", y.data_ptr(), ys[0], ys[1], gate.data_ptr(), gs[0], gs[1], code,
+         _candidate(candidate), reset_at, marks_at, addr(d_h), ds[0], ds[1], d_h_T_at,
+         d_y.data_ptr(), d_gate.data_ptr(), d_h0.data_ptr(), B, T, D, addr(ws), ws_bytes,
+         stream_of(dev))
     return d_y, d_gate, d_h0
 
 
@@ -172,20 +177,16 @@ def step(y: Tensor, gate: Tensor, state: Tensor, *, rows: Optional[Tensor] = Non
     states are the rows ``rows [n]`` (int32, distinct; ``None``: the first ``n``) of ``state
     [S, D]`` (fp32), updated in place. Returns the new states ``h [n, D]`` in ``y``'s dtype. A row
     outside ``[0, S)`` is padding: its ``h`` is zero and no state is touched."""
-    n, D = _shape(y, 2)
-    code = _dtype(y, "y")
-    _strided(y, "y", y)
-    _strided(gate, "gate", y)
-    if state.dim() != 2:
-        raise ValueError(f"state must be [S, {D}], got {tuple(state.shape)}")
-    S = int(state.shape[0])
-    _dense(state, "state", (S, D), torch.float32, y)
-    _dense(rows, "rows", (n,), torch.int32, y)
-    _dense(reset, "reset", (n,), torch.bool, y)
-    h = torch.empty(n, D, dtype=y.dtype, device=y.device)
-    call("hsn_scan_step", ptr(y), y.stride(0), ptr(gate), gate.stride(0), code,
-         _candidate(candidate), ptr(rows), ptr(reset), ptr(state), ptr(h), n, S, D,
-         stream_of(y.device))
+    shape, code, io, dev = _first(y, 2)
+    n, D = shape
+    ys, gs = _strides(y, "y", shape, io, dev), _strides(gate, "gate", shape, io, dev)
+    S = state.shape[0] if state.dim() == 2 else -1
+    state_at = _dense(state, "state", (S, D), torch.float32, dev)
+    rows_at = _dense(rows, "rows", (n,), torch.int32, dev)
+    reset_at = _dense(reset, "reset", (n,), torch.bool, dev)
+    h = torch.empty(shape, dtype=io, device=dev)
+    call("hsn_scan_step", y.data_ptr(), ys[0], gate.data_ptr(), gs[0], code, _candidate(candidate),
+         rows_at, reset_at, state_at, h.data_ptr(), n, S, D, stream_of(dev))
     return h
 
 

@@ -11,13 +11,14 @@ Nothing is kept between calls. For many tokens, or a gradient, there is the grou
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import call, ptr, stream_of
+from ._lib import addr, call, stream_of
 
 __all__ = ["MAX_TOKENS", "MAX_UNITS", "MAX_CHOSEN", "unit_layer", "available"]
 
@@ -27,14 +28,21 @@ _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16,
           torch.bfloat16: _lib.DTYPE_BF16}
 
 
-def _weight(t: Optional[Tensor], name: str, shape: tuple, x: Tensor) -> None:
+def _weight(t: Optional[Tensor], name: str, shape: tuple, dtype: torch.dtype, device) -> None:
     if t is None:
         return
-    if tuple(t.shape) != shape or t.dtype != x.dtype or t.device != x.device:
-        raise ValueError(f"{name} must be {shape} {x.dtype} on {x.device}, got {tuple(t.shape)} "
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {shape} {dtype} on {device}, got {tuple(t.shape)} "
                          f"{t.dtype} on {t.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+@lru_cache(maxsize=1024)
+def _workspace_bytes(n, M, k, d_in, H, d_out, dtype, activation) -> int:
+    out = ctypes.c_int64(0)
+    call("hsn_units_layer_workspace", n, M, k, d_in, H, d_out, dtype, activation, ctypes.byref(out))
+    return out.value
 
 
 def unit_layer(x: Tensor, router: Tensor, W1: Tensor, b1: Optional[Tensor], W2: Tensor,
@@ -51,7 +59,8 @@ def unit_layer(x: Tensor, router: Tensor, W1: Tensor, b1: Optional[Tensor], W2: 
     if x.dim() != 2 or x.dtype not in _DTYPE:
         raise ValueError("x must be [n, d_in] in float32, float16 or bfloat16, got "
                          f"{tuple(x.shape)} {x.dtype}")
-    if x.stride(1) != 1 and x.shape[1] > 1:
+    row, last = x.stride()
+    if last != 1 and x.shape[1] > 1:
         raise ValueError("a row of x must be contiguous")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
@@ -65,21 +74,22 @@ def unit_layer(x: Tensor, router: Tensor, W1: Tensor, b1: Optional[Tensor], W2: 
         raise ValueError(f"k must be in [1, {min(M, MAX_CHOSEN)}], got {k}")
     if n > MAX_TOKENS or M > MAX_UNITS:
         raise ValueError(f"at most {MAX_TOKENS} tokens and {MAX_UNITS} units, got {n} and {M}")
-    _weight(router, "router", (M, d_in), x)
-    _weight(W1, "W1", (M, d_in, H1), x)
-    _weight(b1, "b1", (M, H1), x)
-    _weight(W2, "W2", (M, H, d_out), x)
-    _weight(b2, "b2", (M, d_out), x)
+    io, dev = x.dtype, x.device
+    _weight(router, "router", (M, d_in), io, dev)
+    _weight(W1, "W1", (M, d_in, H1), io, dev)
+    _weight(b1, "b1", (M, H1), io, dev)
+    _weight(W2, "W2", (M, H, d_out), io, dev)
+    _weight(b2, "b2", (M, d_out), io, dev)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (x, router, W1, b1, W2, b2)):
         raise ValueError("unit_layer has no gradient: call it under torch.no_grad()")
-    code, act = _DTYPE[x.dtype], ACTIVATIONS[activation]
-    y = torch.empty(n, d_out, dtype=x.dtype, device=x.device)
-    size = ctypes.c_int64(0)
-    call("hsn_units_layer_workspace", n, M, k, d_in, H, d_out, code, act, ctypes.byref(size))
-    ws = torch.empty(size.value, dtype=torch.uint8, device=x.device)
-    call("hsn_units_layer", ptr(x), x.stride(0), ptr(router), ptr(W1), ptr(b1), ptr(W2), ptr(b2),
-         ptr(y), n, M, k, d_in, H, d_out, code, act, ptr(ws), size.value, stream_of(x.device))
+    code, act = _DTYPE[io], ACTIVATIONS[activation]
+    y = torch.empty((n, d_out), dtype=io, device=dev)
+    size = _workspace_bytes(n, M, k, d_in, H, d_out, code, act)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    call("hsn_units_layer", x.data_ptr(), row, router.data_ptr(), W1.data_ptr(), addr(b1),
+         W2.data_ptr(), addr(b2), y.data_ptr(), n, M, k, d_in, H, d_out, code, act, ws.data_ptr(),
+         size, stream_of(dev))
     return y
 
 
