@@ -5,16 +5,17 @@
 // histogram bins, by lanes, by waves. The order of tokens is the order of score_key(logit), then
 // of the token. A row takes these passes over its logits:
 //   1. the largest logit and its first token (all that a greedy row needs).
-//   2. with top_k up to 512: the k-th largest of the 1024 threads' own largest keys is no larger than
-//      the k-th largest key of the row, so every token that top_k keeps is among those from it on,
-//      some k (1 + k / 2048) of them where the large ones lie anywhere. They (or those from a little
-//      below it on, found by one histogram of the 1024 keys) are gathered
-//      into LDS and sorted there, the other filters and the choice follow on the list, and no other
-//      token's exponential is ever taken.
-//      Else, with a top_k or a top_p: counts and masses in 2048 bins, linear in x over the range where
-//      a weight is not 0 (x > -27.73). They say in which bin the filter cuts. Where the tokens down to
-//      that bin are at most 1024 they are gathered and sorted as above (a third pass); otherwise the
-//      cut is found on the keys' digits (11, 11 and 10 bits), a pass over the row for each.
+//   2. with top_k up to 512, or without a top_k and with a top_p: a list. The k-th largest of the 1024
+//      threads' own largest keys is no larger than the k-th largest key of the row, so every token
+//      that top_k keeps is among those from it on, some k (1 + k / 2048) of them where the large
+//      ones lie anywhere. They (or those from a little below it on, found by one histogram of the 1024
+//      keys) are gathered into LDS and sorted there, the other filters and the choice follow on the
+//      list, and no other token's exponential is ever taken. top_p alone takes some 680 tokens and
+//      the row's whole mass, and is done where they hold its share.
+//      Else: counts and masses in 2048 bins, linear in x over the range where a weight is not 0 (x >
+//      -27.73). They say in which bin a filter cuts, and the bin's tokens, gathered and sorted, at which
+//      token; where a bin has more than 1024 (equal logits), the cut is found on the keys' digits (11, 11
+//      and 10 bits), a pass over the row for each.
 //   3. without a list: the kept weights' sums in the order of tokens, 64 packs of 16 bytes at a time,
 //      then one wave's walk through the 64 packs that hold the answer.
 // What bounds a row is the instructions of one compute unit: the passes over keys are short, an exact
@@ -77,14 +78,16 @@ struct Settings {
         cuts_p = !(top_p >= 1.0f);
     }
     __device__ bool greedy() const { return !(t > 0); }
-    // the list of the tokens from the k-th largest of the threads' maxima on is tried
-    __device__ bool lists() const { return cuts_k && top_k <= kListTop; }
+    // whether a list of the largest tokens is tried, and from the how-many-th largest of the threads'
+    // maxima over `packs` packs on: top_k's, or as many as a list holds (a twelfth of the tokens
+    // where the packs are few)
+    __device__ bool lists() const { return cuts_k ? top_k <= kListTop : cuts_p; }
+    __device__ int list_top(int packs) const { return cuts_k ? top_k : min(kListTop, max(1, packs / 2)); }
 };
 
 struct Shared {
     uint64_t mass[kBins];   // bins; then the sums of 64 packs
     uint32_t count[kBins];
-    uint32_t least[kBins];  // the smallest key of a bin
     uint64_t list[kList];
     uint64_t wave64[kWaves];
     uint32_t wave32[kWaves];
@@ -235,6 +238,10 @@ __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
 }
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return readlane(v, lane); }
 
+__device__ __forceinline__ int bin_of(float x) {
+    return min(kBins - 1, static_cast<int>(-x * kBinScale));
+}
+
 // Inclusive sum over the workgroup in thread order; `total` the whole. Ends with a barrier passed.
 template <typename T>
 __device__ __forceinline__ T block_scan(T v, Shared& s, T& total) {
@@ -258,9 +265,21 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, Shared& s) {
     return group_max<16>(s.wave32[threadIdx.x % kWaves]);
 }
 
+// The number of threads with `flag`, in every thread.
+__device__ __forceinline__ int block_count(bool flag, Shared& s) {
+    if (threadIdx.x == 0) s.n_list = 0;
+    __syncthreads();
+    const uint64_t lanes = ballot(flag);
+    if (lanes && threadIdx.x % kWave == 0) atomicAdd(&s.n_list, uint32_t(__popcll(lanes)));
+    __syncthreads();
+    const int n = static_cast<int>(s.n_list);
+    __syncthreads();
+    return n;
+}
+
 __device__ __forceinline__ void clear_bins(Shared& s) {
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0, s.least[i] = ~0u;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
     __syncthreads();
 }
 
@@ -293,7 +312,7 @@ __device__ __forceinline__ Place find_bin(Shared& s, bool by_count, uint64_t k, 
         const bool before = by_count ? c_at[i] < k : static_cast<double>(base + m_at[i]) < target;
         const bool after = by_count ? c_at[i + 1] < k
                                     : static_cast<double>(base + m_at[i + 1]) < target;
-        if (before && !after && c_at[i + 1] > c_at[i]) {
+        if (before && !after) {
             s.found = b + i;
             s.found_below = static_cast<uint32_t>(c_at[i]);
             s.found_mass = m_at[i];
@@ -363,13 +382,17 @@ __device__ __forceinline__ Cut descend(const Row<E>& row, const Weigh& weigh, Sh
 }
 
 template <typename E, typename F>
-__device__ __forceinline__ uint64_t pack_sum(const Row<E>& row, int p, const v4u& pack, F&& f) {
+__device__ __forceinline__ uint64_t pack_sum(const Row<E>& row, int p, const v4u& pack, F&& f,
+                                             uint64_t (&w)[Row<E>::kVec]) {
     uint64_t sum = 0;
     uint32_t key[Row<E>::kVec];
     Row<E>::keys(pack, key);
 #pragma unroll
-    for (int i = 0; i < Row<E>::kVec; ++i) sum += f(key[i], row.first(p) + i);
-    return p < row.packs ? sum : 0;
+    for (int i = 0; i < Row<E>::kVec; ++i) {
+        w[i] = p < row.packs ? f(key[i], row.first(p) + i) : 0;
+        sum += w[i];
+    }
+    return sum;
 }
 
 // The sums of f(key, token) over 64 packs each, from chunk `from` up to `to`, a wave a sum.
@@ -379,7 +402,8 @@ __device__ __forceinline__ void chunk_sums(const Row<E>& row, int from, int to, 
     for (int c = from + wave; c < to; c += waves) {
         v4u pack[1];
         row.load(c * kWave + lane, 0, pack);
-        const uint64_t sum = wave_scan(pack_sum(row, c * kWave + lane, pack[0], f));
+        uint64_t w[Row<E>::kVec];
+        const uint64_t sum = wave_scan(pack_sum(row, c * kWave + lane, pack[0], f, w));
         if (lane == kWave - 1) sums[c] = sum;
     }
 }
@@ -391,12 +415,12 @@ __device__ __forceinline__ int walk(const Row<E>& row, Shared& s, const uint64_t
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int chunks = (row.packs + kWave - 1) / kWave;
     __syncthreads();
-    for (int i = threadIdx.x; i < kChunks; i += kThreads) s.mass[i] = sums && i < chunks ? sums[i] : 0;
     if (threadIdx.x == 0) s.found = kChunks;
-    __syncthreads();
     if (!sums) chunk_sums(row, 0, chunks, s.mass, f);
     __syncthreads();
-    const uint64_t s0 = s.mass[2 * threadIdx.x], s1 = s.mass[2 * threadIdx.x + 1];
+    if (!sums) sums = s.mass;
+    const int c0 = 2 * threadIdx.x, c1 = c0 + 1;
+    const uint64_t s0 = c0 < chunks ? sums[c0] : 0, s1 = c1 < chunks ? sums[c1] : 0;
     uint64_t total;
     const uint64_t end = block_scan(s0 + s1, s, total);
     const uint64_t r = limit(total);
@@ -414,18 +438,17 @@ __device__ __forceinline__ int walk(const Row<E>& row, Shared& s, const uint64_t
         const int p = c * kWave + lane;
         v4u pack[1];
         row.load(p, 0, pack);
-        const uint64_t sum = pack_sum(row, p, pack[0], f);
+        uint64_t w[Row<E>::kVec];
+        const uint64_t sum = pack_sum(row, p, pack[0], f, w);
         uint64_t run = wave_scan(sum) + s.found_mass - sum;  // before this pack
         if (run <= r && run + sum > r) {
-            uint32_t key[Row<E>::kVec];
-            Row<E>::keys(pack[0], key);
+            int below = 0;  // tokens of the pack before the answer
+#pragma unroll
             for (int i = 0; i < Row<E>::kVec; ++i) {
-                run += f(key[i], row.first(p) + i);
-                if (run > r) {
-                    s.found_below = row.first(p) + i;
-                    break;
-                }
+                run += w[i];
+                below += run <= r;
             }
+            s.found_below = row.first(p) + below;
         }
     }
     __syncthreads();
@@ -495,29 +518,32 @@ __device__ __forceinline__ uint64_t at_share(float u, uint64_t total) {
     return i < total ? i : total - 1;
 }
 
-// The rest of a row on its list of `n` tokens (in LDS, any order): every token that top_k keeps and
-// every one larger than some token of the list. by_count: top_k cuts; else `total` is the row's
-// whole mass, which top_p is a share of.
-__device__ __forceinline__ void finish_list(Shared& s, const Weigh& weigh, int n, bool by_count, int top_k,
-                            float top_p, float min_p, float u, uint64_t total, int64_t* token) {
+// The mass that top_p asks for; a positive one, so that the first token is under it.
+__device__ __forceinline__ double mass_target(float top_p, uint64_t total) {
+    const double target = static_cast<double>(top_p) * static_cast<double>(total);
+    return target > 0 ? target : 1.0;
+}
+
+// The rest of a row on its list of `n` tokens (in LDS, any order), whose `sure` largest are the row's
+// largest. by_count: these are what top_k keeps; else top_p cuts, `total` is the row's whole mass,
+// and where the sure tokens do not hold what top_p keeps the answer is false and nothing is written.
+__device__ __forceinline__ bool finish_list(Shared& s, const Weigh& weigh, int n, bool by_count, int sure,
+                                            float top_p, float min_p, float u, uint64_t total,
+                                            int64_t* token) {
     const int tid = threadIdx.x;
     uint64_t v = tid < n ? s.list[tid] : 0;
     v = sort_down(v, n, s);
     uint32_t key = static_cast<uint32_t>(v >> 32);
     const float e = tid < n ? weigh.e(key) : 0.0f;
-    uint64_t w = tid < n && (!by_count || tid < top_k) ? Weigh::fixed(e) : 0;
+    uint64_t w = tid < min(n, sure) ? Weigh::fixed(e) : 0;
     uint64_t sum;
     const uint64_t run = block_scan(w, s, sum);
-    const double target = static_cast<double>(top_p) * static_cast<double>(by_count ? sum : total);
+    const double target = mass_target(top_p, by_count ? sum : total);
+    if (!by_count && static_cast<double>(sum) < target) return false;
     bool kept = w && (top_p >= 1.0f || static_cast<double>(run - w) < target) && e >= min_p;
     kept |= tid == 0;
     // the kept tokens, the list's first ones, in their order: the least token is the largest complement
-    if (tid == 0) s.n_list = 0;
-    __syncthreads();
-    if (const uint64_t lanes = ballot(kept); lanes && tid % kWave == 0)
-        atomicMax(&s.n_list, uint32_t(tid + kWave - __clzll(lanes)));
-    __syncthreads();
-    const int left = static_cast<int>(s.n_list);
+    const int left = block_count(kept, s);
     v = kept ? (v << 32 | v >> 32) : 0;
     v = sort_down(v, left, s);
     key = static_cast<uint32_t>(v);
@@ -525,12 +551,13 @@ __device__ __forceinline__ void finish_list(Shared& s, const Weigh& weigh, int n
     const uint64_t end = block_scan(w, s, sum);
     const uint64_t r = at_share(u, sum);
     if (w && end > r && end - w <= r) *token = int64_t(uint32_t(~(v >> 32)));
+    return true;
 }
 
-// Every token of packs [from, to) with a key from `least` on into the list; how many there are (the list
-// holds kList).
-template <typename E>
-__device__ __forceinline__ int gather(const Row<E>& row, int from, int to, Shared& s, uint32_t least) {
+// Every token of packs [from, to) with a key from `least` on that `wanted(key)` takes, into the list; how
+// many there are (the list holds kList).
+template <typename E, typename F>
+__device__ __forceinline__ int gather(const Row<E>& row, int from, int to, Shared& s, uint32_t least, F&& wanted) {
     __syncthreads();
     if (threadIdx.x == 0) s.n_list = 0;
     __syncthreads();
@@ -540,7 +567,7 @@ __device__ __forceinline__ int gather(const Row<E>& row, int from, int to, Share
         for (int j = 1; j < Row<E>::kVec; ++j) top = max(top, key[j]);
         if (top < least) return;
         for (int j = 0; j < Row<E>::kVec; ++j) {
-            if (key[j] < least) continue;
+            if (key[j] < least || !wanted(key[j])) continue;
             const uint32_t place = atomicAdd(&s.n_list, 1u);
             if (place < kList) s.list[place] = uint64_t(key[j]) << 32 | uint32_t(~(first + j));
         }
@@ -551,13 +578,28 @@ __device__ __forceinline__ int gather(const Row<E>& row, int from, int to, Share
     return n;
 }
 
-// The mass that top_p asks for; a positive one, so that the first token is under it.
-__device__ __forceinline__ double mass_target(float top_p, uint64_t total) {
-    const double target = static_cast<double>(top_p) * static_cast<double>(total);
-    return target > 0 ? target : 1.0;
+// A filter's cut inside one bin, whose `n` tokens are the list: by_count, the first k tokens stay, else
+// those with a mass before them, `before` and the bin's, under the target. mass_at: what stays, with
+// `before`.
+__device__ __forceinline__ Cut cut_list(Shared& s, const Weigh& weigh, int n, bool by_count, int k,
+                                        double target, uint64_t before, uint64_t& mass_at) {
+    const int tid = threadIdx.x;
+    const uint64_t v = sort_down(tid < n ? s.list[tid] : 0, n, s);
+    const uint32_t key = static_cast<uint32_t>(v >> 32);
+    const uint64_t w = tid < n ? weigh.w(key) : 0;
+    uint64_t sum;
+    const uint64_t run = before + block_scan(w, s, sum);
+    const bool kept = tid < n && (by_count ? tid < k : static_cast<double>(run - w) < target);
+    const int stay = block_count(kept, s);  // the first ones
+    if (tid == stay - 1) s.found = key, s.found_mass = run;
+    __syncthreads();
+    const uint32_t last = s.found;
+    mass_at = s.found_mass;
+    return Cut{last, uint64_t(stay - block_count(tid < n && key > last, s))};
 }
 
-// A token's weight where no filter but min_p cuts; the row's first token always has one.
+// A token's weight where top_k and top_p do not cut (min_p 0: where they have not cut yet); the row's
+// first token always has one.
 struct Plain {
     Weigh weigh;
     float min_p;
@@ -621,7 +663,8 @@ __global__ __launch_bounds__(kThreads) void sample_slices(Args a) {
     find_best(row, from, to, s, mine, best, first);
     if (tid == 0) a.best[at] = best, a.first[at] = first;
     if (set.greedy() || !set.lists()) return;
-    const int n = best > kKeyNegInf ? gather(row, from, to, s, list_from(mine, best, set.top_k, s)) : 0;
+    const int n = best > kKeyNegInf ? gather(row, from, to, s, list_from(mine, best, set.list_top(row.packs), s),
+                                              [](uint32_t) { return true; }) : 0;
     if (tid == 0) a.listed[at] = n;
     if (tid < n) a.lists[int64_t(at) * kList + tid] = s.list[tid];
 }
@@ -635,14 +678,14 @@ __device__ __forceinline__ void best_of_slices(const Args& a, int i, uint32_t& b
 }
 static_assert(kMostSlices == 16, "a row of lanes holds the slices");
 
-// A part of a row's sums of 64 packs' weights, for rows that neither top_k nor top_p cuts: a wave four
+// A part of a row's sums of 64 packs' weights, for rows that top_k does not cut: a wave four
 // sums, so that a batch with few such rows still fills the GPU (64 rows of 131072 in bf16: 16 sums a wave
 // take 32 us).
 template <typename E>
 __global__ __launch_bounds__(kSumThreads) void sample_sums(Args a) {
     const int i = blockIdx.y;
     const Settings set(a, i);
-    if (set.greedy() || set.cuts_k || set.cuts_p) return;
+    if (set.greedy() || set.cuts_k) return;
     const Row<E> row(static_cast<const E*>(a.logits) + i * a.row, a.V);
     uint32_t best;
     int first;
@@ -650,7 +693,8 @@ __global__ __launch_bounds__(kSumThreads) void sample_sums(Args a) {
     if (best <= kKeyNegInf) return;
     const int from = blockIdx.x * kSumChunks;
     const int to = min((row.packs + kWave - 1) / kWave, from + kSumChunks);
-    chunk_sums(row, from, to, a.sums + int64_t(i) * kChunks, Plain{Weigh(best, set.t), set.min_p, first});
+    chunk_sums(row, from, to, a.sums + int64_t(i) * kChunks,
+               Plain{Weigh(best, set.t), set.cuts_p ? 0.0f : set.min_p, first});
 }
 
 // The slices' lists as one: the tokens from the k-th largest of the threads' maxima over them on;
@@ -709,12 +753,28 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
     if (set.lists()) {
         int n;
         if constexpr (kSlices)
-            n = merge_lists(a, i, top_k, best, s);
+            n = merge_lists(a, i, set.list_top(row.packs), best, s);
         else
-            n = gather(row, 0, row.packs, s, list_from(mine, best, top_k, s));
+            n = gather(row, 0, row.packs, s, list_from(mine, best, set.list_top(row.packs), s),
+                       [](uint32_t) { return true; });
         if (n <= kList) {
-            finish_list(s, weigh, n, true, top_k, top_p, min_p, u, 0, a.tokens + i);
-            return;
+            uint64_t total = 0;
+            if (!cuts_k) {
+                uint64_t here = 0;
+                if constexpr (kSlices) {
+                    for (int c = tid; c * kWave < row.packs; c += kThreads)
+                        here += a.sums[int64_t(i) * kChunks + c];
+                } else {
+                    row.template each<1>(0, row.packs, [&](int, const uint32_t (&key)[kVec]) {
+#pragma unroll
+                        for (int j = 0; j < kVec; ++j) here += weigh.w(key[j]);
+                    });
+                }
+                block_scan(here, s, total);
+            }
+            // the slices' lists are whole down to their own ends only, and each has as many as asked for
+            const int sure = cuts_k ? top_k : kSlices ? set.list_top(row.packs) : n;
+            if (finish_list(s, weigh, n, cuts_k, sure, top_p, min_p, u, total, a.tokens + i)) return;
         }
     }
     Cut cut{0, 0};
@@ -727,28 +787,39 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
                 const float x = weigh.x(key[j]);
                 const uint64_t w = Weigh::fixed(Weigh::e_of(x));
                 if (!w) continue;
-                const int bin = min(kBins - 1, static_cast<int>(-x * kBinScale));
+                const int bin = bin_of(x);
                 atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[bin]), (unsigned long long)w);
-                atomicAdd(&s.count[bin], 1u);
-                atomicMin(&s.least[bin], key[j]);
+                if (cuts_k) atomicAdd(&s.count[bin], 1u);
             }
         });
         __syncthreads();
         uint64_t total;
         block_scan(s.mass[2 * tid] + s.mass[2 * tid + 1], s, total);
-        Place at = find_bin(s, cuts_k, top_k, 0.0, 0);
-        const bool by_count = cuts_k && at.found;  // else fewer tokens than top_k have a weight
-        if (!by_count && cuts_p) at = find_bin(s, false, 0, mass_target(top_p, total), 0);
-        if ((by_count || cuts_p) && at.found && at.count_before + at.count <= kList) {
-            const int n = gather(row, 0, row.packs, s, s.least[at.bin]);
-            finish_list(s, weigh, n, by_count, top_k, top_p, min_p, u, total, a.tokens + i);
-            return;
-        }
-        // the earlier of the two filters' cuts
-        if (by_count) cut = descend(row, weigh, s, true, top_k, 0.0, total);
-        if (cuts_p) {
-            uint64_t unused;
-            const Cut c = descend(row, weigh, s, false, 0, mass_target(top_p, total), unused);
+        bool bins = true;
+#pragma unroll 1
+        for (int filter = 0; filter < 2; ++filter) {  // top_k, then top_p of what it keeps
+            const bool by_count = filter == 0;
+            if (by_count ? !cuts_k : !cuts_p) continue;
+            const double target = mass_target(top_p, total);
+            Place at{};
+            int n = kList + 1;
+            if (bins) {
+                at = find_bin(s, by_count, top_k, target, 0);
+                if (!at.found) continue;  // it keeps every token with a weight
+                n = gather(row, 0, row.packs, s, kKeyNegInf + 1, [&](uint32_t k) {
+                    const float x = weigh.x(k);
+                    return x > -30.0f && bin_of(x) == at.bin && weigh.w(k);
+                });
+            }
+            Cut c;
+            uint64_t mass;
+            if (n <= kList) {
+                c = cut_list(s, weigh, n, by_count, top_k - int(at.count_before), target, at.mass_before, mass);
+            } else {
+                c = descend(row, weigh, s, by_count, top_k, target, mass);
+                bins = false;
+            }
+            if (by_count) total = mass;
             if (c.key > cut.key || (c.key == cut.key && c.equal < cut.equal)) cut = c;
         }
     }
@@ -812,7 +883,7 @@ void launch(const Args& a, int n, hipStream_t st) {
     sample_slices<E><<<dim3(a.slices, n), kThreads, 0, st>>>(a);
     // where the settings are the same for all rows, whether any row needs the sums is known here
     const hsn_sample_settings& f = a.settings;
-    const bool cut = (!a.top_k && f.top_k > 0 && f.top_k < a.V) || (!a.top_p && !(f.top_p >= 1.0f));
+    const bool cut = !a.top_k && f.top_k > 0 && f.top_k < a.V;
     if (!cut) {
         const int chunks = (a.slices * a.slice_packs + kWave - 1) / kWave;
         sample_sums<E><<<dim3((chunks + kSumChunks - 1) / kSumChunks, n), kSumThreads, 0, st>>>(a);
