@@ -114,6 +114,27 @@ def host_tables():
     return _tables
 
 
+@lru_cache(maxsize=None)
+def native_calls(*names: str):
+    """``(hsn_amd._calls, the addresses of these entry points)``: the host helper that checks,
+    allocates and calls in one step, when it is built from the current source, else ``None``."""
+    if _build.host_stale("_calls") is not None:
+        return None
+    from . import _calls
+
+    lib = library()
+    return (_calls, *(ctypes.cast(getattr(lib, name), c_void_p).value for name in names))
+
+
+def called(out, name: str):
+    """What a native call returned: its outputs (``None``: it declined the arguments); a status
+    raises as :func:`call` does."""
+    if type(out) is int:
+        message = library().hsn_win_last_error().decode(errors="replace")
+        raise RuntimeError(f"{name}: {STATUS.get(out, out)}: {message}")
+    return out
+
+
 @lru_cache(maxsize=1)
 def library() -> ctypes.CDLL:
     """The loaded library (built in-tree and matching its sources), else ``RuntimeError``."""

@@ -110,49 +110,64 @@ def build(verbose: bool = False, incremental: bool = False) -> Path:
     return LIBRARY
 
 
-#: The host helper module (``hsn_amd/host/tables.cpp``): the trainer's pointer tables, built with
-#: the host compiler against the installed PyTorch's headers and libraries.
-HOST_SOURCE = PKG / "host" / "tables.cpp"
-HOST_MODULE = PKG / "_tables.so"
-HOST_MANIFEST = PKG / "_tables.json"
+#: The host helper modules, built with the host compiler against the installed PyTorch's headers and
+#: libraries: the trainer's pointer tables (``hsn_amd/host/tables.cpp`` -> ``hsn_amd/_tables.so``) and
+#: the language-model operators' calls (``hsn_amd/host/calls.cpp`` -> ``hsn_amd/_calls.so``).
+HOST_MODULES = ("_tables", "_calls")
 
 
-def build_host(verbose: bool = False) -> Path:
-    """Compile ``hsn_amd/_tables.so`` (CPython extension, host code only); returns its path."""
+def _host_paths(name: str) -> tuple[Path, Path, Path]:
+    """``(source, module, manifest)`` of a host helper module."""
+    return PKG / "host" / f"{name[1:]}.cpp", PKG / f"{name}.so", PKG / f"{name}.json"
+
+
+def _build_host(name: str) -> Path:
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
+    source, module, manifest = _host_paths(name)
     torch_lib = str(Path(torch.__file__).resolve().parent / "lib")
-    tmp = HOST_MODULE.with_suffix(".so.tmp")
+    tmp = module.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-isystem{p}" for p in cpp_extension.include_paths()],
            f"-isystem{sysconfig.get_paths()['include']}",
-           str(HOST_SOURCE), "-o", str(tmp),
+           str(source), "-o", str(tmp),
            f"-L{torch_lib}", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python",
            f"-Wl,-rpath,{torch_lib}"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"host helper build failed:\n{proc.stderr[-6000:]}")
-    os.replace(tmp, HOST_MODULE)
-    HOST_MANIFEST.write_text(json.dumps({"source_sha256": _sha(HOST_SOURCE),
-                                         "module_sha256": _sha(HOST_MODULE)}, indent=1) + "\n")
+        raise RuntimeError(f"host helper build failed on {source.name}:\n{proc.stderr[-6000:]}")
+    os.replace(tmp, module)
+    manifest.write_text(json.dumps({"source_sha256": _sha(source),
+                                    "module_sha256": _sha(module)}, indent=1) + "\n")
+    return module
+
+
+def build_host(verbose: bool = False) -> list[Path]:
+    """Compile the host helper modules (CPython extensions, host code only); returns their paths."""
+    import torch  # noqa: F401  (imported once, before the threads)
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(HOST_MODULES)) as pool:
+        modules = list(pool.map(_build_host, HOST_MODULES))
     if verbose:
-        print(f"built {HOST_MODULE} ({HOST_MODULE.stat().st_size} bytes)")
-    return HOST_MODULE
+        for module in modules:
+            print(f"built {module} ({module.stat().st_size} bytes)")
+    return modules
 
 
-def host_stale() -> str | None:
-    """Why ``hsn_amd/_tables.so`` is not the build of the current source, or None."""
-    if not HOST_MODULE.is_file() or not HOST_MANIFEST.is_file():
-        return "hsn_amd/_tables.so is not built"
-    manifest = json.loads(HOST_MANIFEST.read_text())
-    if manifest.get("module_sha256") != _sha(HOST_MODULE):
-        return "hsn_amd/_tables.so differs from its build manifest"
-    if manifest.get("source_sha256") != _sha(HOST_SOURCE):
-        return "hsn_amd/host/tables.cpp changed since hsn_amd/_tables.so was built"
+def host_stale(name: str = "_tables") -> str | None:
+    """Why a host helper module is not the build of its current source, or None."""
+    source, module, manifest_path = _host_paths(name)
+    if not module.is_file() or not manifest_path.is_file():
+        return f"hsn_amd/{module.name} is not built"
+    manifest = json.loads(manifest_path.read_text())
+    if manifest.get("module_sha256") != _sha(module):
+        return f"hsn_amd/{module.name} differs from its build manifest"
+    if manifest.get("source_sha256") != _sha(source):
+        return f"hsn_amd/host/{source.name} changed since hsn_amd/{module.name} was built"
     return None
 
 

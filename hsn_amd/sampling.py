@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import addr, call, stream_of
+from ._lib import addr, call, called, native_calls, stream_of
 
 __all__ = ["MAX_TOKENS", "sample", "available"]
 
@@ -66,6 +66,13 @@ def sample(logits: Tensor, u: Tensor, *, temperature: Union[float, Tensor] = 1.0
     mass exceeds ``u``. A temperature of 0 gives the largest logit's first token. NaN counts as
     ``-inf``; a row without a logit above ``-inf`` gives -1. The settings are numbers, or tensors of
     ``n`` (``top_k`` int32, the others fp32)."""
+    native = native_calls("hsn_sample_workspace", "hsn_sample")
+    if native is not None and logits.is_cuda:
+        calls, size_at, call_at = native
+        out = called(calls.sample(size_at, call_at, stream_of(logits.device), logits, u, temperature,
+                                  top_k, top_p, min_p), "hsn_sample")
+        if out is not None:
+            return out
     if not logits.is_cuda:
         raise ValueError(f"logits are on {logits.device}: the kernels take ROCm device tensors")
     if logits.dim() != 2 or logits.dtype not in _DTYPE:

@@ -11,7 +11,9 @@ autograd node, :func:`step` one position of every running sequence.
 ``y`` and ``gate`` are ``[B, T, D]`` in fp32, bf16 or fp16; their last dimension is contiguous and
 the other two may have any stride (slices of one fused product, a transposed batch). States and
 their cotangents are fp32. Every function requires ROCm tensors and the built HIP library; there is
-no CPU path here. Nothing is kept between calls.
+no CPU path here. Nothing is kept between calls. A call's checks, allocations and launch are one step
+of the host helper ``hsn_amd._calls`` where it is built; without it, and for arguments it declines,
+the same checks run here, where each mismatch has its message.
 """
 
 from __future__ import annotations
@@ -24,7 +26,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import addr, call, stream_of
+from ._lib import addr, call, called, native_calls, stream_of
 
 __all__ = ["SPAN", "forward", "backward", "gated_scan", "GatedScan", "step", "available"]
 
@@ -96,6 +98,14 @@ def forward(y: Tensor, gate: Tensor, reset: Optional[Tensor] = None, h0: Optiona
     """The recurrence over a window: ``h [B, T, D]`` in ``y``'s dtype, the end state ``h_T [B, D]``
     (fp32) and, with ``save``, ``marks``: the states :func:`backward` starts from. ``reset [B, T]``
     is bool, ``h0 [B, D]`` fp32 (``None``: no resets, zero)."""
+    native = native_calls("hsn_scan_workspace", "hsn_scan_forward")
+    if native is not None and y.is_cuda:
+        calls, size_at, call_at = native
+        out = called(calls.scan_forward(size_at, call_at, stream_of(y.device), y, gate, reset, h0,
+                                        CANDIDATES.get(candidate, -1), int(save), SPAN),
+                     "hsn_scan_forward")
+        if out is not None:
+            return {"h": out[0], "h_T": out[1], "marks": out[2]}
     shape, code, io, dev = _first(y, 3)
     B, T, D = shape
     ys, gs = _strides(y, "y", shape, io, dev), _strides(gate, "gate", shape, io, dev)
@@ -119,6 +129,14 @@ def backward(y: Tensor, gate: Tensor, marks: Tensor, reset: Optional[Tensor],
     """``(d_y, d_gate, d_h0)`` from :func:`forward`'s inputs and ``marks`` and the cotangents
     ``d_h [B, T, D]`` (``y``'s dtype) and ``d_h_T [B, D]`` (fp32), either ``None`` where absent.
     The cotangent of the state is fp32; ``d_y`` and ``d_gate`` have ``y``'s dtype."""
+    native = native_calls("hsn_scan_workspace", "hsn_scan_backward")
+    if native is not None and y.is_cuda:
+        calls, size_at, call_at = native
+        out = called(calls.scan_backward(size_at, call_at, stream_of(y.device), y, gate, marks, reset,
+                                         d_h, d_h_T, CANDIDATES.get(candidate, -1), SPAN),
+                     "hsn_scan_backward")
+        if out is not None:
+            return out
     shape, code, io, dev = _first(y, 3)
     B, T, D = shape
     ys, gs = _strides(y, "y", shape, io, dev), _strides(gate, "gate", shape, io, dev)
@@ -177,6 +195,13 @@ def step(y: Tensor, gate: Tensor, state: Tensor, *, rows: Optional[Tensor] = Non
     states are the rows ``rows [n]`` (int32, distinct; ``None``: the first ``n``) of ``state
     [S, D]`` (fp32), updated in place. Returns the new states ``h [n, D]`` in ``y``'s dtype. A row
     outside ``[0, S)`` is padding: its ``h`` is zero and no state is touched."""
+    native = native_calls("hsn_scan_step")
+    if native is not None and y.is_cuda:
+        calls, call_at = native
+        out = called(calls.scan_step(call_at, stream_of(y.device), y, gate, state, rows, reset,
+                                     CANDIDATES.get(candidate, -1)), "hsn_scan_step")
+        if out is not None:
+            return out
     shape, code, io, dev = _first(y, 2)
     n, D = shape
     ys, gs = _strides(y, "y", shape, io, dev), _strides(gate, "gate", shape, io, dev)

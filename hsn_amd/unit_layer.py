@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import addr, call, stream_of
+from ._lib import addr, call, called, native_calls, stream_of
 
 __all__ = ["MAX_TOKENS", "MAX_UNITS", "MAX_CHOSEN", "unit_layer", "available"]
 
@@ -54,6 +54,14 @@ def unit_layer(x: Tensor, router: Tensor, W1: Tensor, b1: Optional[Tensor], W2: 
     ``silu(z[:H]) z[H:]`` (``W1 [M, d_in, 2 H]``); ``W2 [M, H, d_out]``, biases optional. Everything
     has ``x``'s dtype (fp32, bf16 or fp16) and is computed in fp32; nothing is rounded before
     ``y``. ``x``'s rows may lie any distance apart."""
+    native = native_calls("hsn_units_layer_workspace", "hsn_units_layer")
+    if native is not None and x.is_cuda:
+        calls, size_at, call_at = native
+        out = called(calls.unit_layer(size_at, call_at, stream_of(x.device), x, router, W1, b1, W2, b2,
+                                      k, ACTIVATIONS.get(activation, -1), int(activation == "swiglu")),
+                     "hsn_units_layer")
+        if out is not None:
+            return out
     if not x.is_cuda:
         raise ValueError(f"x is on {x.device}: the kernels take ROCm device tensors")
     if x.dim() != 2 or x.dtype not in _DTYPE:
