@@ -70,10 +70,10 @@ Plan plan(int B, int T, int D, int tile) {
     q.tiles = (T + tile - 1) / tile;
     // 256 strips fill the GPU's compute units. Up to 8 tiles a walk is then no slower than the split
     // (backward, 256 strips in fp32: 4 tiles 34 against 40 us), from 16 on the split is faster
-    // (backward in bf16: 32 tiles 187 against 170 us). With fewer strips two tiles' walk costs less
-    // than the launch that clears the exchange's words (6 strips, forward 12.3 against 14.5 us,
-    // backward 12.0 against 15.6 us, called one by one); four tiles' costs more (22 against 15 us).
-    q.split = q.tiles > 2 && (q.strips < 256 || q.tiles > 8);
+    // (backward in bf16: 32 tiles 187 against 170 us). With fewer strips the split is faster from two
+    // tiles on, with the launch that clears its words (6 strips, two tiles: forward 12.3 against 10.0
+    // us, backward 11.2 against 9.8 us).
+    q.split = q.tiles > 1 && (q.strips < 256 || q.tiles > 8);
     const int64_t groups = (q.tiles + kGroup - 1) / kGroup;
     q.words = q.split ? 64 + (q.tiles + groups) * q.strips * kChannels : 0;
     HSN_REQUIRE(q.strips <= INT32_MAX && q.strips * (q.split ? q.tiles : 1) <= INT32_MAX,
