@@ -138,17 +138,21 @@ struct Row {
             __builtin_memcpy(&pack[n], e, 16);
         }
     }
-    // The keys of a pack's logits; NaN counts as -inf.
-    static __device__ __forceinline__ void keys(const v4u& pack, uint32_t (&k)[kVec]) {
+    // A pack's logits, and their keys; NaN counts as -inf.
+    static __device__ __forceinline__ void values(const v4u& pack, float (&l)[kVec]) {
         E e[kVec];
         __builtin_memcpy(e, &pack, 16);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-            const float l = to_f32(e[j]);
-            k[j] = l != l ? kKeyNegInf : score_key(l);
-        }
+        for (int j = 0; j < kVec; ++j) l[j] = to_f32(e[j]);
     }
-    // f(first token, keys) for packs [from, to), the workgroup's threads side by side, N loads in flight.
+    static __device__ __forceinline__ uint32_t key(float l) { return l != l ? kKeyNegInf : score_key(l); }
+    static __device__ __forceinline__ void keys(const v4u& pack, uint32_t (&k)[kVec]) {
+        float l[kVec];
+        values(pack, l);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) k[j] = key(l[j]);
+    }
+    // f(first token, pack) for packs [from, to), the workgroup's threads side by side, N loads in flight.
     template <int N, typename F>
     __device__ __forceinline__ void each(int from, int to, F&& f) const {
         for (int p = from + int(threadIdx.x); p < to; p += N * kThreads) {
@@ -157,13 +161,20 @@ struct Row {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
                 if (p + n * kThreads >= to) break;
-                uint32_t key[kVec];
-                keys(pack[n], key);
-                f(first(p + n * kThreads), key);
+                f(first(p + n * kThreads), pack[n]);
             }
         }
     }
 };
+
+// The largest of a pack's logits, NaN aside.
+template <int N>
+__device__ __forceinline__ float largest(const float (&l)[N]) {
+    float m = l[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) m = __builtin_fmaxf(m, l[j]);
+    return m;
+}
 
 // The weight of a logit by its key: e, and w as the fixed point of e.
 //
@@ -350,7 +361,9 @@ __device__ __forceinline__ Cut descend(const Row<E>& row, const Weigh& weigh, Sh
     for (int level = 1; level <= 3; ++level) {
         const int up = shifts[level - 1], shift = shifts[level], bits = up - shift;
         clear_bins(s);
-        row.template each<1>(0, row.packs, [&](int, const uint32_t (&key)[Row<E>::kVec]) {
+        row.template each<1>(0, row.packs, [&](int, const v4u& pack) {
+            uint32_t key[Row<E>::kVec];
+            Row<E>::keys(pack, key);
             for (int i = 0; i < Row<E>::kVec; ++i) {
                 if (level > 1 && key[i] >> up != prefix) continue;
                 const uint64_t w = weigh.w(key[i]);
@@ -561,15 +574,18 @@ __device__ __forceinline__ int gather(const Row<E>& row, int from, int to, Share
     __syncthreads();
     if (threadIdx.x == 0) s.n_list = 0;
     __syncthreads();
-    row.template each<kBatch>(from, to, [&](int first, const uint32_t (&key)[Row<E>::kVec]) {
-        uint32_t top = key[0];
+    const float edge = key_value(least);  // keys from `least` on are the logits from here on
+    row.template each<kBatch>(from, to, [&](int first, const v4u& pack) {
+        float l[Row<E>::kVec];
+        Row<E>::values(pack, l);
+        if (!(largest(l) >= edge)) return;
 #pragma unroll
-        for (int j = 1; j < Row<E>::kVec; ++j) top = max(top, key[j]);
-        if (top < least) return;
         for (int j = 0; j < Row<E>::kVec; ++j) {
-            if (key[j] < least || !wanted(key[j])) continue;
+            if (!(l[j] >= edge)) continue;
+            const uint32_t key = Row<E>::key(l[j]);
+            if (!wanted(key)) continue;
             const uint32_t place = atomicAdd(&s.n_list, 1u);
-            if (place < kList) s.list[place] = uint64_t(key[j]) << 32 | uint32_t(~(first + j));
+            if (place < kList) s.list[place] = uint64_t(key) << 32 | uint32_t(~(first + j));
         }
     });
     __syncthreads();
@@ -614,12 +630,17 @@ struct Plain {
 template <typename E>
 __device__ __forceinline__ void find_best(const Row<E>& row, int from, int to, Shared& s, uint32_t& mine,
                                           uint32_t& best, int& first) {
-    mine = 0, first = row.V;
-    row.template each<kBatch>(from, to, [&](int at, const uint32_t (&key)[Row<E>::kVec]) {
+    float top = -__builtin_inff();
+    first = row.V;
+    row.template each<kBatch>(from, to, [&](int at, const v4u& pack) {
+        float l[Row<E>::kVec];
+        Row<E>::values(pack, l);
+        if (!(largest(l) > top)) return;
 #pragma unroll
         for (int j = 0; j < Row<E>::kVec; ++j)
-            if (key[j] > mine) mine = key[j], first = at + j;
+            if (l[j] > top) top = l[j], first = at + j;
     });
+    mine = score_key(top);
     best = block_max(mine, s);
     // the least first token: the largest of its complement
     first = ~block_max(mine == best ? ~static_cast<uint32_t>(first) : 0, s);
@@ -765,7 +786,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
                     for (int c = tid; c * kWave < row.packs; c += kThreads)
                         here += a.sums[int64_t(i) * kChunks + c];
                 } else {
-                    row.template each<1>(0, row.packs, [&](int, const uint32_t (&key)[kVec]) {
+                    row.template each<1>(0, row.packs, [&](int, const v4u& pack) {
+                        uint32_t key[kVec];
+                        Row<E>::keys(pack, key);
 #pragma unroll
                         for (int j = 0; j < kVec; ++j) here += weigh.w(key[j]);
                     });
@@ -780,7 +803,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
     Cut cut{0, 0};
     if (cuts_k || cuts_p) {
         clear_bins(s);
-        row.template each<1>(0, row.packs, [&](int, const uint32_t (&key)[kVec]) {
+        row.template each<1>(0, row.packs, [&](int, const v4u& pack) {
+            uint32_t key[kVec];
+            Row<E>::keys(pack, key);
 #pragma unroll
             for (int j = 0; j < kVec; ++j) {
                 if (key[j] == kKeyNegInf) continue;

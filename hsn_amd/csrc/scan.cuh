@@ -20,10 +20,14 @@
 // memory. Tiles are numbered by a ticket, so that whatever a workgroup waits for belongs to one that
 // already runs and publishes without waiting for a later one: every wait ends. Pairs are folded in
 // groups of 32 tiles in a fixed order, so the bits do not depend on who arrives first. Split, the
-// same 8 x 4096 x 2048 take 97 and 170 us (4.2 and 3.9 TB/s of the 3 and 5 elements that have to move),
-// and one row of 32769 x 1024 60 us, which one walk a strip takes 1.0 ms for; at 32 x 256 x 512 in
-// fp32 the walk's 13.6 and 19.4 us are less than the split's 13.6 and 22.7 and the clearing of its words.
+// same 8 x 4096 x 2048 take 100 and 185 us (4.0 and 3.6 TB/s of the 3 and 5 elements that have to
+// move; a copy reaches 4.7), and one row of 32769 x 1024 60 us, which one walk a strip takes 1.0 ms
+// for; at 32 x 256 x 512 in fp32 the walk's 13.6 and 18.8 us are less than the split's and the clearing of its
+// words. What is left between that and a copy is a workgroup's own latencies: its ticket, its loads and
+// its wait follow one another, and the registers allow two workgroups a compute unit to overlap them.
 #pragma once
+
+#include <type_traits>
 
 #include "../../include/hsn_scan.h"
 #include "common.cuh"
@@ -254,8 +258,8 @@ struct Tile {
 };
 
 // The thread's inclusive join over the wave's segments up to its own, from the first on (UP) or
-// from the last on.
-template <int LANES, bool UP, int V>
+// from the last on. RESETS: whether a segment of the wave may be constant.
+template <int LANES, bool UP, bool RESETS, int V>
 __device__ __forceinline__ void wave_join(float (&A)[V], float (&H)[V]) {
     const int lane = lane_id();
 #pragma unroll
@@ -265,7 +269,8 @@ __device__ __forceinline__ void wave_join(float (&A)[V], float (&H)[V]) {
         for (int v = 0; v < V; ++v) {
             const Pair o = UP ? Pair{__shfl_up(A[v], d, kWave), __shfl_up(H[v], d, kWave)}
                               : Pair{__shfl_down(A[v], d, kWave), __shfl_down(H[v], d, kWave)};
-            const Pair m = join(o, {A[v], H[v]});
+            const Pair m = RESETS ? join(o, {A[v], H[v]})
+                                  : Pair{o.A * A[v], __builtin_fmaf(A[v], o.H, H[v])};
             A[v] = has ? m.A : A[v];
             H[v] = has ? m.H : H[v];
         }
@@ -334,21 +339,30 @@ __global__ __launch_bounds__(kThreads) void forward_tiles(Args p) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) x[i][v] *= to_f32(ry[i].e[v]);
         }
+        // most waves have no reset in their segments: they skip what resets cost at every position
+        const bool any = ballot(drop != 0) != 0;
+        auto fold = [&](auto resets_too) {
+            constexpr bool R = decltype(resets_too)::value;
 #pragma unroll
-        for (int v = 0; v < V; ++v) A[v] = 1.0f, H[v] = 0.0f;
+            for (int v = 0; v < V; ++v) A[v] = 1.0f, H[v] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (drop >> i & 1)
+            for (int i = 0; i < S; ++i) {
+                if (R && (drop >> i & 1))
 #pragma unroll
-                for (int v = 0; v < V; ++v) A[v] = -1.0f, H[v] = 0.0f;
+                    for (int v = 0; v < V; ++v) A[v] = -1.0f, H[v] = 0.0f;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                A[v] *= a[i][v];
-                H[v] = __builtin_fmaf(a[i][v], H[v], x[i][v]);
+                for (int v = 0; v < V; ++v) {
+                    A[v] *= a[i][v];
+                    H[v] = __builtin_fmaf(a[i][v], H[v], x[i][v]);
+                }
             }
-        }
+            wave_join<G::kLanes, true, R, V>(A, H);
+        };
+        if (any)
+            fold(std::true_type{});
+        else
+            fold(std::false_type{});
         if (!kSplit && tile + 1 < end) load(tile + 1);
-        wave_join<G::kLanes, true, V>(A, H);
         if (lane >= kWave - G::kLanes)
 #pragma unroll
             for (int v = 0; v < V; ++v) wave_pair[buf][wave][cl * V + v] = {A[v], H[v]};
@@ -383,17 +397,23 @@ __global__ __launch_bounds__(kThreads) void forward_tiles(Args p) {
 #pragma unroll
             for (int v = 0; v < V; ++v) p.marks[(r * spans + t0 / kSpan) * p.D + ch + v] = h[v];
         P o[S];
+        auto walk = [&](auto resets_too) {
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (drop >> i & 1)
+            for (int i = 0; i < S; ++i) {
+                if (decltype(resets_too)::value && (drop >> i & 1))
 #pragma unroll
-                for (int v = 0; v < V; ++v) h[v] = 0.0f;
+                    for (int v = 0; v < V; ++v) h[v] = 0.0f;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                h[v] = __builtin_fmaf(a[i][v], h[v], x[i][v]);
-                o[i].e[v] = from_f32<E>(h[v]);
+                for (int v = 0; v < V; ++v) {
+                    h[v] = __builtin_fmaf(a[i][v], h[v], x[i][v]);
+                    o[i].e[v] = from_f32<E>(h[v]);
+                }
             }
-        }
+        };
+        if (any)
+            walk(std::true_type{});
+        else
+            walk(std::false_type{});
         store_segment<E, V, S>(o, out, p.D, t0, on ? p.T : 0);
     }
 }
@@ -496,8 +516,13 @@ __global__ __launch_bounds__(kThreads) void backward_tiles(Args p) {
                 for (int v = 0; v < V; ++v) M[v] = 0.0f;
         }
         if (!kSplit && turn + 1 < end) load(tile - 1);
-        wave_join<G::kLanes, true, V>(A, H);
-        wave_join<G::kLanes, false, V>(B, M);
+        if (ballot(drop != 0)) {
+            wave_join<G::kLanes, true, true, V>(A, H);
+            wave_join<G::kLanes, false, true, V>(B, M);
+        } else {
+            wave_join<G::kLanes, true, false, V>(A, H);
+            wave_join<G::kLanes, false, false, V>(B, M);
+        }
         if (lane >= kWave - G::kLanes)
 #pragma unroll
             for (int v = 0; v < V; ++v) wave_pair[buf][wave][cl * V + v] = {A[v], H[v]};
