@@ -7,12 +7,13 @@ namespace hsn {
 namespace scan {
 namespace {
 
+// One position of n sequences: a lane a channel, `blocks` workgroups a sequence.
 template <typename E>
 __global__ __launch_bounds__(256) void step(const E* y, int64_t y_row, const E* gate,
                                             int64_t gate_row, int candidate_kind,
                                             const int32_t* rows, const uint8_t* reset,
-                                            float* state, E* h, int S, int D) {
-    const int ch = blockIdx.x * 256 + threadIdx.x, i = blockIdx.y;
+                                            float* state, E* h, int S, int D, int blocks) {
+    const int i = blockIdx.x / blocks, ch = blockIdx.x % blocks * 256 + threadIdx.x;
     if (ch >= D) return;
     const int row = rows ? rows[i] : i;
     float v = 0.0f;
@@ -42,6 +43,7 @@ void check(int B, int T, int D, int dtype, int candidate_kind) {
     HSN_REQUIRE(candidate_kind == HSN_SCAN_TANH || candidate_kind == HSN_SCAN_LINEAR,
                 HSN_ERR_INVALID_ARGUMENT, "unknown candidate");
     HSN_REQUIRE(B >= 0 && T >= 0 && D >= 1, HSN_ERR_INVALID_ARGUMENT, "B, T >= 0 and D >= 1");
+    HSN_REQUIRE(T <= 1 << 30 && D <= 1 << 30, HSN_ERR_SIZE_OVERFLOW, "T, D <= 2^30");
 }
 
 // Every word of the exchange starts at 0 (a kernel, so that the call may be captured).
@@ -194,11 +196,13 @@ extern "C" int hsn_scan_step(const void* y, int64_t y_row, const void* gate, int
     if (n == 0) return HSN_OK;
     HSN_REQUIRE(y && gate && h && (state || S == 0), HSN_ERR_INVALID_ARGUMENT,
                 "a required pointer is NULL");
+    const int64_t blocks = (int64_t(D) + 255) / 256;
+    HSN_REQUIRE(n * blocks <= INT32_MAX, HSN_ERR_SIZE_OVERFLOW, "too many channels for one grid");
     by_dtype(dtype, [&](auto e) {
         using E = decltype(e);
-        step<E><<<dim3((D + 255) / 256, n), 256, 0, as_stream(stream)>>>(
+        step<E><<<static_cast<uint32_t>(n * blocks), 256, 0, as_stream(stream)>>>(
             static_cast<const E*>(y), y_row, static_cast<const E*>(gate), gate_row, candidate_kind,
-            rows, reset, state, static_cast<E*>(h), S, D);
+            rows, reset, state, static_cast<E*>(h), S, D, static_cast<int>(blocks));
     });
     HSN_HIP(hipGetLastError());
     HSN_ABI_END

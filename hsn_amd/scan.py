@@ -24,6 +24,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import addr, call, called, native_calls, stream_of
@@ -170,6 +171,7 @@ class GatedScan(torch.autograd.Function):
         return out["h"], out["h_T"]
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_h, d_h_T):
         y, gate, reset, marks = ctx.saved_tensors
         if d_h is None and d_h_T is None:

@@ -40,6 +40,7 @@ def test_scan_refusals(lib):
     assert _scan_forward(lib, T=4000) == 1 and "workspace" in message()
     assert _scan_forward(lib, T=4000, ws=8, n=1 << 30) == 1 and "aligned" in message()
     assert _scan_forward(lib, B=0) == 0
+    assert _scan_forward(lib, T=(1 << 30) + 1) == 5 and _scan_forward(lib, D=(1 << 30) + 1) == 5
     assert lib.hsn_scan_backward(64, 64, 64, 64, 64, 64, 0, 0, None, None, 64, 64, 64, None, 64, 64, 64,
                                  1, 8, 64, None, 0, None) == 1  # no marks
     assert lib.hsn_scan_step(64, 64, 64, 64, 0, 0, None, None, 64, 64, 5, 4, 64, None) == 1

@@ -303,6 +303,33 @@ def test_step(cuda_device, io, n, S, D, candidate):
             assert torch.equal(pool[row].cpu(), state[row])
 
 
+def test_step_of_many_sequences(cuda_device):
+    """More sequences than one dimension of a grid holds workgroups."""
+    from hsn_amd import scan
+
+    n, D = 70001, 3
+    g = torch.Generator().manual_seed(1)
+    y, gate = torch.randn(n, D, generator=g), torch.randn(n, D, generator=g)
+    state = torch.randn(n, D, generator=g)
+    pool = state.to(cuda_device)
+    h = scan.step(y.to(cuda_device), gate.to(cuda_device), pool)
+    b = torch.sigmoid(gate.double())
+    want = state.double() + b * (torch.tanh(y.double()) - state.double())
+    _check(h, want)
+    _check(pool, want)
+
+
+def test_a_second_derivative_is_refused(cuda_device):
+    from hsn_amd import scan
+
+    y, gate, _, _, _, _ = _problem(1, 20, 4, torch.float32, cuda_device, 0.0)
+    y.requires_grad_()
+    h, _ = scan.gated_scan(y, gate)
+    (d,) = torch.autograd.grad((h * h).sum(), [y], create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
+
+
 def test_step_by_step_is_the_scan(cuda_device):
     """Decoding position by position gives the window's states (the same arithmetic; the scan joins
     spans, so the last bits may differ)."""
