@@ -6,6 +6,9 @@ HIP kernels for MI355X (gfx950), behind the reference's operator interface.
   autograd node with the carried state.
 - :mod:`hsn_amd.kernels.window`, :mod:`hsn_amd.kernels.ops`: drop-in mirrors of the reference's
   ``hsn.kernels.window`` and ``hsn.kernels.ops``.
+- :mod:`hsn_amd.scan`, :mod:`hsn_amd.unit_layer`, :mod:`hsn_amd.sampling`: the gated linear
+  recurrence over whole sequences, a layer of routed units for a few tokens, and the choice of a
+  token, for a recurrent language model's training and answers.
 - :mod:`hsn_amd.workload`: the benchmark's seeded synthetic windows and byte model.
 
 Importing the package initialises no GPU and loads no library; the first operator call does,

@@ -2,9 +2,10 @@
 
 ``python -m hsn_amd.build`` (or ``__graft_entry__.build()``) compiles every source under
 ``hsn_amd/csrc`` with ``hipcc --offload-arch=gfx950`` in parallel and links one shared library
-exporting the C ABI of ``include/hsn_window.h`` and ``include/hsn_ops.h``. A manifest
-(``hsn_amd/libhsn_amd.json``) records the SHA-256 of every source and of the library, so the
-loader can refuse a library built from other sources.
+exporting the C ABI of the headers under ``include/``. A manifest (``hsn_amd/libhsn_amd.json``)
+records the SHA-256 of every source and of the library, so the loader can refuse a library built
+from other sources. The host modules (``hsn_amd/host``: the trainer's pointer tables, the calls of the
+language-model operators) are built beside it, each with a manifest of its own.
 """
 
 from __future__ import annotations
