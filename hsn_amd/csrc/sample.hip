@@ -18,8 +18,12 @@
 //      and 10 bits), a pass over the row for each.
 //   3. without a list: the kept weights' sums in the order of tokens, 64 packs of 16 bytes at a time,
 //      then one wave's walk through the 64 packs that hold the answer.
-// What bounds a row is the instructions of one compute unit: the passes over keys are short, an exact
-// exponential and its fixed point take some 30 instructions.
+// What bounds a row is one workgroup's steps in turn, and in the passes that take exponentials its
+// instructions (an exact one and its fixed point are some 30). One row of 32000 in bf16 with top_k and
+// top_p takes 12 us, of which the list's sorts and scans are half. 64 rows of 131072 in bf16 take 33 us,
+// 12.6 of them the slices' launch; 256 rows of 200003 in fp32 96 us, 59 of them the slices', which read the
+// logits once from HBM and where there are lists once more from the last-level cache (43.9 us at a
+// copy's rate), and 25 the exponentials of the rows that top_k does not cut.
 #include <algorithm>
 #include <type_traits>
 
@@ -39,7 +43,8 @@ constexpr int kBatch = 4;
 constexpr int kBins = 2048, kList = 1024;
 constexpr int kListTop = kList / 2;  // the largest top_k that a list is tried for
 constexpr int kMostSlices = 16;
-constexpr int kSumThreads = 256, kSumChunks = 4 * kSumThreads / kWave;  // of sample_sums
+constexpr int kSumThreads = 256;  // of sample_sums
+constexpr int kAhead = 4;          // sums of 64 packs that a wave makes in one go
 constexpr float kBinScale = kBins / 27.75f;  // 2^-40 = exp(-27.726)
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // score_key(-inf)
 constexpr int kChunks = 2 * kThreads;        // sums of 64 packs: 2^18 / (64 * 4) + 1 at most
@@ -61,6 +66,8 @@ struct Args {
     uint32_t* listed;  // how many tokens the slice's list has; above kList: no list
     uint64_t* lists;
     uint64_t* sums;    // [n, kChunks] sums of 64 packs' weights
+    uint32_t* arrived; // [n] how many parts of the sums are there
+    int parts;         // workgroups a row in sample_parts; 0: sample_sums has made the sums
 };
 
 // A row's settings; NaN and 0 temperatures are greedy.
@@ -408,16 +415,22 @@ __device__ __forceinline__ uint64_t pack_sum(const Row<E>& row, int p, const v4u
     return sum;
 }
 
-// The sums of f(key, token) over 64 packs each, from chunk `from` up to `to`, a wave a sum.
-template <typename E, typename F>
+// The sums of f(key, token) over 64 packs each, from chunk `from` up to `to`, a wave a sum, the loads of
+// N in flight.
+template <int N, typename E, typename F>
 __device__ __forceinline__ void chunk_sums(const Row<E>& row, int from, int to, uint64_t* sums, F&& f) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
-    for (int c = from + wave; c < to; c += waves) {
-        v4u pack[1];
-        row.load(c * kWave + lane, 0, pack);
-        uint64_t w[Row<E>::kVec];
-        const uint64_t sum = wave_scan(pack_sum(row, c * kWave + lane, pack[0], f, w));
-        if (lane == kWave - 1) sums[c] = sum;
+    for (int c = from + wave; c < to; c += N * waves) {
+        v4u pack[N];
+        row.load(c * kWave + lane, waves * kWave, pack);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int at = c + k * waves;
+            if (at >= to) break;
+            uint64_t w[Row<E>::kVec];
+            const uint64_t sum = wave_scan(pack_sum(row, at * kWave + lane, pack[k], f, w));
+            if (lane == kWave - 1) sums[at] = sum;
+        }
     }
 }
 
@@ -429,7 +442,7 @@ __device__ __forceinline__ int walk(const Row<E>& row, Shared& s, const uint64_t
     const int chunks = (row.packs + kWave - 1) / kWave;
     __syncthreads();
     if (threadIdx.x == 0) s.found = kChunks;
-    if (!sums) chunk_sums(row, 0, chunks, s.mass, f);
+    if (!sums) chunk_sums<1>(row, 0, chunks, s.mass, f);
     __syncthreads();
     if (!sums) sums = s.mass;
     const int c0 = 2 * threadIdx.x, c1 = c0 + 1;
@@ -683,6 +696,7 @@ __global__ __launch_bounds__(kThreads) void sample_slices(Args a) {
     int first;
     find_best(row, from, to, s, mine, best, first);
     if (tid == 0) a.best[at] = best, a.first[at] = first;
+    if (tid == 0 && blockIdx.x == 0) a.arrived[i] = 0;
     if (set.greedy() || !set.lists()) return;
     const int n = best > kKeyNegInf ? gather(row, from, to, s, list_from(mine, best, set.list_top(row.packs), s),
                                               [](uint32_t) { return true; }) : 0;
@@ -698,25 +712,6 @@ __device__ __forceinline__ void best_of_slices(const Args& a, int i, uint32_t& b
     first = ~group_max<kMostSlices>(key == best ? ~token : 0);
 }
 static_assert(kMostSlices == 16, "a row of lanes holds the slices");
-
-// A part of a row's sums of 64 packs' weights, for rows that top_k does not cut: a wave four
-// sums, so that a batch with few such rows still fills the GPU (64 rows of 131072 in bf16: 16 sums a wave
-// take 32 us).
-template <typename E>
-__global__ __launch_bounds__(kSumThreads) void sample_sums(Args a) {
-    const int i = blockIdx.y;
-    const Settings set(a, i);
-    if (set.greedy() || set.cuts_k) return;
-    const Row<E> row(static_cast<const E*>(a.logits) + i * a.row, a.V);
-    uint32_t best;
-    int first;
-    best_of_slices(a, i, best, first);
-    if (best <= kKeyNegInf) return;
-    const int from = blockIdx.x * kSumChunks;
-    const int to = min((row.packs + kWave - 1) / kWave, from + kSumChunks);
-    chunk_sums(row, from, to, a.sums + int64_t(i) * kChunks,
-               Plain{Weigh(best, set.t), set.cuts_p ? 0.0f : set.min_p, first});
-}
 
 // The slices' lists as one: the tokens from the k-th largest of the threads' maxima over them on;
 // how many, or more than kList where there is no such list.
@@ -750,9 +745,8 @@ __device__ __forceinline__ int merge_lists(const Args& a, int i, int k, uint32_t
 
 // A row: from its logits, or (kSlices) from what its slices have left.
 template <typename E, bool kSlices>
-__global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
-    __shared__ Shared s;
-    const int i = blockIdx.x, tid = threadIdx.x;
+__device__ __forceinline__ void finish_row(const Args& a, Shared& s, int i) {
+    const int tid = threadIdx.x;
     const Row<E> row(static_cast<const E*>(a.logits) + i * a.row, a.V);
     constexpr int kVec = Row<E>::kVec;
     const Settings set(a, i);
@@ -863,6 +857,62 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
     if (tid == 0) a.tokens[i] = token;
 }
 
+template <typename E>
+__global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
+    __shared__ Shared s;
+    finish_row<E, false>(a, s, blockIdx.x);
+}
+
+// Part `part` of a row's sums of 64 packs' weights, kAhead a wave.
+template <typename E>
+__device__ __forceinline__ void part_sums(const Args& a, int i, int part, const Settings& set, uint32_t best,
+                                          int first) {
+    const Row<E> row(static_cast<const E*>(a.logits) + i * a.row, a.V);
+    const int chunks = kAhead * blockDim.x / kWave, from = part * chunks;
+    const int to = min((row.packs + kWave - 1) / kWave, from + chunks);
+    chunk_sums<kAhead>(row, from, to, a.sums + int64_t(i) * kChunks,
+                       Plain{Weigh(best, set.t), set.cuts_p ? 0.0f : set.min_p, first});
+}
+
+// The sums of all rows that need them: those that top_k does not cut.
+template <typename E>
+__global__ __launch_bounds__(kSumThreads) void sample_sums(Args a) {
+    const int i = blockIdx.y;
+    const Settings set(a, i);
+    if (set.greedy() || set.cuts_k) return;
+    uint32_t best;
+    int first;
+    best_of_slices(a, i, best, first);
+    if (best > kKeyNegInf) part_sums<E>(a, i, blockIdx.x, set, best, first);
+}
+
+// The rows whose slices are there. One that needs the sums has them made by `parts` workgroups, and
+// whoever comes last finishes it; no workgroup waits. Any other row is one workgroup's, at the same time.
+template <typename E>
+__global__ __launch_bounds__(kThreads) void sample_parts(Args a) {
+    __shared__ Shared s;
+    const int parts = max(a.parts, 1), i = blockIdx.x / parts, part = blockIdx.x % parts;
+    if (a.parts) {
+        const Settings set(a, i);
+        uint32_t best;
+        int first;
+        best_of_slices(a, i, best, first);
+        if (set.greedy() || set.cuts_k || best <= kKeyNegInf) {
+            if (part) return;
+        } else {
+            part_sums<E>(a, i, part, set, best, first);
+            __syncthreads();
+            if (threadIdx.x == 0)
+                s.found = __hip_atomic_fetch_add(a.arrived + i, 1u, __ATOMIC_ACQ_REL,
+                                                 __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (s.found != uint32_t(parts - 1)) return;
+            __syncthreads();
+        }
+    }
+    finish_row<E, true>(a, s, i);
+}
+
 }  // namespace
 }  // namespace sample
 }  // namespace hsn
@@ -893,6 +943,7 @@ int64_t layout(Args& a, char* base, int n, int size) {
     };
     a.lists = reinterpret_cast<uint64_t*>(take(8 * parts * kList));
     a.sums = reinterpret_cast<uint64_t*>(take(8 * int64_t(n) * kChunks));
+    a.arrived = reinterpret_cast<uint32_t*>(take(4 * int64_t(n)));
     a.best = reinterpret_cast<uint32_t*>(take(4 * parts));
     a.first = reinterpret_cast<int*>(take(4 * parts));
     a.listed = reinterpret_cast<uint32_t*>(take(4 * parts));
@@ -900,20 +951,29 @@ int64_t layout(Args& a, char* base, int n, int size) {
 }
 
 template <typename E>
-void launch(const Args& a, int n, hipStream_t st) {
+void launch(Args a, int n, hipStream_t st) {
     if (!a.slices) {
-        sample_rows<E, false><<<n, kThreads, 0, st>>>(a);
+        sample_rows<E><<<n, kThreads, 0, st>>>(a);
         return;
     }
     sample_slices<E><<<dim3(a.slices, n), kThreads, 0, st>>>(a);
-    // where the settings are the same for all rows, whether any row needs the sums is known here
+    // Where top_k is the same for all rows, whether they need the sums is known here. A few rows' are made on
+    // the way (64 rows of 131072 in bf16, some of them cut: 32.9 us a call, with a launch of their own 38.3).
+    // Many rows' workgroups would mostly find nothing to do, and a compute unit holds one of them (256
+    // rows of 200003 in fp32: 131 against 96 us).
     const hsn_sample_settings& f = a.settings;
     const bool cut = !a.top_k && f.top_k > 0 && f.top_k < a.V;
-    if (!cut) {
-        const int chunks = (a.slices * a.slice_packs + kWave - 1) / kWave;
-        sample_sums<E><<<dim3((chunks + kSumChunks - 1) / kSumChunks, n), kSumThreads, 0, st>>>(a);
+    const int chunks = (a.slices * a.slice_packs + kWave - 1) / kWave;
+    auto parts = [&](int threads) {
+        const int of = kAhead * threads / kWave;
+        return (chunks + of - 1) / of;
+    };
+    a.parts = cut ? 0 : parts(kThreads);
+    if (int64_t(n) * a.parts > 512) {
+        a.parts = 0;
+        sample_sums<E><<<dim3(parts(kSumThreads), n), kSumThreads, 0, st>>>(a);
     }
-    sample_rows<E, true><<<n, kThreads, 0, st>>>(a);
+    sample_parts<E><<<n * std::max(a.parts, 1), kThreads, 0, st>>>(a);
 }
 
 void check(int n, int V, int dtype) {

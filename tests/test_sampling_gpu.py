@@ -221,6 +221,34 @@ def test_large_vocabularies_follow_the_share(cuda_device, V, io):
         _check_share(logits[0], u, got.cpu(), t, k, p, m)
 
 
+@pytest.mark.parametrize("io,V", [("f32", 100003), ("bf16", 150001)])
+def test_a_rows_token_does_not_depend_on_the_batch(cuda_device, io, V):
+    """A row alone, in a batch of 30 and in one of 120: how the rows are spread over the GPU differs,
+    the sums are of whole numbers and may not."""
+    from hsn_amd import sampling
+
+    n = 120
+    logits, u = _rows(n, V, io, 17)
+    logits[7] = -math.inf  # a row without a token, and one with a single token
+    logits[8, 1:] = -math.inf
+    t, k, p, m = (torch.tensor(c, dtype=d).to(cuda_device) for c, d in zip(
+        zip(*[FILTERS[i % len(FILTERS)] for i in range(n)]),
+        (torch.float32, torch.int32, torch.float32, torch.float32)))
+    logits, u = logits.to(cuda_device), u.to(cuda_device)
+
+    def run(size):
+        return [x for i in range(0, n, size) for x in sampling.sample(
+            logits[i:i + size], u[i:i + size], temperature=t[i:i + size], top_k=k[i:i + size],
+            top_p=p[i:i + size], min_p=m[i:i + size]).tolist()]
+
+    alone = run(1)
+    assert run(30) == alone and run(n) == alone
+    assert alone[7] == -1 and alone[8] == 0
+    plain = [i for i in range(n) if i % len(FILTERS) == 3 and i > 8]  # a temperature and min_p
+    for i in plain[:4]:
+        _check_share(logits[i].float().cpu(), u[i:i + 1].cpu(), torch.tensor(alone[i:i + 1]), *FILTERS[3])
+
+
 def test_settings_as_numbers_and_as_rows(cuda_device):
     from hsn_amd import sampling
 
