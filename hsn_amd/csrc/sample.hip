@@ -20,7 +20,7 @@
 //      then one wave's walk through the 64 packs that hold the answer.
 // What bounds a row is one workgroup's steps in turn, and in the passes that take exponentials its
 // instructions (an exact one and its fixed point are some 30). One row of 32000 in bf16 with top_k and
-// top_p takes 12 us, of which the list's sorts and scans are half. 64 rows of 131072 in bf16 take 33 us,
+// top_p takes 12 us. 64 rows of 131072 in bf16 take 33 us,
 // 12.6 of them the slices' launch; 256 rows of 200003 in fp32 96 us, 59 of them the slices', which read the
 // logits once from HBM and where there are lists once more from the last-level cache (43.9 us at a
 // copy's rate), and 25 the exponentials of the rows that top_k does not cut.
