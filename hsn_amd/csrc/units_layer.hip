@@ -20,11 +20,12 @@
 // tokens: 173 us, the products 98.9 and 60.6 (5.4 and 4.4 TB/s). One launch for both products and the
 // sum, its workgroups waiting for one another through memory, takes 35 to 37 us for the one token.
 //
-// x enters the first product exactly. v is fp32: 16-bit weights multiply it on the 16-bit matrix cores as
-// the sum of two bf16 (16 significant bits, 2^-17 of v at most is lost; one bf16 would lose 2^-9), fp16
-// weights as two bf16 themselves (8 and 3 of their 11 bits, nothing lost), since fp16 has not the range of
-// an unscaled v and fp32 products of widened weights take four times the matrix cores' time. A
-// workgroup makes v for its rows in LDS, 512 rows at a time, with the first weights in flight.
+// x enters the first product exactly, and so does v the second. v is fp32: 16-bit weights multiply it on
+// the 16-bit matrix cores as the sum of three bf16 (8 bits each, all 24 of v's; two would lose up to 2^-16
+// of v, which shows in bf16 results as a rounding the other way here and there), fp16 weights as two bf16
+// themselves (8 and 3 of their 11 bits), since fp16 has not the range of an unscaled v and fp32 products
+// of widened weights take four times the matrix cores' time. A workgroup makes v for its rows in LDS, 512
+// rows at a time, with the first weights in flight.
 #include <algorithm>
 #include <type_traits>
 
@@ -265,6 +266,11 @@ __device__ __forceinline__ float element(v4u row, int m) {
     return to_f32(e[m]);
 }
 
+// The upper 8 significant bits of a value, which are a bf16.
+__device__ __forceinline__ float top_bits(float v) {
+    return __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+}
+
 // Column m of fp16 rows as two bf16 operands: the upper 8 bits of each and the rest.
 __device__ __forceinline__ void column_halves(const v4u (&row)[8], int m, v8bf& hi, v8bf& lo) {
     v4u h, l;
@@ -274,8 +280,7 @@ __device__ __forceinline__ void column_halves(const v4u (&row)[8], int m, v8bf& 
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             whole[k] = __float_as_uint(element<_Float16>(row[2 * i + k], m));
-            const float top = __uint_as_float(whole[k] & 0xffff0000u);
-            const float w = __uint_as_float(whole[k]);
+            const float w = __uint_as_float(whole[k]), top = top_bits(w);
             // an infinite weight is all in `hi`; a NaN stays one
             rest[k] = __builtin_fabsf(w) < __builtin_inff() ? __float_as_uint(w - top) : 0u;
         }
@@ -286,9 +291,10 @@ __device__ __forceinline__ void column_halves(const v4u (&row)[8], int m, v8bf& 
     lo = __builtin_bit_cast(v8bf, l);
 }
 
-// v in LDS: fp32, or two bf16. The rows are padded by 16 bytes, so that 16 tokens' packs lie in
-// different banks.
-template <bool kHalves>
+// v in LDS: fp32, or three bf16 with 8 of its bits each, the upper ones first. The rows are padded by
+// 16 bytes, so that 16 tokens' packs lie in different banks.
+constexpr int kParts = 3;
+template <bool kSplit>
 struct Hidden {
     float v[kTokens][kStage + 4];
     __device__ __forceinline__ void put(int t, int k, const float (&x)[8]) {
@@ -297,18 +303,22 @@ struct Hidden {
 };
 template <>
 struct Hidden<true> {
-    uint16_t hi[kTokens][kStage + 8], lo[kTokens][kStage + 8];
+    uint16_t part[kParts][kTokens][kStage + 8];
     __device__ __forceinline__ void put(int t, int k, const float (&x)[8]) {
-        v8bf h, l;
+        float rest[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            h[j] = static_cast<__bf16>(x[j]);
-            const float rest = x[j] - static_cast<float>(h[j]);
-            // an infinite v is all in hi
-            l[j] = static_cast<__bf16>(__builtin_fabsf(x[j]) < 3e38f ? rest : 0.0f);
+        for (int j = 0; j < 8; ++j) rest[j] = x[j];
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+            v4u pack;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+                pack[j / 2] = upper(__float_as_uint(rest[j]), __float_as_uint(rest[j + 1]));
+            __builtin_memcpy(&part[i][t][k], &pack, 16);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)  // an infinite v is all in the first part
+                rest[j] = __builtin_fabsf(rest[j]) < __builtin_inff() ? rest[j] - top_bits(rest[j]) : 0.0f;
         }
-        __builtin_memcpy(&hi[t][k], &h, 16);
-        __builtin_memcpy(&lo[t][k], &l, 16);
     }
 };
 
@@ -422,22 +432,24 @@ __global__ __launch_bounds__(kThreads, 2) void product(Args a) {
                     for (int m = 0; m < kCols; ++m)
                         acc[m] = mfma(left[j], element<E>(row[j], m), acc[m]);
             } else if constexpr (kDown) {
-                v8bf hi, lo;
-                __builtin_memcpy(&hi, &lds.hidden.hi[t][k - stage], 16);
-                __builtin_memcpy(&lo, &lds.hidden.lo[t][k - stage], 16);
+                v8bf v[kParts];
+#pragma unroll
+                for (int i = 0; i < kParts; ++i)
+                    __builtin_memcpy(&v[i], &lds.hidden.part[i][t][k - stage], 16);
 #pragma unroll
                 for (int m = 0; m < kCols; ++m) {
                     if constexpr (kBf16) {
                         const v8bf w = column<v8bf>(row, m);
-                        acc[m] = mfma(lo, w, acc[m]);
-                        acc[m] = mfma(hi, w, acc[m]);
+#pragma unroll
+                        for (int i = kParts - 1; i >= 0; --i) acc[m] = mfma(v[i], w, acc[m]);
                     } else {
                         v8bf w, rest;
                         column_halves(row, m, w, rest);
-                        acc[m] = mfma(lo, rest, acc[m]);
-                        acc[m] = mfma(lo, w, acc[m]);
-                        acc[m] = mfma(hi, rest, acc[m]);
-                        acc[m] = mfma(hi, w, acc[m]);
+#pragma unroll
+                        for (int i = kParts - 1; i >= 0; --i) {
+                            acc[m] = mfma(v[i], rest, acc[m]);
+                            acc[m] = mfma(v[i], w, acc[m]);
+                        }
                     }
                 }
             } else {

@@ -9,8 +9,7 @@
  * x [n, d_in], router [M, d_in], W1 [M, d_in, H1], b1 [M, H1], W2 [M, H, d_out], b2 [M, d_out] and
  * y [n, d_out] are in `dtype` (HSN_DTYPE_F32, _F16 or _BF16), dense and row-major but for x, whose
  * rows are x_row elements apart; b1 and b2 may be NULL. The weights have the unit bank's layout
- * ([in, out], hsn_ops.h). Products are summed in fp32 and nothing is rounded to 16 bits before y, but
- * v enters its product with 16-bit weights with 16 significant bits (the sum of two bf16).
+ * ([in, out], hsn_ops.h). Products are summed in fp32 and nothing is rounded to 16 bits before y.
  * 1 <= K <= min(M, HSN_UNITS_MAX_CHOSEN), M <= HSN_UNITS_MAX, n <= HSN_UNITS_MAX_TOKENS.
  *
  * workspace: hsn_units_layer_workspace() bytes of device memory, 16-byte aligned; its contents do

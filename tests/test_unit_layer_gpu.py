@@ -216,3 +216,30 @@ def test_refusals(cuda_device):
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("activation", ["gelu", "swiglu"])
+def test_hidden_values_keep_their_bits(cuda_device, io, activation):
+    """Two hidden values of 32 whose 20th significant bit differs, with the weights 1 and -1: the result
+    is that bit. Every product and sum here is exact in fp32 (gelu(32) and silu(32) are 32), so no
+    rounding is allowed for."""
+    from hsn_amd.unit_layer import unit_layer
+
+    dt = IO[io]
+    x = torch.ones(1, 3, dtype=dt)
+    router = torch.ones(1, 3, dtype=dt)
+    W1 = torch.zeros(1, 3, 2 if activation == "gelu" else 4)
+    if activation == "gelu":  # v = 32 + 2^-4 + 2^-14 and 32 + 2^-4
+        W1[0, :, 0] = torch.tensor([32.0, 2.0 ** -4, 2.0 ** -14])
+        W1[0, :, 1] = torch.tensor([32.0, 2.0 ** -4, 0.0])
+    else:  # v = 32 (1 + 2^-9 + 2^-19) and 32 (1 + 2^-9)
+        W1[0, 0, :2] = 32.0
+        W1[0, :, 2] = torch.tensor([1.0, 2.0 ** -9, 2.0 ** -19])
+        W1[0, :, 3] = torch.tensor([1.0, 2.0 ** -9, 0.0])
+    W2 = torch.ones(1, 2, 24)
+    W2[0, 1] = -1.0
+    p = [t.to(dt).to(cuda_device) for t in (x, router, W1, W2)]
+    assert float(p[2].float().cpu().sub(W1).abs().max()) == 0.0
+    got = unit_layer(p[0], p[1], p[2], None, p[3], None, 1, activation=activation)
+    assert bool((got.float() == 2.0 ** -14).all()), got
