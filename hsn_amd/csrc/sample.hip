@@ -415,8 +415,8 @@ __device__ __forceinline__ uint64_t pack_sum(const Row<E>& row, int p, const v4u
     return sum;
 }
 
-// The sums of f(key, token) over 64 packs each, from chunk `from` up to `to`, a wave a sum, the loads of
-// N in flight.
+// The sums of f(key, token) over 64 packs each, from chunk `from` up to `to` (`sums`: the first one's
+// place), a wave a sum, the loads of N in flight.
 template <int N, typename E, typename F>
 __device__ __forceinline__ void chunk_sums(const Row<E>& row, int from, int to, uint64_t* sums, F&& f) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
@@ -429,7 +429,7 @@ __device__ __forceinline__ void chunk_sums(const Row<E>& row, int from, int to, 
             if (at >= to) break;
             uint64_t w[Row<E>::kVec];
             const uint64_t sum = wave_scan(pack_sum(row, at * kWave + lane, pack[k], f, w));
-            if (lane == kWave - 1) sums[at] = sum;
+            if (lane == kWave - 1) sums[at - from] = sum;
         }
     }
 }
@@ -863,14 +863,12 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Args a) {
     finish_row<E, false>(a, s, blockIdx.x);
 }
 
-// Part `part` of a row's sums of 64 packs' weights, kAhead a wave.
+// A row's sums of 64 packs' weights, chunks [from, to) of them, to `sums`.
 template <typename E>
-__device__ __forceinline__ void part_sums(const Args& a, int i, int part, const Settings& set, uint32_t best,
-                                          int first) {
+__device__ __forceinline__ void part_sums(const Args& a, int i, int from, int to, uint64_t* sums,
+                                          const Settings& set, uint32_t best, int first) {
     const Row<E> row(static_cast<const E*>(a.logits) + i * a.row, a.V);
-    const int chunks = kAhead * blockDim.x / kWave, from = part * chunks;
-    const int to = min((row.packs + kWave - 1) / kWave, from + chunks);
-    chunk_sums<kAhead>(row, from, to, a.sums + int64_t(i) * kChunks,
+    chunk_sums<kAhead>(row, from, min((row.packs + kWave - 1) / kWave, to), sums,
                        Plain{Weigh(best, set.t), set.cuts_p ? 0.0f : set.min_p, first});
 }
 
@@ -883,11 +881,17 @@ __global__ __launch_bounds__(kSumThreads) void sample_sums(Args a) {
     uint32_t best;
     int first;
     best_of_slices(a, i, best, first);
-    if (best > kKeyNegInf) part_sums<E>(a, i, blockIdx.x, set, best, first);
+    constexpr int kPart = kAhead * kSumThreads / kWave;  // kAhead a wave
+    const int from = blockIdx.x * kPart;
+    if (best > kKeyNegInf)
+        part_sums<E>(a, i, from, from + kPart, a.sums + int64_t(i) * kChunks + from, set, best, first);
 }
 
 // The rows whose slices are there. One that needs the sums has them made by `parts` workgroups, and
 // whoever comes last finishes it; no workgroup waits. Any other row is one workgroup's, at the same time.
+// A workgroup's sums go through LDS to its first wave, which stores them, releases them to the device and
+// counts: the reader may sit behind another L2, and a wave's release waits for its own stores only. (Sums
+// stored by every wave need a release by every wave: 64 rows of 131072 in bf16 37.6 us.)
 template <typename E>
 __global__ __launch_bounds__(kThreads) void sample_parts(Args a) {
     __shared__ Shared s;
@@ -900,11 +904,19 @@ __global__ __launch_bounds__(kThreads) void sample_parts(Args a) {
         if (set.greedy() || set.cuts_k || best <= kKeyNegInf) {
             if (part) return;
         } else {
-            part_sums<E>(a, i, part, set, best, first);
+            constexpr int kPart = kAhead * kThreads / kWave;
+            static_assert(kPart == kWave, "a part's sums, a lane each");
+            const int from = part * kPart, lane = threadIdx.x;
+            part_sums<E>(a, i, from, from + kPart, s.mass, set, best, first);
             __syncthreads();
-            if (threadIdx.x == 0)
-                s.found = __hip_atomic_fetch_add(a.arrived + i, 1u, __ATOMIC_ACQ_REL,
-                                                 __HIP_MEMORY_SCOPE_AGENT);
+            if (lane < kWave) {
+                const Row<E> row(static_cast<const E*>(a.logits) + i * a.row, a.V);
+                if ((from + lane) * kWave < row.packs) a.sums[int64_t(i) * kChunks + from + lane] = s.mass[lane];
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+                if (lane == 0)
+                    s.found = __hip_atomic_fetch_add(a.arrived + i, 1u, __ATOMIC_ACQ_REL,
+                                                     __HIP_MEMORY_SCOPE_AGENT);
+            }
             __syncthreads();
             if (s.found != uint32_t(parts - 1)) return;
             __syncthreads();

@@ -77,3 +77,39 @@ def test_a_status_raises(cuda_device):
     y = torch.zeros(5, 8, device=cuda_device)
     with pytest.raises(RuntimeError, match="every sequence"):
         scan.step(y, y, torch.zeros(3, 8, device=cuda_device))
+
+
+def test_a_rows_sums_are_out_before_they_are_counted(tmp_path):
+    """The workgroups that share a row's sums count themselves by an atomic, and the last one reads
+    them all. The wave that counts waits for its own stores alone, so any other wave's have to be
+    complete at the barrier before. In the code as built (the sampling's own, from this source), no
+    store lies between the last wait for all of a wave's memory operations and that barrier, nor
+    between the last such wait and the atomic."""
+    import shutil
+    import subprocess
+
+    if build.stale() is not None:
+        pytest.skip("library not built here")
+    objdump = "/opt/rocm/llvm/bin/llvm-objdump"
+    if shutil.which(objdump) is None:
+        pytest.skip("no llvm-objdump")
+    shutil.copy(build.LIBRARY, tmp_path / "lib.so")
+    subprocess.run([objdump, "--offloading", "lib.so"], cwd=tmp_path, check=True, capture_output=True)
+    found = 0
+    for part in sorted(tmp_path.glob("lib.so.*gfx950*")):
+        if b"sample_parts" not in part.read_bytes():
+            continue
+        text = subprocess.run([objdump, "-d", "--no-show-raw-insn", str(part)], check=True,
+                              capture_output=True, text=True).stdout
+        for kernel in text.split("\n\n"):
+            if "sample_parts" not in kernel.strip().split("\n")[0]:
+                continue
+            lines = [line.split("//")[0].strip() for line in kernel.split("\n")]
+            count = next(i for i, line in enumerate(lines) if line.startswith("global_atomic_add"))
+            barrier = max(i for i in range(count) if lines[i].startswith("s_barrier"))
+            for end in (barrier, count):
+                waited = max(i for i in range(end) if "s_waitcnt" in lines[i] and "vmcnt(0)" in lines[i])
+                stores = [line for line in lines[waited:end] if "global_store" in line]
+                assert not stores, stores
+            found += 1
+    assert found == 3  # fp32, fp16, bf16
