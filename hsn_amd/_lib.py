@@ -164,6 +164,15 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name}: {STATUS.get(status, status)}: {message}")
 
 
+def call_on(device, name: str, *args) -> None:
+    """:func:`call` with ``device`` current: an entry point launches on the current device, and the
+    default stream's handle, 0, names no device."""
+    import torch
+
+    with torch.cuda.device(device):
+        call(name, *args)
+
+
 OP_FORWARD, OP_BACKWARD, OP_RECURRENCE, OP_CELL_UPDATE, OP_ROUTE = 0, 1, 2, 3, 4
 
 

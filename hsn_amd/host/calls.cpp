@@ -9,11 +9,14 @@
 //          Python, where each mismatch has its message;
 //   int    the entry point's status, not HSN_OK;
 //   else   the outputs.
+// The tensors' device is current while an entry point runs: it launches on the current device, and the
+// default stream's handle, 0, names no device.
 // Host code only: nothing here runs on a device (CPython C API, linked against the installed PyTorch).
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -115,6 +118,7 @@ PyObject* scan_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     int status = entry<int (*)(int, int, int, int, int, int64_t*)>(size_at)(B, T, D, code, 0, &bytes);
     if (status) return PyLong_FromLong(status);
     const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(y->device());
     const auto on = at::TensorOptions().device(y->device());
     const Tensor h = at::empty({B, T, D}, on.dtype(y->scalar_type()));
     const Tensor h_T = at::empty({B, D}, on.dtype(at::kFloat));
@@ -152,6 +156,7 @@ PyObject* scan_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     int status = entry<int (*)(int, int, int, int, int, int64_t*)>(size_at)(B, T, D, code, 1, &bytes);
     if (status) return PyLong_FromLong(status);
     const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(y->device());
     const auto on = at::TensorOptions().device(y->device());
     const Tensor d_y = at::empty({B, T, D}, on.dtype(y->scalar_type()));
     const Tensor d_gate = at::empty({B, T, D}, on.dtype(y->scalar_type()));
@@ -185,6 +190,7 @@ PyObject* scan_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         !dense(rows, {n}, at::kInt, y->device()) || !dense(reset, {n}, at::kBool, y->device()))
         Py_RETURN_NONE;
     const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(y->device());
     const Tensor h = at::empty({n, D}, at::TensorOptions().device(y->device()).dtype(y->scalar_type()));
     const int status = entry<int (*)(P, int64_t, P, int64_t, int, int, P, P, P, P, int, int, int, P)>(call_at)(
         y->data_ptr(), y->stride(0), gate->data_ptr(), gate->stride(0), code, candidate, address(rows),
@@ -222,6 +228,7 @@ PyObject* unit_layer(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     int status = entry<int (*)(int, int, int, int, int, int, int, int, int64_t*)>(size_at)(
         n, M, k, d_in, H, d_out, code, activation, &bytes);
     if (status) return PyLong_FromLong(status);
+    const c10::DeviceGuard current(device);
     const auto on = at::TensorOptions().device(device);
     const Tensor y = at::empty({n, d_out}, on.dtype(type));
     const Tensor ws = workspace(bytes, on);
@@ -276,6 +283,7 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     int status = entry<int (*)(int, int, int, int64_t*)>(size_at)(n, V, code, &bytes);
     if (status) return PyLong_FromLong(status);
     const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(device);
     const auto on = at::TensorOptions().device(device);
     const Tensor tokens = at::empty({n}, on.dtype(at::kLong));
     const Tensor ws = workspace(bytes, on);

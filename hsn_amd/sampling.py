@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import addr, call, called, native_calls, stream_of
+from ._lib import addr, call, call_on, called, native_calls, stream_of
 
 __all__ = ["MAX_TOKENS", "sample", "available"]
 
@@ -100,7 +100,7 @@ def sample(logits: Tensor, u: Tensor, *, temperature: Union[float, Tensor] = 1.0
     size = _workspace_bytes(n, V, code)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     tokens = torch.empty(n, dtype=torch.int64, device=dev)
-    call("hsn_sample", logits.data_ptr(), row, code, u.data_ptr(), t_at, k_at, p_at, m_at,
+    call_on(dev, "hsn_sample", logits.data_ptr(), row, code, u.data_ptr(), t_at, k_at, p_at, m_at,
          ctypes.byref(_Settings(t, k, p, m)), tokens.data_ptr(), n, V, addr(ws), size,
          stream_of(dev))
     return tokens

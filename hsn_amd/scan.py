@@ -27,7 +27,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import addr, call, called, native_calls, stream_of
+from ._lib import addr, call, call_on, called, native_calls, stream_of
 
 __all__ = ["SPAN", "forward", "backward", "gated_scan", "GatedScan", "step", "available"]
 
@@ -118,7 +118,7 @@ def forward(y: Tensor, gate: Tensor, reset: Optional[Tensor] = None, h0: Optiona
     if save:
         marks = torch.empty((B, -(-T // SPAN), D), dtype=torch.float32, device=dev)
     ws, ws_bytes = _workspace(B, T, D, code, 0, dev)
-    call("hsn_scan_forward", y.data_ptr(), ys[0], ys[1], gate.data_ptr(), gs[0], gs[1], code,
+    call_on(dev, "hsn_scan_forward", y.data_ptr(), ys[0], ys[1], gate.data_ptr(), gs[0], gs[1], code,
          _candidate(candidate), reset_at, h0_at, h.data_ptr(), h_T.data_ptr(), addr(marks), B, T, D,
          addr(ws), ws_bytes, stream_of(dev))
     return {"h": h, "h_T": h_T, "marks": marks}
@@ -149,7 +149,7 @@ def backward(y: Tensor, gate: Tensor, marks: Tensor, reset: Optional[Tensor],
     d_gate = torch.empty(shape, dtype=io, device=dev)
     d_h0 = torch.empty((B, D), dtype=torch.float32, device=dev)
     ws, ws_bytes = _workspace(B, T, D, code, 1, dev)
-    call("hsn_scan_backward", y.data_ptr(), ys[0], ys[1], gate.data_ptr(), gs[0], gs[1], code,
+    call_on(dev, "hsn_scan_backward", y.data_ptr(), ys[0], ys[1], gate.data_ptr(), gs[0], gs[1], code,
          _candidate(candidate), reset_at, marks_at, addr(d_h), ds[0], ds[1], d_h_T_at,
          d_y.data_ptr(), d_gate.data_ptr(), d_h0.data_ptr(), B, T, D, addr(ws), ws_bytes,
          stream_of(dev))
@@ -212,7 +212,7 @@ def step(y: Tensor, gate: Tensor, state: Tensor, *, rows: Optional[Tensor] = Non
     rows_at = _dense(rows, "rows", (n,), torch.int32, dev)
     reset_at = _dense(reset, "reset", (n,), torch.bool, dev)
     h = torch.empty(shape, dtype=io, device=dev)
-    call("hsn_scan_step", y.data_ptr(), ys[0], gate.data_ptr(), gs[0], code, _candidate(candidate),
+    call_on(dev, "hsn_scan_step", y.data_ptr(), ys[0], gate.data_ptr(), gs[0], code, _candidate(candidate),
          rows_at, reset_at, state_at, h.data_ptr(), n, S, D, stream_of(dev))
     return h
 

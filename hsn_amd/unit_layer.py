@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import addr, call, called, native_calls, stream_of
+from ._lib import addr, call, call_on, called, native_calls, stream_of
 
 __all__ = ["MAX_TOKENS", "MAX_UNITS", "MAX_CHOSEN", "unit_layer", "available"]
 
@@ -95,7 +95,7 @@ def unit_layer(x: Tensor, router: Tensor, W1: Tensor, b1: Optional[Tensor], W2: 
     y = torch.empty((n, d_out), dtype=io, device=dev)
     size = _workspace_bytes(n, M, k, d_in, H, d_out, code, act)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    call("hsn_units_layer", x.data_ptr(), row, router.data_ptr(), W1.data_ptr(), addr(b1),
+    call_on(dev, "hsn_units_layer", x.data_ptr(), row, router.data_ptr(), W1.data_ptr(), addr(b1),
          W2.data_ptr(), addr(b2), y.data_ptr(), n, M, k, d_in, H, d_out, code, act, ws.data_ptr(),
          size, stream_of(dev))
     return y
