@@ -21,6 +21,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <initializer_list>
 
 namespace {
 
@@ -85,6 +86,14 @@ bool dense(const Tensor* t, at::IntArrayRef shape, at::ScalarType type, at::Devi
 bool like(const Tensor* t, const Tensor& y) {
     return t && t->scalar_type() == y.scalar_type() && t->device() == y.device() && t->sizes() == y.sizes() &&
            plain(*t) && (t->stride(-1) == 1 || t->size(-1) <= 1);
+}
+
+// Whether the caller wants a gradient with respect to one of these, for an operator that has none.
+bool wants_gradient(std::initializer_list<const Tensor*> of) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : of)
+        if (t && t->requires_grad()) return true;
+    return false;
 }
 
 P address(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
@@ -187,7 +196,8 @@ PyObject* scan_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     const int64_t n = y->size(0), D = y->size(1), S = state->size(0);
     if (code < 0 || candidate < 0 || n > INT32_MAX || D > INT32_MAX || S > INT32_MAX || !like(y, *y) ||
         !like(gate, *y) || !dense(state, {S, D}, at::kFloat, y->device()) ||
-        !dense(rows, {n}, at::kInt, y->device()) || !dense(reset, {n}, at::kBool, y->device()))
+        !dense(rows, {n}, at::kInt, y->device()) || !dense(reset, {n}, at::kBool, y->device()) ||
+        wants_gradient({y, gate, state}))
         Py_RETURN_NONE;
     const at::NoGradGuard no_grad;
     const c10::DeviceGuard current(y->device());
@@ -196,6 +206,8 @@ PyObject* scan_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         y->data_ptr(), y->stride(0), gate->data_ptr(), gate->stride(0), code, candidate, address(rows),
         address(reset), state->data_ptr(), h.data_ptr(), n, S, D, entry<P>(stream));
     if (status) return PyLong_FromLong(status);
+    // an update in place, as autograd sees it; an inference tensor has no version
+    if (n && !state->is_inference()) state->unsafeGetTensorImpl()->bump_version();
     return wrap(h);
     END_HANDLE_TH_ERRORS
 }
@@ -221,9 +233,7 @@ PyObject* unit_layer(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         !dense(b1, {M, H1}, type, device) || !dense(W2, {M, H, d_out}, type, device) ||
         !dense(b2, {M, d_out}, type, device))
         Py_RETURN_NONE;
-    if (at::GradMode::is_enabled())
-        for (const Tensor* t : {x, router, W1, b1, W2, b2})
-            if (t && t->requires_grad()) Py_RETURN_NONE;
+    if (wants_gradient({x, router, W1, b1, W2, b2})) Py_RETURN_NONE;
     int64_t bytes = 0;
     int status = entry<int (*)(int, int, int, int, int, int, int, int, int64_t*)>(size_at)(
         n, M, k, d_in, H, d_out, code, activation, &bytes);

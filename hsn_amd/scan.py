@@ -195,8 +195,8 @@ def step(y: Tensor, gate: Tensor, state: Tensor, *, rows: Optional[Tensor] = Non
          reset: Optional[Tensor] = None, candidate: str = "tanh") -> Tensor:
     """One position of ``n`` running sequences, without a gradient: ``y``, ``gate`` ``[n, D]``; the
     states are the rows ``rows [n]`` (int32, distinct; ``None``: the first ``n``) of ``state
-    [S, D]`` (fp32), updated in place. Returns the new states ``h [n, D]`` in ``y``'s dtype. A row
-    outside ``[0, S)`` is padding: its ``h`` is zero and no state is touched."""
+    [S, D]`` (fp32), updated in place, which autograd counts as such. Returns the new states ``h [n, D]``
+    in ``y``'s dtype. A row outside ``[0, S)`` is padding: its ``h`` is zero and no state is touched."""
     native = native_calls("hsn_scan_step")
     if native is not None and y.is_cuda:
         calls, call_at = native
@@ -211,9 +211,13 @@ def step(y: Tensor, gate: Tensor, state: Tensor, *, rows: Optional[Tensor] = Non
     state_at = _dense(state, "state", (S, D), torch.float32, dev)
     rows_at = _dense(rows, "rows", (n,), torch.int32, dev)
     reset_at = _dense(reset, "reset", (n,), torch.bool, dev)
+    if torch.is_grad_enabled() and (y.requires_grad or gate.requires_grad or state.requires_grad):
+        raise ValueError("step has no gradient: call it under torch.no_grad()")
     h = torch.empty(shape, dtype=io, device=dev)
     call_on(dev, "hsn_scan_step", y.data_ptr(), ys[0], gate.data_ptr(), gs[0], code, _candidate(candidate),
          rows_at, reset_at, state_at, h.data_ptr(), n, S, D, stream_of(dev))
+    if n and not state.is_inference():
+        torch.autograd.graph.increment_version(state)
     return h
 
 

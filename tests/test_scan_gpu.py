@@ -408,3 +408,49 @@ def test_refusals(cuda_device):
             call()
     with pytest.raises(RuntimeError):  # more sequences than states, and no rows
         scan.step(y[:, 0], gate[:, 0], state[:1])
+
+
+@pytest.fixture(params=["helper", "python"])
+def either_way(request, monkeypatch):
+    """With the host helper, and with the Python checks alone."""
+    if request.param == "python":
+        from hsn_amd import scan
+
+        monkeypatch.setattr(scan, "native_calls", lambda *names: None)
+
+
+def test_step_counts_as_an_update_in_place(cuda_device, either_way):
+    """A pool that an operation has saved for its gradient and that the step then updates is refused by
+    that operation's backward, as after any update in place; a step of no sequences updates nothing."""
+    from hsn_amd import scan
+
+    y = torch.randn(2, 8, device=cuda_device)
+    w = torch.ones(3, 8, device=cuda_device, requires_grad=True)
+    state = torch.randn(3, 8, device=cuda_device)
+    out = (w * state).sum()
+    scan.step(y[:0], y[:0], state)
+    torch.autograd.grad(out, [w], retain_graph=True)
+    version = state._version
+    scan.step(y, y, state)
+    assert state._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, [w])
+    with torch.inference_mode():  # such a pool keeps no version, and no operation saves it
+        pool = torch.zeros(2, 8, device=cuda_device)
+        scan.step(y, y, pool)
+    scan.step(y, y, pool)
+    assert bool((pool != 0).any())
+
+
+def test_step_refuses_what_needs_a_gradient(cuda_device, either_way):
+    from hsn_amd import scan
+
+    y, state = torch.randn(2, 8, device=cuda_device), torch.zeros(2, 8, device=cuda_device)
+    for which in range(3):
+        args = [y.clone(), y.clone(), state.clone()]
+        args[which].requires_grad_()
+        with pytest.raises(ValueError, match="no gradient"):
+            scan.step(*args)
+        assert bool((args[2] == 0).all())
+        with torch.no_grad():
+            assert not scan.step(*args).requires_grad
