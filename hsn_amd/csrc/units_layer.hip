@@ -24,8 +24,10 @@
 // the 16-bit matrix cores as the sum of three bf16 (8 bits each, all 24 of v's; two would lose up to 2^-16
 // of v, which shows in bf16 results as a rounding the other way here and there), fp16 weights as two bf16
 // themselves (8 and 3 of their 11 bits), since fp16 has not the range of an unscaled v and fp32 products
-// of widened weights take four times the matrix cores' time. A workgroup makes v for its rows in LDS, 512
-// rows at a time, with the first weights in flight.
+// of widened weights take four times the matrix cores' time. A value's parts have its sign and none is 0
+// unless the value is (2^-126 stands in for a part without bits), so that an infinity on either side gives
+// an infinity and not a NaN. A workgroup makes v for its rows in LDS, 512 rows at a time, with the
+// first weights in flight.
 #include <algorithm>
 #include <type_traits>
 
@@ -271,6 +273,12 @@ __device__ __forceinline__ float top_bits(float v) {
     return __uint_as_float(__float_as_uint(v) & 0xffff0000u);
 }
 
+// What is left of a value after its upper bits, or what stands in for it.
+__device__ __forceinline__ float left_bits(float from, float value) {
+    const float left = from - top_bits(from);  // NaN of an infinity
+    return __builtin_fabsf(left) > 0.0f ? left : __builtin_amdgcn_fmed3f(value, -0x1p-126f, 0x1p-126f);
+}
+
 // Column m of fp16 rows as two bf16 operands: the upper 8 bits of each and the rest.
 __device__ __forceinline__ void column_halves(const v4u (&row)[8], int m, v8bf& hi, v8bf& lo) {
     v4u h, l;
@@ -280,9 +288,8 @@ __device__ __forceinline__ void column_halves(const v4u (&row)[8], int m, v8bf& 
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             whole[k] = __float_as_uint(element<_Float16>(row[2 * i + k], m));
-            const float w = __uint_as_float(whole[k]), top = top_bits(w);
-            // an infinite weight is all in `hi`; a NaN stays one
-            rest[k] = __builtin_fabsf(w) < __builtin_inff() ? __float_as_uint(w - top) : 0u;
+            const float w = __uint_as_float(whole[k]);
+            rest[k] = __float_as_uint(left_bits(w, w));
         }
         h[i] = upper(whole[0], whole[1]);
         l[i] = upper(rest[0], rest[1]);
@@ -316,8 +323,7 @@ struct Hidden<true> {
                 pack[j / 2] = upper(__float_as_uint(rest[j]), __float_as_uint(rest[j + 1]));
             __builtin_memcpy(&part[i][t][k], &pack, 16);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)  // an infinite v is all in the first part
-                rest[j] = __builtin_fabsf(rest[j]) < __builtin_inff() ? rest[j] - top_bits(rest[j]) : 0.0f;
+            for (int j = 0; j < 8; ++j) rest[j] = left_bits(rest[j], x[j]);
         }
     }
 };

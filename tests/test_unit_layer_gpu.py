@@ -243,3 +243,37 @@ def test_hidden_values_keep_their_bits(cuda_device, io, activation):
     assert float(p[2].float().cpu().sub(W1).abs().max()) == 0.0
     got = unit_layer(p[0], p[1], p[2], None, p[3], None, 1, activation=activation)
     assert bool((got.float() == 2.0 ** -14).all()), got
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("where", ["weight", "hidden"])
+def test_an_infinity_of_a_chosen_unit_is_an_infinity(cuda_device, io, where):
+    """An infinite weight W2 gives an infinity of the hidden value's sign, whatever bits that value has
+    (one without low bits, one whose low bits round up or down, a small one); an infinite hidden
+    value one of the weight's sign. Neither is a NaN."""
+    from hsn_amd.unit_layer import unit_layer
+
+    dt, inf = IO[io], float("inf")
+    n, H, d_out = 16, 5, 20
+    W1 = torch.zeros(1, n, H)  # token i picks row i
+    x = torch.eye(n)
+    W1[0, :, 2] = torch.cat([torch.tensor([32.0, 2.0 ** -8]), torch.linspace(0.5, 3.0, n - 2)])
+    b1 = torch.zeros(1, H)
+    W2 = torch.zeros(1, H, d_out)
+    W2[0, 2, ::2], W2[0, 2, 1::2] = 3.0, -0.5
+    if where == "weight":
+        W2[0, 2, 4], W2[0, 2, 7] = inf, -inf
+    else:
+        b1[0, 2] = inf
+    p = [t.to(dt) for t in (x, torch.ones(1, n), W1, b1, W2)]
+    got = unit_layer(*(t.to(cuda_device) for t in p), None, 1).float().cpu()
+    want = L.unit_layer(*p, None, 1)
+    assert not bool(torch.isnan(want).any())
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and not bool(torch.isnan(got).any())
+    assert torch.equal(got[torch.isinf(want)].double(), want[torch.isinf(want)])
+    if where == "weight":
+        assert int(torch.isinf(want).sum()) == 2 * n
+        finite = torch.isfinite(want)
+        _check(got[finite], want[finite], dt)
+    else:
+        assert bool(torch.isinf(want).all())
