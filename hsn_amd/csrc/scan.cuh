@@ -3,7 +3,9 @@
 // A position is a map of the state, h -> a h + x with a = sigmoid(-g), x = sigmoid(g) c; maps join
 // (first (A1, H1), then (A2, H2)) to (A1 A2, A2 H1 + H2), so a span of positions is one pair, and
 // the time axis splits anywhere. A reset makes the map constant; it is marked by a negative A, so
-// that joins select the later value instead of multiplying the earlier one by zero (0 * inf).
+// that joins select the later value instead of multiplying the earlier one by zero (0 * inf). A NaN A
+// counts as constant too: a NaN gate makes the span's value NaN whatever comes in, unless, going backward,
+// a reset between the gate and the span's start drops it.
 //
 // Tile: a workgroup of 512 threads takes 64 channels of one row (128 bytes of 16-bit storage) and
 // kTile positions. A thread has V neighbouring channels (2 where the layout allows, else 1) and a
@@ -87,7 +89,8 @@ struct Pair {
     float A, H;
 };
 
-__device__ __forceinline__ bool constant(float A) { return __float_as_int(A) < 0; }
+// A sign, or a NaN of either.
+__device__ __forceinline__ bool constant(float A) { return __float_as_uint(A) > 0x7f800000u; }
 __device__ __forceinline__ float apply(Pair m, float h) {
     return constant(m.A) ? m.H : __builtin_fmaf(m.A, h, m.H);
 }
@@ -166,10 +169,10 @@ __device__ __forceinline__ uint32_t load_resets(const uint8_t* row, int t0, int 
 // The exchange of pairs between a row's tiles.
 // --------------------------------------------------------------------------------------------
 
-// A pair as one word that is never 0 (A's bits are below 0x7f800000 or negative, plus one; a NaN A
-// has a NaN H, and 0 says the same of such a map).
+// A pair as one word that is never 0 (A's bits are at most 0x7f800000 or negative, plus one; a NaN A as -0,
+// which says the same).
 __device__ __forceinline__ uint64_t pair_word(Pair m) {
-    const uint32_t a = m.A != m.A ? 0u : __float_as_uint(m.A);
+    const uint32_t a = m.A != m.A ? 0x80000000u : __float_as_uint(m.A);
     return uint64_t(a + 1) << 32 | __float_as_uint(m.H);
 }
 __device__ __forceinline__ Pair word_pair(uint64_t w) {

@@ -454,3 +454,33 @@ def test_step_refuses_what_needs_a_gradient(cuda_device, either_way):
         assert bool((args[2] == 0).all())
         with torch.no_grad():
             assert not scan.step(*args).requires_grad
+
+
+@pytest.mark.parametrize("T", [40, 3000])
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+def test_a_nan_gate_after_a_reset_stays_behind_it(cuda_device, T, io):
+    """Backward, a NaN gate makes the cotangents before it NaN only down to the next reset: the
+    positions before that reset belong to another document. The gate follows the reset in one
+    thread's segment, in one wave, in one workgroup, and in another tile."""
+    from hsn_amd import scan
+
+    y, gate, _, h0, d_h, d_h_T = _problem(1, T, 64, IO[io], cuda_device, 0.0, seed=14)
+    resets = [20] if T == 40 else [20, 700, 1400, 2000]
+    after = [2, 9, 17] if T == 40 else [2, 9, 17, 90, 250, 500]
+    reset = torch.zeros(1, T, dtype=torch.bool, device=cuda_device)
+    reset[0, resets] = True
+    for channel, far in enumerate(after):
+        for at in resets:
+            gate[0, at + far, channel] = float("nan")
+    gate[0, resets[-1], 40] = -float("nan")  # the reset's own position
+    d_h[0, -1, 41] = float("inf")
+    p = (y, gate, reset, h0, d_h, None)
+    marks = scan.forward(y, gate, reset, h0)["marks"]
+    got = scan.backward(y, gate, marks, reset, d_h, None)
+    want = L.scan_backward(*_cpu(*p))
+    for g, w, what in zip(got, want, ("d_y", "d_gate", "d_h0")):
+        assert torch.equal(torch.isfinite(g).cpu(), torch.isfinite(w)), what
+        finite = torch.isfinite(w)
+        _check(g.cpu()[finite], w[finite], g.dtype, what)
+    assert bool(torch.isfinite(got[2]).all())
+    assert bool(torch.isfinite(got[0][0, :resets[0]]).all())
