@@ -22,7 +22,8 @@ __global__ __launch_bounds__(256) void step(const E* y, int64_t y_row, const E* 
         float a, b;
         gates(to_f32(gate[i * gate_row + ch]), a, b);
         const float old = reset && reset[i] ? 0.0f : *at;
-        v = __builtin_fmaf(a, old, b * candidate<E>(to_f32(y[i * y_row + ch]), candidate_kind));
+        const float in = to_f32(y[i * y_row + ch]);
+        v = __builtin_fmaf(a, old, candidate_kind == HSN_SCAN_TANH ? b * tanh_of<E>(in) : linear_share(b) * in);
         *at = v;
     }
     h[int64_t(i) * D + ch] = from_f32<E>(v);

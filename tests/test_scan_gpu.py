@@ -484,3 +484,27 @@ def test_a_nan_gate_after_a_reset_stays_behind_it(cuda_device, T, io):
         _check(g.cpu()[finite], w[finite], g.dtype, what)
     assert bool(torch.isfinite(got[2]).all())
     assert bool(torch.isfinite(got[0][0, :resets[0]]).all())
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [1, 300])
+def test_positions_masked_by_the_lowest_value_keep_the_state(cuda_device, io, T):
+    """Masked positions hold the type's lowest value in the gate and in the linear candidate alike
+    (a mask laid over both halves of one product): their share is 0, so that candidate counts for
+    nothing, in the state as in the gradients. The definition's product is 0 there, exactly."""
+    from hsn_amd import scan
+
+    y, gate, _, h0, d_h, d_h_T = _problem(2, T, 64, IO[io], cuda_device, 0.0, seed=T)
+    masked = torch.zeros(T, dtype=torch.bool)
+    masked[::3] = True
+    low = torch.finfo(IO[io]).min
+    y[:, masked], gate[:, masked] = low, low
+    y[0, masked] = -low
+    gate[0, masked] = -float("inf")
+    out, grads = _both_ways((y, gate, None, h0, d_h, d_h_T), "linear")
+    assert float(grads[0][:, masked].abs().max()) == 0.0
+    assert float(grads[1][:, masked].abs().max()) == 0.0
+    assert torch.equal(out["h"][:, 0], h0.to(IO[io]))
+    pool = h0.clone()
+    h = scan.step(y[:, 0], gate[:, 0], pool, candidate="linear")
+    assert torch.equal(pool, h0) and torch.equal(h, h0.to(IO[io]))
