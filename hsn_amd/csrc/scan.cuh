@@ -559,7 +559,6 @@ __global__ __launch_bounds__(kThreads) void backward_tiles(Args p) {
                 h[v] = lane >= G::kLanes ? apply(m, h[v]) : h[v];
             }
         }
-        constexpr float slope = kTanh ? -1.0f : 0.0f;  // c' = 1 - c^2, or 1
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             if (drop >> i & 1)
@@ -570,7 +569,7 @@ __global__ __launch_bounds__(kThreads) void backward_tiles(Args p) {
                 const float cand = c[i][v], share = b[i][v];
                 c[i][v] = a[i][v] * share * (cand - h[v]);
                 h[v] = __builtin_fmaf(a[i][v], h[v], share * cand);
-                b[i][v] = share * __builtin_fmaf(slope * cand, cand, 1.0f);
+                if constexpr (kTanh) b[i][v] = share * __builtin_fmaf(-cand, cand, 1.0f);  // c' = 1 - c^2
             }
         }
         float mu[V];

@@ -508,3 +508,18 @@ def test_positions_masked_by_the_lowest_value_keep_the_state(cuda_device, io, T)
     pool = h0.clone()
     h = scan.step(y[:, 0], gate[:, 0], pool, candidate="linear")
     assert torch.equal(pool, h0) and torch.equal(h, h0.to(IO[io]))
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+def test_an_infinite_linear_candidate_has_a_finite_gradient(cuda_device, io):
+    """The linear candidate's derivative is 1 whatever its value: d_y of an infinite candidate is the
+    share of its cotangent."""
+    from hsn_amd import scan
+
+    y, gate, _, h0, d_h, d_h_T = _problem(1, 50, 64, IO[io], cuda_device, 0.0, seed=15)
+    y[0, 20, 3], y[0, 30, 5] = float("inf"), -float("inf")
+    marks = scan.forward(y, gate, None, h0, candidate="linear")["marks"]
+    got = scan.backward(y, gate, marks, None, d_h, d_h_T, candidate="linear")[0]
+    want = L.scan_backward(*_cpu(y, gate, None, h0, d_h, d_h_T), "linear")[0]
+    assert bool(torch.isfinite(want).all())
+    _check(got, want, IO[io])
