@@ -122,6 +122,14 @@ def _host_paths(name: str) -> tuple[Path, Path, Path]:
     return PKG / "host" / f"{name[1:]}.cpp", PKG / f"{name}.so", PKG / f"{name}.json"
 
 
+def _host_digest(source: Path) -> str:
+    """Digest of what a host helper module depends on here: its source and the C ABI's headers."""
+    h = hashlib.sha256(source.read_bytes())
+    for path in sorted((ROOT / "include").glob("*.h")):
+        h.update(path.read_bytes())
+    return h.hexdigest()
+
+
 def _build_host(name: str) -> Path:
     import sysconfig
 
@@ -142,7 +150,7 @@ def _build_host(name: str) -> Path:
     if proc.returncode != 0:
         raise RuntimeError(f"host helper build failed on {source.name}:\n{proc.stderr[-6000:]}")
     os.replace(tmp, module)
-    manifest.write_text(json.dumps({"source_sha256": _sha(source),
+    manifest.write_text(json.dumps({"source_sha256": _host_digest(source),
                                     "module_sha256": _sha(module)}, indent=1) + "\n")
     return module
 
@@ -167,8 +175,8 @@ def host_stale(name: str = "_tables") -> str | None:
     manifest = json.loads(manifest_path.read_text())
     if manifest.get("module_sha256") != _sha(module):
         return f"hsn_amd/{module.name} differs from its build manifest"
-    if manifest.get("source_sha256") != _sha(source):
-        return f"hsn_amd/host/{source.name} changed since hsn_amd/{module.name} was built"
+    if manifest.get("source_sha256") != _host_digest(source):
+        return f"hsn_amd/host/{source.name} or a header changed since hsn_amd/{module.name} was built"
     return None
 
 

@@ -23,6 +23,9 @@
 #include <cstdint>
 #include <initializer_list>
 
+#include "../../include/hsn_sample.h"
+#include "../../include/hsn_units_layer.h"
+
 namespace {
 
 using at::Tensor;
@@ -228,7 +231,8 @@ PyObject* unit_layer(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     const int code = dtype_code(type);
     const int64_t n = x->size(0), d_in = x->size(1), M = W2->size(0), H = W2->size(1), d_out = W2->size(2);
     const int64_t H1 = gated ? 2 * H : H;
-    if (code < 0 || !like(x, *x) || k < 1 || k > M || n > 64 || M > 256 || d_in > 65536 || H > 65536 ||
+    if (code < 0 || !like(x, *x) || k < 1 || k > M || k > HSN_UNITS_MAX_CHOSEN ||
+        n > HSN_UNITS_MAX_TOKENS || M > HSN_UNITS_MAX || d_in > 65536 || H > 65536 ||
         d_out > 65536 || !dense(router, {M, d_in}, type, device) || !dense(W1, {M, d_in, H1}, type, device) ||
         !dense(b1, {M, H1}, type, device) || !dense(W2, {M, H, d_out}, type, device) ||
         !dense(b2, {M, d_out}, type, device))
@@ -268,7 +272,7 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     const int code = dtype_code(logits->scalar_type());
     const auto device = logits->device();
     const int64_t n = logits->size(0), V = logits->size(1);
-    if (code < 0 || n > INT32_MAX || V < 1 || V > 262144 || !like(logits, *logits) ||
+    if (code < 0 || n > INT32_MAX || V < 1 || V > HSN_SAMPLE_MAX_TOKENS || !like(logits, *logits) ||
         !dense(u, {n}, at::kFloat, device))
         Py_RETURN_NONE;
     // a setting: a row's values in a tensor, or one number

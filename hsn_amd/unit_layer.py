@@ -20,9 +20,10 @@ from torch import Tensor
 from . import _lib
 from ._lib import addr, call, call_on, called, native_calls, stream_of
 
-__all__ = ["MAX_TOKENS", "MAX_UNITS", "MAX_CHOSEN", "unit_layer", "available"]
+__all__ = ["MAX_TOKENS", "MAX_UNITS", "MAX_CHOSEN", "MAX_WIDTH", "unit_layer", "available"]
 
 MAX_TOKENS, MAX_UNITS, MAX_CHOSEN = 64, 256, 16
+MAX_WIDTH = 65536
 ACTIVATIONS = {"gelu": 0, "swiglu": 1}
 _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16,
           torch.bfloat16: _lib.DTYPE_BF16}
@@ -82,6 +83,8 @@ def unit_layer(x: Tensor, router: Tensor, W1: Tensor, b1: Optional[Tensor], W2: 
         raise ValueError(f"k must be in [1, {min(M, MAX_CHOSEN)}], got {k}")
     if n > MAX_TOKENS or M > MAX_UNITS:
         raise ValueError(f"at most {MAX_TOKENS} tokens and {MAX_UNITS} units, got {n} and {M}")
+    if max(d_in, H, d_out) > MAX_WIDTH:
+        raise ValueError(f"widths of at most {MAX_WIDTH}, got d_in {d_in}, H {H} and d_out {d_out}")
     io, dev = x.dtype, x.device
     _weight(router, "router", (M, d_in), io, dev)
     _weight(W1, "W1", (M, d_in, H1), io, dev)

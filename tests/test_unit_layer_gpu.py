@@ -277,3 +277,21 @@ def test_an_infinity_of_a_chosen_unit_is_an_infinity(cuda_device, io, where):
         _check(got[finite], want[finite], dt)
     else:
         assert bool(torch.isinf(want).all())
+
+
+def test_refusals_are_the_same_with_and_without_the_host_helper(cuda_device, monkeypatch):
+    """More chosen units than the layer takes, where the bank has as many; wider than it takes."""
+    import hsn_amd.unit_layer as module
+
+    def refused():
+        p = [t.to(cuda_device) for t in _problem(2, 32, 4, 8, 8, 8, "f32", "gelu", True)]
+        with pytest.raises(ValueError, match="k must be in"):
+            module.unit_layer(*p, 17)
+        x, router = torch.zeros(1, 65537, device=cuda_device), torch.zeros(2, 65537, device=cuda_device)
+        W1, W2 = torch.zeros(2, 65537, 4, device=cuda_device), torch.zeros(2, 4, 4, device=cuda_device)
+        with pytest.raises(ValueError, match="65536"):
+            module.unit_layer(x, router, W1, None, W2, None, 1)
+
+    refused()
+    monkeypatch.setattr(module, "native_calls", lambda *names: None)
+    refused()
