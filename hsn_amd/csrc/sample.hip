@@ -993,6 +993,8 @@ void check(int n, int V, int dtype) {
                 HSN_ERR_UNSUPPORTED_DTYPE, "logits must be F32, F16 or BF16");
     HSN_REQUIRE(n >= 0 && V >= 1, HSN_ERR_INVALID_ARGUMENT, "n >= 0 and V >= 1");
     HSN_REQUIRE(V <= HSN_SAMPLE_MAX_TOKENS, HSN_ERR_SIZE_OVERFLOW, "at most 2^18 tokens");
+    // a workgroup a row, and a grid's dimension holds fewer than 2^32 threads
+    HSN_REQUIRE(n < (int64_t(1) << 32) / kThreads, HSN_ERR_SIZE_OVERFLOW, "fewer than 2^22 rows");
 }
 
 }  // namespace

@@ -217,7 +217,7 @@ struct ExchangeLds {
 __device__ __forceinline__ float exchange(const Args& p, ExchangeLds& lds, int k, int strip,
                                           Pair total, float start) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    uint64_t* pairs = p.box + 64 + strip * kChannels + lane;
+    uint64_t* pairs = p.box + 64 + int64_t(strip) * kChannels + lane;
     const int64_t line = int64_t(p.strips) * kChannels;
     uint64_t* prefix = pairs + p.tiles * line;
     if (wave == 0) publish(pairs + k * line, pair_word(total));

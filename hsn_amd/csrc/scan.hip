@@ -47,6 +47,13 @@ void check(int B, int T, int D, int dtype, int candidate_kind) {
     HSN_REQUIRE(T <= 1 << 30 && D <= 1 << 30, HSN_ERR_SIZE_OVERFLOW, "T, D <= 2^30");
 }
 
+// A grid's dimension holds fewer than 2^32 threads.
+uint32_t grid(int64_t blocks, int threads) {
+    HSN_REQUIRE(blocks < (int64_t(1) << 32) / threads, HSN_ERR_SIZE_OVERFLOW,
+                "too many rows and channels for one grid");
+    return static_cast<uint32_t>(blocks);
+}
+
 // Every word of the exchange starts at 0 (a kernel, so that the call may be captured).
 __global__ __launch_bounds__(256) void clear(uint4* box, int64_t n) {
     const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
@@ -79,8 +86,7 @@ Plan plan(int B, int T, int D, int tile) {
     q.split = q.tiles > 1 && (q.strips < 256 || q.tiles > 8);
     const int64_t groups = (q.tiles + kGroup - 1) / kGroup;
     q.words = q.split ? 64 + (q.tiles + groups) * q.strips * kChannels : 0;
-    HSN_REQUIRE(q.strips <= INT32_MAX && q.strips * (q.split ? q.tiles : 1) <= INT32_MAX,
-                HSN_ERR_SIZE_OVERFLOW, "too many rows and channels for one grid");
+    grid(q.strips * (q.split ? q.tiles : 1), kThreads);
     return q;
 }
 
@@ -104,7 +110,7 @@ void run(Args& p, const Plan& q, int dtype, int vec, bool back, void* workspace,
                     "the workspace must be aligned to 16 bytes");
         p.box = static_cast<uint64_t*>(workspace);
         const int64_t n = q.words / 2;
-        clear<<<static_cast<uint32_t>((n + 255) / 256), 256, 0, st>>>(
+        clear<<<grid((n + 255) / 256, 256), 256, 0, st>>>(
             reinterpret_cast<uint4*>(p.box), n);
     }
     by_dtype(dtype, [&](auto e) {
@@ -115,7 +121,7 @@ void run(Args& p, const Plan& q, int dtype, int vec, bool back, void* workspace,
 }
 
 void run_empty(const float* from, float* to, int64_t n, hipStream_t st) {
-    carry_over<<<static_cast<uint32_t>((n + 255) / 256), 256, 0, st>>>(from, to, n);
+    carry_over<<<grid((n + 255) / 256, 256), 256, 0, st>>>(from, to, n);
     HSN_HIP(hipGetLastError());
 }
 
@@ -198,10 +204,10 @@ extern "C" int hsn_scan_step(const void* y, int64_t y_row, const void* gate, int
     HSN_REQUIRE(y && gate && h && (state || S == 0), HSN_ERR_INVALID_ARGUMENT,
                 "a required pointer is NULL");
     const int64_t blocks = (int64_t(D) + 255) / 256;
-    HSN_REQUIRE(n * blocks <= INT32_MAX, HSN_ERR_SIZE_OVERFLOW, "too many channels for one grid");
+    const uint32_t all = grid(n * blocks, 256);
     by_dtype(dtype, [&](auto e) {
         using E = decltype(e);
-        step<E><<<static_cast<uint32_t>(n * blocks), 256, 0, as_stream(stream)>>>(
+        step<E><<<all, 256, 0, as_stream(stream)>>>(
             static_cast<const E*>(y), y_row, static_cast<const E*>(gate), gate_row, candidate_kind,
             rows, reset, state, static_cast<E*>(h), S, D, static_cast<int>(blocks));
     });

@@ -15,7 +15,7 @@
  *     weights exceeds floor(u W), W the kept weights' sum.
  * logits [n, V] in `dtype` (HSN_DTYPE_F32, _F16 or _BF16), rows `row` elements apart. u, temperature,
  * top_k, top_p and min_p are arrays of n on the device; each of the four settings may be NULL, and
- * then `settings` holds it for every row. tokens [n] is int64. 1 <= V <= 2^18.
+ * then `settings` holds it for every row. tokens [n] is int64. 1 <= V <= 2^18, n < 2^22.
  *
  * Nothing is allocated and nothing is kept between calls, so the call may be captured in a graph.
  * `stream` is a hipStream_t (NULL: the default stream). The call returns once the work is

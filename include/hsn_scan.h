@@ -7,7 +7,8 @@
  * Shapes: B rows, T positions, D channels. y and gate are [B, T, D] in `dtype` (HSN_DTYPE_F32,
  * _F16 or _BF16) with the last index contiguous and any row and position strides, counted in
  * elements; every other tensor is dense and row-major. reset holds 0 or 1. States (h0, h_T, marks,
- * state and their cotangents) are fp32, and everything is computed in fp32. T and D are at most 2^30.
+ * state and their cotangents) are fp32, and everything is computed in fp32. T and D are at most 2^30, and
+ * a call whose rows, channels and spans of time need more workgroups than one grid holds is refused.
  *
  * Caller-allocated outputs; nothing is allocated and nothing is kept between calls, so every call
  * may be captured in a graph. `stream` is a hipStream_t (NULL: the default stream). Functions

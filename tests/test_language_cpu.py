@@ -61,6 +61,24 @@ def test_scan_workspace(lib):
     assert lib.hsn_scan_workspace(1 << 20, 1 << 20, 64, 0, 0, ctypes.byref(size)) == 5
 
 
+def test_sizes_past_one_grid(lib):
+    """A dimension of a grid holds fewer than 2^32 threads: what needs more is refused by name."""
+    size = ctypes.c_int64(-1)
+
+    def message():
+        return lib.hsn_win_last_error().decode()
+
+    # 1024 tiles of 256 positions, 512 threads each
+    assert lib.hsn_scan_workspace((1 << 13) - 1, 1 << 18, 64, 2, 0, ctypes.byref(size)) == 0
+    assert lib.hsn_scan_workspace(1 << 13, 1 << 18, 64, 2, 0, ctypes.byref(size)) == 5
+    assert _scan_forward(lib, B=1 << 23) == 5 and "one grid" in message()
+    assert _scan_forward(lib, B=1 << 30, T=0) == 5 and "one grid" in message()
+    assert lib.hsn_scan_step(64, 64, 64, 64, 0, 0, None, None, 64, 64, 1 << 24, 1 << 24, 1, None) == 5
+    assert "one grid" in message()
+    assert _sample(lib, n=1 << 22) == 5 and "rows" in message()
+    assert lib.hsn_sample_workspace(1 << 22, 8, 0, ctypes.byref(size)) == 5
+
+
 def _units(lib, **change):
     a = dict(x=64, x_row=16, router=64, W1=64, b1=None, W2=64, b2=None, y=64, n=2, M=4, K=2, d_in=16,
              H=8, d_out=16, dtype=0, activation=0, ws=256, bytes=1 << 20)
