@@ -99,6 +99,9 @@ SIGNATURES: dict[str, list] = {
     "hsn_sample": [P, L, I, P, P, P, P, P, P, P, I, I, P, L, P],
 }
 
+#: the entry points' sizes are C ints, and ctypes would cut a larger number to its lower bits
+SIZE_LIMIT = 2 ** 31
+
 _lock = threading.Lock()
 
 

@@ -82,6 +82,8 @@ def sample(logits: Tensor, u: Tensor, *, temperature: Union[float, Tensor] = 1.0
     dev = logits.device
     if not 1 <= V <= MAX_TOKENS:
         raise ValueError(f"V must be in [1, {MAX_TOKENS}], got {V}")
+    if n >= _lib.SIZE_LIMIT:
+        raise ValueError(f"sizes are below 2^31, got {n} rows")
     row, last = logits.stride()
     if last != 1 and V > 1:
         raise ValueError("a row of logits must be contiguous")

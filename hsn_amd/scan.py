@@ -55,6 +55,8 @@ def _first(y: Tensor, dims: int) -> tuple:
                          f"{tuple(shape)}")
     if dtype not in _DTYPE:
         raise ValueError(f"y must be float32, float16 or bfloat16, got {dtype}")
+    if max(shape) >= _lib.SIZE_LIMIT:
+        raise ValueError(f"sizes are below 2^31, got {tuple(shape)}")
     return shape, _DTYPE[dtype], dtype, y.device
 
 
@@ -208,6 +210,8 @@ def step(y: Tensor, gate: Tensor, state: Tensor, *, rows: Optional[Tensor] = Non
     n, D = shape
     ys, gs = _strides(y, "y", shape, io, dev), _strides(gate, "gate", shape, io, dev)
     S = state.shape[0] if state.dim() == 2 else -1
+    if S >= _lib.SIZE_LIMIT:
+        raise ValueError(f"sizes are below 2^31, got a pool of {S} states")
     state_at = _dense(state, "state", (S, D), torch.float32, dev)
     rows_at = _dense(rows, "rows", (n,), torch.int32, dev)
     reset_at = _dense(reset, "reset", (n,), torch.bool, dev)
