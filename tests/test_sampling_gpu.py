@@ -305,3 +305,50 @@ def test_refusals(cuda_device):
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("V", [32000, 131072, 262144])
+def test_large_vocabularies_in_fp16(cuda_device, V):
+    from hsn_amd import sampling
+
+    logits, _ = _rows(1, V, "f16", V + 1)
+    u = (torch.arange(64) + 0.5) / 64
+    for n in (64, 3):  # whole rows or few slices, and many slices
+        rows = logits.expand(n, V).to(cuda_device)
+        for settings in ((1.0, 0, 1.0, 0.0), (1.0, 64, 1.0, 0.0), (0.8, 0, 0.8, 0.01), (1.0, 0, 1.0, 0.001)):
+            t, k, p, m = settings
+            got = sampling.sample(rows, u[:n].to(cuda_device), temperature=t, top_k=k, top_p=p, min_p=m)
+            _check_share(logits[0], u[:n], got.cpu(), *settings)
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V", [9500, 140000])
+@pytest.mark.parametrize("k,level", [(5700, 1.0), (5700, 2.0), (2000, 2.0), (0, 1.0), (5700, None), (0, None)])
+def test_cuts_among_thousands_of_equal_logits(cuda_device, io, V, k, level):
+    """200 tokens of 3, 3000 of 2 and 6000 of 1, anywhere in the row: top_k (above what a list holds) and
+    top_p each cut among more equal tokens than are sorted in one place. top_p lies half a token's
+    mass from its edges and u in the middle of a token's share, so fp32 decides nothing."""
+    from hsn_amd import sampling
+
+    g = torch.Generator().manual_seed(k + V)
+    row = torch.full((V,), -math.inf)
+    row[torch.randperm(V, generator=g)[:9200]] = torch.tensor([3.0] * 200 + [2.0] * 3000 + [1.0] * 6000)
+    row = row.to(IO[io])
+    p = 1.0
+    if level is not None:
+        all_kept = L.kept_tokens(row.float(), 1.0, k, 1.0, 0.0)
+        total = sum(w for _, w in all_kept)
+        inside = [i for i, (j, _) in enumerate(all_kept) if float(row[j]) == level]
+        cut = inside[len(inside) * 2 // 3]
+        p = (sum(w for _, w in all_kept[:cut]) + 0.5 * all_kept[cut][1]) / total
+    p = float(torch.tensor(p, dtype=torch.float32))
+    kept = sorted(L.kept_tokens(row.float(), 1.0, k, p, 0.0))
+    total, run, at = sum(w for _, w in kept), 0.0, []
+    for j, w in kept:
+        at.append((j, (run + 0.5 * w) / total))
+        run += w
+    picks = [at[i] for i in (0, 1, len(at) // 3, len(at) // 2, len(at) - 2, len(at) - 1)]
+    u = torch.tensor([v for _, v in picks], dtype=torch.float32)
+    rows = row.expand(len(picks), V).to(cuda_device)
+    got = sampling.sample(rows, u.to(cuda_device), top_k=k, top_p=p)
+    assert got.tolist() == [j for j, _ in picks]

@@ -523,3 +523,51 @@ def test_an_infinite_linear_candidate_has_a_finite_gradient(cuda_device, io):
     want = L.scan_backward(*_cpu(y, gate, None, h0, d_h, d_h_T), "linear")[0]
     assert bool(torch.isfinite(want).all())
     _check(got, want, IO[io])
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("candidate", ["tanh", "linear"])
+@pytest.mark.parametrize("B,T,D,reset_p,layout", [
+    (256, 300, 40, 0.05, "fused"), (64, 129, 250, 0.0, "dense"), (128, 1000, 99, 1 / 300, "dense"),
+    (300, 257, 7, 0.05, "fused"), (260, 512, 64, 1 / 100, "positions_first"), (256, 1024, 33, 0.0, "odd_start")])
+def test_a_walk_over_several_tiles(cuda_device, io, candidate, B, T, D, reset_p, layout):
+    """Rows and channels enough for the GPU and a few tiles: a workgroup walks them one after the other,
+    with the next one's loads in flight. Two to eight tiles, the last one whole, ragged or of a
+    single position, one and two channels a thread."""
+    import ctypes
+
+    from hsn_amd import _lib
+
+    size = ctypes.c_int64(-1)
+    for backward in (0, 1):  # no exchange between workgroups, and more than a tile backward and in fp32
+        _lib.call("hsn_scan_workspace", B, T, D, {"f32": 0, "f16": 1, "bf16": 2}[io], backward, ctypes.byref(size))
+        assert size.value == 0
+    assert 128 < T <= 1024
+    _both_ways(_problem(B, T, D, IO[io], cuda_device, reset_p, seed=B + D, layout=layout), candidate)
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+def test_what_a_reset_drops_in_a_walk(cuda_device, io):
+    """The walk's carry over tiles: a start state of infinity or NaN ends at the reset, forward, and a
+    cotangent of either backward."""
+    from hsn_amd import scan
+
+    B, T, D = 256, 700, 20
+    y, gate, _, h0, d_h, d_h_T = _problem(B, T, D, IO[io], cuda_device, 0.0, seed=31)
+    reset = torch.zeros(B, T, dtype=torch.bool, device=cuda_device)
+    at = torch.arange(B) * 2 + 100  # in every tile but the first and the last
+    reset[torch.arange(B), at] = True
+    before = (torch.arange(T)[None, :] < at[:, None]).to(cuda_device)
+    h0[:, 5], h0[:, 6] = float("inf"), float("nan")
+    d_h_T[:, 8], d_h_T[:, 9] = float("nan"), float("inf")
+    out = scan.forward(y, gate, reset, h0)
+    clean = scan.forward(y, gate, reset, torch.where(torch.isfinite(h0), h0, 0.0))
+    after = ~before[..., None].expand(-1, -1, D)
+    assert torch.equal(out["h"][after], clean["h"][after]) and torch.equal(out["h_T"], clean["h_T"])
+    assert bool(torch.isnan(out["h"][..., 6][before]).all())
+    got = scan.backward(y, gate, clean["marks"], reset, d_h, d_h_T)
+    want = scan.backward(y, gate, clean["marks"], reset, d_h, torch.where(torch.isfinite(d_h_T), d_h_T, 0.0))
+    rows = before[..., None].expand(-1, -1, D)
+    assert torch.equal(got[0][rows], want[0][rows]) and torch.equal(got[1][rows], want[1][rows])
+    assert torch.equal(got[2], want[2])
+    assert bool(torch.isnan(got[0][..., 8][~before]).all())

@@ -295,3 +295,15 @@ def test_refusals_are_the_same_with_and_without_the_host_helper(cuda_device, mon
     refused()
     monkeypatch.setattr(module, "native_calls", lambda *names: None)
     refused()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("like_one", [False, True])
+@pytest.mark.parametrize("activation,H,d_out", [("gelu", 1100, 1000), ("swiglu", 1024, 1032)])
+def test_hidden_values_in_several_stages(cuda_device, io, like_one, activation, H, d_out):
+    """40 units over 8 to 17 column tiles leave a workgroup all rows of W2: its hidden values pass
+    through LDS 512 at a time, two or three times, with the next weights in flight over the refill.
+    Alike, one unit has all 40 tokens, in three groups of up to 16."""
+    p = _problem(40, 40, 2, 24, H, d_out, io, activation, True, seed=H, like_one=like_one)
+    got = _run(p, 2, activation, cuda_device)
+    _check(got, L.unit_layer(*p, 2, activation), IO[io])
