@@ -571,3 +571,47 @@ def test_what_a_reset_drops_in_a_walk(cuda_device, io):
     assert torch.equal(got[0][rows], want[0][rows]) and torch.equal(got[1][rows], want[1][rows])
     assert torch.equal(got[2], want[2])
     assert bool(torch.isnan(got[0][..., 8][~before]).all())
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+def test_small_shares_are_right_to_parts_of_themselves(cuda_device, io):
+    """One position from a zero state: h = b y, so h_T / y is the share itself, d_y = b d_h_T, and its
+    complement shows in d_h0 = a d_h_T where a is small (large gates). The exponent's rounding is
+    2^-24 |g| log2(e) in base 2, that is |g| 2^-24 of the share, log2(e)'s own |g| 1.4e-8; a few
+    ulps for the rest."""
+    from hsn_amd import scan
+
+    g = torch.tensor([-0.25, -1.0, -12.0, -30.0, -69.0, -80.0]).repeat(8)
+    g = torch.cat([g, -g]).to(IO[io])
+    y = torch.linspace(0.5, 2.0, g.numel()).to(IO[io])
+    one = torch.ones(1, g.numel())
+    args = [t.reshape(1, 1, -1).to(cuda_device) for t in (y, g)]
+    out = scan.forward(*args, candidate="linear")
+    _, _, d_h0 = scan.backward(*args, out["marks"], None, None, one.to(cuda_device), candidate="linear")
+    g, y = g.double(), y.double()
+    room = g.abs() * (2.0 ** -24 + 1.4e-8) + 8 * 2.0 ** -24
+    b, a = 1 / (1 + torch.exp(-g)), 1 / (1 + torch.exp(g))
+    assert bool(((out["h_T"][0].double().cpu() / (b * y) - 1).abs() <= room).all())
+    assert bool(((d_h0[0].double().cpu() / a - 1).abs() <= room).all())
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+def test_small_candidates_are_right_to_parts_of_themselves(cuda_device, io):
+    """tanh(y) itself, from a gate of +inf: h_T = tanh(y). From the limit on it is 1 - 2 / (1 + e): the
+    exponential, the sum and the reciprocal are off by 2.5 ulps of 1/2 together, twice that and the
+    last rounding 2.7e-7 of 1. Below the limit the series' next term (17 y^7 / 315 in fp32, y^3 / 3 in
+    16 bits) and four roundings."""
+    from hsn_amd import scan
+
+    y = torch.cat([torch.logspace(-6, 0.5, 256), torch.tensor([0.125, 0.1249, 0.0078125, 0.0078])])
+    y = torch.cat([y, -y]).to(IO[io])
+    gate = torch.full_like(y, float("inf"))
+    args = [t.reshape(1, 1, -1).to(cuda_device) for t in (y, gate)]
+    got = scan.forward(*args, save=False)["h_T"][0].double().cpu()
+    want = torch.tanh(y.double())
+    off = (got / want - 1).abs()
+    if io == "f32":
+        room = torch.where(y.abs() < 0.125, 17 / 315 * y.double() ** 6 + 4 * 2.0 ** -24, 2.7e-7 / want.abs())
+    else:
+        room = torch.where(y.abs() < 0.0078125, y.double() ** 2 / 3 + 2.0 ** -24, 2.7e-7 / want.abs())
+    assert bool((off <= room).all()), float(off.max())
