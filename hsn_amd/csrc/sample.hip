@@ -22,8 +22,8 @@
 // instructions (an exact one and its fixed point are some 30). One row of 32000 in bf16 with top_k and
 // top_p takes 12 us. 64 rows of 131072 in bf16 take 33 us,
 // 12.6 of them the slices' launch; 256 rows of 200003 in fp32 96 us, 59 of them the slices', which read the
-// logits once from HBM and where there are lists once more from the last-level cache (43.9 us at a
-// copy's rate), and 25 the exponentials of the rows that top_k does not cut.
+// logits once from HBM and where there are lists once more from the last-level cache (38.5 us at a
+// copy's 5.3 TB/s), and 25 the exponentials of the rows that top_k does not cut.
 #include <algorithm>
 #include <type_traits>
 
@@ -970,7 +970,7 @@ void launch(Args a, int n, hipStream_t st) {
     }
     sample_slices<E><<<dim3(a.slices, n), kThreads, 0, st>>>(a);
     // Where top_k is the same for all rows, whether they need the sums is known here. A few rows' are made on
-    // the way (64 rows of 131072 in bf16, some of them cut: 32.9 us a call, with a launch of their own 38.3).
+    // the way (64 rows of 131072 in bf16, some of them cut: 33.5 us a call, with a launch of their own 38.3).
     // Many rows' workgroups would mostly find nothing to do, and a compute unit holds one of them (256
     // rows of 200003 in fp32: 131 against 96 us).
     const hsn_sample_settings& f = a.settings;

@@ -22,9 +22,9 @@
 // memory. Tiles are numbered by a ticket, so that whatever a workgroup waits for belongs to one that
 // already runs and publishes without waiting for a later one: every wait ends. Pairs are folded in
 // groups of 32 tiles in a fixed order, so the bits do not depend on who arrives first. Split, the
-// same 8 x 4096 x 2048 take 100 and 185 us (4.0 and 3.6 TB/s of the 3 and 5 elements that have to
-// move; a copy reaches 4.7), and one row of 32769 x 1024 60 us, which one walk a strip takes 1.0 ms
-// for; at 32 x 256 x 512 in fp32 the walk's 13.6 and 18.8 us are less than the split's and the clearing of its
+// same 8 x 4096 x 2048 take 104 and 184 us (3.9 and 3.6 TB/s of the 3 and 5 elements that have to
+// move; a copy reaches 5.3), and one row of 32769 x 1024 64 us, which one walk a strip takes 1.0 ms
+// for; at 32 x 256 x 512 in fp32 the walk's 13.5 and 19.5 us are less than the split's and the clearing of its
 // words. What is left between that and a copy is a workgroup's own latencies: its ticket, its loads and
 // its wait follow one another, and the registers allow two workgroups a compute unit to overlap them.
 #pragma once
@@ -60,7 +60,7 @@ struct Args {
 // e/(1+e) with e = exp(-g), neither a difference from 1 (1 - b would leave nothing of a small a). The
 // exponent's rounding and that of log2(e) leave e right to 1.25 |g| 2^-24 of itself, so a small share is
 // right to that and a few ulps (7.5e-7 at |g| = 10, 4.5e-6 at 60); the product in two parts takes 3% more
-// time (8 x 4096 x 2048 in bf16, forward and backward: 292 us, not 283). e stops at 2^126, so that a is 1 and b 2^-126 for every g below
+// time (8 x 4096 x 2048 in bf16, forward and backward: 288 us, not 280). e stops at 2^126, so that a is 1 and b 2^-126 for every g below
 // -87 and not inf * 0; the minimum keeps a NaN.
 __device__ __forceinline__ void gates(float g, float& a, float& b) {
     const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(-kLog2e * g, 126.0f));
@@ -72,8 +72,8 @@ __device__ __forceinline__ void gates(float g, float& a, float& b) {
 // difference of equals, the series y - y^3/3 + 2 y^5/15 (fp32 storage: below 1/8 the next term,
 // 17 y^7 / 315, is at most 2.1e-7 of y) or y alone (16-bit storage: below 1/128 it is off by at most
 // 1.6e-7 of 1, as the other form is, and 2e-5 of itself, a 24th of fp16's rounding of y and a 190th of
-// bf16's). The fp32 states of 16-bit inputs take the latter too; the series takes 3% more time there
-// (8 x 4096 x 2048 in bf16, forward and backward: 292 us, not 283).
+// bf16's). The fp32 states of 16-bit inputs take the latter too; the series takes 4% more time there
+// (8 x 4096 x 2048 in bf16, forward and backward: 292 us, not 280).
 template <typename E>
 __device__ __forceinline__ float tanh_of(float y) {
     const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * y);
@@ -645,7 +645,7 @@ void launch_backward_as(const Args& p, bool split, hipStream_t st) {
         backward_tiles<E, V, kBackwardPer / V, false, kTanh><<<p.strips, kThreads, 0, st>>>(p);
 }
 // A kernel a candidate: with both in one, the registers of the split passes in 16 bits pass 128 and a compute
-// unit holds one workgroup instead of two (8 x 4096 x 2048 forward and backward: 403 us instead of 282).
+// unit holds one workgroup instead of two (8 x 4096 x 2048 forward and backward: 403 us instead of 280).
 template <typename E, int V>
 void launch_forward_as(const Args& p, bool split, hipStream_t st) {
     p.candidate == HSN_SCAN_TANH ? launch_forward_as<E, V, true>(p, split, st)

@@ -82,7 +82,8 @@ Plan plan(int B, int T, int D, int tile) {
     // (backward, 256 strips in fp32: 4 tiles 34 against 40 us), from 16 on the split is faster
     // (backward in bf16: 32 tiles 187 against 170 us). With fewer strips the split is faster from two
     // tiles on, with the launch that clears its words (6 strips, two tiles: forward 12.3 against 10.0
-    // us, backward 11.2 against 9.8 us).
+    // us, backward 11.2 against 9.8 us). Neither way is timed between 6 and 256 strips, nor between 4 and
+    // 32 tiles but for these.
     q.split = q.tiles > 1 && (q.strips < 256 || q.tiles > 8);
     const int64_t groups = (q.tiles + kGroup - 1) / kGroup;
     q.words = q.split ? 64 + (q.tiles + groups) * q.strips * kChannels : 0;

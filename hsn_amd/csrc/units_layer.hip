@@ -15,10 +15,12 @@
 // products 16x16x32, the m-th with the columns c0 + m of the lanes. Rows are split over a workgroup's
 // waves and, where units and column tiles are few, over workgroups, so that some 512 workgroups
 // keep the loads of two steps each in flight.
-// One token, 8 of 64 gated units of 2048 x 1024 in bf16: 34 us, the products 15.8 and 11.3 (4.2 and 3.0
+// One token, 8 of 64 gated units of 2048 x 1024 in bf16: 35 us, the products 16.1 and 11.8 (4.2 and 2.8
 // TB/s); 256 workgroups a product are as fast, 1024 take 40 us, and 48 with one step a wave. 32 such
-// tokens: 173 us, the products 98.9 and 60.6 (5.4 and 4.4 TB/s). One launch for both products and the
-// sum, its workgroups waiting for one another through memory, takes 35 to 37 us for the one token.
+// tokens: 175 us, the products 100 and 61 (5.3 and 4.3 TB/s). One launch for both products and the
+// sum, its workgroups waiting for one another through memory, measured 35 to 37 us against 34.4 for the one
+// token, 13.1 against 16.0 for one of 2 of 8 units of 256 x 512 in fp32, and 31.3 against 33.4 for 5 tokens of
+// 3 of 12 units of 999 x 1234 in fp16; where it would begin to lose is not measured, and no rule takes it.
 //
 // x enters the first product exactly, and so does v the second. v is fp32: 16-bit weights multiply it on
 // the 16-bit matrix cores as the sum of three bf16 (8 bits each, all 24 of v's; two would lose up to 2^-16
@@ -600,7 +602,7 @@ int64_t layout(Args& a, const void* W1, const void* W2, char* base, int size) {
 template <typename E>
 void launch(Args a, hipStream_t st) {
     // The choice is the first product's where all tokens' units are a thread each, which saves a
-    // launch (of 4 us), else a launch of its own.
+    // kernel of 4.7 us, else a launch of its own.
     a.choose_inline = a.n * a.M <= kThreads;
     route<E><<<dim3(a.n, (a.M + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
     if (!a.choose_inline) choose<<<a.n, kThreads, 0, st>>>(a);

@@ -7,10 +7,13 @@
  * Shapes: B rows, T positions, D channels. y and gate are [B, T, D] in `dtype` (HSN_DTYPE_F32,
  * _F16 or _BF16) with the last index contiguous and any row and position strides, counted in
  * elements; every other tensor is dense and row-major. reset holds 0 or 1. States (h0, h_T, marks,
- * state and their cotangents) are fp32, and everything is computed in fp32: a share b or 1 - b to about
- * (1.25 |g| + 8) 2^-24 of itself, a tanh to 2.7e-7 and, where that is more, to 3e-6 of itself (fp32 inputs)
- * or 4e-5 (16-bit ones). T and D are at most 2^30, and
- * a call whose rows, channels and spans of time need more workgroups than one grid holds is refused.
+ * state and their cotangents) are fp32. T and D are at most 2^30, and a call whose rows, channels and
+ * spans of time need more workgroups than one grid holds is refused.
+ *
+ * Everything is computed in fp32: a share b or 1 - b is right to about (1.25 |g| + 8) 2^-24 of
+ * itself, a tanh to 2.7e-7 and to 3e-6 of itself (fp32 inputs) or 4e-5 (16-bit ones). A state that is
+ * not finite ends at the next reset; until then a NaN stays one, and an infinity stays one or, where
+ * spans are joined, becomes a NaN.
  *
  * Caller-allocated outputs; nothing is allocated and nothing is kept between calls, so every call
  * may be captured in a graph. `stream` is a hipStream_t (NULL: the default stream). Functions
