@@ -1,6 +1,7 @@
 """The C ABI of ``libhsn_amd.so`` (``include/hsn_window.h``, ``include/hsn_ops.h``,
 ``include/hsn_trainer.h``, ``include/hsn_sweep.h``, ``include/hsn_round.h``,
-``include/hsn_scan.h``, ``include/hsn_units_layer.h``, ``include/hsn_sample.h``) via ctypes.
+``include/hsn_scan.h``, ``include/hsn_units_layer.h``, ``include/hsn_sample.h``,
+``include/hsn_clip.h``) via ctypes.
 
 The library is the product: every operator in :mod:`hsn_amd` reaches the GPU through these
 entry points, and nothing here falls back to another implementation. :func:`library` raises a
@@ -13,7 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_void_p
 from functools import lru_cache
 
 from . import build as _build
@@ -30,7 +31,7 @@ STATUS = {
 }
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
-P, I, F, L = c_void_p, c_int, c_float, c_int64
+P, I, F, L, D = c_void_p, c_int, c_float, c_int64, c_double
 
 #: argument types of every exported entry point, in declaration order of the headers
 SIGNATURES: dict[str, list] = {
@@ -97,6 +98,8 @@ SIGNATURES: dict[str, list] = {
     "hsn_units_layer": [P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P, L, P],
     "hsn_sample_workspace": [I, I, I, P],
     "hsn_sample": [P, L, I, P, P, P, P, P, P, P, I, I, P, L, P],
+    "hsn_clip_workspace": [P, I, P],
+    "hsn_clip": [P, P, P, P, I, D, P, P, L, P],
 }
 
 #: the entry points' sizes are C ints, and ctypes would cut a larger number to its lower bits

@@ -1,5 +1,5 @@
 // The calls of a decoded token in one step from the interpreter: the language-model operators'
-// Python mirrors (hsn_amd/scan.py, unit_layer.py, sampling.py) check their tensors, allocate outputs
+// Python mirrors (hsn_amd/scan.py, unit_layer.py, sampling.py, grad_clip.py) check their tensors, allocate outputs
 // and workspace and call the C entry point through this module where it is built. Made in the
 // interpreter, the checks, allocations and the conversion of some twenty arguments cost 4 to 6 us a
 // call, more than the kernel of a single position; here they cost about 1 us.
@@ -22,6 +22,7 @@
 
 #include <cstdint>
 #include <initializer_list>
+#include <vector>
 
 #include "../../include/hsn_sample.h"
 #include "../../include/hsn_units_layer.h"
@@ -310,6 +311,76 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// A list or tuple of tensors, held while it is read.
+struct List {
+    PyObject* seq = nullptr;
+    explicit List(PyObject* o) : seq(PyList_Check(o) || PyTuple_Check(o) ? Py_NewRef(o) : nullptr) {}
+    List(const List&) = delete;
+    List& operator=(const List&) = delete;
+    ~List() { Py_XDECREF(seq); }
+    Py_ssize_t size() const { return seq ? PySequence_Fast_GET_SIZE(seq) : 0; }
+    const Tensor* at(Py_ssize_t i) const {
+        PyObject* o = PySequence_Fast_GET_ITEM(seq, i);
+        return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+    }
+};
+
+// grad_clip(workspace, clip, stream, grads, outs, max_norm): outs None: the norm and the coefficient alone
+PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Arguments in{args, args + n_args};
+    const int64_t size_at = in.integer(), call_at = in.integer(), stream = in.integer();
+    const List grads(in.next());
+    PyObject* const outs_given = in.next();
+    const List outs(outs_given);
+    const double max_norm = in.number();
+    const Py_ssize_t n = grads.size();
+    const bool writes = outs_given != Py_None;
+    if (!in.ok || n < 1 || n > INT32_MAX || (writes && outs.size() != n) || !(max_norm >= 0.0))
+        Py_RETURN_NONE;
+    std::vector<void*> at(static_cast<size_t>(2 * n));
+    std::vector<int64_t> numels(static_cast<size_t>(n));
+    std::vector<int> codes(static_cast<size_t>(n));
+    const Tensor* first = grads.at(0);
+    if (!first || !first->is_cuda()) Py_RETURN_NONE;
+    const auto device = first->device();
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const Tensor* g = grads.at(i);
+        if (!g || g->device() != device || !plain(*g) || !g->is_non_overlapping_and_dense() ||
+            wants_gradient({g}))
+            Py_RETURN_NONE;
+        codes[i] = dtype_code(g->scalar_type());
+        if (codes[i] < 0) Py_RETURN_NONE;
+        numels[i] = g->numel();
+        at[i] = g->data_ptr();
+        if (!writes) continue;
+        const Tensor* o = outs.at(i);
+        if (!o || o->device() != device || !plain(*o) || o->scalar_type() != g->scalar_type() ||
+            o->sizes() != g->sizes() || wants_gradient({o}))
+            Py_RETURN_NONE;
+        for (int64_t d = 0; numels[i] && d < g->dim(); ++d)
+            if (g->size(d) > 1 && o->stride(d) != g->stride(d)) Py_RETURN_NONE;
+        at[n + i] = o->data_ptr();
+    }
+    int64_t bytes = 0;
+    int status = entry<int (*)(const int64_t*, int, int64_t*)>(size_at)(numels.data(), n, &bytes);
+    if (status) return PyLong_FromLong(status);
+    const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(device);
+    const auto on = at::TensorOptions().device(device);
+    const Tensor result = at::empty({2}, on.dtype(at::kDouble));
+    const Tensor ws = workspace(bytes, on);
+    status = entry<int (*)(void* const*, void* const*, const int64_t*, const int*, int, double, P, P, int64_t,
+                           P)>(call_at)(at.data(), writes ? at.data() + n : nullptr, numels.data(),
+                                        codes.data(), n, max_norm, result.data_ptr(), ws.data_ptr(), bytes,
+                                        entry<P>(stream));
+    if (status) return PyLong_FromLong(status);
+    for (Py_ssize_t i = 0; writes && i < n; ++i)  // an update in place, as autograd sees it
+        if (!outs.at(i)->is_inference()) outs.at(i)->unsafeGetTensorImpl()->bump_version();
+    return Py_BuildValue("(NN)", wrap(result.narrow(0, 0, 1)), wrap(result.narrow(0, 1, 1)));
+    END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyCFunction fast() {
     return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F));
@@ -327,6 +398,8 @@ PyMethodDef kMethods[] = {
      "(workspace, layer, stream, x, router, W1, b1, W2, b2, k, activation, gated) -> y"},
     {"sample", fast<sample>(), METH_FASTCALL,
      "(workspace, sample, stream, logits, u, temperature, top_k, top_p, min_p) -> tokens"},
+    {"grad_clip", fast<grad_clip>(), METH_FASTCALL,
+     "(workspace, clip, stream, grads, outs, max_norm) -> (norm, coefficient)"},
     {nullptr, nullptr, 0, nullptr},
 };
 
