@@ -1,0 +1,553 @@
+// Log probabilities of given tokens with the entropy, the most probable alternatives and the gradient
+// (include/hsn_score.h).
+//
+// Forward: one pass over the logits. A thread keeps the running largest logit m, S = sum e^(l - m) and
+// W = sum e^(l - m) (l - m) of what it has seen, raised to a new m once a batch of packs; lanes, waves and
+// a row's parts are joined in a fixed order. Where alternatives are wanted, each wave also keeps a list
+// of candidates in LDS: what is at least as large as the k-th largest of its lanes' own largest logits so
+// far (k of the wave's logits are, so nothing below it can be among the row's k largest), which few
+// batches after the first have. A list that is full is cut to its k largest. Sorted lists of waves and
+// parts are merged by one wave, a list a lane.
+//
+// Backward: d = g ([j = t] - p) - h p (log p + H), a pack at a time from the logits and four numbers a row.
+//
+// Both are bound by memory where rows are many: the forward reads n V logits, the backward reads and
+// writes as many.
+#include <algorithm>
+
+#include "../../include/hsn_score.h"
+#include "abi_util.h"
+#include "packs.cuh"
+
+namespace hsn {
+namespace score {
+namespace {
+
+constexpr int kBatch = 4;      // packs a thread has in flight
+constexpr int kMostParts = 64;  // of a row: a lane each when they are joined
+constexpr int kList = 256;      // candidates of a wave
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kLog2 = 1.4426950408889634f;
+constexpr uint32_t kKeyNegInf = 0x007fffffu;  // score_key(-inf)
+constexpr uint64_t kNone = uint64_t(kKeyNegInf) << 32 | 0xffffffffu;  // no candidate is this small
+
+struct Args {
+    const void* logits;
+    int64_t row;
+    const void* tokens;
+    int64_t token_stride;
+    bool wide;  // 64-bit tokens
+    float *logprob, *entropy, *top_logprobs;
+    int64_t* top_tokens;
+    float4* stats;
+    int V, top, parts, part_packs;
+    float4* part_sums;     // [n, parts] m, S, W
+    uint64_t* part_lists;  // [n, parts, top]
+    // backward
+    const float *g, *h;
+    int64_t g_stride, h_stride;
+    void* d_logits;
+    __device__ __forceinline__ int64_t token(int i) const {
+        return wide ? static_cast<const int64_t*>(tokens)[i * token_stride]
+                    : static_cast<const int32_t*>(tokens)[i * token_stride];
+    }
+};
+
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2); }
+
+// m, S and W of some logits. Of none: the lowest number, 0 and 0.
+struct Sums {
+    float m = kLowest, S = 0.0f, W = 0.0f;
+    // The same sums from a reference `to` >= m. What is not finite in m and to enters S by the logits alone.
+    __device__ __forceinline__ void raise(float to) {
+        const float d = fmaxf(m - to, -1e30f);  // the difference may leave fp32's range
+        const float f = exp_of(d);
+        W = f * __builtin_fmaf(d, S, W);
+        S = f * S;
+        m = to;
+    }
+    __device__ __forceinline__ void add(const Sums& o) {
+        S += o.S;
+        W += o.W;
+    }
+};
+
+__device__ __forceinline__ float wave_largest(float v) {
+    v = fmaxf(v, dpp_f32<dpp::kXor1>(v));
+    v = fmaxf(v, dpp_f32<dpp::kXor2>(v));
+    v = fmaxf(v, dpp_f32<dpp::kHalfMirror>(v));
+    v = fmaxf(v, dpp_f32<dpp::kRor8>(v));
+    RowPair r = pair16(__float_as_uint(v));
+    v = fmaxf(__uint_as_float(r.lo), __uint_as_float(r.hi));
+    r = pair32(__float_as_uint(v));
+    return fmaxf(__uint_as_float(r.lo), __uint_as_float(r.hi));
+}
+
+__device__ __forceinline__ Sums wave_join(Sums s) {
+    s.raise(wave_largest(s.m));
+    s.S = group_sum<kWave>(s.S);
+    s.W = group_sum<kWave>(s.W);
+    return s;
+}
+
+// ------------------------------------------------------------------------------------------
+// Candidates: 64-bit numbers, the logit's order above the token's (the lower token the larger).
+// ------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return __uint_as_float(k ^ (static_cast<int32_t>(k) < 0 ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ uint64_t candidate(float l, int token) {
+    return uint64_t(score_key(l)) << 32 | (0xffffffffu - static_cast<uint32_t>(token));
+}
+
+__device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
+    const uint32_t hi = static_cast<uint32_t>(v >> 32);
+    const uint32_t most = group_max<kWave>(hi);
+    const uint32_t lo = group_max<kWave>(hi == most ? static_cast<uint32_t>(v) : 0u);
+    return uint64_t(most) << 32 | lo;
+}
+
+// What a wave wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+}
+
+struct Candidates {
+    uint64_t* list;  // kList of this wave's, in LDS
+    int k, count = 0;
+    uint64_t above = kNone;  // candidates are larger than this
+    float from = -__builtin_inff();  // and their logits at least this
+    float lane_most = -__builtin_inff();
+    __device__ Candidates(uint64_t* l, int top) : list(l), k(top) {}
+
+    // Leaves the k largest, sorted.
+    __device__ void cut() {
+        wave_fence();
+        const int lane = lane_id();
+        constexpr int kEach = kList / kWave;
+        uint64_t mine[kEach], kept = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) mine[i] = i * kWave + lane < count ? list[i * kWave + lane] : 0;
+        const int n = min(count, k);
+        for (int r = 0; r < n; ++r) {
+            uint64_t most = mine[0];
+#pragma unroll
+            for (int i = 1; i < kEach; ++i) most = mine[i] > most ? mine[i] : most;
+            most = wave_largest(most);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) mine[i] = mine[i] == most ? 0 : mine[i];
+            if (lane == r) kept = most;
+            if (r == k - 1) above = most;
+        }
+        wave_fence();
+        if (lane < n) list[lane] = kept;
+        count = n;
+        from = fmaxf(from, key_value(static_cast<uint32_t>(above >> 32)));
+    }
+
+    // Raises the bound to the k-th largest of the lanes' largest (to 16 bits of its key, from below).
+    __device__ __forceinline__ void bound() {
+        const uint32_t key = score_key(lane_most);
+        uint32_t least = 0;
+        for (int bit = 31; bit >= 16; --bit) {
+            const uint32_t test = least | 1u << bit;
+            if (__popcll(ballot(key >= test)) >= k) least = test;
+        }
+        if (least > kKeyNegInf) from = fmaxf(from, key_value(least));
+    }
+
+    template <typename E, int N>
+    __device__ __forceinline__ void take(const Pack<E> (&v)[N], const float (&most)[N], float batch_most,
+                                         const int (&first)[N]) {
+        lane_most = fmaxf(lane_most, batch_most);
+        if (!ballot(batch_most >= from)) return;
+        bound();
+#pragma unroll
+        for (int b = 0; b < N; ++b) {
+            if (!ballot(most[b] >= from)) continue;
+#pragma unroll
+            for (int j = 0; j < Pack<E>::kN; ++j) {
+                const float l = v[b][j];
+                const uint64_t c = candidate(l, first[b] + j);
+                put(l, c);
+            }
+        }
+    }
+    __device__ __forceinline__ void put(float l, uint64_t c) {
+        uint64_t lanes = ballot(l >= from && c > above);
+        if (!lanes) return;
+        if (count + __popcll(lanes) > kList) {
+            cut();
+            lanes = ballot(l >= from && c > above);
+        }
+        if (lanes >> lane_id() & 1) list[count + lanes_below(lanes)] = c;
+        count += __popcll(lanes);
+    }
+};
+
+// The k largest of `lists` sorted lists (a lane each, `each` numbers apart, 0 behind the last), lane r the
+// r-th.
+__device__ __forceinline__ uint64_t merge(const uint64_t* all, int lists, int each, int k) {
+    const int lane = lane_id();
+    const uint64_t* mine = all + lane * each;
+    int at = 0;
+    uint64_t head = lane < lists ? mine[0] : 0, kept = 0;
+    for (int r = 0; r < k; ++r) {
+        const uint64_t most = wave_largest(head);
+        if (lane == r) kept = most;
+        if (head == most && most) head = ++at < k ? mine[at] : 0;
+    }
+    return kept;
+}
+
+// A row's values from its sums: one wave, lane 0 and the lanes of the alternatives.
+template <typename E>
+__device__ __forceinline__ void write_row(const Args& a, int i, const Sums& s, uint64_t best) {
+    const int lane = lane_id();
+    const bool none = s.S == 0.0f;
+    const float rest = none ? 0.0f : logf(s.S);
+    if (lane == 0) {
+        const int64_t t = a.token(i);
+        float logprob = 0.0f;
+        if (t >= 0 && t < a.V) {
+            const float l = to_f32(static_cast<const E*>(a.logits)[i * a.row + t]);
+            logprob = none ? -__builtin_inff() : (l - s.m) - rest;
+            if (s.S != s.S) logprob = s.S;
+        }
+        const float entropy = none ? 0.0f : rest - s.W / s.S;
+        a.logprob[i] = logprob;
+        a.entropy[i] = entropy;
+        if (a.stats) a.stats[i] = make_float4(s.m, none ? 0.0f : 1.0f / s.S, rest, entropy);
+    }
+    if (lane < a.top) {
+        const bool there = best != 0;
+        const float l = key_value(static_cast<uint32_t>(best >> 32));
+        a.top_tokens[int64_t(i) * a.top + lane] = 
+            there ? int64_t(0xffffffffu - static_cast<uint32_t>(best)) : int64_t(-1);
+        a.top_logprobs[int64_t(i) * a.top + lane] = there ? (l - s.m) - rest : -__builtin_inff();
+    }
+}
+
+// A workgroup a part of a row.
+template <typename E, int WAVES, bool TOP>
+__global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
+    constexpr int kThreads = WAVES * kWave, kN = Pack<E>::kN;
+    __shared__ float wave_sums[WAVES][3];
+    __shared__ uint64_t lists[TOP ? WAVES : 1][TOP ? kList : 1];
+    const int i = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const int wave = uniform(threadIdx.x / kWave), lane = lane_id();
+    const E* row = static_cast<const E*>(a.logits) + i * a.row;
+    const int packs = a.V / kN;  // whole ones
+    const int begin = part * a.part_packs;
+    const int end = part + 1 == a.parts ? packs : min(packs, begin + a.part_packs);
+    Sums s;
+    Candidates c(lists[TOP ? wave : 0], a.top);
+    const auto batch = [&](const auto& v, const auto& first) {
+        constexpr int N = sizeof(v) / sizeof(v[0]);
+        float most[N];
+#pragma unroll
+        for (int b = 0; b < N; ++b) {
+            most[b] = v[b][0];
+#pragma unroll
+            for (int j = 1; j < kN; ++j) most[b] = fmaxf(most[b], v[b][j]);
+        }
+        float all = most[0];
+#pragma unroll
+        for (int b = 1; b < N; ++b) all = fmaxf(all, most[b]);
+        s.raise(fmaxf(s.m, all));
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                const float x = v[b][j] - s.m;
+                const float e = exp_of(x);
+                s.S += e;
+                s.W = __builtin_fmaf(e, fmaxf(x, -200.0f), s.W);  // e is 0 there, and x may be -inf
+            }
+        if constexpr (TOP) c.take(v, most, all, first);
+    };
+    const auto nothing = [] {
+        Pack<E> v;
+#pragma unroll
+        for (int j = 0; j < kN; ++j) v.e[j] = from_f32<E>(-__builtin_inff());
+        return v;
+    };
+    // (the loop is the same for all lanes: the candidates' lists are the wave's)
+    for (int p0 = begin; p0 < end; p0 += kBatch * kThreads) {
+        Pack<E> v[kBatch];
+        int first[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int p = p0 + b * kThreads + int(threadIdx.x);
+            v[b] = p < end ? load_pack(row + int64_t(p) * kN) : nothing();
+            first[b] = p * kN;
+        }
+        batch(v, first);
+    }
+    if (part + 1 == a.parts && packs * kN < a.V && wave == 0) {  // the elements after the last pack
+        Pack<E> v[1] = {nothing()};
+        const int first[1] = {packs * kN + lane};
+        if (first[0] < a.V) v[0].e[0] = row[first[0]];
+        batch(v, first);
+    }
+    s = wave_join(s);
+    if constexpr (TOP) {
+        c.cut();
+        if (lane >= c.count && lane < a.top) c.list[lane] = 0;
+    }
+    if constexpr (WAVES > 1) {
+        if (lane == 0) wave_sums[wave][0] = s.m, wave_sums[wave][1] = s.S, wave_sums[wave][2] = s.W;
+        __syncthreads();
+        if (wave) return;
+        float m = s.m;
+        for (int w = 1; w < WAVES; ++w) m = fmaxf(m, wave_sums[w][0]);
+        s.raise(m);  // wave 0's own
+        for (int w = 1; w < WAVES; ++w) {
+            Sums o;
+            o.m = wave_sums[w][0], o.S = wave_sums[w][1], o.W = wave_sums[w][2];
+            o.raise(m);
+            s.add(o);
+        }
+    } else if constexpr (TOP) {
+        wave_fence();
+    }
+    uint64_t best = 0;
+    if constexpr (TOP) best = merge(&lists[0][0], WAVES, kList, a.top);
+    if (a.parts == 1) {
+        write_row<E>(a, i, s, best);
+    } else {
+        if (lane == 0) a.part_sums[blockIdx.x] = make_float4(s.m, s.S, s.W, 0.0f);
+        if (TOP && lane < a.top) a.part_lists[int64_t(blockIdx.x) * a.top + lane] = best;
+    }
+}
+
+// The parts of a row joined, a wave a row.
+template <typename E, bool TOP>
+__global__ __launch_bounds__(kWave) void score_join(const Args a) {
+    __shared__ uint64_t lists[TOP ? kMostParts * HSN_SCORE_MAX_TOP : 1];
+    const int i = blockIdx.x, lane = lane_id();
+    Sums s;
+    if (lane < a.parts) {
+        const float4 v = a.part_sums[int64_t(i) * a.parts + lane];
+        s.m = v.x, s.S = v.y, s.W = v.z;
+    }
+    if constexpr (TOP) {
+        const uint64_t* from = a.part_lists + int64_t(i) * a.parts * a.top;
+        for (int j = lane; j < a.parts * a.top; j += kWave) lists[j] = from[j];
+        wave_fence();
+    }
+    s = wave_join(s);
+    uint64_t best = 0;
+    if constexpr (TOP) best = merge(lists, a.parts, a.top, a.top);
+    write_row<E>(a, i, s, best);
+}
+
+// A workgroup a part of a row.
+template <typename E, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void score_grad(const Args a) {
+    constexpr int kThreads = WAVES * kWave, kN = Pack<E>::kN;
+    const int i = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const E* row = static_cast<const E*>(a.logits) + i * a.row;
+    E* to = static_cast<E*>(a.d_logits) + int64_t(i) * a.V;
+    const float4 stats = a.stats[i];
+    const float m = stats.x, r = stats.y, rest = stats.z, entropy = stats.w;
+    const int64_t given = a.token(i);
+    const bool skipped = given < 0 || given >= a.V || r == 0.0f;
+    const int t = skipped ? -1 : static_cast<int>(given);
+    const float g = a.g && !skipped ? a.g[i * a.g_stride] : 0.0f;
+    const float h = a.h ? a.h[i * a.h_stride] : 0.0f;
+    const float lift = entropy - rest;  // log p + H = x + lift
+    const auto grad = [&](float l) {
+        const float x = l - m;
+        const float p = exp_of(x) * r;
+        return -p * __builtin_fmaf(h, fmaxf(x, -200.0f) + lift, g);
+    };
+    const int packs = a.V / kN;
+    const int begin = part * a.part_packs;
+    const int end = part + 1 == a.parts ? packs : min(packs, begin + a.part_packs);
+    for (int p = begin + int(threadIdx.x); p < end; p += kBatch * kThreads) {
+        Pack<E> v[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (p + b * kThreads < end) v[b] = load_pack(row + int64_t(p + b * kThreads) * kN);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (p + b * kThreads >= end) break;
+            const int first = (p + b * kThreads) * kN;
+            float d[kN];
+#pragma unroll
+            for (int j = 0; j < kN; ++j) d[j] = grad(v[b][j]);
+            if (static_cast<uint32_t>(t - first) < kN) {
+#pragma unroll
+                for (int j = 0; j < kN; ++j) d[j] += first + j == t ? g : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < kN; ++j) v[b].e[j] = from_f32<E>(d[j]);
+            store_pack(to + first, v[b]);
+        }
+    }
+    if (part + 1 == a.parts) {
+        const int j = packs * kN + int(threadIdx.x);
+        if (j < a.V) to[j] = from_f32<E>(grad(to_f32(row[j])) + (j == t ? g : 0.0f));
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// Launches.
+// ------------------------------------------------------------------------------------------
+
+int size_of(int dtype) { return dtype == HSN_DTYPE_F32 ? 4 : 2; }
+
+// Waves of a workgroup and parts of a row.
+struct Plan {
+    int waves, parts, part_packs;
+};
+
+Plan plan_of(int n, int V, int dtype) {
+    const int64_t packs = std::max<int64_t>(1, V / (16 / size_of(dtype)));
+    Plan p;
+    p.waves = packs <= 2 * kBatch * kWave ? 1 : 4;
+    const int64_t batch = int64_t(kBatch) * p.waves * kWave;
+    const int64_t wanted = (2048 + n - 1) / std::max(n, 1);
+    const int64_t parts = std::max<int64_t>(1, std::min({wanted, packs / batch, int64_t(kMostParts)}));
+    p.part_packs = static_cast<int>((packs + parts - 1) / parts);
+    p.parts = static_cast<int>((packs + p.part_packs - 1) / p.part_packs);
+    return p;
+}
+
+int64_t layout(Args& a, char* at, int n, int top) {
+    if (a.parts == 1) return 0;
+    a.part_sums = reinterpret_cast<float4*>(at);
+    const int64_t sums = 16 * int64_t(n) * a.parts;
+    a.part_lists = reinterpret_cast<uint64_t*>(at + sums);
+    return sums + 8 * int64_t(n) * a.parts * top;
+}
+
+template <typename E, bool TOP>
+void launch_forward(const Args& a, const Plan& p, int n, hipStream_t st) {
+    if (p.waves == 1)
+        score_rows<E, 1, TOP><<<n * p.parts, kWave, 0, st>>>(a);
+    else
+        score_rows<E, 4, TOP><<<n * p.parts, 4 * kWave, 0, st>>>(a);
+    HSN_HIP(hipGetLastError());
+    if (p.parts > 1) score_join<E, TOP><<<n, kWave, 0, st>>>(a);
+}
+
+template <typename E>
+void launch_backward(const Args& a, const Plan& p, int n, hipStream_t st) {
+    if (p.waves == 1)
+        score_grad<E, 1><<<n * p.parts, kWave, 0, st>>>(a);
+    else
+        score_grad<E, 4><<<n * p.parts, 4 * kWave, 0, st>>>(a);
+}
+
+void check(int n, int V, int dtype, int top) {
+    HSN_REQUIRE(dtype == HSN_DTYPE_F32 || dtype == HSN_DTYPE_F16 || dtype == HSN_DTYPE_BF16,
+                HSN_ERR_UNSUPPORTED_DTYPE, "logits must be F32, F16 or BF16");
+    HSN_REQUIRE(n >= 0 && V >= 1, HSN_ERR_INVALID_ARGUMENT, "n >= 0 and V >= 1");
+    HSN_REQUIRE(top >= 0 && top <= HSN_SCORE_MAX_TOP, HSN_ERR_INVALID_ARGUMENT, "top in [0, 32]");
+    HSN_REQUIRE(V <= HSN_SCORE_MAX_TOKENS, HSN_ERR_SIZE_OVERFLOW, "at most 2^24 tokens");
+    // a grid's dimension holds fewer than 2^32 threads, four waves a row
+    HSN_REQUIRE(n < 1 << 24, HSN_ERR_SIZE_OVERFLOW, "fewer than 2^24 rows");
+    HSN_REQUIRE(int64_t(n) * V < int64_t(1) << 40, HSN_ERR_SIZE_OVERFLOW, "fewer than 2^40 logits");
+}
+
+void check_rows(const void* logits, int dtype, const void* tokens, int token_bytes) {
+    HSN_REQUIRE(logits && tokens, HSN_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
+    HSN_REQUIRE(reinterpret_cast<uintptr_t>(logits) % size_of(dtype) == 0, HSN_ERR_INVALID_ARGUMENT,
+                "logits must be aligned to their type");
+    HSN_REQUIRE(token_bytes == 8 || token_bytes == 4, HSN_ERR_INVALID_ARGUMENT, "token_bytes is 8 or 4");
+}
+
+}  // namespace
+}  // namespace score
+}  // namespace hsn
+
+using namespace hsn;
+using namespace hsn::score;
+
+extern "C" int hsn_score_workspace(int n, int V, int dtype, int top, int64_t* bytes) {
+    HSN_ABI_BEGIN
+    check(n, V, dtype, top);
+    HSN_REQUIRE(bytes, HSN_ERR_INVALID_ARGUMENT, "bytes must not be NULL");
+    Args a{};
+    a.parts = plan_of(n, V, dtype).parts;
+    *bytes = layout(a, nullptr, n, top);
+    HSN_ABI_END
+}
+
+extern "C" int hsn_score_forward(const void* logits, int64_t row, int dtype, const void* tokens,
+                                 int64_t token_stride, int token_bytes, float* logprob, float* entropy,
+                                 int64_t* top_tokens, float* top_logprobs, float* stats, int n, int V,
+                                 int top, void* workspace, int64_t workspace_bytes, void* stream) {
+    HSN_ABI_BEGIN
+    check(n, V, dtype, top);
+    if (n == 0) return HSN_OK;
+    check_rows(logits, dtype, tokens, token_bytes);
+    HSN_REQUIRE(logprob && entropy && (top == 0 || (top_tokens && top_logprobs)), HSN_ERR_INVALID_ARGUMENT,
+                "a required pointer is NULL");
+    HSN_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 16 == 0, HSN_ERR_INVALID_ARGUMENT,
+                "stats must be aligned to 16 bytes");
+    const Plan p = plan_of(n, V, dtype);
+    Args a{};
+    a.logits = logits, a.row = row, a.tokens = tokens, a.token_stride = token_stride;
+    a.wide = token_bytes == 8;
+    a.logprob = logprob, a.entropy = entropy, a.top_tokens = top_tokens, a.top_logprobs = top_logprobs;
+    a.stats = reinterpret_cast<float4*>(stats);
+    a.V = V, a.top = top, a.parts = p.parts, a.part_packs = p.part_packs;
+    const int64_t bytes = layout(a, static_cast<char*>(workspace), n, top);
+    HSN_REQUIRE(!bytes || (workspace && workspace_bytes >= bytes), HSN_ERR_INVALID_ARGUMENT,
+                "the workspace is too small");
+    HSN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, HSN_ERR_INVALID_ARGUMENT,
+                "the workspace must be aligned to 16 bytes");
+    hipStream_t st = as_stream(stream);
+    const auto with = [&](auto e) {
+        using E = decltype(e);
+        if (top)
+            launch_forward<E, true>(a, p, n, st);
+        else
+            launch_forward<E, false>(a, p, n, st);
+    };
+    if (dtype == HSN_DTYPE_F32)
+        with(float{});
+    else if (dtype == HSN_DTYPE_F16)
+        with(_Float16{});
+    else
+        with(bf16_t{});
+    HSN_HIP(hipGetLastError());
+    HSN_ABI_END
+}
+
+extern "C" int hsn_score_backward(const void* logits, int64_t row, int dtype, const void* tokens,
+                                  int64_t token_stride, int token_bytes, const float* stats,
+                                  const float* d_logprob, int64_t g_stride, const float* d_entropy,
+                                  int64_t h_stride, void* d_logits, int n, int V, void* stream) {
+    HSN_ABI_BEGIN
+    check(n, V, dtype, 0);
+    if (n == 0) return HSN_OK;
+    check_rows(logits, dtype, tokens, token_bytes);
+    HSN_REQUIRE(stats && d_logits, HSN_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
+    HSN_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 16 == 0, HSN_ERR_INVALID_ARGUMENT,
+                "stats must be aligned to 16 bytes");
+    HSN_REQUIRE(reinterpret_cast<uintptr_t>(d_logits) % size_of(dtype) == 0, HSN_ERR_INVALID_ARGUMENT,
+                "d_logits must be aligned to their type");
+    const Plan p = plan_of(n, V, dtype);
+    Args a{};
+    a.logits = logits, a.row = row, a.tokens = tokens, a.token_stride = token_stride;
+    a.wide = token_bytes == 8;
+    a.stats = reinterpret_cast<float4*>(const_cast<float*>(stats));
+    a.V = V, a.parts = p.parts, a.part_packs = p.part_packs;
+    a.g = d_logprob, a.g_stride = g_stride, a.h = d_entropy, a.h_stride = h_stride;
+    a.d_logits = d_logits;
+    hipStream_t st = as_stream(stream);
+    if (dtype == HSN_DTYPE_F32)
+        launch_backward<float>(a, p, n, st);
+    else if (dtype == HSN_DTYPE_F16)
+        launch_backward<_Float16>(a, p, n, st);
+    else
+        launch_backward<bf16_t>(a, p, n, st);
+    HSN_HIP(hipGetLastError());
+    HSN_ABI_END
+}

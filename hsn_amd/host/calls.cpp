@@ -1,8 +1,8 @@
 // The calls of a decoded token in one step from the interpreter: the language-model operators'
-// Python mirrors (hsn_amd/scan.py, unit_layer.py, sampling.py, grad_clip.py) check their tensors, allocate outputs
-// and workspace and call the C entry point through this module where it is built. Made in the
-// interpreter, the checks, allocations and the conversion of some twenty arguments cost 4 to 6 us a
-// call, more than the kernel of a single position; here they cost about 1 us.
+// Python mirrors (hsn_amd/scan.py, unit_layer.py, sampling.py, scoring.py, grad_clip.py) check their
+// tensors, allocate outputs and workspace and call the C entry point through this module where it is
+// built. Made in the interpreter, the checks, allocations and the conversion of some twenty arguments
+// cost 4 to 6 us a call, more than the kernel of a single position; here they cost about 1 us.
 //
 // Every function takes the C entry points' addresses and the raw stream, and returns
 //   None   a check failed: nothing was allocated or launched, and the caller makes the same checks in
@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "../../include/hsn_sample.h"
+#include "../../include/hsn_score.h"
 #include "../../include/hsn_units_layer.h"
 
 namespace {
@@ -311,6 +312,88 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// Logits [n, V] whose rows are contiguous, and a token a row (int64 or int32).
+struct Rows {
+    const Tensor *logits, *tokens;
+    int code = -1, token_bytes = 0;
+    int64_t n = 0, V = 0;
+    bool ok = false;
+    Rows(const Tensor* l, const Tensor* t) : logits(l), tokens(t) {
+        if (!l || !t || l->dim() != 2 || !l->is_cuda()) return;
+        code = dtype_code(l->scalar_type());
+        n = l->size(0), V = l->size(1);
+        token_bytes = t->scalar_type() == at::kLong ? 8 : t->scalar_type() == at::kInt ? 4 : 0;
+        ok = code >= 0 && token_bytes && V >= 1 && V <= HSN_SCORE_MAX_TOKENS && n < 1 << 24 &&
+             n * V < int64_t(1) << 40 && like(l, *l) && t->dim() == 1 && t->size(0) == n &&
+             t->device() == l->device() && plain(*t);
+    }
+};
+
+// score_forward(workspace, forward, stream, logits, tokens, top, save)
+PyObject* score_forward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Arguments in{args, args + n_args};
+    const int64_t size_at = in.integer(), call_at = in.integer(), stream = in.integer();
+    const Tensor *logits = in.tensor(), *tokens = in.tensor();
+    const int64_t top = in.integer(), save = in.integer();
+    if (!in.ok || top < 0 || top > HSN_SCORE_MAX_TOP) Py_RETURN_NONE;
+    const Rows rows(logits, tokens);
+    if (!rows.ok) Py_RETURN_NONE;
+    int64_t bytes = 0;
+    int status = entry<int (*)(int, int, int, int, int64_t*)>(size_at)(rows.n, rows.V, rows.code, top, &bytes);
+    if (status) return PyLong_FromLong(status);
+    const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(logits->device());
+    const auto on = at::TensorOptions().device(logits->device());
+    const Tensor logprob = at::empty({rows.n}, on.dtype(at::kFloat));
+    const Tensor entropy = at::empty({rows.n}, on.dtype(at::kFloat));
+    Tensor top_tokens, top_logprobs, stats;
+    if (top) {
+        top_tokens = at::empty({rows.n, top}, on.dtype(at::kLong));
+        top_logprobs = at::empty({rows.n, top}, on.dtype(at::kFloat));
+    }
+    if (save) stats = at::empty({rows.n, 4}, on.dtype(at::kFloat));
+    const Tensor ws = workspace(bytes, on);
+    status = entry<int (*)(P, int64_t, int, P, int64_t, int, P, P, P, P, P, int, int, int, P, int64_t, P)>(
+        call_at)(logits->data_ptr(), logits->stride(0), rows.code, tokens->data_ptr(), tokens->stride(0),
+                 rows.token_bytes, logprob.data_ptr(), entropy.data_ptr(),
+                 top ? top_tokens.data_ptr() : nullptr, top ? top_logprobs.data_ptr() : nullptr,
+                 save ? stats.data_ptr() : nullptr, rows.n, rows.V, top, bytes ? ws.data_ptr() : nullptr, bytes,
+                 entry<P>(stream));
+    if (status) return PyLong_FromLong(status);
+    return Py_BuildValue("(NNNNN)", wrap(logprob), wrap(entropy), wrap(top_tokens), wrap(top_logprobs),
+                         wrap(stats));
+    END_HANDLE_TH_ERRORS
+}
+
+// score_backward(backward, stream, logits, tokens, stats, d_logprob, d_entropy)
+PyObject* score_backward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Arguments in{args, args + n_args};
+    const int64_t call_at = in.integer(), stream = in.integer();
+    const Tensor *logits = in.tensor(), *tokens = in.tensor(), *stats = in.tensor();
+    const Tensor *g = in.tensor(), *h = in.tensor();
+    if (!in.ok || !stats) Py_RETURN_NONE;
+    const Rows rows(logits, tokens);
+    if (!rows.ok || !dense(stats, {rows.n, 4}, at::kFloat, logits->device())) Py_RETURN_NONE;
+    for (const Tensor* t : {g, h})
+        if (t && (t->dim() != 1 || t->size(0) != rows.n || t->scalar_type() != at::kFloat ||
+                  t->device() != logits->device() || !plain(*t)))
+            Py_RETURN_NONE;
+    const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(logits->device());
+    const Tensor d = at::empty({rows.n, rows.V},
+                               at::TensorOptions().device(logits->device()).dtype(logits->scalar_type()));
+    const int status =
+        entry<int (*)(P, int64_t, int, P, int64_t, int, P, P, int64_t, P, int64_t, P, int, int, P)>(call_at)(
+            logits->data_ptr(), logits->stride(0), rows.code, tokens->data_ptr(), tokens->stride(0),
+            rows.token_bytes, stats->data_ptr(), address(g), g ? g->stride(0) : 0, address(h),
+            h ? h->stride(0) : 0, d.data_ptr(), rows.n, rows.V, entry<P>(stream));
+    if (status) return PyLong_FromLong(status);
+    return wrap(d);
+    END_HANDLE_TH_ERRORS
+}
+
 // A list or tuple of tensors, held while it is read.
 struct List {
     PyObject* seq = nullptr;
@@ -398,6 +481,11 @@ PyMethodDef kMethods[] = {
      "(workspace, layer, stream, x, router, W1, b1, W2, b2, k, activation, gated) -> y"},
     {"sample", fast<sample>(), METH_FASTCALL,
      "(workspace, sample, stream, logits, u, temperature, top_k, top_p, min_p) -> tokens"},
+    {"score_forward", fast<score_forward>(), METH_FASTCALL,
+     "(workspace, forward, stream, logits, tokens, top, save) -> (logprob, entropy, top_tokens, "
+     "top_logprobs, stats)"},
+    {"score_backward", fast<score_backward>(), METH_FASTCALL,
+     "(backward, stream, logits, tokens, stats, d_logprob, d_entropy) -> d_logits"},
     {"grad_clip", fast<grad_clip>(), METH_FASTCALL,
      "(workspace, clip, stream, grads, outs, max_norm) -> (norm, coefficient)"},
     {nullptr, nullptr, 0, nullptr},
