@@ -1,7 +1,7 @@
 """The C ABI of ``libhsn_amd.so`` (``include/hsn_window.h``, ``include/hsn_ops.h``,
 ``include/hsn_trainer.h``, ``include/hsn_sweep.h``, ``include/hsn_round.h``,
 ``include/hsn_scan.h``, ``include/hsn_units_layer.h``, ``include/hsn_sample.h``,
-``include/hsn_score.h``, ``include/hsn_clip.h``) via ctypes.
+``include/hsn_score.h``, ``include/hsn_unit_router.h``, ``include/hsn_clip.h``) via ctypes.
 
 The library is the product: every operator in :mod:`hsn_amd` reaches the GPU through these
 entry points, and nothing here falls back to another implementation. :func:`library` raises a
@@ -101,6 +101,9 @@ SIGNATURES: dict[str, list] = {
     "hsn_score_workspace": [I, I, I, I, P],
     "hsn_score_forward": [P, L, I, P, L, I, P, P, P, P, P, I, I, I, P, L, P],
     "hsn_score_backward": [P, L, I, P, L, I, P, P, L, P, L, P, I, I, P],
+    "hsn_unit_router_workspace": [I, I, I, P],
+    "hsn_unit_router_forward": [P, L, I, P, P, P, P, P, P, I, I, I, P, L, P],
+    "hsn_unit_router_backward": [P, L, I, P, P, P, P, L, P, P, I, I, I, P],
     "hsn_clip_workspace": [P, I, P],
     "hsn_clip": [P, P, P, P, I, D, P, P, L, P],
 }

@@ -1,6 +1,6 @@
 // The calls of a decoded token in one step from the interpreter: the language-model operators'
-// Python mirrors (hsn_amd/scan.py, unit_layer.py, sampling.py, scoring.py, grad_clip.py) check their
-// tensors, allocate outputs and workspace and call the C entry point through this module where it is
+// Python mirrors (hsn_amd/scan.py, unit_layer.py, sampling.py, scoring.py, unit_router.py, grad_clip.py)
+// check their tensors, allocate outputs and workspace and call the C entry point through this module where it is
 // built. Made in the interpreter, the checks, allocations and the conversion of some twenty arguments
 // cost 4 to 6 us a call, more than the kernel of a single position; here they cost about 1 us.
 //
@@ -26,6 +26,7 @@
 
 #include "../../include/hsn_sample.h"
 #include "../../include/hsn_score.h"
+#include "../../include/hsn_unit_router.h"
 #include "../../include/hsn_units_layer.h"
 
 namespace {
@@ -394,6 +395,77 @@ PyObject* score_backward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// unit_router_forward(workspace, forward, stream, logits, k, valid)
+PyObject* unit_router_forward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Arguments in{args, args + n_args};
+    const int64_t size_at = in.integer(), call_at = in.integer(), stream = in.integer();
+    const Tensor* logits = in.tensor();
+    const int64_t k = in.integer();
+    const Tensor* valid = in.tensor();
+    if (!in.ok || !logits || logits->dim() != 2 || !logits->is_cuda()) Py_RETURN_NONE;
+    const auto device = logits->device();
+    const int code = dtype_code(logits->scalar_type());
+    const int64_t n = logits->size(0), M = logits->size(1);
+    if (code < 0 || n >= 1 << 30 || M < 1 || M > HSN_ROUTER_MAX_UNITS || k < 1 || k > M ||
+        k > HSN_ROUTER_MAX_CHOSEN || !like(logits, *logits) || !dense(valid, {n}, at::kBool, device))
+        Py_RETURN_NONE;
+    int64_t bytes = 0;
+    int status = entry<int (*)(int, int, int, int64_t*)>(size_at)(n, M, code, &bytes);
+    if (status) return PyLong_FromLong(status);
+    const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(device);
+    const auto on = at::TensorOptions().device(device);
+    const Tensor units = at::empty({n, k}, on.dtype(at::kLong));
+    const Tensor shares = at::empty({n, k}, on.dtype(at::kFloat));
+    const Tensor tally = at::empty({M + 1}, on.dtype(at::kLong));
+    const Tensor probs = at::empty({M}, on.dtype(at::kFloat));
+    const Tensor balance = at::empty({}, on.dtype(at::kFloat));
+    const Tensor ws = workspace(bytes, on);
+    status = entry<int (*)(P, int64_t, int, P, P, P, P, P, P, int, int, int, P, int64_t, P)>(call_at)(
+        logits->data_ptr(), logits->stride(0), code, address(valid), units.data_ptr(), shares.data_ptr(),
+        tally.data_ptr(), probs.data_ptr(), balance.data_ptr(), n, M, k, ws.data_ptr(), bytes,
+        entry<P>(stream));
+    if (status) return PyLong_FromLong(status);
+    return Py_BuildValue("(NNNNNN)", wrap(units), wrap(shares), wrap(balance), wrap(tally.narrow(0, 0, M)),
+                         wrap(probs), wrap(tally));
+    END_HANDLE_TH_ERRORS
+}
+
+// unit_router_backward(backward, stream, logits, units, tally, d_shares, d_balance, valid)
+PyObject* unit_router_backward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Arguments in{args, args + n_args};
+    const int64_t call_at = in.integer(), stream = in.integer();
+    const Tensor *logits = in.tensor(), *units = in.tensor(), *tally = in.tensor();
+    const Tensor *g = in.tensor(), *d_balance = in.tensor(), *valid = in.tensor();
+    if (!in.ok || !logits || !units || !tally || logits->dim() != 2 || units->dim() != 2 || !logits->is_cuda())
+        Py_RETURN_NONE;
+    const auto device = logits->device();
+    const int code = dtype_code(logits->scalar_type());
+    const int64_t n = logits->size(0), M = logits->size(1), k = units->size(1);
+    if (code < 0 || n >= 1 << 30 || M < 1 || M > HSN_ROUTER_MAX_UNITS || k < 1 || k > M ||
+        k > HSN_ROUTER_MAX_CHOSEN || !like(logits, *logits) || !dense(valid, {n}, at::kBool, device) ||
+        !dense(units, {n, k}, at::kLong, device) || !dense(tally, {M + 1}, at::kLong, device))
+        Py_RETURN_NONE;
+    if (g && (g->dim() != 2 || g->size(0) != n || g->size(1) != k || g->scalar_type() != at::kFloat ||
+              g->device() != device || !plain(*g) || (g->stride(1) != 1 && k > 1)))
+        Py_RETURN_NONE;
+    if (d_balance && (d_balance->numel() != 1 || d_balance->scalar_type() != at::kFloat ||
+                      d_balance->device() != device || !plain(*d_balance)))
+        Py_RETURN_NONE;
+    const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(device);
+    const Tensor d = at::empty({n, M}, at::TensorOptions().device(device).dtype(logits->scalar_type()));
+    const int status =
+        entry<int (*)(P, int64_t, int, P, P, P, P, int64_t, P, P, int, int, int, P)>(call_at)(
+            logits->data_ptr(), logits->stride(0), code, address(valid), units->data_ptr(), tally->data_ptr(),
+            address(g), g ? g->stride(0) : 0, address(d_balance), d.data_ptr(), n, M, k, entry<P>(stream));
+    if (status) return PyLong_FromLong(status);
+    return wrap(d);
+    END_HANDLE_TH_ERRORS
+}
+
 // A list or tuple of tensors, held while it is read.
 struct List {
     PyObject* seq = nullptr;
@@ -486,6 +558,10 @@ PyMethodDef kMethods[] = {
      "top_logprobs, stats)"},
     {"score_backward", fast<score_backward>(), METH_FASTCALL,
      "(backward, stream, logits, tokens, stats, d_logprob, d_entropy) -> d_logits"},
+    {"unit_router_forward", fast<unit_router_forward>(), METH_FASTCALL,
+     "(workspace, forward, stream, logits, k, valid) -> (units, shares, balance, counts, probs, tally)"},
+    {"unit_router_backward", fast<unit_router_backward>(), METH_FASTCALL,
+     "(backward, stream, logits, units, tally, d_shares, d_balance, valid) -> d_logits"},
     {"grad_clip", fast<grad_clip>(), METH_FASTCALL,
      "(workspace, clip, stream, grads, outs, max_norm) -> (norm, coefficient)"},
     {nullptr, nullptr, 0, nullptr},
