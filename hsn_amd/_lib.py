@@ -1,7 +1,8 @@
 """The C ABI of ``libhsn_amd.so`` (``include/hsn_window.h``, ``include/hsn_ops.h``,
 ``include/hsn_trainer.h``, ``include/hsn_sweep.h``, ``include/hsn_round.h``,
 ``include/hsn_scan.h``, ``include/hsn_units_layer.h``, ``include/hsn_sample.h``,
-``include/hsn_score.h``, ``include/hsn_unit_router.h``, ``include/hsn_clip.h``) via ctypes.
+``include/hsn_embed.h``, ``include/hsn_score.h``, ``include/hsn_unit_router.h``,
+``include/hsn_clip.h``) via ctypes.
 
 The library is the product: every operator in :mod:`hsn_amd` reaches the GPU through these
 entry points, and nothing here falls back to another implementation. :func:`library` raises a
@@ -98,6 +99,9 @@ SIGNATURES: dict[str, list] = {
     "hsn_units_layer": [P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P, L, P],
     "hsn_sample_workspace": [I, I, I, P],
     "hsn_sample": [P, L, I, P, P, P, P, P, P, P, I, I, P, L, P],
+    "hsn_embed_forward": [P, L, L, I, P, L, I, F, P, I, I, I, I, I, P],
+    "hsn_embed_workspace": [I, I, I, I, I, P],
+    "hsn_embed_backward": [P, L, L, I, P, L, L, I, F, P, I, I, I, I, I, P, L, P],
     "hsn_score_workspace": [I, I, I, I, P],
     "hsn_score_forward": [P, L, I, P, L, I, P, P, P, P, P, I, I, I, P, L, P],
     "hsn_score_backward": [P, L, I, P, L, I, P, P, L, P, L, P, I, I, P],

@@ -1,0 +1,673 @@
+// The embedding of tokens and its gradient (include/hsn_embed.h).
+//
+// Forward: a copy of rows. A group of lanes takes a slice of a row, several positions in flight.
+//
+// Backward: the positions are sorted by token, and then every sum is over neighbours. The sort is by digits
+// of up to ten bits from the lowest on, stable, so a token's positions stay in order: a workgroup counts a
+// tile's digits, and the next launch ranks the tile's entries (lanes of a wave with the same digit find each
+// other by ballots) and adds up where they go from all tiles' counts; up to 4096 positions are sorted by
+// one workgroup in LDS. The sums are taken over chunks of the sorted list, one as long as the other, so a
+// token that fills a tenth of the text costs no workgroup more than another: a group of lanes walks a
+// chunk with a slice of the columns, writes the rows that begin and end inside it, and leaves the sums
+// that cross a border to a last launch, which adds them in order. Workgroups of the same launch write the
+// rows that no token names.
+//
+// What bounds it is memory: the cotangents are read once, the table's gradient is written once.
+#include <algorithm>
+#include <string>
+
+#include "../../include/hsn_embed.h"
+#include "abi_util.h"
+#include "packs.cuh"
+
+namespace hsn {
+namespace embed {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kDigit = 10, kBins = 1 << kDigit;
+constexpr int kSmall = 4096, kSmallThreads = 512, kSmallWaves = kSmallThreads / kWave;
+constexpr int kBatch = 8;       // entries of a chunk in flight
+constexpr int kZeroRows = 64;   // rows that a workgroup looks through for those without a token
+
+struct Entry {
+    uint32_t token;  // V: padding, behind all others
+    uint32_t position;
+};
+
+struct Args {
+    const void* tokens;
+    int64_t token_b, token_t;
+    bool wide;  // 64-bit tokens
+    const void* rows;  // the table, or the cotangents
+    int64_t row_b, row_t;
+    float scale;
+    void* out;
+    uint32_t n, T, V;
+    int D, slices;  // of 64 packs (or 16) of a row
+    // the sort
+    const Entry* from;
+    Entry* to;
+    uint32_t* counts;  // [tiles, kBins]
+    int tiles, shift, bits;
+    // the sums
+    int chunk, chunks, sum_groups;  // sum_groups: workgroups of sums before those that write zeros
+    float* parts;  // [chunks, 2, D]: the sum that comes from the chunk before, the one that begins here
+    __device__ __forceinline__ int64_t at(uint32_t i, int64_t b, int64_t t) const {
+        if (T == n) return i * t;
+        const uint32_t r = i / T;
+        return r * b + int64_t(i - r * T) * t;
+    }
+    __device__ __forceinline__ uint32_t token(uint32_t i) const {
+        const int64_t o = at(i, token_b, token_t);
+        const int64_t t = wide ? static_cast<const int64_t*>(tokens)[o] : static_cast<const int32_t*>(tokens)[o];
+        return t >= 0 && t < V ? static_cast<uint32_t>(t) : V;
+    }
+};
+
+// kN elements at any address, from or to fp32. Of `there` the first ones alone.
+template <typename E, int N>
+__device__ __forceinline__ void load_some(const E* p, int there, float (&v)[N]) {
+    if (there >= N) {
+        E e[N];
+        __builtin_memcpy(e, p, sizeof(e));
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = to_f32(e[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = j < there ? to_f32(p[j]) : 0.0f;
+    }
+}
+template <typename E, int N>
+__device__ __forceinline__ void store_some(E* p, int there, const float (&v)[N]) {
+    if (there >= N) {
+        E e[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) e[j] = from_f32<E>(v[j]);
+        __builtin_memcpy(p, e, sizeof(e));
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < there) p[j] = from_f32<E>(v[j]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// Forward.
+// ------------------------------------------------------------------------------------------
+
+// A group of G lanes a slice of a row (blockIdx.y), several positions in flight.
+template <typename E, typename O, int G>
+__global__ __launch_bounds__(kThreads) void gather(const Args a) {
+    constexpr int kN = 16 / sizeof(E), kGroups = kThreads / G, kFlight = 4;
+    const int column = (int(blockIdx.y) * G + int(threadIdx.x % G)) * kN, there = a.D - column;
+    if (there <= 0) return;
+    const E* table = static_cast<const E*>(a.rows) + column;
+    O* out = static_cast<O*>(a.out) + column;
+    const uint32_t step = gridDim.x * kGroups;
+    for (uint32_t i = blockIdx.x * kGroups + threadIdx.x / G; i < a.n; i += kFlight * step) {
+        uint32_t token[kFlight];
+        float v[kFlight][kN];
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) token[f] = i + f * step < a.n ? a.token(i + f * step) : a.V;
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) v[f][j] = 0.0f;
+            if (token[f] < a.V) load_some(table + token[f] * a.row_t, there, v[f]);
+        }
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) {
+            if (i + f * step >= a.n) break;
+            if (token[f] < a.V)
+#pragma unroll
+                for (int j = 0; j < kN; ++j) v[f][j] *= a.scale;
+            store_some(out + int64_t(i + f * step) * a.D, there, v[f]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// The sort.
+// ------------------------------------------------------------------------------------------
+
+// What a wave wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Each entry's place among the wave's entries of the same digit, in order; `count` (the wave's, zero
+// before) then holds how many of each there are.
+template <int N, typename C>
+__device__ __forceinline__ void rank_wave(const uint32_t (&digit)[N], int bits, C* count, uint32_t (&rank)[N]) {
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+        uint64_t same = ~uint64_t(0);
+        for (int b = 0; b < bits; ++b) {
+            const bool set = digit[r] >> b & 1;
+            const uint64_t lanes = ballot(set);
+            same &= set ? lanes : ~lanes;
+        }
+        const uint32_t before = lanes_below(same), base = count[digit[r]];
+        rank[r] = base + before;
+        wave_fence();
+        if (before == 0) count[digit[r]] = static_cast<C>(base + __popcll(same));
+        wave_fence();
+    }
+}
+
+// Exclusive sum over the workgroup's threads, in their order. `s`: a word a wave.
+template <int WAVES>
+__device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t* s) {
+    const int lane = lane_id(), wave = threadIdx.x / kWave;
+    uint32_t sum = v;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const uint32_t o = __shfl_up(sum, d, kWave);
+        sum += lane >= d ? o : 0;
+    }
+    if (lane == kWave - 1) s[wave] = sum;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) sum += s[w];
+    return sum - v;
+}
+
+__global__ __launch_bounds__(kSmallThreads) void sort_small(const Args a) {
+    constexpr int kItems = kSmall / kSmallThreads, kMine = kBins / kSmallThreads;
+    __shared__ Entry list[kSmall];
+    __shared__ uint16_t count[kSmallWaves][kBins];
+    __shared__ uint32_t s[kSmallWaves];
+    const int wave = uniform(threadIdx.x / kWave), lane = lane_id();
+    Entry e[kItems];
+    uint32_t digit[kItems], rank[kItems];
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+        const uint32_t i = (wave * kItems + r) * kWave + lane;
+        e[r] = {i < a.n ? a.token(i) : ~0u, i};  // (what is behind the end stays there: every digit is the largest)
+    }
+    for (int shift = 0; shift < a.bits; shift += kDigit) {
+        const int bits = min(kDigit, a.bits - shift);
+        for (int b = threadIdx.x; b < kSmallWaves * kBins; b += kSmallThreads) (&count[0][0])[b] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kItems; ++r) digit[r] = e[r].token >> shift & ((1u << bits) - 1);
+        rank_wave(digit, bits, count[wave], rank);
+        __syncthreads();
+        uint32_t total[kMine], all = 0;
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) {
+            total[b] = 0;
+            for (int w = 0; w < kSmallWaves; ++w) {  // the waves' counts become what is before them
+                const uint32_t c = count[w][threadIdx.x * kMine + b];
+                count[w][threadIdx.x * kMine + b] = static_cast<uint16_t>(total[b]);
+                total[b] += c;
+            }
+            all += total[b];
+        }
+        uint32_t before = block_before<kSmallWaves>(all, s);
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) {
+            for (int w = 0; w < kSmallWaves; ++w)
+                count[w][threadIdx.x * kMine + b] += static_cast<uint16_t>(before);
+            before += total[b];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kItems; ++r) list[count[wave][digit[r]] + rank[r]] = e[r];
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kItems; ++r) e[r] = list[(wave * kItems + r) * kWave + lane];
+    }
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+        const uint32_t i = (wave * kItems + r) * kWave + lane;
+        if (i < a.n) a.to[i] = e[r];
+    }
+}
+
+// Entry i before this pass: the first one reads the tokens.
+__device__ __forceinline__ Entry entry_of(const Args& a, uint32_t i) {
+    return a.from ? a.from[i] : Entry{a.token(i), i};
+}
+
+template <int ITEMS>
+__global__ __launch_bounds__(kThreads) void count_digits(const Args a) {
+    __shared__ uint32_t count[kBins];
+    for (int b = threadIdx.x; b < kBins; b += kThreads) count[b] = 0;
+    __syncthreads();
+    const uint32_t begin = blockIdx.x * (kThreads * ITEMS), mask = (1u << a.bits) - 1;
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        const uint32_t i = begin + r * kThreads + threadIdx.x;
+        if (i < a.n) atomicAdd(&count[(a.from ? a.from[i].token : a.token(i)) >> a.shift & mask], 1u);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += kThreads) a.counts[int64_t(blockIdx.x) * kBins + b] = count[b];
+}
+
+template <int ITEMS>
+__global__ __launch_bounds__(kThreads) void move_entries(const Args a) {
+    constexpr int kMine = kBins / kThreads;
+    __shared__ uint32_t count[kWaves][kBins];
+    __shared__ uint32_t s[kWaves];
+    const int wave = uniform(threadIdx.x / kWave), lane = lane_id();
+    for (int b = threadIdx.x; b < kWaves * kBins; b += kThreads) (&count[0][0])[b] = 0;
+    const uint32_t begin = blockIdx.x * (kThreads * ITEMS) + wave * (kWave * ITEMS) + lane;
+    Entry e[ITEMS];
+    uint32_t digit[ITEMS], rank[ITEMS];
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        const uint32_t i = begin + r * kWave;
+        e[r] = i < a.n ? entry_of(a, i) : Entry{~0u, 0};  // (not moved, and behind all others)
+        digit[r] = e[r].token >> a.shift & ((1u << a.bits) - 1);
+    }
+    __syncthreads();
+    rank_wave(digit, a.bits, count[wave], rank);
+    // where a digit's entries of this tile begin: all entries of lower digits, those of earlier tiles
+    uint32_t total[kMine] = {}, earlier[kMine] = {}, all = 0;
+    const uint32_t first = threadIdx.x * kMine;
+#pragma unroll 4
+    for (int t = 0; t < a.tiles; ++t) {
+        const uint4 c = *reinterpret_cast<const uint4*>(a.counts + int64_t(t) * kBins + first);
+        const uint32_t v[kMine] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) {
+            total[b] += v[b];
+            earlier[b] += t < static_cast<int>(blockIdx.x) ? v[b] : 0;
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < kMine; ++b) all += total[b];
+    uint32_t before = block_before<kWaves>(all, s);  // (passes a barrier: the waves' counts are there)
+#pragma unroll
+    for (int b = 0; b < kMine; ++b) {
+        uint32_t at = before + earlier[b];
+        for (int w = 0; w < kWaves; ++w) {
+            const uint32_t c = count[w][first + b];
+            count[w][first + b] = at;
+            at += c;
+        }
+        before += total[b];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+        if (begin + r * kWave < a.n) a.to[count[wave][digit[r]] + rank[r]] = e[r];
+}
+
+// ------------------------------------------------------------------------------------------
+// The sums.
+// ------------------------------------------------------------------------------------------
+
+// The first entry of the sorted list whose token is at least `token`, by one wave: 64 probes a step.
+__device__ __forceinline__ uint32_t first_of(const Args& a, uint32_t token) {
+    uint32_t lo = 0, hi = a.n;  // entries before lo are smaller, from hi on not
+    while (lo < hi) {
+        const uint64_t span = hi - lo;
+        const uint32_t probe = lo + static_cast<uint32_t>(span * lane_id() / kWave);
+        const uint64_t smaller = ballot(a.from[probe].token < token);  // the lowest lanes
+        const int k = __popcll(smaller);
+        const uint32_t new_hi = k < kWave ? lo + static_cast<uint32_t>(span * k / kWave) : hi;
+        lo = k ? lo + static_cast<uint32_t>(span * (k - 1) / kWave) + 1 : lo;
+        hi = new_hi;
+    }
+    return lo;
+}
+
+// Zeros into the rows [first, first + kZeroRows) that no token names.
+template <typename T>
+__device__ void write_zeros(const Args& a, uint32_t first) {
+    __shared__ uint32_t named[2], range[2];
+    const int wave = uniform(threadIdx.x / kWave);
+    const uint32_t end = min(first + kZeroRows, a.V);
+    if (threadIdx.x < 2) named[threadIdx.x] = 0;
+    if (wave < 2) {
+        const uint32_t at = first_of(a, wave ? end : first);
+        if (lane_id() == 0) range[wave] = at;
+    }
+    __syncthreads();
+    for (uint32_t i = range[0] + threadIdx.x; i < range[1]; i += kThreads) {
+        const uint32_t r = a.from[i].token - first;
+        atomicOr(&named[r / 32], 1u << r % 32);
+    }
+    __syncthreads();
+    constexpr int kN = 16 / sizeof(T);
+    const float zeros[kN] = {};
+    T* out = static_cast<T*>(a.out);
+    for (uint32_t v = first; v < end; ++v) {
+        if (named[(v - first) / 32] >> (v - first) % 32 & 1) continue;
+        for (int c = threadIdx.x * kN; c < a.D; c += kThreads * kN)
+            store_some(out + int64_t(v) * a.D + c, a.D - c, zeros);
+    }
+}
+
+// A group of G lanes a chunk of the sorted list and a slice of the columns.
+template <typename E, typename T, int G>
+__global__ __launch_bounds__(kThreads) void sum_chunks(const Args a) {
+    constexpr int kN = 16 / sizeof(E);
+    if (static_cast<int>(blockIdx.x) >= a.sum_groups) {
+        write_zeros<T>(a, (blockIdx.x - a.sum_groups) * kZeroRows);
+        return;
+    }
+    const int unit = blockIdx.x * (kThreads / G) + threadIdx.x / G;
+    const int chunk = unit / a.slices;
+    const int column = ((unit - chunk * a.slices) * G + int(threadIdx.x % G)) * kN;
+    const int there = a.D - column;
+    if (chunk >= a.chunks || there <= 0) return;
+    const E* d_out = static_cast<const E*>(a.rows) + column;
+    T* out = static_cast<T*>(a.out) + column;
+    const uint32_t begin = static_cast<uint32_t>(chunk) * a.chunk, end = min(begin + a.chunk, a.n);
+    const uint32_t before = begin ? a.from[begin - 1].token : ~0u, after = end < a.n ? a.from[end].token : ~0u;
+    float sum[kN] = {};
+    uint32_t token = a.from[begin].token;
+    bool comes = token == before;  // the sum began in an earlier chunk
+    const auto leave = [&](bool goes) {
+        if (token >= a.V) return;
+        if (comes || goes) {
+            store_some(a.parts + (int64_t(chunk) * 2 + (comes ? 0 : 1)) * a.D + column, there, sum);
+            return;
+        }
+        float v[kN];
+#pragma unroll
+        for (int j = 0; j < kN; ++j) v[j] = sum[j] * a.scale;
+        store_some(out + int64_t(token) * a.D, there, v);
+    };
+    for (uint32_t i = begin; i < end; i += kBatch) {
+        Entry e[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) e[b] = i + b < end ? a.from[i + b] : Entry{a.V, 0};
+        float v[kBatch][kN];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (e[b].token < a.V) load_some(d_out + a.at(e[b].position, a.row_b, a.row_t), there, v[b]);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (i + b >= end) break;
+            if (e[b].token != token) {
+                leave(false);
+                token = e[b].token;
+                comes = false;
+#pragma unroll
+                for (int j = 0; j < kN; ++j) sum[j] = 0.0f;
+            }
+            if (token >= a.V) return;  // padding from here on
+#pragma unroll
+            for (int j = 0; j < kN; ++j) sum[j] += v[b][j];
+        }
+    }
+    leave(token == after);
+}
+
+// The sum that begins in a chunk and goes on behind it, if there is one: a workgroup a slice of 64 packs,
+// a quarter of the parts a wave.
+template <typename E, typename T>
+__global__ __launch_bounds__(kThreads) void join_chunks(const Args a) {
+    constexpr int kN = 16 / sizeof(E), kFlight = 8;
+    __shared__ float sums[kWaves][kN][kWave];
+    const int chunk = blockIdx.x / a.slices, slice = blockIdx.x - chunk * a.slices;
+    const int wave = uniform(threadIdx.x / kWave), lane = lane_id();
+    const uint32_t begin = static_cast<uint32_t>(chunk) * a.chunk, end = begin + a.chunk;
+    if (end >= a.n) return;
+    const uint32_t token = a.from[end].token;
+    if (token >= a.V || a.from[end - 1].token != token) return;
+    if (begin && a.from[begin - 1].token == token) return;  // (so is its first: it began earlier)
+    int parts = 1;  // this chunk's, and those of the chunks that begin with the token
+    for (;;) {
+        const int64_t at = (int64_t(chunk) + parts + lane) * a.chunk;
+        const uint64_t same = ballot(at < a.n && a.from[at < a.n ? at : 0].token == token);
+        const int run = ~same ? __builtin_ctzll(~same) : kWave;
+        parts += run;
+        if (run < kWave) break;
+    }
+    const int column = (slice * kWave + lane) * kN, there = a.D - column;
+    const int from = static_cast<int>(int64_t(parts) * wave / kWaves);
+    const int to = static_cast<int>(int64_t(parts) * (wave + 1) / kWaves);
+    float sum[kN] = {};
+    if (there > 0) {
+        for (int p = from; p < to; p += kFlight) {
+            float v[kFlight][kN];
+#pragma unroll
+            for (int f = 0; f < kFlight; ++f)
+                if (p + f < to)
+                    load_some(a.parts + (int64_t(chunk + p + f) * 2 + (p + f ? 0 : 1)) * a.D + column, there, v[f]);
+#pragma unroll
+            for (int f = 0; f < kFlight; ++f)
+                if (p + f < to)
+#pragma unroll
+                    for (int j = 0; j < kN; ++j) sum[j] += v[f][j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kN; ++j) sums[wave][j][lane] = sum[j];
+    __syncthreads();
+    if (wave || there <= 0) return;
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+        for (int w = 1; w < kWaves; ++w) sum[j] += sums[w][j][lane];
+        sum[j] *= a.scale;
+    }
+    store_some(static_cast<T*>(a.out) + int64_t(token) * a.D + column, there, sum);
+}
+
+// ------------------------------------------------------------------------------------------
+// Launches.
+// ------------------------------------------------------------------------------------------
+
+int size_of(int dtype) { return dtype == HSN_DTYPE_F32 ? 4 : 2; }
+int packs_of(int D, int dtype) { return (D * size_of(dtype) + 15) / 16; }
+int lanes_of(int D, int dtype) { return packs_of(D, dtype) <= 16 ? 16 : kWave; }
+
+void check(int B, int T, int V, int D, int dtype, int other) {
+    for (int t : {dtype, other})
+        HSN_REQUIRE(t == HSN_DTYPE_F32 || t == HSN_DTYPE_F16 || t == HSN_DTYPE_BF16, HSN_ERR_UNSUPPORTED_DTYPE,
+                    "rows must be F32, F16 or BF16");
+    HSN_REQUIRE(B >= 0 && T >= 0 && V >= 1 && D >= 1, HSN_ERR_INVALID_ARGUMENT,
+                "B >= 0, T >= 0, V >= 1 and D >= 1");
+    HSN_REQUIRE(V <= HSN_EMBED_MAX_TOKENS && D <= HSN_EMBED_MAX_WIDTH, HSN_ERR_SIZE_OVERFLOW,
+                "V at most 2^24 and D at most 65536");
+    HSN_REQUIRE(int64_t(B) * T < 1 << 26, HSN_ERR_SIZE_OVERFLOW, "fewer than 2^26 tokens");
+}
+
+void check_rows(const void* p, int dtype, const char* name) {
+    HSN_REQUIRE(p && reinterpret_cast<uintptr_t>(p) % size_of(dtype) == 0, HSN_ERR_INVALID_ARGUMENT,
+                std::string(name) + " must be there and aligned to its type");
+}
+
+// One row of positions where the strides allow it.
+void set_tokens(Args& a, const void* tokens, int64_t b, int64_t t, int bytes, int B, int T) {
+    HSN_REQUIRE(tokens, HSN_ERR_INVALID_ARGUMENT, "tokens is NULL");
+    HSN_REQUIRE(bytes == 8 || bytes == 4, HSN_ERR_INVALID_ARGUMENT, "token_bytes is 8 or 4");
+    a.tokens = tokens, a.token_b = b, a.token_t = t, a.wide = bytes == 8;
+    a.n = static_cast<uint32_t>(B) * T, a.T = T;
+    if (B == 1 || (b == T * t && a.row_b == T * a.row_t)) {
+        a.T = a.n;
+    } else if (T == 1) {
+        a.token_t = b, a.row_t = a.row_b, a.T = a.n;
+    }
+}
+
+template <typename F>
+void with_type(int dtype, F&& f) {
+    if (dtype == HSN_DTYPE_F32)
+        f(float{});
+    else if (dtype == HSN_DTYPE_F16)
+        f(_Float16{});
+    else
+        f(bf16_t{});
+}
+
+// Chunks of the sorted list: as long as leaves some 8192 groups of lanes to fill the GPU, 8 entries (one
+// batch of loads) at least.
+int chunk_of(int64_t n, int D, int dtype) {
+    const int lanes = lanes_of(D, dtype);
+    const int64_t slices = (packs_of(D, dtype) + lanes - 1) / lanes;
+    const int64_t groups = 8192 * (kWave / lanes);
+    int chunk = kBatch;
+    while (chunk < 1024 && n * slices > groups * chunk) chunk *= 2;
+    return chunk;
+}
+
+// Entries a tile: the next launch reads all tiles' counts in every workgroup.
+int items_of(int64_t n) { return n <= 1 << 17 ? 8 : 32; }
+
+struct Workspace {
+    Entry *a, *b;
+    uint32_t* counts;
+    float* parts;
+    int64_t bytes;
+};
+
+Workspace layout(char* at, int64_t n, int D, int dtype) {
+    char* const begin = at;
+    const auto take = [&](int64_t bytes) {
+        char* p = at;
+        at += (bytes + 15) / 16 * 16;
+        return p;
+    };
+    Workspace w;
+    const bool small = n <= kSmall;
+    const int64_t tile = kThreads * items_of(n), chunk = chunk_of(n, D, dtype);
+    w.a = reinterpret_cast<Entry*>(take(8 * n));
+    w.b = reinterpret_cast<Entry*>(take(small ? 0 : 8 * n));
+    w.counts = reinterpret_cast<uint32_t*>(take(small ? 0 : (n + tile - 1) / tile * kBins * 4));
+    w.parts = reinterpret_cast<float*>(take((n + chunk - 1) / chunk * 2 * D * 4));
+    w.bytes = std::max<int64_t>(16, at - begin);
+    return w;
+}
+
+// The entries in the order of their tokens; returns where they are.
+const Entry* sort(Args a, const Workspace& w, hipStream_t st) {
+    int bits = 1;
+    while (a.V >> bits) ++bits;  // padding is V
+    if (a.n <= kSmall) {
+        a.to = w.a, a.bits = bits;
+        sort_small<<<1, kSmallThreads, 0, st>>>(a);
+        HSN_HIP(hipGetLastError());
+        return w.a;
+    }
+    const int passes = (bits + kDigit - 1) / kDigit;
+    const int items = items_of(a.n);
+    a.tiles = static_cast<int>((a.n + kThreads * items - 1) / (kThreads * items));
+    a.counts = w.counts;
+    a.bits = (bits + passes - 1) / passes;
+    for (int p = 0; p < passes; ++p) {
+        a.shift = p * a.bits;
+        a.to = p % 2 ? w.b : w.a;
+        if (items == 8) {
+            count_digits<8><<<a.tiles, kThreads, 0, st>>>(a);
+            HSN_HIP(hipGetLastError());
+            move_entries<8><<<a.tiles, kThreads, 0, st>>>(a);
+        } else {
+            count_digits<32><<<a.tiles, kThreads, 0, st>>>(a);
+            HSN_HIP(hipGetLastError());
+            move_entries<32><<<a.tiles, kThreads, 0, st>>>(a);
+        }
+        HSN_HIP(hipGetLastError());
+        a.from = a.to;
+    }
+    return a.from;
+}
+
+// A grid's dimension holds fewer than 2^32 threads.
+int grid_of(int64_t groups) {
+    HSN_REQUIRE(groups < (int64_t(1) << 32) / kThreads, HSN_ERR_SIZE_OVERFLOW,
+                "more workgroups than one grid holds");
+    return static_cast<int>(groups);
+}
+
+}  // namespace
+}  // namespace embed
+}  // namespace hsn
+
+using namespace hsn;
+using namespace hsn::embed;
+
+extern "C" int hsn_embed_forward(const void* tokens, int64_t token_b, int64_t token_t, int token_bytes,
+                                 const void* table, int64_t table_row, int table_dtype, float scale, void* out,
+                                 int out_dtype, int B, int T, int V, int D, void* stream) {
+    HSN_ABI_BEGIN
+    check(B, T, V, D, table_dtype, out_dtype);
+    if (B == 0 || T == 0) return HSN_OK;
+    check_rows(table, table_dtype, "table");
+    check_rows(out, out_dtype, "out");
+    Args a{};
+    a.rows = table, a.scale = scale, a.out = out, a.V = V, a.D = D;
+    set_tokens(a, tokens, token_b, token_t, token_bytes, B, T);
+    a.row_t = table_row;
+    hipStream_t st = as_stream(stream);
+    with_type(table_dtype, [&](auto e) {
+        with_type(out_dtype, [&](auto o) {
+            using E = decltype(e);
+            using O = decltype(o);
+            const int lanes = lanes_of(D, table_dtype), groups = kThreads / lanes;
+            a.slices = (packs_of(D, table_dtype) + lanes - 1) / lanes;
+            // some 4096 workgroups: 16 a compute unit
+            const int most = std::max(1, 4096 / a.slices);
+            const dim3 grid(std::min<int>((a.n + groups - 1) / groups, most), a.slices);
+            if (lanes == 16)
+                gather<E, O, 16><<<grid, kThreads, 0, st>>>(a);
+            else
+                gather<E, O, kWave><<<grid, kThreads, 0, st>>>(a);
+        });
+    });
+    HSN_HIP(hipGetLastError());
+    HSN_ABI_END
+}
+
+extern "C" int hsn_embed_workspace(int B, int T, int V, int D, int d_out_dtype, int64_t* bytes) {
+    HSN_ABI_BEGIN
+    check(B, T, V, D, d_out_dtype, d_out_dtype);
+    HSN_REQUIRE(bytes, HSN_ERR_INVALID_ARGUMENT, "bytes must not be NULL");
+    *bytes = layout(nullptr, int64_t(B) * T, D, d_out_dtype).bytes;
+    HSN_ABI_END
+}
+
+extern "C" int hsn_embed_backward(const void* tokens, int64_t token_b, int64_t token_t, int token_bytes,
+                                  const void* d_out, int64_t d_out_b, int64_t d_out_t, int d_out_dtype,
+                                  float scale, void* d_table, int table_dtype, int B, int T, int V, int D,
+                                  void* workspace, int64_t workspace_bytes, void* stream) {
+    HSN_ABI_BEGIN
+    check(B, T, V, D, d_out_dtype, table_dtype);
+    check_rows(d_table, table_dtype, "d_table");
+    HSN_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, HSN_ERR_INVALID_ARGUMENT,
+                "the workspace must be there and aligned to 16 bytes");
+    Args a{};
+    a.scale = scale, a.out = d_table, a.V = V, a.D = D;
+    const int64_t n = int64_t(B) * T;
+    if (n) {
+        check_rows(d_out, d_out_dtype, "d_out");
+        a.rows = d_out, a.row_b = d_out_b, a.row_t = d_out_t;
+        set_tokens(a, tokens, token_b, token_t, token_bytes, B, T);
+    }
+    const Workspace w = layout(static_cast<char*>(workspace), n, D, d_out_dtype);
+    HSN_REQUIRE(workspace_bytes >= w.bytes, HSN_ERR_INVALID_ARGUMENT, "the workspace is too small");
+    const int lanes = lanes_of(D, d_out_dtype), groups = kThreads / lanes;
+    a.slices = (packs_of(D, d_out_dtype) + lanes - 1) / lanes;
+    a.chunk = chunk_of(n, D, d_out_dtype);
+    a.chunks = static_cast<int>((n + a.chunk - 1) / a.chunk);
+    const int64_t units = int64_t(a.chunks) * a.slices, zeros = (V + kZeroRows - 1) / kZeroRows;
+    const int grid = grid_of((units + groups - 1) / groups + zeros);
+    const int joins = grid_of(int64_t(a.chunks) * ((packs_of(D, d_out_dtype) + kWave - 1) / kWave));
+    a.sum_groups = grid - static_cast<int>(zeros);
+    a.parts = w.parts;
+    hipStream_t st = as_stream(stream);
+    if (n) a.from = sort(a, w, st);
+    with_type(d_out_dtype, [&](auto e) {
+        with_type(table_dtype, [&](auto t) {
+            using E = decltype(e);
+            using T_ = decltype(t);
+            if (lanes == 16)
+                sum_chunks<E, T_, 16><<<grid, kThreads, 0, st>>>(a);
+            else
+                sum_chunks<E, T_, kWave><<<grid, kThreads, 0, st>>>(a);
+            HSN_HIP(hipGetLastError());
+            if (a.chunks < 2) return;
+            Args j = a;
+            j.slices = (packs_of(D, d_out_dtype) + kWave - 1) / kWave;
+            join_chunks<E, T_><<<joins, kThreads, 0, st>>>(j);
+            HSN_HIP(hipGetLastError());
+        });
+    });
+    HSN_ABI_END
+}

@@ -1,8 +1,9 @@
-// The calls of a decoded token in one step from the interpreter: the language-model operators'
-// Python mirrors (hsn_amd/scan.py, unit_layer.py, sampling.py, scoring.py, unit_router.py, grad_clip.py)
-// check their tensors, allocate outputs and workspace and call the C entry point through this module where it is
-// built. Made in the interpreter, the checks, allocations and the conversion of some twenty arguments
-// cost 4 to 6 us a call, more than the kernel of a single position; here they cost about 1 us.
+// The calls of a decoded token and of a training step's operators in one step from the interpreter: the
+// language-model operators' Python mirrors (hsn_amd/scan.py, unit_layer.py, sampling.py, embedding.py,
+// scoring.py, unit_router.py, grad_clip.py) check their tensors, allocate outputs and workspace and call
+// the C entry point through this module where it is built. Made in the interpreter, the checks,
+// allocations and the conversion of some twenty arguments cost 4 to 6 us a call, more than the kernel of a
+// single position; here they cost about 1 us.
 //
 // Every function takes the C entry points' addresses and the raw stream, and returns
 //   None   a check failed: nothing was allocated or launched, and the caller makes the same checks in
@@ -24,6 +25,7 @@
 #include <initializer_list>
 #include <vector>
 
+#include "../../include/hsn_embed.h"
 #include "../../include/hsn_sample.h"
 #include "../../include/hsn_score.h"
 #include "../../include/hsn_unit_router.h"
@@ -313,6 +315,94 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// Tokens of any shape as B rows of T; a shape that is neither is not `ok`.
+struct Tokens {
+    int64_t B = 1, T = 1, stride_b = 0, stride_t = 0;
+    int bytes = 0;
+    bool ok = false;
+    explicit Tokens(const Tensor* t) {
+        if (!t || !t->is_cuda() || !plain(*t)) return;
+        bytes = t->scalar_type() == at::kLong ? 8 : t->scalar_type() == at::kInt ? 4 : 0;
+        const int64_t dims = t->dim();
+        if (dims == 1) {
+            T = t->size(0), stride_t = t->stride(0);
+        } else if (dims == 2) {
+            B = t->size(0), T = t->size(1), stride_b = t->stride(0), stride_t = t->stride(1);
+        } else if (dims > 2) {
+            return;
+        }
+        ok = bytes && B <= INT32_MAX && T <= INT32_MAX && B * T < 1 << 26;
+    }
+};
+
+// embed_forward(forward, stream, tokens, table, scale, dtype)
+PyObject* embed_forward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Arguments in{args, args + n_args};
+    const int64_t call_at = in.integer(), stream = in.integer();
+    const Tensor *tokens = in.tensor(), *table = in.tensor();
+    const double scale = in.number();
+    const int64_t out_code = in.integer();
+    if (!in.ok || !table || table->dim() != 2 || !table->is_cuda() || out_code < 0) Py_RETURN_NONE;
+    const Tokens of(tokens);
+    const int code = dtype_code(table->scalar_type());
+    const int64_t V = table->size(0), D = table->size(1);
+    if (!of.ok || code < 0 || tokens->device() != table->device() || !like(table, *table) || V < 1 ||
+        V > HSN_EMBED_MAX_TOKENS || D < 1 || D > HSN_EMBED_MAX_WIDTH)
+        Py_RETURN_NONE;
+    const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(table->device());
+    std::vector<int64_t> shape = tokens->sizes().vec();
+    shape.push_back(D);
+    const auto type = out_code == 0 ? at::kFloat : out_code == 1 ? at::kHalf : at::kBFloat16;
+    const Tensor out = at::empty(shape, at::TensorOptions().device(table->device()).dtype(type));
+    const int status = entry<int (*)(P, int64_t, int64_t, int, P, int64_t, int, float, P, int, int, int, int,
+                                     int, P)>(call_at)(
+        tokens->data_ptr(), of.stride_b, of.stride_t, of.bytes, table->data_ptr(), table->stride(0), code,
+        static_cast<float>(scale), out.data_ptr(), out_code, of.B, of.T, V, D, entry<P>(stream));
+    if (status) return PyLong_FromLong(status);
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// embed_backward(workspace, backward, stream, tokens, d_out, V, scale, dtype)
+PyObject* embed_backward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Arguments in{args, args + n_args};
+    const int64_t size_at = in.integer(), call_at = in.integer(), stream = in.integer();
+    const Tensor *tokens = in.tensor(), *d_out = in.tensor();
+    const int64_t V = in.integer();
+    const double scale = in.number();
+    const int64_t out_code = in.integer();
+    if (!in.ok || !d_out || !d_out->is_cuda() || out_code < 0) Py_RETURN_NONE;
+    const Tokens of(tokens);
+    const int code = dtype_code(d_out->scalar_type());
+    if (!of.ok || code < 0 || tokens->device() != d_out->device() || d_out->dim() != tokens->dim() + 1 ||
+        !like(d_out, *d_out) || V < 1 || V > HSN_EMBED_MAX_TOKENS)
+        Py_RETURN_NONE;
+    for (int64_t d = 0; d < tokens->dim(); ++d)
+        if (tokens->size(d) != d_out->size(d)) Py_RETURN_NONE;
+    const int64_t D = d_out->size(-1), dims = tokens->dim();
+    if (D < 1 || D > HSN_EMBED_MAX_WIDTH) Py_RETURN_NONE;
+    int64_t bytes = 0;
+    int status = entry<int (*)(int, int, int, int, int, int64_t*)>(size_at)(of.B, of.T, V, D, code, &bytes);
+    if (status) return PyLong_FromLong(status);
+    const at::NoGradGuard no_grad;
+    const c10::DeviceGuard current(d_out->device());
+    const auto on = at::TensorOptions().device(d_out->device());
+    const auto type = out_code == 0 ? at::kFloat : out_code == 1 ? at::kHalf : at::kBFloat16;
+    const Tensor d_table = at::empty({V, D}, on.dtype(type));
+    const Tensor ws = workspace(bytes, on);
+    status = entry<int (*)(P, int64_t, int64_t, int, P, int64_t, int64_t, int, float, P, int, int, int, int,
+                           int, P, int64_t, P)>(call_at)(
+        tokens->data_ptr(), of.stride_b, of.stride_t, of.bytes, d_out->data_ptr(),
+        dims == 2 ? d_out->stride(0) : 0, dims ? d_out->stride(dims - 1) : 0, code, static_cast<float>(scale),
+        d_table.data_ptr(), out_code, of.B, of.T, V, D, ws.data_ptr(), bytes, entry<P>(stream));
+    if (status) return PyLong_FromLong(status);
+    return wrap(d_table);
+    END_HANDLE_TH_ERRORS
+}
+
 // Logits [n, V] whose rows are contiguous, and a token a row (int64 or int32).
 struct Rows {
     const Tensor *logits, *tokens;
@@ -553,6 +643,10 @@ PyMethodDef kMethods[] = {
      "(workspace, layer, stream, x, router, W1, b1, W2, b2, k, activation, gated) -> y"},
     {"sample", fast<sample>(), METH_FASTCALL,
      "(workspace, sample, stream, logits, u, temperature, top_k, top_p, min_p) -> tokens"},
+    {"embed_forward", fast<embed_forward>(), METH_FASTCALL,
+     "(forward, stream, tokens, table, scale, dtype) -> out"},
+    {"embed_backward", fast<embed_backward>(), METH_FASTCALL,
+     "(workspace, backward, stream, tokens, d_out, V, scale, dtype) -> d_table"},
     {"score_forward", fast<score_forward>(), METH_FASTCALL,
      "(workspace, forward, stream, logits, tokens, top, save) -> (logprob, entropy, top_tokens, "
      "top_logprobs, stats)"},
