@@ -5,8 +5,8 @@
 // Backward: the positions are sorted by token, and then every sum is over neighbours. The sort is by digits
 // of up to ten bits from the lowest on, stable, so a token's positions stay in order: a workgroup counts a
 // tile's digits, and the next launch ranks the tile's entries (lanes of a wave with the same digit find each
-// other by ballots) and adds up where they go from all tiles' counts; up to 4096 positions are sorted by
-// one workgroup in LDS. The sums are taken over chunks of the sorted list, one as long as the other, so a
+// other by ballots) and adds up where they go from all tiles' counts. Up to 16384 positions need one launch:
+// each workgroup counts, for a few entries, what lies before them in the whole list. The sums are taken over chunks of the sorted list, one as long as the other, so a
 // token that fills a tenth of the text costs no workgroup more than another: a group of lanes walks a
 // chunk with a slice of the columns, writes the rows that begin and end inside it, and leaves the sums
 // that cross a border to a last launch, which adds them in order. Workgroups of the same launch write the
@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kDigit = 10, kBins = 1 << kDigit;
-constexpr int kSmall = 4096, kSmallThreads = 512, kSmallWaves = kSmallThreads / kWave;
+constexpr int kSmall = 16384, kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
 constexpr int kBatch = 8;       // entries of a chunk in flight
 constexpr int kZeroRows = 64;   // rows that a workgroup looks through for those without a token
 
@@ -65,7 +65,7 @@ struct Args {
     }
 };
 
-// kN elements at any address, from or to fp32. Of `there` the first ones alone.
+// N elements at any address, from or to fp32. A row of fewer than N has `there` of them.
 template <typename E, int N>
 __device__ __forceinline__ void load_some(const E* p, int there, float (&v)[N]) {
     if (there >= N) {
@@ -92,6 +92,14 @@ __device__ __forceinline__ void store_some(E* p, int there, const float (&v)[N])
     }
 }
 
+// The first of N columns of a lane: a row's last pack ends with the row, and where it overlaps the one before
+// both lanes compute and write the same values. (Its elements one by one, each with a branch and a wait of
+// its own, took most of a narrow row's time.)
+template <int N>
+__device__ __forceinline__ int column_of(int pack, int D) {
+    return max(0, min(pack * N, D - N));
+}
+
 // ------------------------------------------------------------------------------------------
 // Forward.
 // ------------------------------------------------------------------------------------------
@@ -100,8 +108,9 @@ __device__ __forceinline__ void store_some(E* p, int there, const float (&v)[N])
 template <typename E, typename O, int G>
 __global__ __launch_bounds__(kThreads) void gather(const Args a) {
     constexpr int kN = 16 / sizeof(E), kGroups = kThreads / G, kFlight = 4;
-    const int column = (int(blockIdx.y) * G + int(threadIdx.x % G)) * kN, there = a.D - column;
-    if (there <= 0) return;
+    const int pack = int(blockIdx.y) * G + int(threadIdx.x % G);
+    if (pack * kN >= a.D) return;
+    const int column = column_of<kN>(pack, a.D), there = a.D - column;
     const E* table = static_cast<const E*>(a.rows) + column;
     O* out = static_cast<O*>(a.out) + column;
     const uint32_t step = gridDim.x * kGroups;
@@ -173,57 +182,41 @@ __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t* s) {
     return sum - v;
 }
 
-__global__ __launch_bounds__(kSmallThreads) void sort_small(const Args a) {
-    constexpr int kItems = kSmall / kSmallThreads, kMine = kBins / kSmallThreads;
-    __shared__ Entry list[kSmall];
-    __shared__ uint16_t count[kSmallWaves][kBins];
-    __shared__ uint32_t s[kSmallWaves];
+// The whole list of up to R 1024 positions in one launch: entry i's place is the number of entries with a
+// smaller token and of earlier ones with the same. A wave holds a sixteenth of the list, 64 entries a
+// register, and counts for one entry after the other: a comparison of 64 is one vector instruction, its
+// ballot's bits are counted by scalar ones. With k' = 2 k + (1 for the entries' own 64 and later ones), k' < 2
+// k_i + 1 says k < k_i there and k <= k_i before; what is equal and earlier among the entries' own 64 is
+// added by one wave. 8192 entries take 5 us, where two digits by two launches each took 24.
+template <int R>
+__global__ __launch_bounds__(kSmallThreads) void sort_small(const Args a, int entries) {
+    __shared__ int counts[kSmallWaves][kWave];
     const int wave = uniform(threadIdx.x / kWave), lane = lane_id();
-    Entry e[kItems];
-    uint32_t digit[kItems], rank[kItems];
+    const uint32_t first = blockIdx.x * entries, own = first / kWave;
+    uint32_t key[R];
 #pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-        const uint32_t i = (wave * kItems + r) * kWave + lane;
-        e[r] = {i < a.n ? a.token(i) : ~0u, i};  // (what is behind the end stays there: every digit is the largest)
+    for (int r = 0; r < R; ++r) {
+        const uint32_t block = wave * R + r, i = block * kWave + lane;
+        key[r] = 2 * (i < a.n ? a.token(i) : 1u << 30) + (block >= own ? 1 : 0);
     }
-    for (int shift = 0; shift < a.bits; shift += kDigit) {
-        const int bits = min(kDigit, a.bits - shift);
-        for (int b = threadIdx.x; b < kSmallWaves * kBins; b += kSmallThreads) (&count[0][0])[b] = 0;
-        __syncthreads();
+    const uint32_t mine = first + lane;  // the lane's entry, of the first `entries` lanes
+    const uint32_t token = lane < entries && mine < a.n ? a.token(mine) : 0;
+    uint32_t near = ~0u;
+    if (wave == 0 && own * kWave + lane < a.n) near = a.token(own * kWave + lane);
+    int count = 0;
+    for (int i = 0; i < entries; ++i) {
+        const uint32_t t = readlane(token, i);
+        int c = 0;
 #pragma unroll
-        for (int r = 0; r < kItems; ++r) digit[r] = e[r].token >> shift & ((1u << bits) - 1);
-        rank_wave(digit, bits, count[wave], rank);
-        __syncthreads();
-        uint32_t total[kMine], all = 0;
-#pragma unroll
-        for (int b = 0; b < kMine; ++b) {
-            total[b] = 0;
-            for (int w = 0; w < kSmallWaves; ++w) {  // the waves' counts become what is before them
-                const uint32_t c = count[w][threadIdx.x * kMine + b];
-                count[w][threadIdx.x * kMine + b] = static_cast<uint16_t>(total[b]);
-                total[b] += c;
-            }
-            all += total[b];
-        }
-        uint32_t before = block_before<kSmallWaves>(all, s);
-#pragma unroll
-        for (int b = 0; b < kMine; ++b) {
-            for (int w = 0; w < kSmallWaves; ++w)
-                count[w][threadIdx.x * kMine + b] += static_cast<uint16_t>(before);
-            before += total[b];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kItems; ++r) list[count[wave][digit[r]] + rank[r]] = e[r];
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kItems; ++r) e[r] = list[(wave * kItems + r) * kWave + lane];
+        for (int r = 0; r < R; ++r) c += __popcll(ballot(key[r] < 2 * t + 1));
+        if (wave == 0) c += __popcll(ballot(near == t && own * kWave + lane < first + i));
+        if (lane == i) count = c;
     }
-#pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-        const uint32_t i = (wave * kItems + r) * kWave + lane;
-        if (i < a.n) a.to[i] = e[r];
-    }
+    counts[wave][lane] = count;
+    __syncthreads();
+    if (wave || lane >= entries || mine >= a.n) return;
+    for (int w = 1; w < kSmallWaves; ++w) count += counts[w][lane];
+    a.to[count] = {token, mine};
 }
 
 // Entry i before this pass: the first one reads the tokens.
@@ -316,7 +309,7 @@ __device__ __forceinline__ uint32_t first_of(const Args& a, uint32_t token) {
 }
 
 // Zeros into the rows [first, first + kZeroRows) that no token names.
-template <typename T>
+template <typename T, int G>
 __device__ void write_zeros(const Args& a, uint32_t first) {
     __shared__ uint32_t named[2], range[2];
     const int wave = uniform(threadIdx.x / kWave);
@@ -335,10 +328,12 @@ __device__ void write_zeros(const Args& a, uint32_t first) {
     constexpr int kN = 16 / sizeof(T);
     const float zeros[kN] = {};
     T* out = static_cast<T*>(a.out);
-    for (uint32_t v = first; v < end; ++v) {
+    for (uint32_t v = first + threadIdx.x / G; v < end; v += kThreads / G) {
         if (named[(v - first) / 32] >> (v - first) % 32 & 1) continue;
-        for (int c = threadIdx.x * kN; c < a.D; c += kThreads * kN)
+        for (int pack = threadIdx.x % G; pack * kN < a.D; pack += G) {
+            const int c = column_of<kN>(pack, a.D);
             store_some(out + int64_t(v) * a.D + c, a.D - c, zeros);
+        }
     }
 }
 
@@ -347,14 +342,14 @@ template <typename E, typename T, int G>
 __global__ __launch_bounds__(kThreads) void sum_chunks(const Args a) {
     constexpr int kN = 16 / sizeof(E);
     if (static_cast<int>(blockIdx.x) >= a.sum_groups) {
-        write_zeros<T>(a, (blockIdx.x - a.sum_groups) * kZeroRows);
+        write_zeros<T, G>(a, (blockIdx.x - a.sum_groups) * kZeroRows);
         return;
     }
     const int unit = blockIdx.x * (kThreads / G) + threadIdx.x / G;
     const int chunk = unit / a.slices;
-    const int column = ((unit - chunk * a.slices) * G + int(threadIdx.x % G)) * kN;
-    const int there = a.D - column;
-    if (chunk >= a.chunks || there <= 0) return;
+    const int pack = (unit - chunk * a.slices) * G + int(threadIdx.x % G);
+    if (chunk >= a.chunks || pack * kN >= a.D) return;
+    const int column = column_of<kN>(pack, a.D), there = a.D - column;
     const E* d_out = static_cast<const E*>(a.rows) + column;
     T* out = static_cast<T*>(a.out) + column;
     const uint32_t begin = static_cast<uint32_t>(chunk) * a.chunk, end = min(begin + a.chunk, a.n);
@@ -420,7 +415,8 @@ __global__ __launch_bounds__(kThreads) void join_chunks(const Args a) {
         parts += run;
         if (run < kWave) break;
     }
-    const int column = (slice * kWave + lane) * kN, there = a.D - column;
+    const int pack = slice * kWave + lane, column = column_of<kN>(pack, a.D);
+    const int there = pack * kN < a.D ? a.D - column : 0;
     const int from = static_cast<int>(int64_t(parts) * wave / kWaves);
     const int to = static_cast<int>(int64_t(parts) * (wave + 1) / kWaves);
     float sum[kN] = {};
@@ -541,8 +537,14 @@ const Entry* sort(Args a, const Workspace& w, hipStream_t st) {
     int bits = 1;
     while (a.V >> bits) ++bits;  // padding is V
     if (a.n <= kSmall) {
-        a.to = w.a, a.bits = bits;
-        sort_small<<<1, kSmallThreads, 0, st>>>(a);
+        a.to = w.a;
+        const int entries = a.n <= 8192 ? 16 : 32, grid = (a.n + entries - 1) / entries;
+        const int held = (a.n + kSmallThreads - 1) / kSmallThreads;
+        (held <= 1   ? sort_small<1>
+         : held <= 2 ? sort_small<2>
+         : held <= 4 ? sort_small<4>
+         : held <= 8 ? sort_small<8>
+                     : sort_small<16>)<<<grid, kSmallThreads, 0, st>>>(a, entries);
         HSN_HIP(hipGetLastError());
         return w.a;
     }
@@ -600,15 +602,18 @@ extern "C" int hsn_embed_forward(const void* tokens, int64_t token_b, int64_t to
         with_type(out_dtype, [&](auto o) {
             using E = decltype(e);
             using O = decltype(o);
-            const int lanes = lanes_of(D, table_dtype), groups = kThreads / lanes;
-            a.slices = (packs_of(D, table_dtype) + lanes - 1) / lanes;
+            const int packs = packs_of(D, table_dtype);
+            const int lanes = packs <= 16 ? 16 : packs <= kWave ? kWave : kThreads, groups = kThreads / lanes;
+            a.slices = (packs + lanes - 1) / lanes;
             // some 4096 workgroups: 16 a compute unit
             const int most = std::max(1, 4096 / a.slices);
             const dim3 grid(std::min<int>((a.n + groups - 1) / groups, most), a.slices);
             if (lanes == 16)
                 gather<E, O, 16><<<grid, kThreads, 0, st>>>(a);
-            else
+            else if (lanes == kWave)
                 gather<E, O, kWave><<<grid, kThreads, 0, st>>>(a);
+            else
+                gather<E, O, kThreads><<<grid, kThreads, 0, st>>>(a);
         });
     });
     HSN_HIP(hipGetLastError());
