@@ -28,6 +28,7 @@ constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kDigit = 10, kBins = 1 << kDigit;
 constexpr int kSmall = 16384, kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
 constexpr int kBatch = 8;       // entries of a chunk in flight
+constexpr int kCounts = 16;     // tiles' counts in flight
 constexpr int kZeroRows = 64;   // rows that a workgroup looks through for those without a token
 
 struct Entry {
@@ -53,51 +54,70 @@ struct Args {
     // the sums
     int chunk, chunks, sum_groups;  // sum_groups: workgroups of sums before those that write zeros
     float* parts;  // [chunks, 2, D]: the sum that comes from the chunk before, the one that begins here
-    __device__ __forceinline__ int64_t at(uint32_t i, int64_t b, int64_t t) const {
-        if (T == n) return i * t;
-        const uint32_t r = i / T;
-        return r * b + int64_t(i - r * T) * t;
-    }
-    __device__ __forceinline__ uint32_t token(uint32_t i) const {
-        const int64_t o = at(i, token_b, token_t);
-        const int64_t t = wide ? static_cast<const int64_t*>(tokens)[o] : static_cast<const int32_t*>(tokens)[o];
-        return t >= 0 && t < V ? static_cast<uint32_t>(t) : V;
-    }
 };
 
-// N elements at any address, from or to fp32. A row of fewer than N has `there` of them.
-template <typename E, int N>
-__device__ __forceinline__ void load_some(const E* p, int there, float (&v)[N]) {
-    if (there >= N) {
-        E e[N];
-        __builtin_memcpy(e, p, sizeof(e));
+// Positions' offsets, and their tokens (V: padding). The branches are taken once for all N, so that the loads
+// are in flight together: each in a branch of its own, every one waits for the one before.
+template <int N>
+__device__ __forceinline__ void offsets_of(const Args& a, const uint32_t (&i)[N], int64_t b, int64_t t,
+                                           int64_t (&at)[N]) {
+    if (a.T == a.n) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = to_f32(e[j]);
+        for (int f = 0; f < N; ++f) at[f] = i[f] * t;
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = j < there ? to_f32(p[j]) : 0.0f;
+        for (int f = 0; f < N; ++f) {
+            const uint32_t r = i[f] / a.T;
+            at[f] = r * b + int64_t(i[f] - r * a.T) * t;
+        }
     }
 }
-template <typename E, int N>
-__device__ __forceinline__ void store_some(E* p, int there, const float (&v)[N]) {
-    if (there >= N) {
-        E e[N];
+template <int N>
+__device__ __forceinline__ void tokens_of(const Args& a, const uint32_t (&i)[N], uint32_t (&token)[N]) {
+    int64_t at[N], raw[N];
+    offsets_of(a, i, a.token_b, a.token_t, at);
+    if (a.wide) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) e[j] = from_f32<E>(v[j]);
-        __builtin_memcpy(p, e, sizeof(e));
+        for (int f = 0; f < N; ++f) raw[f] = static_cast<const int64_t*>(a.tokens)[at[f]];
     } else {
+        int32_t narrow[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j < there) p[j] = from_f32<E>(v[j]);
+        for (int f = 0; f < N; ++f) narrow[f] = static_cast<const int32_t*>(a.tokens)[at[f]];
+#pragma unroll
+        for (int f = 0; f < N; ++f) raw[f] = narrow[f];
     }
+#pragma unroll
+    for (int f = 0; f < N; ++f) token[f] = raw[f] >= 0 && raw[f] < a.V ? static_cast<uint32_t>(raw[f]) : a.V;
 }
 
-// The first of N columns of a lane: a row's last pack ends with the row, and where it overlaps the one before
+// A product rounded to fp32, whatever it is rounded to next: left to itself, the compiler takes fp16 products
+// by an instruction that rounds once in some places and not in others.
+__device__ __forceinline__ float times(float a, float b) {
+    float p = a * b;
+    asm("" : "+v"(p));
+    return p;
+}
+
+// F times N elements, and N elements, at any address.
+template <typename E, int F, int N>
+__device__ __forceinline__ void load_some(const E* p, const int64_t (&at)[F], E (&v)[F][N]) {
+#pragma unroll
+    for (int f = 0; f < F; ++f) __builtin_memcpy(v[f], p + at[f], sizeof(v[f]));
+}
+template <typename E, int N>
+__device__ __forceinline__ void store_some(E* p, const float (&v)[N]) {
+    E e[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) e[j] = from_f32<E>(v[j]);
+    __builtin_memcpy(p, e, sizeof(e));
+}
+
+// The first of a lane's N columns: a row's last pack ends with the row, and where it overlaps the one before
 // both lanes compute and write the same values. (Its elements one by one, each with a branch and a wait of
-// its own, took most of a narrow row's time.)
+// its own, took most of a narrow row's time.) Rows of less than a pack have one column a lane.
 template <int N>
 __device__ __forceinline__ int column_of(int pack, int D) {
-    return max(0, min(pack * N, D - N));
+    return min(pack * N, D - N);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -105,33 +125,32 @@ __device__ __forceinline__ int column_of(int pack, int D) {
 // ------------------------------------------------------------------------------------------
 
 // A group of G lanes a slice of a row (blockIdx.y), several positions in flight.
-template <typename E, typename O, int G>
+template <typename E, typename O, int G, int kN>
 __global__ __launch_bounds__(kThreads) void gather(const Args a) {
-    constexpr int kN = 16 / sizeof(E), kGroups = kThreads / G, kFlight = 4;
+    constexpr int kGroups = kThreads / G, kFlight = 4;
     const int pack = int(blockIdx.y) * G + int(threadIdx.x % G);
     if (pack * kN >= a.D) return;
-    const int column = column_of<kN>(pack, a.D), there = a.D - column;
+    const int column = column_of<kN>(pack, a.D);
     const E* table = static_cast<const E*>(a.rows) + column;
     O* out = static_cast<O*>(a.out) + column;
     const uint32_t step = gridDim.x * kGroups;
     for (uint32_t i = blockIdx.x * kGroups + threadIdx.x / G; i < a.n; i += kFlight * step) {
-        uint32_t token[kFlight];
-        float v[kFlight][kN];
+        uint32_t position[kFlight], token[kFlight];
+        int64_t at[kFlight];
+        E e[kFlight][kN];
 #pragma unroll
-        for (int f = 0; f < kFlight; ++f) token[f] = i + f * step < a.n ? a.token(i + f * step) : a.V;
+        for (int f = 0; f < kFlight; ++f) position[f] = min(i + f * step, a.n - 1);
+        tokens_of(a, position, token);
 #pragma unroll
-        for (int f = 0; f < kFlight; ++f) {
-#pragma unroll
-            for (int j = 0; j < kN; ++j) v[f][j] = 0.0f;
-            if (token[f] < a.V) load_some(table + token[f] * a.row_t, there, v[f]);
-        }
+        for (int f = 0; f < kFlight; ++f) at[f] = min(token[f], a.V - 1) * a.row_t;
+        load_some(table, at, e);
 #pragma unroll
         for (int f = 0; f < kFlight; ++f) {
             if (i + f * step >= a.n) break;
-            if (token[f] < a.V)
+            float v[kN];
 #pragma unroll
-                for (int j = 0; j < kN; ++j) v[f][j] *= a.scale;
-            store_some(out + int64_t(i + f * step) * a.D, there, v[f]);
+            for (int j = 0; j < kN; ++j) v[j] = token[f] < a.V ? times(to_f32(e[f][j]), a.scale) : 0.0f;
+            store_some(out + int64_t(i + f * step) * a.D, v);
         }
     }
 }
@@ -187,29 +206,33 @@ __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t* s) {
 // register, and counts for one entry after the other: a comparison of 64 is one vector instruction, its
 // ballot's bits are counted by scalar ones. With k' = 2 k + (1 for the entries' own 64 and later ones), k' < 2
 // k_i + 1 says k < k_i there and k <= k_i before; what is equal and earlier among the entries' own 64 is
-// added by one wave. 8192 entries take 5 us, where two digits by two launches each took 24.
+// added by one wave. 8192 entries take 10 us, where two digits by two launches each took 24; the scalar
+// counts bound it.
 template <int R>
 __global__ __launch_bounds__(kSmallThreads) void sort_small(const Args a, int entries) {
     __shared__ int counts[kSmallWaves][kWave];
     const int wave = uniform(threadIdx.x / kWave), lane = lane_id();
     const uint32_t first = blockIdx.x * entries, own = first / kWave;
-    uint32_t key[R];
+    // the list; then the lane's entry (of the first `entries` lanes) and the lane's of the entries' own 64
+    uint32_t at[R + 2], key[R + 2];
+    const uint32_t mine = first + lane, beside = own * kWave + lane;
+#pragma unroll
+    for (int r = 0; r < R; ++r) at[r] = min((wave * R + r) * kWave + lane, a.n - 1);
+    at[R] = min(mine, a.n - 1), at[R + 1] = min(beside, a.n - 1);
+    tokens_of(a, at, key);
+    const uint32_t token = key[R], near = beside < a.n ? key[R + 1] : ~0u;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const uint32_t block = wave * R + r, i = block * kWave + lane;
-        key[r] = 2 * (i < a.n ? a.token(i) : 1u << 30) + (block >= own ? 1 : 0);
+        const uint32_t block = wave * R + r;
+        key[r] = 2 * (block * kWave + lane < a.n ? key[r] : 1u << 30) + (block >= own ? 1 : 0);
     }
-    const uint32_t mine = first + lane;  // the lane's entry, of the first `entries` lanes
-    const uint32_t token = lane < entries && mine < a.n ? a.token(mine) : 0;
-    uint32_t near = ~0u;
-    if (wave == 0 && own * kWave + lane < a.n) near = a.token(own * kWave + lane);
     int count = 0;
     for (int i = 0; i < entries; ++i) {
         const uint32_t t = readlane(token, i);
         int c = 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) c += __popcll(ballot(key[r] < 2 * t + 1));
-        if (wave == 0) c += __popcll(ballot(near == t && own * kWave + lane < first + i));
+        if (wave == 0) c += __popcll(ballot(near == t && beside < first + i));
         if (lane == i) count = c;
     }
     counts[wave][lane] = count;
@@ -219,22 +242,34 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small(const Args a, int en
     a.to[count] = {token, mine};
 }
 
-// Entry i before this pass: the first one reads the tokens.
-__device__ __forceinline__ Entry entry_of(const Args& a, uint32_t i) {
-    return a.from ? a.from[i] : Entry{a.token(i), i};
+// Entries before this pass: the first one reads the tokens.
+template <int N>
+__device__ __forceinline__ void entries_of(const Args& a, const uint32_t (&i)[N], Entry (&e)[N]) {
+    if (a.from) {
+#pragma unroll
+        for (int r = 0; r < N; ++r) e[r] = a.from[i[r]];
+    } else {
+        uint32_t token[N];
+        tokens_of(a, i, token);
+#pragma unroll
+        for (int r = 0; r < N; ++r) e[r] = {token[r], i[r]};
+    }
 }
 
 template <int ITEMS>
 __global__ __launch_bounds__(kThreads) void count_digits(const Args a) {
     __shared__ uint32_t count[kBins];
     for (int b = threadIdx.x; b < kBins; b += kThreads) count[b] = 0;
-    __syncthreads();
     const uint32_t begin = blockIdx.x * (kThreads * ITEMS), mask = (1u << a.bits) - 1;
+    uint32_t i[ITEMS];
+    Entry e[ITEMS];
 #pragma unroll
-    for (int r = 0; r < ITEMS; ++r) {
-        const uint32_t i = begin + r * kThreads + threadIdx.x;
-        if (i < a.n) atomicAdd(&count[(a.from ? a.from[i].token : a.token(i)) >> a.shift & mask], 1u);
-    }
+    for (int r = 0; r < ITEMS; ++r) i[r] = min(begin + r * kThreads + threadIdx.x, a.n - 1);
+    entries_of(a, i, e);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+        if (begin + r * kThreads + threadIdx.x < a.n) atomicAdd(&count[e[r].token >> a.shift & mask], 1u);
     __syncthreads();
     for (int b = threadIdx.x; b < kBins; b += kThreads) a.counts[int64_t(blockIdx.x) * kBins + b] = count[b];
 }
@@ -250,26 +285,32 @@ __global__ __launch_bounds__(kThreads) void move_entries(const Args a) {
     Entry e[ITEMS];
     uint32_t digit[ITEMS], rank[ITEMS];
 #pragma unroll
-    for (int r = 0; r < ITEMS; ++r) {
-        const uint32_t i = begin + r * kWave;
-        e[r] = i < a.n ? entry_of(a, i) : Entry{~0u, 0};  // (not moved, and behind all others)
-        digit[r] = e[r].token >> a.shift & ((1u << a.bits) - 1);
+    for (int r = 0; r < ITEMS; ++r) rank[r] = min(begin + r * kWave, a.n - 1);
+    entries_of(a, rank, e);
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {  // what is behind the end is not moved, and behind all others
+        digit[r] = (begin + r * kWave < a.n ? e[r].token : ~0u) >> a.shift & ((1u << a.bits) - 1);
     }
-    __syncthreads();
-    rank_wave(digit, a.bits, count[wave], rank);
     // where a digit's entries of this tile begin: all entries of lower digits, those of earlier tiles
     uint32_t total[kMine] = {}, earlier[kMine] = {}, all = 0;
     const uint32_t first = threadIdx.x * kMine;
-#pragma unroll 4
-    for (int t = 0; t < a.tiles; ++t) {
-        const uint4 c = *reinterpret_cast<const uint4*>(a.counts + int64_t(t) * kBins + first);
-        const uint32_t v[kMine] = {c.x, c.y, c.z, c.w};
+    for (int t0 = 0; t0 < a.tiles; t0 += kCounts) {
+        uint4 c[kCounts];
 #pragma unroll
-        for (int b = 0; b < kMine; ++b) {
-            total[b] += v[b];
-            earlier[b] += t < static_cast<int>(blockIdx.x) ? v[b] : 0;
+        for (int f = 0; f < kCounts; ++f)
+            c[f] = *reinterpret_cast<const uint4*>(a.counts + int64_t(min(t0 + f, a.tiles - 1)) * kBins + first);
+#pragma unroll
+        for (int f = 0; f < kCounts; ++f) {
+            const uint32_t v[kMine] = {c[f].x, c[f].y, c[f].z, c[f].w};
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) {
+                total[b] += t0 + f < a.tiles ? v[b] : 0;
+                earlier[b] += t0 + f < static_cast<int>(blockIdx.x) ? v[b] : 0;
+            }
         }
     }
+    __syncthreads();
+    rank_wave(digit, a.bits, count[wave], rank);
 #pragma unroll
     for (int b = 0; b < kMine; ++b) all += total[b];
     uint32_t before = block_before<kWaves>(all, s);  // (passes a barrier: the waves' counts are there)
@@ -309,7 +350,7 @@ __device__ __forceinline__ uint32_t first_of(const Args& a, uint32_t token) {
 }
 
 // Zeros into the rows [first, first + kZeroRows) that no token names.
-template <typename T, int G>
+template <typename T, int G, int kN>
 __device__ void write_zeros(const Args& a, uint32_t first) {
     __shared__ uint32_t named[2], range[2];
     const int wave = uniform(threadIdx.x / kWave);
@@ -325,31 +366,27 @@ __device__ void write_zeros(const Args& a, uint32_t first) {
         atomicOr(&named[r / 32], 1u << r % 32);
     }
     __syncthreads();
-    constexpr int kN = 16 / sizeof(T);
     const float zeros[kN] = {};
     T* out = static_cast<T*>(a.out);
     for (uint32_t v = first + threadIdx.x / G; v < end; v += kThreads / G) {
         if (named[(v - first) / 32] >> (v - first) % 32 & 1) continue;
-        for (int pack = threadIdx.x % G; pack * kN < a.D; pack += G) {
-            const int c = column_of<kN>(pack, a.D);
-            store_some(out + int64_t(v) * a.D + c, a.D - c, zeros);
-        }
+        for (int pack = threadIdx.x % G; pack * kN < a.D; pack += G)
+            store_some(out + int64_t(v) * a.D + column_of<kN>(pack, a.D), zeros);
     }
 }
 
 // A group of G lanes a chunk of the sorted list and a slice of the columns.
-template <typename E, typename T, int G>
+template <typename E, typename T, int G, int kN>
 __global__ __launch_bounds__(kThreads) void sum_chunks(const Args a) {
-    constexpr int kN = 16 / sizeof(E);
     if (static_cast<int>(blockIdx.x) >= a.sum_groups) {
-        write_zeros<T, G>(a, (blockIdx.x - a.sum_groups) * kZeroRows);
+        write_zeros<T, G, (kN < 16 / int(sizeof(T)) ? kN : 16 / int(sizeof(T)))>(a, (blockIdx.x - a.sum_groups) * kZeroRows);
         return;
     }
     const int unit = blockIdx.x * (kThreads / G) + threadIdx.x / G;
     const int chunk = unit / a.slices;
     const int pack = (unit - chunk * a.slices) * G + int(threadIdx.x % G);
     if (chunk >= a.chunks || pack * kN >= a.D) return;
-    const int column = column_of<kN>(pack, a.D), there = a.D - column;
+    const int column = column_of<kN>(pack, a.D);
     const E* d_out = static_cast<const E*>(a.rows) + column;
     T* out = static_cast<T*>(a.out) + column;
     const uint32_t begin = static_cast<uint32_t>(chunk) * a.chunk, end = min(begin + a.chunk, a.n);
@@ -360,35 +397,38 @@ __global__ __launch_bounds__(kThreads) void sum_chunks(const Args a) {
     const auto leave = [&](bool goes) {
         if (token >= a.V) return;
         if (comes || goes) {
-            store_some(a.parts + (int64_t(chunk) * 2 + (comes ? 0 : 1)) * a.D + column, there, sum);
+            store_some(a.parts + (int64_t(chunk) * 2 + (comes ? 0 : 1)) * a.D + column, sum);
             return;
         }
         float v[kN];
 #pragma unroll
-        for (int j = 0; j < kN; ++j) v[j] = sum[j] * a.scale;
-        store_some(out + int64_t(token) * a.D, there, v);
+        for (int j = 0; j < kN; ++j) v[j] = times(sum[j], a.scale);
+        store_some(out + int64_t(token) * a.D, v);
     };
     for (uint32_t i = begin; i < end; i += kBatch) {
-        Entry e[kBatch];
+        uint32_t tokens[kBatch], position[kBatch];
+        int64_t at[kBatch];
+        E v[kBatch][kN];
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) e[b] = i + b < end ? a.from[i + b] : Entry{a.V, 0};
-        float v[kBatch][kN];
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-            if (e[b].token < a.V) load_some(d_out + a.at(e[b].position, a.row_b, a.row_t), there, v[b]);
+        for (int b = 0; b < kBatch; ++b) {
+            const Entry e = a.from[min(i + b, end - 1)];
+            tokens[b] = e.token, position[b] = e.position;
+        }
+        offsets_of(a, position, a.row_b, a.row_t, at);
+        load_some(d_out, at, v);
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             if (i + b >= end) break;
-            if (e[b].token != token) {
+            if (tokens[b] != token) {
                 leave(false);
-                token = e[b].token;
+                token = tokens[b];
                 comes = false;
 #pragma unroll
                 for (int j = 0; j < kN; ++j) sum[j] = 0.0f;
             }
             if (token >= a.V) return;  // padding from here on
 #pragma unroll
-            for (int j = 0; j < kN; ++j) sum[j] += v[b][j];
+            for (int j = 0; j < kN; ++j) sum[j] += to_f32(v[b][j]);
         }
     }
     leave(token == after);
@@ -396,17 +436,18 @@ __global__ __launch_bounds__(kThreads) void sum_chunks(const Args a) {
 
 // The sum that begins in a chunk and goes on behind it, if there is one: a workgroup a slice of 64 packs,
 // a quarter of the parts a wave.
-template <typename E, typename T>
+template <typename T, int kN>
 __global__ __launch_bounds__(kThreads) void join_chunks(const Args a) {
-    constexpr int kN = 16 / sizeof(E), kFlight = 8;
+    constexpr int kFlight = 8;
     __shared__ float sums[kWaves][kN][kWave];
     const int chunk = blockIdx.x / a.slices, slice = blockIdx.x - chunk * a.slices;
     const int wave = uniform(threadIdx.x / kWave), lane = lane_id();
     const uint32_t begin = static_cast<uint32_t>(chunk) * a.chunk, end = begin + a.chunk;
     if (end >= a.n) return;
-    const uint32_t token = a.from[end].token;
-    if (token >= a.V || a.from[end - 1].token != token) return;
-    if (begin && a.from[begin - 1].token == token) return;  // (so is its first: it began earlier)
+    const uint32_t token = a.from[end].token, last = a.from[end - 1].token;
+    const uint32_t before = a.from[begin ? begin - 1 : 0].token;
+    if (token >= a.V || last != token) return;
+    if (begin && before == token) return;  // (so is its first: it began earlier)
     int parts = 1;  // this chunk's, and those of the chunks that begin with the token
     for (;;) {
         const int64_t at = (int64_t(chunk) + parts + lane) * a.chunk;
@@ -416,17 +457,20 @@ __global__ __launch_bounds__(kThreads) void join_chunks(const Args a) {
         if (run < kWave) break;
     }
     const int pack = slice * kWave + lane, column = column_of<kN>(pack, a.D);
-    const int there = pack * kN < a.D ? a.D - column : 0;
+    const bool there = pack * kN < a.D;
     const int from = static_cast<int>(int64_t(parts) * wave / kWaves);
     const int to = static_cast<int>(int64_t(parts) * (wave + 1) / kWaves);
     float sum[kN] = {};
-    if (there > 0) {
+    if (there) {
         for (int p = from; p < to; p += kFlight) {
             float v[kFlight][kN];
+            int64_t at[kFlight];
 #pragma unroll
-            for (int f = 0; f < kFlight; ++f)
-                if (p + f < to)
-                    load_some(a.parts + (int64_t(chunk + p + f) * 2 + (p + f ? 0 : 1)) * a.D + column, there, v[f]);
+            for (int f = 0; f < kFlight; ++f) {
+                const int q = min(p + f, to - 1);
+                at[f] = (int64_t(chunk + q) * 2 + (q ? 0 : 1)) * a.D + column;
+            }
+            load_some(a.parts, at, v);
 #pragma unroll
             for (int f = 0; f < kFlight; ++f)
                 if (p + f < to)
@@ -437,13 +481,13 @@ __global__ __launch_bounds__(kThreads) void join_chunks(const Args a) {
 #pragma unroll
     for (int j = 0; j < kN; ++j) sums[wave][j][lane] = sum[j];
     __syncthreads();
-    if (wave || there <= 0) return;
+    if (wave || !there) return;
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
         for (int w = 1; w < kWaves; ++w) sum[j] += sums[w][j][lane];
-        sum[j] *= a.scale;
+        sum[j] = times(sum[j], a.scale);
     }
-    store_some(static_cast<T*>(a.out) + int64_t(token) * a.D + column, there, sum);
+    store_some(static_cast<T*>(a.out) + int64_t(token) * a.D + column, sum);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -451,7 +495,9 @@ __global__ __launch_bounds__(kThreads) void join_chunks(const Args a) {
 // ------------------------------------------------------------------------------------------
 
 int size_of(int dtype) { return dtype == HSN_DTYPE_F32 ? 4 : 2; }
-int packs_of(int D, int dtype) { return (D * size_of(dtype) + 15) / 16; }
+// A lane's columns: 16 bytes of a row's type, or one column of rows that have less.
+int columns_of(int D, int dtype) { return D * size_of(dtype) < 16 ? 1 : 16 / size_of(dtype); }
+int packs_of(int D, int dtype) { return (D + columns_of(D, dtype) - 1) / columns_of(D, dtype); }
 int lanes_of(int D, int dtype) { return packs_of(D, dtype) <= 16 ? 16 : kWave; }
 
 void check(int B, int T, int V, int D, int dtype, int other) {
@@ -493,19 +539,19 @@ void with_type(int dtype, F&& f) {
         f(bf16_t{});
 }
 
-// Chunks of the sorted list: as long as leaves some 8192 groups of lanes to fill the GPU, 8 entries (one
+// Chunks of the sorted list: as long as leaves some 4096 waves to fill the GPU, 8 entries (one
 // batch of loads) at least.
 int chunk_of(int64_t n, int D, int dtype) {
     const int lanes = lanes_of(D, dtype);
     const int64_t slices = (packs_of(D, dtype) + lanes - 1) / lanes;
-    const int64_t groups = 8192 * (kWave / lanes);
+    const int64_t groups = 4096 * (kWave / lanes);
     int chunk = kBatch;
     while (chunk < 1024 && n * slices > groups * chunk) chunk *= 2;
     return chunk;
 }
 
 // Entries a tile: the next launch reads all tiles' counts in every workgroup.
-int items_of(int64_t n) { return n <= 1 << 17 ? 8 : 32; }
+int items_of(int64_t n) { return n <= 1 << 16 ? 4 : n <= 1 << 18 ? 8 : 32; }
 
 struct Workspace {
     Entry *a, *b;
@@ -556,15 +602,13 @@ const Entry* sort(Args a, const Workspace& w, hipStream_t st) {
     for (int p = 0; p < passes; ++p) {
         a.shift = p * a.bits;
         a.to = p % 2 ? w.b : w.a;
-        if (items == 8) {
-            count_digits<8><<<a.tiles, kThreads, 0, st>>>(a);
-            HSN_HIP(hipGetLastError());
-            move_entries<8><<<a.tiles, kThreads, 0, st>>>(a);
-        } else {
-            count_digits<32><<<a.tiles, kThreads, 0, st>>>(a);
-            HSN_HIP(hipGetLastError());
-            move_entries<32><<<a.tiles, kThreads, 0, st>>>(a);
-        }
+        (items == 4   ? count_digits<4>
+         : items == 8 ? count_digits<8>
+                      : count_digits<32>)<<<a.tiles, kThreads, 0, st>>>(a);
+        HSN_HIP(hipGetLastError());
+        (items == 4   ? move_entries<4>
+         : items == 8 ? move_entries<8>
+                      : move_entries<32>)<<<a.tiles, kThreads, 0, st>>>(a);
         HSN_HIP(hipGetLastError());
         a.from = a.to;
     }
@@ -608,12 +652,11 @@ extern "C" int hsn_embed_forward(const void* tokens, int64_t token_b, int64_t to
             // some 4096 workgroups: 16 a compute unit
             const int most = std::max(1, 4096 / a.slices);
             const dim3 grid(std::min<int>((a.n + groups - 1) / groups, most), a.slices);
-            if (lanes == 16)
-                gather<E, O, 16><<<grid, kThreads, 0, st>>>(a);
-            else if (lanes == kWave)
-                gather<E, O, kWave><<<grid, kThreads, 0, st>>>(a);
-            else
-                gather<E, O, kThreads><<<grid, kThreads, 0, st>>>(a);
+            constexpr int kN = 16 / sizeof(E);
+            (columns_of(D, table_dtype) == 1 ? gather<E, O, 16, 1>
+             : lanes == 16                   ? gather<E, O, 16, kN>
+             : lanes == kWave                ? gather<E, O, kWave, kN>
+                                             : gather<E, O, kThreads, kN>)<<<grid, kThreads, 0, st>>>(a);
         });
     });
     HSN_HIP(hipGetLastError());
@@ -662,15 +705,16 @@ extern "C" int hsn_embed_backward(const void* tokens, int64_t token_b, int64_t t
         with_type(table_dtype, [&](auto t) {
             using E = decltype(e);
             using T_ = decltype(t);
-            if (lanes == 16)
-                sum_chunks<E, T_, 16><<<grid, kThreads, 0, st>>>(a);
-            else
-                sum_chunks<E, T_, kWave><<<grid, kThreads, 0, st>>>(a);
+            constexpr int kN = 16 / sizeof(E);
+            const bool narrow = columns_of(D, d_out_dtype) == 1;
+            (narrow        ? sum_chunks<E, T_, 16, 1>
+             : lanes == 16 ? sum_chunks<E, T_, 16, kN>
+                           : sum_chunks<E, T_, kWave, kN>)<<<grid, kThreads, 0, st>>>(a);
             HSN_HIP(hipGetLastError());
             if (a.chunks < 2) return;
             Args j = a;
             j.slices = (packs_of(D, d_out_dtype) + kWave - 1) / kWave;
-            join_chunks<E, T_><<<joins, kThreads, 0, st>>>(j);
+            (narrow ? join_chunks<T_, 1> : join_chunks<T_, kN>)<<<joins, kThreads, 0, st>>>(j);
             HSN_HIP(hipGetLastError());
         });
     });

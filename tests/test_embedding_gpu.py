@@ -55,13 +55,15 @@ def _check(tokens, V, D, dev, table="f32", out="f32", scale=1.0, seed=0):
 @pytest.mark.parametrize("out", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("table", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("shape,V,D", [((1,), 1, 1), ((7,), 5, 3), ((3, 50), 40, 100), ((2, 33), 1000, 64),
-                                       ((5, 101), 70, 520), ((60,), 20, 2055)])
+                                       ((5, 101), 70, 520), ((60,), 20, 2055), ((40,), 9, 4), ((41,), 99, 5),
+                                       ((42,), 80, 7), ((43,), 81, 8), ((44,), 65, 9)])
 def test_rows_and_gradient(cuda_device, shape, V, D, table, out):
     _check(_tokens(shape, V, V + D), V, D, cuda_device, table, out, scale=1.0 if V % 2 else 2.5)
 
 
 @pytest.mark.parametrize("n,V", [(4095, 700), (4096, 3), (4097, 50000), (2048 * 3, 1023), (2048 * 3 + 1, 1024),
-                                 (12345, 262144), (9000, (1 << 20) + 1), (5000, 1 << 24)])
+                                 (12345, 262144), (9000, (1 << 20) + 1), (5000, 1 << 24), (16384, 900),
+                                 (16385, 901), (20000, 262144), (17000, (1 << 20) + 1), (70000, 1023)])
 @pytest.mark.parametrize("D", [1, 9])
 def test_sorts(cuda_device, n, V, D):
     """Sizes around the sort's: one workgroup's list, whole tiles, one to three digits."""
