@@ -101,11 +101,13 @@ __device__ __forceinline__ uint64_t candidate(float l, int token) {
     return uint64_t(score_key(l)) << 32 | (0xffffffffu - static_cast<uint32_t>(token));
 }
 
+// The largest of a wave's numbers, that are different or 0.
 __device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
-    const uint32_t hi = static_cast<uint32_t>(v >> 32);
+    const uint32_t hi = static_cast<uint32_t>(v >> 32), lo = static_cast<uint32_t>(v);
     const uint32_t most = group_max<kWave>(hi);
-    const uint32_t lo = group_max<kWave>(hi == most ? static_cast<uint32_t>(v) : 0u);
-    return uint64_t(most) << 32 | lo;
+    const uint64_t lanes = ballot(hi == most);
+    if (__popcll(lanes) == 1) return uint64_t(most) << 32 | readlane(lo, __builtin_ctzll(lanes));
+    return uint64_t(most) << 32 | group_max<kWave>(hi == most ? lo : 0u);
 }
 
 // What a wave wrote to LDS is there for its other lanes.
@@ -159,31 +161,56 @@ struct Candidates {
     }
 
     template <typename E, int N>
-    __device__ __forceinline__ void take(const Pack<E> (&v)[N], const float (&most)[N], float batch_most,
-                                         const int (&first)[N]) {
-        lane_most = fmaxf(lane_most, batch_most);
-        if (!ballot(batch_most >= from)) return;
-        bound();
+    __device__ __forceinline__ void take(const Pack<E> (&v)[N], const float (&most)[N], const int (&first)[N]) {
 #pragma unroll
         for (int b = 0; b < N; ++b) {
             if (!ballot(most[b] >= from)) continue;
 #pragma unroll
             for (int j = 0; j < Pack<E>::kN; ++j) {
                 const float l = v[b][j];
-                const uint64_t c = candidate(l, first[b] + j);
-                put(l, c);
+                if (ballot(l >= from)) put(l, candidate(l, first[b] + j));
             }
         }
     }
     __device__ __forceinline__ void put(float l, uint64_t c) {
         uint64_t lanes = ballot(l >= from && c > above);
-        if (!lanes) return;
         if (count + __popcll(lanes) > kList) {
             cut();
             lanes = ballot(l >= from && c > above);
         }
         if (lanes >> lane_id() & 1) list[count + lanes_below(lanes)] = c;
         count += __popcll(lanes);
+    }
+    // The list's numbers from the bound on, at most 64, to `to`, where `*filled` counts them.
+    __device__ __forceinline__ void leave(uint64_t* to, uint32_t* filled) {
+        wave_fence();
+        const int lane = lane_id();
+        constexpr int kEach = kList / kWave;
+        uint64_t c[kEach], lanes[kEach];
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            c[i] = i * kWave + lane < count ? list[i * kWave + lane] : 0;
+            lanes[i] = ballot(c[i] && key_value(static_cast<uint32_t>(c[i] >> 32)) >= from);
+            n += __popcll(lanes[i]);
+        }
+        if (n > kWave) {  // (equal logits, or a row whose every next logit is a new largest one)
+            cut();
+            wave_fence();
+            c[0] = lane < count ? list[lane] : 0;
+            lanes[0] = ballot(c[0] != 0);
+            n = count;
+#pragma unroll
+            for (int i = 1; i < kEach; ++i) lanes[i] = 0;
+        }
+        int at = 0;
+        if (lane == 0) at = static_cast<int>(atomicAdd(filled, static_cast<uint32_t>(n)));
+        at = uniform(at);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (lanes[i] >> lane & 1) to[at + lanes_below(lanes[i])] = c[i];
+            at += __popcll(lanes[i]);
+        }
     }
 };
 
@@ -230,12 +257,37 @@ __device__ __forceinline__ void write_row(const Args& a, int i, const Sums& s, u
     }
 }
 
+template <typename E>
+__device__ __forceinline__ Pack<E> no_pack() {
+    Pack<E> v;
+#pragma unroll
+    for (int j = 0; j < Pack<E>::kN; ++j) v.e[j] = from_f32<E>(-__builtin_inff());
+    return v;
+}
+
+// The k-th largest of the workgroup's 64 columns' largest logits is a bound for its candidates: k different
+// logits are as large. A column is a lane of every wave; about k logits are above its bound (64 ln(64 / (64 -
+// k)) where they lie anywhere), 24 for k = 20.
+template <int WAVES>
+__device__ __forceinline__ void share_bound(Candidates& c, float (*columns)[kWave]) {
+    if constexpr (WAVES > 1) {
+        const int wave = threadIdx.x / kWave, lane = lane_id();
+        columns[wave][lane] = c.lane_most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) c.lane_most = fmaxf(c.lane_most, columns[w][lane]);
+    }
+    c.bound();
+}
+
 // A workgroup a part of a row.
 template <typename E, int WAVES, bool TOP>
 __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
     constexpr int kThreads = WAVES * kWave, kN = Pack<E>::kN;
     __shared__ float wave_sums[WAVES][3];
-    __shared__ uint64_t lists[TOP ? WAVES : 1][TOP ? kList : 1];
+    __shared__ uint64_t lists[TOP ? WAVES : 1][TOP ? kList : 1], left[TOP ? kThreads : 1], sorted[kWave];
+    __shared__ float columns[TOP ? WAVES : 1][kWave];
+    __shared__ uint32_t filled;
     const int i = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     const int wave = uniform(threadIdx.x / kWave), lane = lane_id();
     const E* row = static_cast<const E*>(a.logits) + i * a.row;
@@ -244,6 +296,7 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
     const int end = part + 1 == a.parts ? packs : min(packs, begin + a.part_packs);
     Sums s;
     Candidates c(lists[TOP ? wave : 0], a.top);
+    bool first_batch = true;
     const auto batch = [&](const auto& v, const auto& first) {
         constexpr int N = sizeof(v) / sizeof(v[0]);
         float most[N];
@@ -266,13 +319,17 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
                 s.S += e;
                 s.W = __builtin_fmaf(e, fmaxf(x, -200.0f), s.W);  // e is 0 there, and x may be -inf
             }
-        if constexpr (TOP) c.take(v, most, all, first);
-    };
-    const auto nothing = [] {
-        Pack<E> v;
-#pragma unroll
-        for (int j = 0; j < kN; ++j) v.e[j] = from_f32<E>(-__builtin_inff());
-        return v;
+        if constexpr (TOP) {
+            c.lane_most = fmaxf(c.lane_most, all);
+            if (first_batch) {  // (the same for all waves of the workgroup)
+                share_bound<WAVES>(c, columns);
+                c.take(v, most, first);
+            } else if (ballot(all >= c.from)) {
+                c.bound();
+                c.take(v, most, first);
+            }
+            first_batch = false;
+        }
     };
     // (the loop is the same for all lanes: the candidates' lists are the wave's)
     for (int p0 = begin; p0 < end; p0 += kBatch * kThreads) {
@@ -281,25 +338,48 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const int p = p0 + b * kThreads + int(threadIdx.x);
-            v[b] = p < end ? load_pack(row + int64_t(p) * kN) : nothing();
+            v[b] = load_pack(row + int64_t(min(p, end - 1)) * kN);
+            if (p >= end) v[b] = no_pack<E>();
             first[b] = p * kN;
         }
         batch(v, first);
     }
-    if (part + 1 == a.parts && packs * kN < a.V && wave == 0) {  // the elements after the last pack
-        Pack<E> v[1] = {nothing()};
-        const int first[1] = {packs * kN + lane};
+    if (part + 1 == a.parts && packs * kN < a.V) {  // the elements after the last pack, wave 0's
+        Pack<E> v[1] = {no_pack<E>()};
+        const int first[1] = {packs * kN + int(threadIdx.x)};
         if (first[0] < a.V) v[0].e[0] = row[first[0]];
         batch(v, first);
     }
     s = wave_join(s);
+    if (lane == 0) wave_sums[wave][0] = s.m, wave_sums[wave][1] = s.S, wave_sums[wave][2] = s.W;
+    uint64_t best = 0;
     if constexpr (TOP) {
-        c.cut();
-        if (lane >= c.count && lane < a.top) c.list[lane] = 0;
+        if constexpr (WAVES > 1) __syncthreads();  // the columns are read
+        if (threadIdx.x == 0) filled = 0;
+        if (wave == 0) sorted[lane] = 0;
+        share_bound<WAVES>(c, columns);
+        if constexpr (WAVES == 1) wave_fence();
+        c.leave(left, &filled);
+        if constexpr (WAVES > 1)
+            __syncthreads();
+        else
+            wave_fence();
+        const int n = static_cast<int>(filled);
+        if (static_cast<int>(threadIdx.x) < n) {
+            const uint64_t mine = left[threadIdx.x];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += left[j] > mine;
+            if (rank < a.top) sorted[rank] = mine;
+        }
+        if constexpr (WAVES > 1)
+            __syncthreads();
+        else
+            wave_fence();
+        if (wave) return;
+        best = lane < a.top ? sorted[lane] : 0;
     }
     if constexpr (WAVES > 1) {
-        if (lane == 0) wave_sums[wave][0] = s.m, wave_sums[wave][1] = s.S, wave_sums[wave][2] = s.W;
-        __syncthreads();
+        if constexpr (!TOP) __syncthreads();
         if (wave) return;
         float m = s.m;
         for (int w = 1; w < WAVES; ++w) m = fmaxf(m, wave_sums[w][0]);
@@ -310,11 +390,7 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
             o.raise(m);
             s.add(o);
         }
-    } else if constexpr (TOP) {
-        wave_fence();
     }
-    uint64_t best = 0;
-    if constexpr (TOP) best = merge(&lists[0][0], WAVES, kList, a.top);
     if (a.parts == 1) {
         write_row<E>(a, i, s, best);
     } else {
@@ -405,16 +481,32 @@ struct Plan {
     int waves, parts, part_packs;
 };
 
-Plan plan_of(int n, int V, int dtype) {
-    const int64_t packs = std::max<int64_t>(1, V / (16 / size_of(dtype)));
+Plan split(int waves, int64_t packs, int64_t parts) {
     Plan p;
-    p.waves = packs <= 2 * kBatch * kWave ? 1 : 4;
-    const int64_t batch = int64_t(kBatch) * p.waves * kWave;
-    const int64_t wanted = (2048 + n - 1) / std::max(n, 1);
-    const int64_t parts = std::max<int64_t>(1, std::min({wanted, packs / batch, int64_t(kMostParts)}));
+    p.waves = waves;
+    parts = std::max<int64_t>(1, std::min<int64_t>(parts, kMostParts));
     p.part_packs = static_cast<int>((packs + parts - 1) / parts);
     p.parts = static_cast<int>((packs + p.part_packs - 1) / p.part_packs);
     return p;
+}
+
+// Some 2048 workgroups of four waves fill the GPU. Fewer rows than an eighth of that take 16 waves each
+// before they take parts: a part costs the second launch (1 x 32000 bf16: 21.5 us in three parts of four
+// waves).
+Plan plan_forward(int n, int V, int dtype) {
+    const int64_t packs = std::max<int64_t>(1, V / (16 / size_of(dtype)));
+    if (packs <= 2 * kBatch * kWave) return split(1, packs, 1);
+    if (n <= 256) {
+        const int64_t batch = kBatch * 16 * kWave;
+        return split(16, packs, std::min<int64_t>((packs + batch - 1) / batch, 512 / std::max(n, 1)));
+    }
+    return split(4, packs, std::min<int64_t>((2047 + n) / n, packs / (kBatch * 4 * kWave)));
+}
+
+Plan plan_backward(int n, int V, int dtype) {
+    const int64_t packs = std::max<int64_t>(1, V / (16 / size_of(dtype)));
+    const int waves = packs <= 2 * kBatch * kWave ? 1 : 4;
+    return split(waves, packs, std::min<int64_t>((2047 + n) / std::max(n, 1), packs / (kBatch * waves * kWave)));
 }
 
 int64_t layout(Args& a, char* at, int n, int top) {
@@ -427,10 +519,9 @@ int64_t layout(Args& a, char* at, int n, int top) {
 
 template <typename E, bool TOP>
 void launch_forward(const Args& a, const Plan& p, int n, hipStream_t st) {
-    if (p.waves == 1)
-        score_rows<E, 1, TOP><<<n * p.parts, kWave, 0, st>>>(a);
-    else
-        score_rows<E, 4, TOP><<<n * p.parts, 4 * kWave, 0, st>>>(a);
+    (p.waves == 1   ? score_rows<E, 1, TOP>
+     : p.waves == 4 ? score_rows<E, 4, TOP>
+                    : score_rows<E, 16, TOP>)<<<n * p.parts, p.waves * kWave, 0, st>>>(a);
     HSN_HIP(hipGetLastError());
     if (p.parts > 1) score_join<E, TOP><<<n, kWave, 0, st>>>(a);
 }
@@ -473,7 +564,7 @@ extern "C" int hsn_score_workspace(int n, int V, int dtype, int top, int64_t* by
     check(n, V, dtype, top);
     HSN_REQUIRE(bytes, HSN_ERR_INVALID_ARGUMENT, "bytes must not be NULL");
     Args a{};
-    a.parts = plan_of(n, V, dtype).parts;
+    a.parts = plan_forward(n, V, dtype).parts;
     *bytes = layout(a, nullptr, n, top);
     HSN_ABI_END
 }
@@ -490,7 +581,7 @@ extern "C" int hsn_score_forward(const void* logits, int64_t row, int dtype, con
                 "a required pointer is NULL");
     HSN_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 16 == 0, HSN_ERR_INVALID_ARGUMENT,
                 "stats must be aligned to 16 bytes");
-    const Plan p = plan_of(n, V, dtype);
+    const Plan p = plan_forward(n, V, dtype);
     Args a{};
     a.logits = logits, a.row = row, a.tokens = tokens, a.token_stride = token_stride;
     a.wide = token_bytes == 8;
@@ -533,7 +624,7 @@ extern "C" int hsn_score_backward(const void* logits, int64_t row, int dtype, co
                 "stats must be aligned to 16 bytes");
     HSN_REQUIRE(reinterpret_cast<uintptr_t>(d_logits) % size_of(dtype) == 0, HSN_ERR_INVALID_ARGUMENT,
                 "d_logits must be aligned to their type");
-    const Plan p = plan_of(n, V, dtype);
+    const Plan p = plan_backward(n, V, dtype);
     Args a{};
     a.logits = logits, a.row = row, a.tokens = tokens, a.token_stride = token_stride;
     a.wide = token_bytes == 8;
