@@ -332,16 +332,24 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
         }
     };
     // (the loop is the same for all lanes: the candidates' lists are the wave's)
+    Pack<E> next[kBatch];
+    const auto load = [&](int p0) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            next[b] = load_pack(row + int64_t(min(p0 + b * kThreads + int(threadIdx.x), end - 1)) * kN);
+    };
+    if (begin < end) load(begin);
     for (int p0 = begin; p0 < end; p0 += kBatch * kThreads) {
         Pack<E> v[kBatch];
         int first[kBatch];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const int p = p0 + b * kThreads + int(threadIdx.x);
-            v[b] = load_pack(row + int64_t(min(p, end - 1)) * kN);
+            v[b] = next[b];
             if (p >= end) v[b] = no_pack<E>();
             first[b] = p * kN;
         }
+        if (p0 + kBatch * kThreads < end) load(p0 + kBatch * kThreads);
         batch(v, first);
     }
     if (part + 1 == a.parts && packs * kN < a.V) {  // the elements after the last pack, wave 0's
@@ -490,17 +498,24 @@ Plan split(int waves, int64_t packs, int64_t parts) {
     return p;
 }
 
-// Some 2048 workgroups of four waves fill the GPU. Fewer rows than an eighth of that take 16 waves each
-// before they take parts: a part costs the second launch (1 x 32000 bf16: 21.5 us in three parts of four
-// waves).
+// The forward's, with packs a row, from sweeps over n rows of V bf16 logits with five alternatives (us):
+// - a batch of a wave or two: a wave a row.
+// - a batch of four waves: those, whatever n is (64 x 8192: 8.0, by 16 waves 9.2).
+// - a batch of 16 waves, of no more than 256 rows: those, without the second launch (1 x 32000 with 20
+//   alternatives: 8.9, by parts 13); and so all rows where n is above 128, as their waves fill the GPU (200 x
+//   262144: 33, four waves in four parts 39).
+// - up to 128 longer rows: parts of one batch of four waves, as far as 1024 workgroups go (1 x 131071: 10.7
+//   in 16 parts, 16.8 by 16 waves; 64 x 131071: 15 to 16 in 4 to 16 parts, 20 by 16 waves).
+// - more rows: four waves each, in parts of at least eight batches while there are fewer than 1024 rows (300 x
+//   262144: 46 in 4 parts, 58 in one; but 301 x 50021 in fp32 31 in one and 34 in three).
 Plan plan_forward(int n, int V, int dtype) {
     const int64_t packs = std::max<int64_t>(1, V / (16 / size_of(dtype)));
-    if (packs <= 2 * kBatch * kWave) return split(1, packs, 1);
-    if (n <= 256) {
-        const int64_t batch = kBatch * 16 * kWave;
-        return split(16, packs, std::min<int64_t>((packs + batch - 1) / batch, 512 / std::max(n, 1)));
-    }
-    return split(4, packs, std::min<int64_t>((2047 + n) / n, packs / (kBatch * 4 * kWave)));
+    const int64_t batch = kBatch * 4 * kWave, fill = 1024 / std::max(n, 1);
+    if (packs <= batch / 2) return split(1, packs, 1);
+    if (packs <= batch) return split(4, packs, 1);
+    if (n > 256) return split(4, packs, std::min<int64_t>(fill, packs / (8 * batch)));
+    if (packs <= 4 * batch || n > 128) return split(16, packs, 1);
+    return split(4, packs, std::min<int64_t>(fill, (packs + batch - 1) / batch));
 }
 
 Plan plan_backward(int n, int V, int dtype) {
