@@ -8,7 +8,8 @@
 // before it scales, which costs it less than a third launch.
 //
 // What bounds it is memory: the list is read twice, the second time from the last-level cache where it
-// fits, and written once.
+// fits, and written once. A run is scaled from its end, which was read last, and long lists are stored past
+// the cache: 64 tensors of 4 M fp32 elements take 596 us, 615 from the begin and with ordinary stores.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -58,13 +59,19 @@ struct Walk {
     const List<ROWS>& l;
     uint32_t c, end;
     int t;
-    __device__ Walk(const List<ROWS>& list) : l(list) {
+    // from the run's first chunk on, or (`backward`) from its last
+    __device__ Walk(const List<ROWS>& list, bool backward = false) : l(list) {
         c = static_cast<uint32_t>(uint64_t(blockIdx.x) * l.chunks / gridDim.x);
         end = static_cast<uint32_t>(uint64_t(blockIdx.x + 1) * l.chunks / gridDim.x);
+        if (backward) {
+            const uint32_t last = end;
+            end = c;
+            c = last;
+        }
         int lo = 0, hi = l.n;  // the last tensor that begins at or before chunk c
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if (l.first[mid] <= c)
+            if (l.first[mid] <= (backward ? c - 1 : c))
                 lo = mid;
             else
                 hi = mid;
@@ -74,6 +81,11 @@ struct Walk {
     __device__ __forceinline__ bool more() {
         if (c >= end) return false;
         if (t + 1 < l.n && c >= l.first[t + 1]) ++t;  // (no tensor is without a chunk)
+        return true;
+    }
+    __device__ __forceinline__ bool back() {
+        if (c <= end) return false;
+        if (--c < l.first[t]) --t;
         return true;
     }
     __device__ __forceinline__ int type() const { return static_cast<int>(l.at[0][t] >> 62); }
@@ -142,7 +154,7 @@ __device__ __forceinline__ E scaled(float g, double by) {
     return from_f32<E>(static_cast<float>(static_cast<double>(g) * by));
 }
 
-template <typename E>
+template <bool STREAM, typename E>
 __device__ __forceinline__ void scale_chunk(const E* p, E* q, int count, double by) {
     constexpr int kN = Pack<E>::kN, kPacks = kChunk / (kThreads * kN);
     if (count == kChunk) {
@@ -153,7 +165,7 @@ __device__ __forceinline__ void scale_chunk(const E* p, E* q, int count, double 
         for (int i = 0; i < kPacks; ++i) {
 #pragma unroll
             for (int j = 0; j < kN; ++j) v[i].e[j] = scaled<E>(v[i][j], by);
-            store_pack(q + (i * kThreads + threadIdx.x) * kN, v[i]);
+            store_pack<STREAM>(q + (i * kThreads + threadIdx.x) * kN, v[i]);
         }
         return;
     }
@@ -162,13 +174,15 @@ __device__ __forceinline__ void scale_chunk(const E* p, E* q, int count, double 
             Pack<E> v = load_pack(p + o);
 #pragma unroll
             for (int j = 0; j < kN; ++j) v.e[j] = scaled<E>(v[j], by);
-            store_pack(q + o, v);
+            store_pack<false>(q + o, v);
         } else {
             for (int j = o; j < count; ++j) q[j] = scaled<E>(to_f32(p[j]), by);
         }
     }
 }
 
+// STREAM: what is written goes past the cache.
+template <bool STREAM>
 __global__ __launch_bounds__(kThreads) void scale(const List<2> l) {
     __shared__ double s[kWaves];
     double sum = 0.0;
@@ -181,13 +195,13 @@ __global__ __launch_bounds__(kThreads) void scale(const List<2> l) {
         l.result[1] = by;
     }
     if (l.in_place && by == 1.0) return;
-    for (Walk<2> w(l); w.more(); ++w.c) {
+    for (Walk<2> w(l, true); w.back();) {
         if (w.type() == HSN_DTYPE_F32)
-            scale_chunk(w.base<const float>(0), w.base<float>(1), w.count(), by);
+            scale_chunk<STREAM>(w.base<const float>(0), w.base<float>(1), w.count(), by);
         else if (w.type() == HSN_DTYPE_F16)
-            scale_chunk(w.base<const _Float16>(0), w.base<_Float16>(1), w.count(), by);
+            scale_chunk<STREAM>(w.base<const _Float16>(0), w.base<_Float16>(1), w.count(), by);
         else
-            scale_chunk(w.base<const bf16_t>(0), w.base<bf16_t>(1), w.count(), by);
+            scale_chunk<STREAM>(w.base<const bf16_t>(0), w.base<bf16_t>(1), w.count(), by);
     }
 }
 
@@ -338,11 +352,14 @@ extern "C" int hsn_clip(const void* const* grads, void* const* outs, const int64
     l.partials = static_cast<double*>(workspace);
     l.n_partials = n_partials, l.max_norm = max_norm, l.result = result, l.in_place = in_place;
     l.writes_result = true;
+    int64_t written_bytes = 0;
+    for (int j = 0; outs && j < n; ++j) written_bytes += numels[j] * size_of(dtypes[j]);
+    const auto kernel = written_bytes > kStream ? scale<true> : scale<false>;
     const std::vector<Part> written = outs ? parts_of<2>(numels, n) : std::vector<Part>();
-    if (written.empty()) scale<<<1, kThreads, 0, st>>>(l);
+    if (written.empty()) kernel<<<1, kThreads, 0, st>>>(l);
     for (const Part& part : written) {
         fill<2>(l, part, {grads, outs}, numels, dtypes);
-        scale<<<grid_of(part, written.size()), kThreads, 0, st>>>(l);
+        kernel<<<grid_of(part, written.size()), kThreads, 0, st>>>(l);
         l.writes_result = false;
     }
     HSN_HIP(hipGetLastError());

@@ -23,9 +23,31 @@ __device__ __forceinline__ Pack<E> load_pack(const E* p) {
     __builtin_memcpy(&v, p, 16);
     return v;
 }
-template <typename E>
+
+// Outputs beyond half of the last-level cache are stored past it, which leaves it to what is read again (the
+// logits' second reading, say): see the kernels for what each gains. Smaller ones stay in it for whoever
+// reads them next.
+constexpr int64_t kStream = int64_t(128) << 20;
+
+template <int BYTES>
+__device__ __forceinline__ void stream_bytes(void* p, const void* v) {
+    typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
+    static_assert(BYTES % 16 == 0, "packs");
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+        words w;
+        __builtin_memcpy(&w, static_cast<const char*>(v) + 16 * i, 16);
+        __builtin_nontemporal_store(w, reinterpret_cast<words*>(static_cast<char*>(p) + 16 * i));
+    }
+}
+
+// (A template: of two branches that store the same, the compiler makes one ordinary store.)
+template <bool STREAM, typename E>
 __device__ __forceinline__ void store_pack(E* p, const Pack<E>& v) {
-    __builtin_memcpy(p, &v, 16);
+    if constexpr (STREAM)
+        stream_bytes<16>(p, &v);
+    else
+        __builtin_memcpy(p, &v, 16);
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
