@@ -159,12 +159,6 @@ __global__ __launch_bounds__(kThreads) void gather(const Args a) {
 // The sort.
 // ------------------------------------------------------------------------------------------
 
-// What a wave wrote to LDS is there for its other lanes.
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // Each entry's place among the wave's entries of the same digit, in order; `count` (the wave's, zero
 // before) then holds how many of each there are.
 template <int N, typename C>
@@ -179,9 +173,9 @@ __device__ __forceinline__ void rank_wave(const uint32_t (&digit)[N], int bits, 
         }
         const uint32_t before = lanes_below(same), base = count[digit[r]];
         rank[r] = base + before;
-        wave_fence();
+        wave_order();
         if (before == 0) count[digit[r]] = static_cast<C>(base + __popcll(same));
-        wave_fence();
+        wave_order();
     }
 }
 

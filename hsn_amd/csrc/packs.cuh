@@ -50,6 +50,13 @@ __device__ __forceinline__ void store_pack(E* p, const Pack<E>& v) {
         __builtin_memcpy(p, &v, 16);
 }
 
+// Between a wave's accesses to LDS by different lanes: a wave's LDS instructions are carried out in their
+// order, so it is enough that the compiler keeps it. (A fence would wait for loads in flight as well.)
+__device__ __forceinline__ void wave_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (int mask = 32; mask; mask >>= 1) v += __shfl_xor(v, mask, kWave);

@@ -110,12 +110,6 @@ __device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
     return uint64_t(most) << 32 | group_max<kWave>(hi == most ? lo : 0u);
 }
 
-// What a wave wrote to LDS is there for its other lanes.
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-}
-
 struct Candidates {
     uint64_t* list;  // kList of this wave's, in LDS
     int k, count = 0;
@@ -126,7 +120,7 @@ struct Candidates {
 
     // Leaves the k largest, sorted.
     __device__ void cut() {
-        wave_fence();
+        wave_order();
         const int lane = lane_id();
         constexpr int kEach = kList / kWave;
         uint64_t mine[kEach], kept = 0;
@@ -143,7 +137,7 @@ struct Candidates {
             if (lane == r) kept = most;
             if (r == k - 1) above = most;
         }
-        wave_fence();
+        wave_order();
         if (lane < n) list[lane] = kept;
         count = n;
         from = fmaxf(from, key_value(static_cast<uint32_t>(above >> 32)));
@@ -183,7 +177,7 @@ struct Candidates {
     }
     // The list's numbers from the bound on, at most 64, to `to`, where `*filled` counts them.
     __device__ __forceinline__ void leave(uint64_t* to, uint32_t* filled) {
-        wave_fence();
+        wave_order();
         const int lane = lane_id();
         constexpr int kEach = kList / kWave;
         uint64_t c[kEach], lanes[kEach];
@@ -196,7 +190,7 @@ struct Candidates {
         }
         if (n > kWave) {  // (equal logits, or a row whose every next logit is a new largest one)
             cut();
-            wave_fence();
+            wave_order();
             c[0] = lane < count ? list[lane] : 0;
             lanes[0] = ballot(c[0] != 0);
             n = count;
@@ -366,12 +360,12 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
         if (threadIdx.x == 0) filled = 0;
         if (wave == 0) sorted[lane] = 0;
         share_bound<WAVES>(c, columns);
-        if constexpr (WAVES == 1) wave_fence();
+        if constexpr (WAVES == 1) wave_order();
         c.leave(left, &filled);
         if constexpr (WAVES > 1)
             __syncthreads();
         else
-            wave_fence();
+            wave_order();
         const int n = static_cast<int>(filled);
         if (static_cast<int>(threadIdx.x) < n) {
             const uint64_t mine = left[threadIdx.x];
@@ -382,7 +376,7 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
         if constexpr (WAVES > 1)
             __syncthreads();
         else
-            wave_fence();
+            wave_order();
         if (wave) return;
         best = lane < a.top ? sorted[lane] : 0;
     }
@@ -420,7 +414,7 @@ __global__ __launch_bounds__(kWave) void score_join(const Args a) {
     if constexpr (TOP) {
         const uint64_t* from = a.part_lists + int64_t(i) * a.parts * a.top;
         for (int j = lane; j < a.parts * a.top; j += kWave) lists[j] = from[j];
-        wave_fence();
+        wave_order();
     }
     s = wave_join(s);
     uint64_t best = 0;

@@ -2,10 +2,11 @@
 // (include/hsn_unit_router.h).
 //
 // A token is a group of G lanes with four units each (G the power of two that holds M), so a wave takes
-// 64 / G tokens at a time, and maxima and sums over a token are lane steps. The k units are chosen one after
-// the other: the group's largest key, its first lane, that lane's first unit. Each lane adds the
-// probabilities and counts of its own units over all tokens that it meets; lanes, waves and at last
-// workgroups are added in a fixed order, so the sums repeat, and a second launch makes the balance of them.
+// 64 / G tokens at a time, and maxima and sums over a token are lane steps. A unit's key is its logit's order
+// above its number, so keys differ; a lane sorts its four, and the group's largest first key is the next
+// unit chosen, k times, without a branch. Each lane adds the probabilities of its own units over all tokens
+// that it meets; lanes, waves and at last workgroups are added in a fixed order, so the sums repeat, and a
+// second launch makes the balance of them. Counts are whole numbers, added in LDS in any order.
 //
 // The backward takes the probabilities again from the logits. The chosen slots of a wave's tokens go through
 // LDS to the lanes that hold their units.
@@ -20,13 +21,12 @@ namespace router {
 namespace {
 
 constexpr int kEach = 4;  // units a lane
-constexpr int kWaves = 8, kThreads = kWaves * kWave;
-constexpr int kMostGroups = 512;        // workgroups of the forward: two a compute unit
-constexpr int kMostBackward = 2048;
-constexpr int kFlush = 128;             // tokens that a lane adds in fp32
-constexpr int kFinish = 1024, kFinishUnits = 16, kFinishSlices = kFinish / kFinishUnits;
+constexpr int kWaves = 16, kThreads = kWaves * kWave;
+constexpr int kMostGroups = 256;  // workgroups of the forward: one a compute unit, its sums are few to add
+constexpr int kMostBackward = 1024;
+constexpr int kFlush = 128;       // tokens that a lane adds in fp32
+constexpr int kFinish = 1024;
 constexpr float kLog2 = 1.4426950408889634f;
-constexpr uint32_t kKeyNegInf = 0x007fffffu;  // score_key(-inf)
 
 struct Args {
     const void* logits;
@@ -37,12 +37,10 @@ struct Args {
     int64_t* tally;
     float *probs, *balance;
     int n, M, k;
-    // workspace: of each forward workgroup; of each workgroup that finishes
+    // workspace: of each forward workgroup
     double* part_probs;     // [groups, M]
-    uint32_t* part_counts;  // [groups, M + 1], the live tokens last
-    double* part_dot;       // [finishing]: sum of c_e prob_e
-    int64_t* part_chosen;   // [finishing]: sum of c_e
-    uint32_t* arrived;
+    uint32_t* part_counts;  // [groups, M]
+    uint32_t* part_rows;    // [groups]: live tokens
     int groups;
     // backward
     const float *g, *d_balance;
@@ -76,93 +74,148 @@ __device__ __forceinline__ uint64_t of_group(uint64_t lanes) {
     return lanes >> (lane_id() / G * G) & ((uint64_t(1) << (G % kWave)) - 1);
 }
 
-// A lane's four logits of a token; -inf behind the last unit and where there is no token.
+// A lane's four logits of a token; -inf behind the last unit.
 template <typename E>
-__device__ __forceinline__ void load_units(const E* row, int unit, int M, bool there, float (&x)[kEach]) {
-    if (there && unit + kEach <= M) {
-        E e[kEach];
-        __builtin_memcpy(e, row + unit, sizeof(e));
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) x[j] = to_f32(e[j]);
+struct Four {
+    E e[kEach];
+};
+template <typename E>
+__device__ __forceinline__ Four<E> load_units(const E* row, int unit, int M) {
+    Four<E> v;
+    if (unit + kEach <= M) {
+        __builtin_memcpy(&v, row + unit, sizeof(v));
     } else {
 #pragma unroll
-        for (int j = 0; j < kEach; ++j)
-            x[j] = there && unit + j < M ? to_f32(row[unit + j]) : -__builtin_inff();
+        for (int j = 0; j < kEach; ++j) v.e[j] = unit + j < M ? row[unit + j] : from_f32<E>(-__builtin_inff());
     }
+    return v;
+}
+
+// A unit's key: the larger the logit, and among equal ones the lower the unit, the larger; NaN above all,
+// and 0 for -inf, which is never chosen.
+template <typename E>
+struct Order {  // 16 bits: the logit's order in the upper half
+    using Key = uint32_t;
+    static constexpr uint32_t kInf = sizeof(E) == 2 && __is_same(E, _Float16) ? 0x7c00 : 0x7f80;
+    static __device__ __forceinline__ Key key(E e, int unit) {
+        const uint32_t u = __builtin_bit_cast(uint16_t, e);
+        uint32_t k = u & 0x8000 ? u ^ 0xffff : u | 0x8000;
+        k = u == 0x8000 ? 0x8000 : k;                 // -0 as 0
+        k = (u & 0x7fff) > kInf ? 0xffff : k;         // NaN
+        return u == (0x8000 | kInf) ? 0 : k << 16 | (0xffffu - unit);
+    }
+    static __device__ __forceinline__ float value(Key k) {
+        k >>= 16;
+        return to_f32(__builtin_bit_cast(E, static_cast<uint16_t>(k & 0x8000 ? k ^ 0x8000 : k ^ 0xffff)));
+    }
+    static __device__ __forceinline__ int unit(Key k) { return 0xffff - static_cast<int>(k & 0xffff); }
+    template <int G>
+    static __device__ __forceinline__ Key largest(Key k) {
+        return group_max<G>(k);
+    }
+};
+template <>
+struct Order<float> {
+    using Key = uint64_t;
+    static __device__ __forceinline__ Key key(float x, int unit) {
+        return x == -__builtin_inff() ? 0 : uint64_t(score_key(x)) << 32 | (0xffffffffu - unit);
+    }
+    static __device__ __forceinline__ float value(Key key) {
+        const uint32_t k = static_cast<uint32_t>(key >> 32);
+        return __uint_as_float(k ^ (static_cast<int32_t>(k) < 0 ? 0x80000000u : 0xffffffffu));
+    }
+    static __device__ __forceinline__ int unit(Key k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
+    template <int G>
+    static __device__ __forceinline__ Key largest(Key k) {
+        const uint32_t hi = static_cast<uint32_t>(k >> 32), most = group_max<G>(hi);
+        return uint64_t(most) << 32 | group_max<G>(hi == most ? static_cast<uint32_t>(k) : 0u);
+    }
+};
+
+template <typename K>
+__device__ __forceinline__ void order(K& a, K& b) {
+    const K hi = a > b ? a : b;
+    b = a > b ? b : a;
+    a = hi;
 }
 
 template <typename E, int G>
 __global__ __launch_bounds__(kThreads) void route_tokens(const Args a) {
     constexpr int kTokens = kWave / G;  // a wave takes at a time
+    constexpr int kSlots = (HSN_ROUTER_MAX_CHOSEN + G - 1) / G;  // slots that a lane of a group writes
+    using O = Order<E>;
+    using Key = typename O::Key;
     __shared__ double probs[kWaves][G * kEach];
-    __shared__ uint32_t counts[kWaves][G * kEach], rows[kWaves];
+    __shared__ uint32_t counts[G * kEach], rows;
     const int wave = uniform(threadIdx.x / kWave), lane = lane_id(), sub = lane % G, unit = sub * kEach;
+    for (int u = threadIdx.x; u < G * kEach; u += kThreads) counts[u] = 0;
+    if (threadIdx.x == 0) rows = 0;
+    __syncthreads();
     const E* logits = static_cast<const E*>(a.logits);
     float sum[kEach] = {};
     double whole[kEach] = {};
-    uint32_t count[kEach] = {}, live_tokens = 0;
-    const int step = a.groups * kWaves * kTokens;
+    uint32_t live_tokens = 0;
+    const int64_t step = int64_t(a.groups) * kWaves * kTokens;
+    int64_t t = (int64_t(blockIdx.x) * kWaves + wave) * kTokens;
+    // the next tokens' logits are in flight while these are worked on (a token behind the last one: the last)
+    Four<E> next;
+    bool next_valid = false;
+    const auto load = [&](int64_t from) {
+        const int64_t i = from + lane / G, at = i < a.n ? i : a.n - 1;
+        next = load_units(logits + at * a.row, unit, a.M);
+        next_valid = a.valid ? a.valid[at] : true;
+    };
+    if (t < a.n) load(t);
     int turn = 0;
-    for (int64_t t = (int64_t(blockIdx.x) * kWaves + wave) * kTokens; t < a.n; t += step) {
+    for (; t < a.n; t += step) {
         const int64_t i = t + lane / G;
-        const bool there = i < a.n;
-        float x[kEach];
-        load_units(logits + i * a.row, unit, a.M, there, x);
-        const bool wanted = there && (!a.valid || a.valid[i]);
-        uint32_t key[kEach];
-        int rank[kEach];
+        const bool there = i < a.n, wanted = there && next_valid;
+        const Four<E> v = next;
+        if (t + step < a.n) load(t + step);
+        Key key[kEach];
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            key[j] = score_key(x[j]);
-            key[j] = wanted && key[j] > kKeyNegInf ? key[j] : 0;  // 0: not to be chosen
-            rank[j] = -1;
-        }
-        float m = 0.0f, chosen = 0.0f;
-        int found = 0;
-        for (int r = 0; r < a.k; ++r) {
-            const uint32_t mine = umax(umax(key[0], key[1]), umax(key[2], key[3]));
-            const uint32_t most = group_max<G>(mine);
-            const float value =
-                __uint_as_float(most ^ (static_cast<int32_t>(most) < 0 ? 0x80000000u : 0xffffffffu));
-            if (r == 0) m = value;
-            if (most) {
-                chosen += exp_of(value - m);
-                found = r + 1;
-            }
-            const uint64_t lanes = of_group<G>(ballot(mine == most));
-            if (most && sub == __builtin_ctzll(lanes)) {
-                bool open = true;
+        for (int j = 0; j < kEach; ++j) key[j] = wanted ? O::key(v.e[j], unit + j) : 0;
+        order(key[0], key[1]), order(key[2], key[3]), order(key[0], key[2]), order(key[1], key[3]);
+        order(key[1], key[2]);
+        Key kept[kSlots], first = 0;
 #pragma unroll
-                for (int j = 0; j < kEach; ++j) {
-                    const bool it = open && key[j] == most;
-                    open = open && !it;
-                    rank[j] = it ? r : rank[j];
-                    key[j] = it ? 0 : key[j];
-                }
+        for (int q = 0; q < kSlots; ++q) {
+            kept[q] = 0;
+            const int some = min(G, a.k - q * G);
+            for (int s = 0; s < some; ++s) {
+                const Key most = O::template largest<G>(key[0]);
+                if (q == 0 && s == 0) first = most;
+                const bool mine = key[0] == most;
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) key[j] = mine ? (j + 1 < kEach ? key[j + 1 < kEach ? j + 1 : j] : 0) : key[j];
+                kept[q] = sub == s ? most : kept[q];
             }
         }
-        const bool live = found > 0;
+        const bool live = first != 0;
+        const float m = O::value(first);
         float e[kEach];
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) e[j] = live ? exp_of(x[j] - m) : 0.0f;
-        const float total = group_sum<G>((e[0] + e[1]) + (e[2] + e[3]));
-        const float part = live ? 1.0f / total : 0.0f, share = live ? 1.0f / chosen : 0.0f;
+        for (int j = 0; j < kEach; ++j) e[j] = exp_of(to_f32(v.e[j]) - m);
+        const float part = 1.0f / group_sum<G>((e[0] + e[1]) + (e[2] + e[3]));
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            sum[j] += e[j] * part;
-            if (rank[j] >= 0) {
-                ++count[j];
-                a.units[i * a.k + rank[j]] = unit + j;
-                a.shares[i * a.k + rank[j]] = e[j] * share;
-            }
+        for (int j = 0; j < kEach; ++j) sum[j] += live ? e[j] * part : 0.0f;
+        float w[kSlots], chosen = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kSlots; ++q) {
+            w[q] = kept[q] ? exp_of(O::value(kept[q]) - m) : 0.0f;
+            chosen += w[q];
         }
-        if (there && sub == 0) {
-            live_tokens += live;
-            for (int r = found; r < a.k; ++r) {
-                a.units[i * a.k + r] = -1;
-                a.shares[i * a.k + r] = 0.0f;
-            }
+        const float share = 1.0f / group_sum<G>(chosen);
+#pragma unroll
+        for (int q = 0; q < kSlots; ++q) {
+            const int r = q * G + sub;
+            if (r >= a.k || !there) continue;
+            const int u = O::unit(kept[q]);
+            a.units[i * a.k + r] = kept[q] ? u : -1;
+            a.shares[i * a.k + r] = kept[q] ? w[q] * share : 0.0f;
+            if (kept[q]) atomicAdd(&counts[u], 1u);
         }
+        live_tokens += live && sub == 0;
         if (++turn % kFlush == 0) {
 #pragma unroll
             for (int j = 0; j < kEach; ++j) whole[j] += sum[j], sum[j] = 0.0f;
@@ -173,104 +226,81 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Args a) {
     for (int j = 0; j < kEach; ++j) {
         whole[j] += sum[j];
 #pragma unroll
-        for (int mask = G; mask < kWave; mask *= 2) {
-            whole[j] += __shfl_xor(whole[j], mask, kWave);
-            count[j] += __shfl_xor(count[j], mask, kWave);
-        }
+        for (int mask = G; mask < kWave; mask *= 2) whole[j] += __shfl_xor(whole[j], mask, kWave);
+        if (lane < G) probs[wave][unit + j] = whole[j];
     }
-#pragma unroll
-    for (int mask = G; mask < kWave; mask *= 2) live_tokens += __shfl_xor(live_tokens, mask, kWave);
-    if (lane < G) {
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            probs[wave][unit + j] = whole[j];
-            counts[wave][unit + j] = count[j];
-        }
-        if (lane == 0) rows[wave] = live_tokens;
-    }
+    if (live_tokens) atomicAdd(&rows, live_tokens);
     __syncthreads();
-    for (int u = threadIdx.x; u <= a.M; u += kThreads) {
+    for (int u = threadIdx.x; u < a.M; u += kThreads) {
         double p = 0.0;
-        uint32_t c = 0;
-        for (int w = 0; w < kWaves; ++w) {
-            if (u < a.M) p += probs[w][u];
-            c += u < a.M ? counts[w][u] : rows[w];
-        }
-        if (u < a.M) a.part_probs[int64_t(blockIdx.x) * a.M + u] = p;
-        a.part_counts[int64_t(blockIdx.x) * (a.M + 1) + u] = c;
+        for (int w = 0; w < kWaves; ++w) p += probs[w][u];
+        a.part_probs[int64_t(blockIdx.x) * a.M + u] = p;
+        a.part_counts[int64_t(blockIdx.x) * a.M + u] = counts[u];
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.arrived = 0;  // for the launch after this one
+    if (threadIdx.x == 0) a.part_rows[blockIdx.x] = rows;
 }
 
-// The workgroups' sums added, 16 units a workgroup; the last one that arrives makes the balance.
-__global__ __launch_bounds__(kFinish) void route_finish(const Args a) {
-    __shared__ double probs[kFinishSlices][kFinishUnits];
-    __shared__ int64_t counts[kFinishSlices][kFinishUnits], rows[kFinishSlices];
-    const int u = blockIdx.x * kFinishUnits + threadIdx.x % kFinishUnits, slice = threadIdx.x / kFinishUnits;
-    double p = 0.0;
-    int64_t c = 0, r = 0;
-    for (int g = slice; g < a.groups; g += kFinishSlices) {
-        if (u < a.M) {
-            p += a.part_probs[int64_t(g) * a.M + u];
-            c += a.part_counts[int64_t(g) * (a.M + 1) + u];
+// The workgroups' sums added and the balance, by one workgroup: a thread a unit and a slice of them.
+__global__ __launch_bounds__(kFinish) void route_finish(const Args a, int units) {  // units: a power of two >= M
+    constexpr int kFinishWaves = kFinish / kWave, kFlight = 8;
+    __shared__ double probs[kFinish], s[kFinishWaves];
+    __shared__ uint64_t counts[kFinish];
+    const int u = threadIdx.x % units, slice = threadIdx.x / units, slices = kFinish / units;
+    const int at = min(u, a.M - 1);
+    double p = 0.0, r = 0.0;
+    uint64_t c = 0;
+    for (int g0 = slice; g0 < a.groups; g0 += slices * kFlight) {
+        double q[kFlight];
+        uint32_t d[kFlight];
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) {
+            const int64_t g = min(g0 + f * slices, a.groups - 1);
+            q[f] = a.part_probs[g * a.M + at];
+            d[f] = a.part_counts[g * a.M + at];
         }
-        r += a.part_counts[int64_t(g) * (a.M + 1) + a.M];
-    }
-    probs[slice][threadIdx.x % kFinishUnits] = p;
-    counts[slice][threadIdx.x % kFinishUnits] = c;
-    if (threadIdx.x % kFinishUnits == 0) rows[slice] = r;
-    __syncthreads();
-    if (threadIdx.x >= kWave) return;
-    const int lane = threadIdx.x;
-    r = rows[lane];  // 64 slices: a lane each
 #pragma unroll
-    for (int mask = 32; mask; mask >>= 1) r += __shfl_xor(r, mask, kWave);
-    // four lanes a unit, a quarter of the slices each
-    p = 0.0, c = 0;
-    for (int s = lane / kFinishUnits; s < kFinishSlices; s += kWave / kFinishUnits) {
-        p += probs[s][lane % kFinishUnits];
-        c += counts[s][lane % kFinishUnits];
+        for (int f = 0; f < kFlight; ++f) {
+            const bool there = g0 + f * slices < a.groups;
+            p += there ? q[f] : 0.0;
+            c += there ? d[f] : 0;
+        }
     }
-#pragma unroll
-    for (int mask = kFinishUnits; mask < kWave; mask *= 2) {
+    if (static_cast<int>(threadIdx.x) < a.groups) r = a.part_rows[threadIdx.x];
+    // the lanes of a wave that hold the same unit, then the threads that still do
+    for (int mask = units; mask < kWave; mask *= 2) {
         p += __shfl_xor(p, mask, kWave);
         c += __shfl_xor(c, mask, kWave);
     }
-    p /= static_cast<double>(r > 0 ? r : 1);
-    const bool mine = lane < kFinishUnits && u < a.M;
-    if (mine) {
-        a.tally[u] = c;
-        a.probs[u] = static_cast<float>(p);
-    }
-    double dot = mine ? static_cast<double>(c) * p : 0.0;
-    int64_t chosen = mine ? c : 0;
-#pragma unroll
-    for (int mask = 32; mask; mask >>= 1) {
-        dot += __shfl_xor(dot, mask, kWave);
-        chosen += __shfl_xor(chosen, mask, kWave);
-    }
-    if (lane) return;
-    if (blockIdx.x == 0) a.tally[a.M] = r;
-    if (gridDim.x > 1) {
-        a.part_dot[blockIdx.x] = dot;
-        a.part_chosen[blockIdx.x] = chosen;
-        __threadfence();  // this lane's own stores, before it counts itself
-        if (atomicAdd(a.arrived, 1u) + 1 < gridDim.x) return;
-        __threadfence();
-        dot = 0.0, chosen = 0;
-        for (uint32_t g = 0; g < gridDim.x; ++g) {
-            dot += __hip_atomic_load(a.part_dot + g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            chosen += __hip_atomic_load(a.part_chosen + g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    probs[threadIdx.x] = p;
+    counts[threadIdx.x] = c;
+    r = block_sum<kFinishWaves>(r, s);  // (passes a barrier)
+    p = 0.0, c = 0;
+    if (static_cast<int>(threadIdx.x) < a.M) {
+        for (int i = threadIdx.x; i < kFinish; i += max(units, kWave)) {
+            p += probs[i];
+            c += counts[i];
         }
+        p /= r > 0.0 ? r : 1.0;
+        a.tally[threadIdx.x] = static_cast<int64_t>(c);
+        a.probs[threadIdx.x] = static_cast<float>(p);
     }
-    *a.balance = static_cast<float>(a.M * dot / static_cast<double>(chosen > 0 ? chosen : 1));
+    const double chosen = block_sum<kFinishWaves>(static_cast<double>(c), s);
+    const double dot = block_sum<kFinishWaves>(static_cast<double>(c) * p, s);
+    if (threadIdx.x == 0) {
+        a.tally[a.M] = static_cast<int64_t>(r);
+        *a.balance = static_cast<float>(a.M * dot / (chosen > 0.0 ? chosen : 1.0));
+    }
 }
+static_assert(kMostGroups <= kFinish, "a thread a workgroup's live tokens");
 
 constexpr int kBackWaves = 4, kBackThreads = kBackWaves * kWave;
 
 template <typename E, int G>
 __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
     constexpr int kTokens = kWave / G;
+    // slots of a wave's tokens that a lane brings: k is at most 16 and at most the units
+    constexpr int kMostK = G * kEach < HSN_ROUTER_MAX_CHOSEN ? G * kEach : HSN_ROUTER_MAX_CHOSEN;
+    constexpr int kSlots = (kTokens * kMostK + kWave - 1) / kWave;
     __shared__ float2 slots[kBackWaves][kTokens][G * kEach];  // whether a unit is chosen, its cotangent
     const int wave = uniform(threadIdx.x / kWave), lane = lane_id(), sub = lane % G, unit = sub * kEach;
     float2* const mine = slots[wave][lane / G] + unit;
@@ -292,29 +322,50 @@ __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
     const float pull = a.d_balance && rows > 0
                            ? static_cast<float>(static_cast<double>(*a.d_balance) * a.M / static_cast<double>(rows))
                            : 0.0f;
-    const int step = gridDim.x * kBackWaves * kTokens;
-    for (int64_t t = (int64_t(blockIdx.x) * kBackWaves + wave) * kTokens; t < a.n; t += step) {
+    int token_of[kSlots], rank_of[kSlots];  // of the slots that the lane brings
+#pragma unroll
+    for (int q = 0; q < kSlots; ++q) {
+        const int s = q * kWave + lane;
+        token_of[q] = s / a.k;
+        rank_of[q] = s - token_of[q] * a.k;
+    }
+    const int64_t step = int64_t(gridDim.x) * kBackWaves * kTokens;
+    int64_t t = (int64_t(blockIdx.x) * kBackWaves + wave) * kTokens;
+    Four<E> next;
+    bool next_valid = false;
+    int64_t next_unit[kSlots];
+    float next_g[kSlots];
+    const auto bring = [&](int64_t from) {
+        const int64_t i = from + lane / G, at = i < a.n ? i : a.n - 1;
+        next = load_units(logits + at * a.row, unit, a.M);
+        next_valid = a.valid ? a.valid[at] : true;
+        if (a.g) {
+#pragma unroll
+            for (int q = 0; q < kSlots; ++q) {
+                const int64_t j = from + token_of[q] < a.n ? from + token_of[q] : a.n - 1;
+                next_unit[q] = a.units[j * a.k + rank_of[q]];
+                next_g[q] = a.g[j * a.g_row + rank_of[q]];
+            }
+        }
+    };
+    if (t < a.n) bring(t);
+    for (; t < a.n; t += step) {
         const int64_t i = t + lane / G;
-        const bool there = i < a.n;
+        const bool there = i < a.n, wanted = there && next_valid;
         float x[kEach];
-        load_units(logits + i * a.row, unit, a.M, there, x);
-        const bool wanted = there && (!a.valid || a.valid[i]);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) x[j] = to_f32(next.e[j]);
         if (a.g) {
 #pragma unroll
             for (int j = 0; j < kEach; ++j) mine[j] = make_float2(0.0f, 0.0f);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-            __builtin_amdgcn_wave_barrier();
-            const int64_t left = a.n - t;
-            const int n_slots = static_cast<int>(left < kTokens ? left : kTokens) * a.k;
-            for (int s = lane; s < n_slots; s += kWave) {
-                const int token = s / a.k;
-                const int64_t u = a.units[t * a.k + s];
-                if (u >= 0 && u < a.M)
-                    slots[wave][token][u] = make_float2(1.0f, a.g[(t + token) * a.g_row + (s - token * a.k)]);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-            __builtin_amdgcn_wave_barrier();
+            wave_order();
+#pragma unroll
+            for (int q = 0; q < kSlots; ++q)
+                if (token_of[q] < kTokens && t + token_of[q] < a.n && next_unit[q] >= 0 && next_unit[q] < a.M)
+                    slots[wave][token_of[q]][next_unit[q]] = make_float2(1.0f, next_g[q]);
+            wave_order();
         }
+        if (t + step < a.n) bring(t + step);
         const float m = group_largest<G>(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
         const bool strange = x[0] != x[0] || x[1] != x[1] || x[2] != x[2] || x[3] != x[3];
         const bool live = wanted && (m > -__builtin_inff() || of_group<G>(ballot(strange)) != 0);
@@ -381,8 +432,6 @@ int groups_of(int n, int M) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostGroups, (n + tokens - 1) / tokens)));
 }
 
-int finishing(int M) { return (M + kFinishUnits - 1) / kFinishUnits; }
-
 int64_t layout(Args& a, char* at) {
     char* const begin = at;
     const auto take = [&](int64_t bytes) {
@@ -391,10 +440,8 @@ int64_t layout(Args& a, char* at) {
         return p;
     };
     a.part_probs = reinterpret_cast<double*>(take(8 * int64_t(a.groups) * a.M));
-    a.part_counts = reinterpret_cast<uint32_t*>(take(4 * int64_t(a.groups) * (a.M + 1)));
-    a.part_dot = reinterpret_cast<double*>(take(8 * finishing(a.M)));
-    a.part_chosen = reinterpret_cast<int64_t*>(take(8 * finishing(a.M)));
-    a.arrived = reinterpret_cast<uint32_t*>(take(4));
+    a.part_counts = reinterpret_cast<uint32_t*>(take(4 * int64_t(a.groups) * a.M));
+    a.part_rows = reinterpret_cast<uint32_t*>(take(4 * int64_t(a.groups)));
     return at - begin;
 }
 
@@ -472,7 +519,9 @@ extern "C" int hsn_unit_router_forward(const void* logits, int64_t row, int dtyp
         });
     });
     HSN_HIP(hipGetLastError());
-    route_finish<<<finishing(M), kFinish, 0, st>>>(a);
+    int units = 1;
+    while (units < M) units *= 2;
+    route_finish<<<1, kFinish, 0, st>>>(a, units);
     HSN_HIP(hipGetLastError());
     HSN_ABI_END
 }
