@@ -57,9 +57,32 @@ __device__ __forceinline__ void wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// A double's halves through the lanes (an LDS shuffle costs five times as much).
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, uint64_t(dpp_u32<CTRL>(static_cast<uint32_t>(u >> 32))) << 32 |
+                                          dpp_u32<CTRL>(static_cast<uint32_t>(u)));
+}
+__device__ __forceinline__ double rows_sum(RowPair lo, RowPair hi) {
+    return __builtin_bit_cast(double, uint64_t(hi.lo) << 32 | lo.lo) +
+           __builtin_bit_cast(double, uint64_t(hi.hi) << 32 | lo.hi);
+}
+// The sum over the lanes of a wave whose numbers differ by multiples of G, in each of them.
+template <int G = 1>
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int mask = 32; mask; mask >>= 1) v += __shfl_xor(v, mask, kWave);
+    if constexpr (G <= 1) v += dpp_f64<dpp::kXor1>(v);
+    if constexpr (G <= 2) v += dpp_f64<dpp::kXor2>(v);
+    if constexpr (G <= 4) v += dpp_f64<0x124>(v);  // row_ror:4
+    if constexpr (G <= 8) v += dpp_f64<dpp::kRor8>(v);
+    if constexpr (G <= 16) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        v = rows_sum(pair16(static_cast<uint32_t>(u)), pair16(static_cast<uint32_t>(u >> 32)));
+    }
+    if constexpr (G <= 32) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        v = rows_sum(pair32(static_cast<uint32_t>(u)), pair32(static_cast<uint32_t>(u >> 32)));
+    }
     return v;
 }
 

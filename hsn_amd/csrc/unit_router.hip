@@ -20,8 +20,6 @@ namespace hsn {
 namespace router {
 namespace {
 
-constexpr int kEach = 4;  // units a lane
-constexpr int kWaves = 16, kThreads = kWaves * kWave;
 constexpr int kMostGroups = 256;  // workgroups of the forward: one a compute unit, its sums are few to add
 constexpr int kMostBackward = 1024;
 constexpr int kFlush = 128;       // tokens that a lane adds in fp32
@@ -74,41 +72,44 @@ __device__ __forceinline__ uint64_t of_group(uint64_t lanes) {
     return lanes >> (lane_id() / G * G) & ((uint64_t(1) << (G % kWave)) - 1);
 }
 
-// A lane's four logits of a token; -inf behind the last unit.
-template <typename E>
-struct Four {
-    E e[kEach];
+// A lane's units are EACH from `begin` on, of which those from `own` on are its own: the last ones of M end
+// with M, so that a token's logits are read by whole packs. (Where some lanes read their elements one by
+// one, all of them unpack what they read at once and wait for it, and no load stays in flight.) Fewer
+// than four units have a lane each.
+template <typename E, int EACH>
+struct Units {
+    E e[EACH];
 };
-template <typename E>
-__device__ __forceinline__ Four<E> load_units(const E* row, int unit, int M) {
-    Four<E> v;
-    if (unit + kEach <= M) {
-        __builtin_memcpy(&v, row + unit, sizeof(v));
-    } else {
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) v.e[j] = unit + j < M ? row[unit + j] : from_f32<E>(-__builtin_inff());
+template <int EACH>
+struct Place {
+    int begin, own;
+    __device__ Place(int sub, int M) {
+        begin = max(0, min(sub * EACH, M - EACH));
+        own = min(sub * EACH - begin, EACH);  // EACH: none
     }
+    __device__ __forceinline__ bool mine(int j) const { return j >= own; }
+};
+template <typename E, int EACH>
+__device__ __forceinline__ Units<E, EACH> load_units(const E* p) {
+    Units<E, EACH> v;
+    __builtin_memcpy(&v, p, sizeof(v));
     return v;
 }
 
 // A unit's key: the larger the logit, and among equal ones the lower the unit, the larger; NaN above all,
 // and 0 for -inf, which is never chosen.
 template <typename E>
-struct Order {  // 16 bits: the logit's order in the upper half
+struct Order {  // a 16-bit logit in fp32 leaves at least 13 low bits free: 8 for the unit
+    static_assert(HSN_ROUTER_MAX_UNITS <= 256, "8 bits hold a unit");
     using Key = uint32_t;
-    static constexpr uint32_t kInf = sizeof(E) == 2 && __is_same(E, _Float16) ? 0x7c00 : 0x7f80;
-    static __device__ __forceinline__ Key key(E e, int unit) {
-        const uint32_t u = __builtin_bit_cast(uint16_t, e);
-        uint32_t k = u & 0x8000 ? u ^ 0xffff : u | 0x8000;
-        k = u == 0x8000 ? 0x8000 : k;                 // -0 as 0
-        k = (u & 0x7fff) > kInf ? 0xffff : k;         // NaN
-        return u == (0x8000 | kInf) ? 0 : k << 16 | (0xffffu - unit);
+    static __device__ __forceinline__ Key key(float x, int unit, uint32_t mask) {
+        const uint32_t k = (score_key(x) & 0xffffff00u) | (255u - unit);
+        return x == -__builtin_inff() ? 0 : k & mask;
     }
     static __device__ __forceinline__ float value(Key k) {
-        k >>= 16;
-        return to_f32(__builtin_bit_cast(E, static_cast<uint16_t>(k & 0x8000 ? k ^ 0x8000 : k ^ 0xffff)));
+        return __uint_as_float(static_cast<int32_t>(k) < 0 ? (k & 0xffffff00u) ^ 0x80000000u : ~(k | 0xffu));
     }
-    static __device__ __forceinline__ int unit(Key k) { return 0xffff - static_cast<int>(k & 0xffff); }
+    static __device__ __forceinline__ int unit(Key k) { return 255 - static_cast<int>(k & 255); }
     template <int G>
     static __device__ __forceinline__ Key largest(Key k) {
         return group_max<G>(k);
@@ -117,8 +118,9 @@ struct Order {  // 16 bits: the logit's order in the upper half
 template <>
 struct Order<float> {
     using Key = uint64_t;
-    static __device__ __forceinline__ Key key(float x, int unit) {
-        return x == -__builtin_inff() ? 0 : uint64_t(score_key(x)) << 32 | (0xffffffffu - unit);
+    static __device__ __forceinline__ Key key(float x, int unit, uint32_t mask) {
+        const uint32_t k = x == -__builtin_inff() ? 0 : mask;
+        return uint64_t(score_key(x) & k) << 32 | ((0xffffffffu - unit) & k);
     }
     static __device__ __forceinline__ float value(Key key) {
         const uint32_t k = static_cast<uint32_t>(key >> 32);
@@ -139,44 +141,54 @@ __device__ __forceinline__ void order(K& a, K& b) {
     a = hi;
 }
 
-template <typename E, int G>
-__global__ __launch_bounds__(kThreads) void route_tokens(const Args a) {
+template <typename E, int G, int EACH, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void route_tokens(const Args a) {
     constexpr int kTokens = kWave / G;  // a wave takes at a time
-    constexpr int kSlots = (HSN_ROUTER_MAX_CHOSEN + G - 1) / G;  // slots that a lane of a group writes
+    constexpr int kThreads = WAVES * kWave;
+    // slots that a lane of a group writes: k is at most 16 and at most the units
+    constexpr int kMostK = G * EACH < HSN_ROUTER_MAX_CHOSEN ? G * EACH : HSN_ROUTER_MAX_CHOSEN;
+    constexpr int kSlots = (kMostK + G - 1) / G;
     using O = Order<E>;
     using Key = typename O::Key;
-    __shared__ double probs[kWaves][G * kEach];
-    __shared__ uint32_t counts[G * kEach], rows;
-    const int wave = uniform(threadIdx.x / kWave), lane = lane_id(), sub = lane % G, unit = sub * kEach;
-    for (int u = threadIdx.x; u < G * kEach; u += kThreads) counts[u] = 0;
+    __shared__ double probs[WAVES][G * EACH];
+    __shared__ uint32_t counts[G * EACH], rows;
+    const int wave = uniform(threadIdx.x / kWave), lane = lane_id(), sub = lane % G;
+    const Place<EACH> place(sub, a.M);
+    for (int u = threadIdx.x; u < G * EACH; u += kThreads) counts[u] = 0;
     if (threadIdx.x == 0) rows = 0;
-    __syncthreads();
-    const E* logits = static_cast<const E*>(a.logits);
-    float sum[kEach] = {};
-    double whole[kEach] = {};
+    const E* logits = static_cast<const E*>(a.logits) + place.begin;
+    float sum[EACH] = {};
+    double whole[EACH] = {};
     uint32_t live_tokens = 0;
-    const int64_t step = int64_t(a.groups) * kWaves * kTokens;
-    int64_t t = (int64_t(blockIdx.x) * kWaves + wave) * kTokens;
+    const int64_t step = int64_t(a.groups) * WAVES * kTokens;
+    int64_t t = (int64_t(blockIdx.x) * WAVES + wave) * kTokens;
     // the next tokens' logits are in flight while these are worked on (a token behind the last one: the last)
-    Four<E> next;
-    bool next_valid = false;
+    Units<E, EACH> next;
+    uint8_t next_valid = 1;
     const auto load = [&](int64_t from) {
         const int64_t i = from + lane / G, at = i < a.n ? i : a.n - 1;
-        next = load_units(logits + at * a.row, unit, a.M);
-        next_valid = a.valid ? a.valid[at] : true;
+        next = load_units<E, EACH>(logits + at * a.row);
+        if (a.valid) next_valid = a.valid[at];
     };
     if (t < a.n) load(t);
+    __syncthreads();
     int turn = 0;
     for (; t < a.n; t += step) {
         const int64_t i = t + lane / G;
-        const bool there = i < a.n, wanted = there && next_valid;
-        const Four<E> v = next;
-        if (t + step < a.n) load(t + step);
-        Key key[kEach];
+        const bool there = i < a.n;
+        float x[EACH];
+        Key key[EACH];
+        const uint32_t mask = there && next_valid ? 0xffffffffu : 0;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) key[j] = wanted ? O::key(v.e[j], unit + j) : 0;
-        order(key[0], key[1]), order(key[2], key[3]), order(key[0], key[2]), order(key[1], key[3]);
-        order(key[1], key[2]);
+        for (int j = 0; j < EACH; ++j) {
+            x[j] = place.mine(j) ? to_f32(next.e[j]) : -__builtin_inff();
+            key[j] = O::key(x[j], place.begin + j, mask);
+        }
+        if (t + step < a.n) load(t + step);
+        if constexpr (EACH == 4) {
+            order(key[0], key[1]), order(key[2], key[3]), order(key[0], key[2]), order(key[1], key[3]);
+            order(key[1], key[2]);
+        }
         Key kept[kSlots], first = 0;
 #pragma unroll
         for (int q = 0; q < kSlots; ++q) {
@@ -187,18 +199,22 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Args a) {
                 if (q == 0 && s == 0) first = most;
                 const bool mine = key[0] == most;
 #pragma unroll
-                for (int j = 0; j < kEach; ++j) key[j] = mine ? (j + 1 < kEach ? key[j + 1 < kEach ? j + 1 : j] : 0) : key[j];
+                for (int j = 0; j + 1 < EACH; ++j) key[j] = mine ? key[j + 1] : key[j];
+                key[EACH - 1] = mine ? 0 : key[EACH - 1];
                 kept[q] = sub == s ? most : kept[q];
             }
         }
         const bool live = first != 0;
         const float m = O::value(first);
-        float e[kEach];
+        float e[EACH], total = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) e[j] = exp_of(to_f32(v.e[j]) - m);
-        const float part = 1.0f / group_sum<G>((e[0] + e[1]) + (e[2] + e[3]));
+        for (int j = 0; j < EACH; ++j) {
+            e[j] = exp_of(x[j] - m);
+            total += e[j];
+        }
+        const float part = 1.0f / group_sum<G>(total);
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) sum[j] += live ? e[j] * part : 0.0f;
+        for (int j = 0; j < EACH; ++j) sum[j] += live ? e[j] * part : 0.0f;
         float w[kSlots], chosen = 0.0f;
 #pragma unroll
         for (int q = 0; q < kSlots; ++q) {
@@ -218,22 +234,21 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Args a) {
         live_tokens += live && sub == 0;
         if (++turn % kFlush == 0) {
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) whole[j] += sum[j], sum[j] = 0.0f;
+            for (int j = 0; j < EACH; ++j) whole[j] += sum[j], sum[j] = 0.0f;
         }
     }
     // lanes that hold the same units, then waves
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        whole[j] += sum[j];
-#pragma unroll
-        for (int mask = G; mask < kWave; mask *= 2) whole[j] += __shfl_xor(whole[j], mask, kWave);
-        if (lane < G) probs[wave][unit + j] = whole[j];
+    for (int j = 0; j < EACH; ++j) {
+        const double v = wave_sum<G>(whole[j] + sum[j]);
+        if (lane < G && place.mine(j)) probs[wave][place.begin + j] = v;
     }
     if (live_tokens) atomicAdd(&rows, live_tokens);
     __syncthreads();
     for (int u = threadIdx.x; u < a.M; u += kThreads) {
         double p = 0.0;
-        for (int w = 0; w < kWaves; ++w) p += probs[w][u];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) p += probs[w][u];
         a.part_probs[int64_t(blockIdx.x) * a.M + u] = p;
         a.part_counts[int64_t(blockIdx.x) * a.M + u] = counts[u];
     }
@@ -242,8 +257,8 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Args a) {
 
 // The workgroups' sums added and the balance, by one workgroup: a thread a unit and a slice of them.
 __global__ __launch_bounds__(kFinish) void route_finish(const Args a, int units) {  // units: a power of two >= M
-    constexpr int kFinishWaves = kFinish / kWave, kFlight = 8;
-    __shared__ double probs[kFinish], s[kFinishWaves];
+    constexpr int kFlight = 8;
+    __shared__ double probs[kFinish], s[3][kFinish / kWave];
     __shared__ uint64_t counts[kFinish];
     const int u = threadIdx.x % units, slice = threadIdx.x / units, slices = kFinish / units;
     const int at = min(u, a.M - 1);
@@ -273,7 +288,13 @@ __global__ __launch_bounds__(kFinish) void route_finish(const Args a, int units)
     }
     probs[threadIdx.x] = p;
     counts[threadIdx.x] = c;
-    r = block_sum<kFinishWaves>(r, s);  // (passes a barrier)
+    const int wave = threadIdx.x / kWave;
+    r = wave_sum(r);
+    if (threadIdx.x % kWave == 0) s[0][wave] = r;
+    __syncthreads();
+    if (threadIdx.x >= HSN_ROUTER_MAX_UNITS) return;  // (whole waves, that pass no further barrier)
+    r = 0.0;
+    for (int w = 0; w < kMostGroups / kWave; ++w) r += s[0][w];
     p = 0.0, c = 0;
     if (static_cast<int>(threadIdx.x) < a.M) {
         for (int i = threadIdx.x; i < kFinish; i += max(units, kWave)) {
@@ -284,40 +305,44 @@ __global__ __launch_bounds__(kFinish) void route_finish(const Args a, int units)
         a.tally[threadIdx.x] = static_cast<int64_t>(c);
         a.probs[threadIdx.x] = static_cast<float>(p);
     }
-    const double chosen = block_sum<kFinishWaves>(static_cast<double>(c), s);
-    const double dot = block_sum<kFinishWaves>(static_cast<double>(c) * p, s);
+    const double chosen = wave_sum(static_cast<double>(c)), dot = wave_sum(static_cast<double>(c) * p);
+    if (threadIdx.x % kWave == 0) s[1][wave] = chosen, s[2][wave] = dot;
+    __syncthreads();
     if (threadIdx.x == 0) {
+        double all = 0.0, balance = 0.0;
+        for (int w = 0; w < HSN_ROUTER_MAX_UNITS / kWave; ++w) all += s[1][w], balance += s[2][w];
         a.tally[a.M] = static_cast<int64_t>(r);
-        *a.balance = static_cast<float>(a.M * dot / (chosen > 0.0 ? chosen : 1.0));
+        *a.balance = static_cast<float>(a.M * balance / (all > 0.0 ? all : 1.0));
     }
 }
 static_assert(kMostGroups <= kFinish, "a thread a workgroup's live tokens");
 
 constexpr int kBackWaves = 4, kBackThreads = kBackWaves * kWave;
 
-template <typename E, int G>
+template <typename E, int G, int EACH>
 __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
     constexpr int kTokens = kWave / G;
     // slots of a wave's tokens that a lane brings: k is at most 16 and at most the units
-    constexpr int kMostK = G * kEach < HSN_ROUTER_MAX_CHOSEN ? G * kEach : HSN_ROUTER_MAX_CHOSEN;
+    constexpr int kMostK = G * EACH < HSN_ROUTER_MAX_CHOSEN ? G * EACH : HSN_ROUTER_MAX_CHOSEN;
     constexpr int kSlots = (kTokens * kMostK + kWave - 1) / kWave;
-    __shared__ float2 slots[kBackWaves][kTokens][G * kEach];  // whether a unit is chosen, its cotangent
-    const int wave = uniform(threadIdx.x / kWave), lane = lane_id(), sub = lane % G, unit = sub * kEach;
-    float2* const mine = slots[wave][lane / G] + unit;
-    const E* logits = static_cast<const E*>(a.logits);
+    __shared__ float2 slots[kBackWaves][kTokens][G * EACH];  // whether a unit is chosen, its cotangent
+    const int wave = uniform(threadIdx.x / kWave), lane = lane_id(), sub = lane % G;
+    const Place<EACH> place(sub, a.M);
+    float2* const mine = slots[wave][lane / G];
+    const E* logits = static_cast<const E*>(a.logits) + place.begin;
     E* to = static_cast<E*>(a.d_logits);
-    float load[kEach];
+    float load[EACH];
     double all = 0.0;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const double c = unit + j < a.M ? static_cast<double>(a.tally[unit + j]) : 0.0;
+    for (int j = 0; j < EACH; ++j) {
+        const double c = place.mine(j) ? static_cast<double>(a.tally[place.begin + j]) : 0.0;
         load[j] = static_cast<float>(c);
         all += c;
     }
 #pragma unroll
     for (int mask = 1; mask < G; mask *= 2) all += __shfl_xor(all, mask, kWave);
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) load[j] = all > 0.0 ? static_cast<float>(load[j] / all) : 0.0f;
+    for (int j = 0; j < EACH; ++j) load[j] = all > 0.0 ? static_cast<float>(load[j] / all) : 0.0f;
     const int64_t rows = a.tally[a.M];
     const float pull = a.d_balance && rows > 0
                            ? static_cast<float>(static_cast<double>(*a.d_balance) * a.M / static_cast<double>(rows))
@@ -331,14 +356,14 @@ __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
     }
     const int64_t step = int64_t(gridDim.x) * kBackWaves * kTokens;
     int64_t t = (int64_t(blockIdx.x) * kBackWaves + wave) * kTokens;
-    Four<E> next;
-    bool next_valid = false;
+    Units<E, EACH> next;
+    uint8_t next_valid = 1;
     int64_t next_unit[kSlots];
     float next_g[kSlots];
     const auto bring = [&](int64_t from) {
         const int64_t i = from + lane / G, at = i < a.n ? i : a.n - 1;
-        next = load_units(logits + at * a.row, unit, a.M);
-        next_valid = a.valid ? a.valid[at] : true;
+        next = load_units<E, EACH>(logits + at * a.row);
+        if (a.valid) next_valid = a.valid[at];
         if (a.g) {
 #pragma unroll
             for (int q = 0; q < kSlots; ++q) {
@@ -352,12 +377,13 @@ __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
     for (; t < a.n; t += step) {
         const int64_t i = t + lane / G;
         const bool there = i < a.n, wanted = there && next_valid;
-        float x[kEach];
+        float x[EACH];
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) x[j] = to_f32(next.e[j]);
+        for (int j = 0; j < EACH; ++j) x[j] = place.mine(j) ? to_f32(next.e[j]) : -__builtin_inff();
         if (a.g) {
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) mine[j] = make_float2(0.0f, 0.0f);
+            for (int j = 0; j < EACH; ++j)
+                if (place.mine(j)) mine[place.begin + j] = make_float2(0.0f, 0.0f);
             wave_order();
 #pragma unroll
             for (int q = 0; q < kSlots; ++q)
@@ -366,29 +392,38 @@ __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
             wave_order();
         }
         if (t + step < a.n) bring(t + step);
-        const float m = group_largest<G>(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-        const bool strange = x[0] != x[0] || x[1] != x[1] || x[2] != x[2] || x[3] != x[3];
-        const bool live = wanted && (m > -__builtin_inff() || of_group<G>(ballot(strange)) != 0);
-        float p[kEach], d[kEach];
+        float m = x[0];
+        bool strange = false;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) p[j] = exp_of(x[j] - m);
-        const float part = 1.0f / group_sum<G>((p[0] + p[1]) + (p[2] + p[3]));
+        for (int j = 0; j < EACH; ++j) {
+            m = fmaxf(m, x[j]);
+            strange = strange || x[j] != x[j];
+        }
+        m = group_largest<G>(m);
+        const bool live = wanted && (m > -__builtin_inff() || of_group<G>(ballot(strange)) != 0);
+        float p[EACH], d[EACH], total = 0.0f;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            p[j] = exp_of(x[j] - m);
+            total += p[j];
+        }
+        const float part = 1.0f / group_sum<G>(total);
         float toward = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
+        for (int j = 0; j < EACH; ++j) {
             p[j] *= part;
             toward = __builtin_fmaf(p[j], load[j], toward);
         }
         toward = group_sum<G>(toward);
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) d[j] = pull * p[j] * (load[j] - toward);
+        for (int j = 0; j < EACH; ++j) d[j] = pull * p[j] * (load[j] - toward);
         if (a.g) {
             float mass = 0.0f, mean = 0.0f;
-            float2 v[kEach];
+            float2 v[EACH];
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) {
-                v[j] = mine[j];
-                const float q = v[j].x != 0.0f ? p[j] : 0.0f;
+            for (int j = 0; j < EACH; ++j) {
+                v[j] = mine[place.begin + j];
+                const float q = v[j].x != 0.0f && place.mine(j) ? p[j] : 0.0f;
                 mass += q;
                 mean = __builtin_fmaf(q, v[j].y, mean);
             }
@@ -397,20 +432,20 @@ __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
             const float share = mass != 0.0f ? 1.0f / mass : 0.0f;  // (no unit chosen: 0)
             mean *= share;
 #pragma unroll
-            for (int j = 0; j < kEach; ++j)
+            for (int j = 0; j < EACH; ++j)
                 if (v[j].x != 0.0f) d[j] = __builtin_fmaf(p[j] * share, v[j].y - mean, d[j]);
         }
         if (!there) continue;
-        E out[kEach];
+        E out[EACH];
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) out[j] = from_f32<E>(live ? d[j] : 0.0f);
-        E* at = to + i * a.M + unit;
-        if (unit + kEach <= a.M) {
+        for (int j = 0; j < EACH; ++j) out[j] = from_f32<E>(live ? d[j] : 0.0f);
+        E* at = to + i * a.M + place.begin;
+        if (place.own == 0) {
             __builtin_memcpy(at, out, sizeof(out));
         } else {
 #pragma unroll
-            for (int j = 0; j < kEach; ++j)
-                if (unit + j < a.M) at[j] = out[j];
+            for (int j = 0; j < EACH; ++j)
+                if (place.mine(j)) at[j] = out[j];
         }
     }
 }
@@ -421,14 +456,20 @@ __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
 
 int size_of(int dtype) { return dtype == HSN_DTYPE_F32 ? 4 : 2; }
 
-int lanes_of(int M) {  // G
+// A token's lanes (G) and a lane's units.
+int lanes_of(int M) {
+    if (M < 4) return 4;
     int g = 1;
-    while (g * kEach < M) g *= 2;
+    while (g * 4 < M) g *= 2;
     return g;
 }
 
+// Waves of a forward workgroup: 16 where the tokens keep a workgroup of them on each compute unit busy, else 4,
+// which leaves a SIMD to a wave.
+int waves_of(int n, int M) { return n > int64_t(kMostGroups) * 4 * (kWave / lanes_of(M)) ? 16 : 4; }
+
 int groups_of(int n, int M) {
-    const int64_t tokens = int64_t(kWaves) * (kWave / lanes_of(M));
+    const int64_t tokens = int64_t(waves_of(n, M)) * (kWave / lanes_of(M));
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostGroups, (n + tokens - 1) / tokens)));
 }
 
@@ -448,14 +489,16 @@ int64_t layout(Args& a, char* at) {
 template <typename F>
 void with_lanes(int M, F&& f) {
     using std::integral_constant;
+    constexpr integral_constant<int, 4> four;
+    if (M < 4) return f(four, integral_constant<int, 1>());
     switch (lanes_of(M)) {
-        case 1: return f(integral_constant<int, 1>());
-        case 2: return f(integral_constant<int, 2>());
-        case 4: return f(integral_constant<int, 4>());
-        case 8: return f(integral_constant<int, 8>());
-        case 16: return f(integral_constant<int, 16>());
-        case 32: return f(integral_constant<int, 32>());
-        default: return f(integral_constant<int, 64>());
+        case 1: return f(integral_constant<int, 1>(), four);
+        case 2: return f(integral_constant<int, 2>(), four);
+        case 4: return f(four, four);
+        case 8: return f(integral_constant<int, 8>(), four);
+        case 16: return f(integral_constant<int, 16>(), four);
+        case 32: return f(integral_constant<int, 32>(), four);
+        default: return f(integral_constant<int, 64>(), four);
     }
 }
 template <typename F>
@@ -514,8 +557,12 @@ extern "C" int hsn_unit_router_forward(const void* logits, int64_t row, int dtyp
                 "the workspace must be aligned to 16 bytes");
     hipStream_t st = as_stream(stream);
     with_type(dtype, [&](auto e) {
-        with_lanes(M, [&](auto g) {
-            route_tokens<decltype(e), decltype(g)::value><<<a.groups, kThreads, 0, st>>>(a);
+        with_lanes(M, [&](auto g, auto each) {
+            using E = decltype(e);
+            constexpr int kG = decltype(g)::value, kEach = decltype(each)::value;
+            const int waves = waves_of(n, M);
+            (waves == 4 ? route_tokens<E, kG, kEach, 4>
+                        : route_tokens<E, kG, kEach, 16>)<<<a.groups, waves * kWave, 0, st>>>(a);
         });
     });
     HSN_HIP(hipGetLastError());
@@ -543,11 +590,11 @@ extern "C" int hsn_unit_router_backward(const void* logits, int64_t row, int dty
     a.g = d_shares, a.g_row = g_row, a.d_balance = d_balance, a.d_logits = d_logits;
     hipStream_t st = as_stream(stream);
     with_type(dtype, [&](auto e) {
-        with_lanes(M, [&](auto g) {
-            constexpr int kG = decltype(g)::value;
+        with_lanes(M, [&](auto g, auto each) {
+            constexpr int kG = decltype(g)::value, kEach = decltype(each)::value;
             const int64_t tokens = int64_t(kBackWaves) * (kWave / kG);
             const int grid = static_cast<int>(std::min<int64_t>(kMostBackward, (n + tokens - 1) / tokens));
-            route_backward<decltype(e), kG><<<grid, kBackThreads, 0, st>>>(a);
+            route_backward<decltype(e), kG, kEach><<<grid, kBackThreads, 0, st>>>(a);
         });
     });
     HSN_HIP(hipGetLastError());
