@@ -209,53 +209,25 @@ __global__ __launch_bounds__(kThreads) void scale(const List<2> l) {
 // The launches of a pass.
 // ------------------------------------------------------------------------------------------
 
-// Where the launches of a pass with ROWS operands begin and end, tensors without an element left out.
-struct Part {
-    std::vector<int> tensors;
-    uint32_t chunks = 0;
-};
+constexpr int64_t kMostChunks = (int64_t(1) << 32) - 1;  // of a list
 
-template <int ROWS>
-std::vector<Part> parts_of(const int64_t* numels, int n) {
-    std::vector<Part> parts;
-    for (int j = 0; j < n; ++j) {
-        if (numels[j] == 0) continue;
-        const int64_t chunks = (numels[j] + kChunk - 1) / kChunk;
-        HSN_REQUIRE(chunks < (int64_t(1) << 31), HSN_ERR_SIZE_OVERFLOW,
-                    "a tensor has 2^43 elements or more");
-        if (parts.empty() || parts.back().tensors.size() == List<ROWS>::kTensors ||
-            parts.back().chunks + chunks >= (int64_t(1) << 32))
-            parts.emplace_back();
-        parts.back().tensors.push_back(j);
-        parts.back().chunks += static_cast<uint32_t>(chunks);
-    }
-    return parts;
+int launches_of(int n, int tensors) { return std::max(1, (n + tensors - 1) / tensors); }
+// Workgroups of a launch, of so many.
+int grid_of(uint32_t chunks, int launches) {
+    return static_cast<int>(std::min<uint32_t>(chunks, std::max(kFewest, kPartials / launches)));
 }
-
-int grid_of(const Part& part, size_t launches) {
-    const uint32_t most = std::max(kFewest, kPartials / static_cast<int>(launches));
-    return static_cast<int>(std::min(part.chunks, most));
-}
-
-int partials_of(const std::vector<Part>& parts) {
-    int total = 0;
-    for (const Part& part : parts) total += grid_of(part, parts.size());
-    return total;
+int most_partials(int n) {
+    const int launches = launches_of(n, List<1>::kTensors);
+    return std::max(kPartials, kFewest * launches);
 }
 
 template <int ROWS>
-void fill(List<ROWS>& l, const Part& part, const void* const* const (&rows)[ROWS], const int64_t* numels,
-          const int* dtypes) {
-    uint32_t chunk = 0;
-    l.n = 0;
-    for (int j : part.tensors) {
-        const uint64_t last = static_cast<uint64_t>((numels[j] - 1) % kChunk);
-        for (int r = 0; r < ROWS; ++r)
-            l.at[r][l.n] = reinterpret_cast<uintptr_t>(rows[r][j]) | last << 48 | uint64_t(dtypes[j]) << 62;
-        l.first[l.n++] = chunk;
-        chunk += static_cast<uint32_t>((numels[j] + kChunk - 1) / kChunk);
-    }
-    l.chunks = chunk;
+void append(List<ROWS>& l, const void* const (&rows)[ROWS], int64_t numel, int dtype) {
+    const uint64_t last = static_cast<uint64_t>((numel - 1) % kChunk);
+    for (int r = 0; r < ROWS; ++r)
+        l.at[r][l.n] = reinterpret_cast<uintptr_t>(rows[r]) | last << 48 | uint64_t(dtype) << 62;
+    l.first[l.n++] = l.chunks;
+    l.chunks += static_cast<uint32_t>((numel + kChunk - 1) / kChunk);
 }
 
 int64_t size_of(int dtype) { return dtype == HSN_DTYPE_F32 ? 4 : 2; }
@@ -269,30 +241,30 @@ struct Range {
 // What is written lies apart from everything else, a tensor's own gradient in place aside.
 void check_apart(const void* const* grads, void* const* outs, const int64_t* numels, const int* dtypes, int n) {
     std::vector<Range> written;
+    written.reserve(n);
+    bool sorted = true;
     for (int j = 0; j < n; ++j)
         if (numels[j]) {
             const uintptr_t at = reinterpret_cast<uintptr_t>(outs[j]);
+            sorted = sorted && (written.empty() || written.back().from <= at);
             written.push_back({at, at + static_cast<uintptr_t>(numels[j] * size_of(dtypes[j])), j});
         }
-    std::sort(written.begin(), written.end());
+    if (written.empty()) return;
+    if (!sorted) std::sort(written.begin(), written.end());
     for (size_t i = 1; i < written.size(); ++i)
         HSN_REQUIRE(written[i].from >= written[i - 1].to, HSN_ERR_INVALID_ARGUMENT,
                     "tensors " + std::to_string(written[i - 1].j) + " and " + std::to_string(written[i].j) +
                         " to be written overlap");
+    const uintptr_t first = written.front().from, last = written.back().to;
     for (int j = 0; j < n; ++j) {
         if (!numels[j] || grads[j] == outs[j]) continue;
         const uintptr_t from = reinterpret_cast<uintptr_t>(grads[j]);
         const uintptr_t to = from + static_cast<uintptr_t>(numels[j] * size_of(dtypes[j]));
+        if (to <= first || from >= last) continue;
         auto it = std::lower_bound(written.begin(), written.end(), Range{to, 0, 0});  // begins at or after the end
         HSN_REQUIRE(it == written.begin() || std::prev(it)->to <= from, HSN_ERR_INVALID_ARGUMENT,
                     "a tensor to be written overlaps gradient " + std::to_string(j));
     }
-}
-
-void check(const int64_t* numels, int n) {
-    HSN_REQUIRE(n >= 0 && (n == 0 || numels), HSN_ERR_INVALID_ARGUMENT, "bad tensor list");
-    for (int j = 0; j < n; ++j)
-        HSN_REQUIRE(numels[j] >= 0, HSN_ERR_INVALID_ARGUMENT, "a tensor's element count is negative");
 }
 
 }  // namespace
@@ -304,9 +276,9 @@ using namespace hsn::clip;
 
 extern "C" int hsn_clip_workspace(const int64_t* numels, int n, int64_t* bytes) {
     HSN_ABI_BEGIN
-    check(numels, n);
+    HSN_REQUIRE(n >= 0 && (n == 0 || numels), HSN_ERR_INVALID_ARGUMENT, "bad tensor list");
     HSN_REQUIRE(bytes, HSN_ERR_INVALID_ARGUMENT, "bytes must not be NULL");
-    *bytes = 8 * int64_t(std::max(1, partials_of(parts_of<1>(numels, n))));
+    *bytes = 8 * int64_t(most_partials(n));
     HSN_ABI_END
 }
 
@@ -314,54 +286,70 @@ extern "C" int hsn_clip(const void* const* grads, void* const* outs, const int64
                         int n, double max_norm, double* result, void* workspace, int64_t workspace_bytes,
                         void* stream) {
     HSN_ABI_BEGIN
-    check(numels, n);
-    HSN_REQUIRE(n == 0 || (grads && dtypes), HSN_ERR_INVALID_ARGUMENT, "a required list is NULL");
+    HSN_REQUIRE(n >= 0 && (n == 0 || (grads && numels && dtypes)), HSN_ERR_INVALID_ARGUMENT, "bad tensor list");
     HSN_REQUIRE(result && workspace, HSN_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
     HSN_REQUIRE(max_norm >= 0.0, HSN_ERR_INVALID_ARGUMENT, "max_norm >= 0");
-    bool in_place = true;
-    for (int j = 0; j < n; ++j) {
-        HSN_REQUIRE(dtypes[j] == HSN_DTYPE_F32 || dtypes[j] == HSN_DTYPE_F16 || dtypes[j] == HSN_DTYPE_BF16,
-                    HSN_ERR_UNSUPPORTED_DTYPE, "a gradient must be F32, F16 or BF16");
-        if (!numels[j]) continue;
-        HSN_REQUIRE(grads[j] && (!outs || outs[j]), HSN_ERR_INVALID_ARGUMENT, "a tensor's address is NULL");
-        for (const void* p : {grads[j], outs ? static_cast<const void*>(outs[j]) : grads[j]})
-            HSN_REQUIRE(reinterpret_cast<uintptr_t>(p) <= kAddress &&
-                            reinterpret_cast<uintptr_t>(p) % size_of(dtypes[j]) == 0,
-                        HSN_ERR_INVALID_ARGUMENT, "a tensor's address is not aligned to its type");
-        in_place = in_place && outs && outs[j] == grads[j];
-    }
-    if (outs) check_apart(grads, outs, numels, dtypes, n);
-    const std::vector<Part> parts = parts_of<1>(numels, n);
-    const int n_partials = partials_of(parts);
-    HSN_REQUIRE(workspace_bytes >= 8 * int64_t(std::max(1, n_partials)), HSN_ERR_INVALID_ARGUMENT,
+    HSN_REQUIRE(workspace_bytes >= 8 * int64_t(most_partials(n)), HSN_ERR_INVALID_ARGUMENT,
                 "the workspace is too small");
     HSN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 8 == 0, HSN_ERR_INVALID_ARGUMENT,
                 "the workspace must be aligned to 8 bytes");
+    bool in_place = true;
+    int filled = 0;  // tensors with an element
+    int64_t chunks = 0, written_bytes = 0;
+    for (int j = 0; j < n; ++j) {
+        HSN_REQUIRE(dtypes[j] == HSN_DTYPE_F32 || dtypes[j] == HSN_DTYPE_F16 || dtypes[j] == HSN_DTYPE_BF16,
+                    HSN_ERR_UNSUPPORTED_DTYPE, "a gradient must be F32, F16 or BF16");
+        HSN_REQUIRE(numels[j] >= 0, HSN_ERR_INVALID_ARGUMENT, "a tensor's element count is negative");
+        if (!numels[j]) continue;
+        const uintptr_t g = reinterpret_cast<uintptr_t>(grads[j]);
+        const uintptr_t o = outs ? reinterpret_cast<uintptr_t>(outs[j]) : g;
+        HSN_REQUIRE(g && o, HSN_ERR_INVALID_ARGUMENT, "a tensor's address is NULL");
+        HSN_REQUIRE((g | o) <= kAddress && (g | o) % size_of(dtypes[j]) == 0, HSN_ERR_INVALID_ARGUMENT,
+                    "a tensor's address is not aligned to its type");
+        in_place = in_place && g == o;
+        chunks += (numels[j] - 1) / kChunk + 1;
+        HSN_REQUIRE(chunks <= kMostChunks, HSN_ERR_SIZE_OVERFLOW, "the list has 2^44 elements or more");
+        written_bytes += numels[j] * size_of(dtypes[j]);
+        ++filled;
+    }
+    if (outs) check_apart(grads, outs, numels, dtypes, n);
     hipStream_t st = as_stream(stream);
-    double* at = static_cast<double*>(workspace);
-    for (const Part& part : parts) {
-        List<1> l{};
-        fill<1>(l, part, {grads}, numels, dtypes);
-        l.partials = at;
-        const int grid = grid_of(part, parts.size());
+    double* const partials = static_cast<double*>(workspace);
+    int n_partials = 0;
+    List<1> l;
+    l.n = 0, l.chunks = 0;
+    const int launches = launches_of(filled, List<1>::kTensors);
+    for (int j = 0, left = filled; left; ++j) {
+        if (!numels[j]) continue;
+        append<1>(l, {grads[j]}, numels[j], dtypes[j]);
+        if (--left && l.n < List<1>::kTensors) continue;
+        l.partials = partials + n_partials;
+        const int grid = grid_of(l.chunks, launches);
         squares<<<grid, kThreads, 0, st>>>(l);
         HSN_HIP(hipGetLastError());
-        at += grid;
+        n_partials += grid;
+        l.n = 0, l.chunks = 0;
     }
-    List<2> l{};
-    l.partials = static_cast<double*>(workspace);
-    l.n_partials = n_partials, l.max_norm = max_norm, l.result = result, l.in_place = in_place;
-    l.writes_result = true;
-    int64_t written_bytes = 0;
-    for (int j = 0; outs && j < n; ++j) written_bytes += numels[j] * size_of(dtypes[j]);
-    const auto kernel = written_bytes > kStream ? scale<true> : scale<false>;
-    const std::vector<Part> written = outs ? parts_of<2>(numels, n) : std::vector<Part>();
-    if (written.empty()) kernel<<<1, kThreads, 0, st>>>(l);
-    for (const Part& part : written) {
-        fill<2>(l, part, {grads, outs}, numels, dtypes);
-        kernel<<<grid_of(part, written.size()), kThreads, 0, st>>>(l);
-        l.writes_result = false;
+    List<2> m;
+    m.n = 0, m.chunks = 0;
+    m.partials = partials, m.n_partials = n_partials, m.max_norm = max_norm, m.result = result;
+    m.in_place = in_place && outs;
+    m.writes_result = true;
+    const auto kernel = outs && written_bytes > kStream ? scale<true> : scale<false>;
+    if (!outs || !filled) {
+        kernel<<<1, kThreads, 0, st>>>(m);
+        HSN_HIP(hipGetLastError());
+        return HSN_OK;
     }
-    HSN_HIP(hipGetLastError());
+    const int writes = launches_of(filled, List<2>::kTensors);
+    for (int j = 0, left = filled; left; ++j) {
+        if (!numels[j]) continue;
+        append<2>(m, {grads[j], outs[j]}, numels[j], dtypes[j]);
+        if (--left && m.n < List<2>::kTensors) continue;
+        kernel<<<grid_of(m.chunks, writes), kThreads, 0, st>>>(m);
+        HSN_HIP(hipGetLastError());
+        m.n = 0, m.chunks = 0;
+        m.writes_result = false;
+    }
     HSN_ABI_END
 }

@@ -566,9 +566,16 @@ struct List {
     Py_ssize_t size() const { return seq ? PySequence_Fast_GET_SIZE(seq) : 0; }
     const Tensor* at(Py_ssize_t i) const {
         PyObject* o = PySequence_Fast_GET_ITEM(seq, i);
-        return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+        const bool exact = reinterpret_cast<PyObject*>(Py_TYPE(o)) == THPVariableClass;  // (the usual case)
+        return exact || THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
     }
 };
+
+// data_ptr() of a tensor that has a storage, inlined: a list has hundreds of them.
+void* address_of(const at::TensorImpl* t) {
+    char* const base = static_cast<char*>(t->unsafe_storage().unsafeGetStorageImpl()->mutable_data());
+    return base + t->storage_offset() * t->itemsize();
+}
 
 // grad_clip(workspace, clip, stream, grads, outs, max_norm): outs None: the norm and the coefficient alone
 PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
@@ -589,23 +596,29 @@ PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     const Tensor* first = grads.at(0);
     if (!first || !first->is_cuda()) Py_RETURN_NONE;
     const auto device = first->device();
+    const bool recording = at::GradMode::is_enabled(), in_place = outs_given == grads.seq;
     for (Py_ssize_t i = 0; i < n; ++i) {
-        const Tensor* g = grads.at(i);
-        if (!g || g->device() != device || !plain(*g) || !g->is_non_overlapping_and_dense() ||
-            wants_gradient({g}))
-            Py_RETURN_NONE;
-        codes[i] = dtype_code(g->scalar_type());
-        if (codes[i] < 0) Py_RETURN_NONE;
+        const Tensor* given = grads.at(i);
+        if (!given || !plain(*given) || (recording && given->requires_grad())) Py_RETURN_NONE;
+        const at::TensorImpl* g = given->unsafeGetTensorImpl();
+        codes[i] = dtype_code(given->scalar_type());
+        if (codes[i] < 0 || g->device() != device || !g->is_non_overlapping_and_dense()) Py_RETURN_NONE;
         numels[i] = g->numel();
-        at[i] = g->data_ptr();
+        at[i] = address_of(g);
         if (!writes) continue;
-        const Tensor* o = outs.at(i);
-        if (!o || o->device() != device || !plain(*o) || o->scalar_type() != g->scalar_type() ||
-            o->sizes() != g->sizes() || wants_gradient({o}))
+        if (in_place) {
+            at[n + i] = at[i];
+            continue;
+        }
+        const Tensor* out = outs.at(i);
+        if (!out || !plain(*out) || (recording && out->requires_grad())) Py_RETURN_NONE;
+        const at::TensorImpl* o = out->unsafeGetTensorImpl();
+        const at::IntArrayRef sizes = g->sizes(), strides = g->strides(), others = o->strides();
+        if (out->scalar_type() != given->scalar_type() || o->device() != device || o->sizes() != sizes)
             Py_RETURN_NONE;
-        for (int64_t d = 0; numels[i] && d < g->dim(); ++d)
-            if (g->size(d) > 1 && o->stride(d) != g->stride(d)) Py_RETURN_NONE;
-        at[n + i] = o->data_ptr();
+        for (size_t d = 0; numels[i] && d < sizes.size(); ++d)
+            if (sizes[d] > 1 && others[d] != strides[d]) Py_RETURN_NONE;
+        at[n + i] = address_of(o);
     }
     int64_t bytes = 0;
     int status = entry<int (*)(const int64_t*, int, int64_t*)>(size_at)(numels.data(), n, &bytes);
@@ -620,8 +633,10 @@ PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                                         codes.data(), n, max_norm, result.data_ptr(), ws.data_ptr(), bytes,
                                         entry<P>(stream));
     if (status) return PyLong_FromLong(status);
-    for (Py_ssize_t i = 0; writes && i < n; ++i)  // an update in place, as autograd sees it
-        if (!outs.at(i)->is_inference()) outs.at(i)->unsafeGetTensorImpl()->bump_version();
+    for (Py_ssize_t i = 0; writes && i < n; ++i) {  // an update in place, as autograd sees it
+        at::TensorImpl* o = outs.at(i)->unsafeGetTensorImpl();
+        if (!o->is_inference()) o->bump_version();
+    }
     return Py_BuildValue("(NN)", wrap(result.narrow(0, 0, 1)), wrap(result.narrow(0, 1, 1)));
     END_HANDLE_TH_ERRORS
 }
