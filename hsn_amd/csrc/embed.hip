@@ -5,7 +5,7 @@
 // Backward: the positions are sorted by token, and then every sum is over neighbours. The sort is by digits
 // of up to ten bits from the lowest on, stable, so a token's positions stay in order: a workgroup counts a
 // tile's digits, and the next launch ranks the tile's entries (lanes of a wave with the same digit find each
-// other by ballots) and adds up where they go from all tiles' counts. Up to 16384 positions need one launch:
+// other by ballots) and adds up where they go from all tiles' counts. Up to 8192 positions need one launch:
 // each workgroup counts, for a few entries, what lies before them in the whole list. The sums are taken over chunks of the sorted list, one as long as the other, so a
 // token that fills a tenth of the text costs no workgroup more than another: a group of lanes walks a
 // chunk with a slice of the columns, writes the rows that begin and end inside it, and leaves the sums
@@ -26,7 +26,8 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kDigit = 10, kBins = 1 << kDigit;
-constexpr int kSmall = 16384, kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
+constexpr int kSmall = 8192, kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
+constexpr int kEntries = 16;    // that a workgroup of the short sort places
 constexpr int kBatch = 8;       // entries of a chunk in flight
 constexpr int kCounts = 16;     // tiles' counts in flight
 constexpr int kZeroRows = 64;   // rows that a workgroup looks through for those without a token
@@ -201,13 +202,13 @@ __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t* s) {
 // ballot's bits are counted by scalar ones. With k' = 2 k + (1 for the entries' own 64 and later ones), k' < 2
 // k_i + 1 says k < k_i there and k <= k_i before; what is equal and earlier among the entries' own 64 is
 // added by one wave. 8192 entries take 10 us, where two digits by two launches each took 24; the scalar
-// counts bound it.
+// counts bound it, and 16384 take longer (26) than by digits.
 template <int R>
-__global__ __launch_bounds__(kSmallThreads) void sort_small(const Args a, int entries) {
+__global__ __launch_bounds__(kSmallThreads) void sort_small(const Args a) {
     __shared__ int counts[kSmallWaves][kWave];
     const int wave = uniform(threadIdx.x / kWave), lane = lane_id();
-    const uint32_t first = blockIdx.x * entries, own = first / kWave;
-    // the list; then the lane's entry (of the first `entries` lanes) and the lane's of the entries' own 64
+    const uint32_t first = blockIdx.x * kEntries, own = first / kWave;
+    // the list; then the lane's entry (of the first kEntries lanes) and the lane's of the entries' own 64
     uint32_t at[R + 2], key[R + 2];
     const uint32_t mine = first + lane, beside = own * kWave + lane;
 #pragma unroll
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small(const Args a, int en
         key[r] = 2 * (block * kWave + lane < a.n ? key[r] : 1u << 30) + (block >= own ? 1 : 0);
     }
     int count = 0;
-    for (int i = 0; i < entries; ++i) {
+    for (int i = 0; i < kEntries; ++i) {
         const uint32_t t = readlane(token, i);
         int c = 0;
 #pragma unroll
@@ -231,7 +232,7 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small(const Args a, int en
     }
     counts[wave][lane] = count;
     __syncthreads();
-    if (wave || lane >= entries || mine >= a.n) return;
+    if (wave || lane >= kEntries || mine >= a.n) return;
     for (int w = 1; w < kSmallWaves; ++w) count += counts[w][lane];
     a.to[count] = {token, mine};
 }
@@ -578,13 +579,12 @@ const Entry* sort(Args a, const Workspace& w, hipStream_t st) {
     while (a.V >> bits) ++bits;  // padding is V
     if (a.n <= kSmall) {
         a.to = w.a;
-        const int entries = a.n <= 8192 ? 16 : 32, grid = (a.n + entries - 1) / entries;
+        const int grid = (a.n + kEntries - 1) / kEntries;
         const int held = (a.n + kSmallThreads - 1) / kSmallThreads;
         (held <= 1   ? sort_small<1>
          : held <= 2 ? sort_small<2>
          : held <= 4 ? sort_small<4>
-         : held <= 8 ? sort_small<8>
-                     : sort_small<16>)<<<grid, kSmallThreads, 0, st>>>(a, entries);
+                     : sort_small<8>)<<<grid, kSmallThreads, 0, st>>>(a);
         HSN_HIP(hipGetLastError());
         return w.a;
     }
