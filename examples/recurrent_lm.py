@@ -1,14 +1,16 @@
 """A small recurrent language model on this package's operators, from training to answering.
 
-The model reads tokens through the gated linear recurrence (:mod:`hsn_amd.scan`) and answers through
-a bank of units that a router chooses (two a token):
+The model reads tokens (:mod:`hsn_amd.embedding`) through the gated linear recurrence
+(:mod:`hsn_amd.scan`) and answers through a bank of units that a router chooses (two a token):
 
     x = embed[token];  y | gate = x Wz;  h = scan(y, gate);  o = units(h);  logits = o out^T
 
 Training runs whole windows: the recurrence as one autograd node with its state carried from window
-to window, the units as the grouped unit MLP of :mod:`hsn_amd.kernels.ops`. Answering reads the
-prompt with one forward scan, and then takes a token at a time: one position of the recurrence on a
-pool of states (:func:`hsn_amd.scan.step`), the unit layer for a few tokens
+to window, the units' choice with its balance loss (:mod:`hsn_amd.unit_router`), the units as the grouped
+unit MLP of :mod:`hsn_amd.kernels.ops`, the loss from the tokens' log probabilities
+(:mod:`hsn_amd.scoring`), and the gradients clipped by their global norm (:mod:`hsn_amd.grad_clip`).
+Answering reads the prompt with one forward scan, and then takes a token at a time: one position of the
+recurrence on a pool of states (:func:`hsn_amd.scan.step`), the unit layer for a few tokens
 (:func:`hsn_amd.unit_layer.unit_layer`) and the choice of a token from given random numbers
 (:func:`hsn_amd.sampling.sample`). The decoded position is a HIP graph, replayed for every token.
 
@@ -29,7 +31,7 @@ from torch import Tensor
 if __name__ == "__main__":
     sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
-from hsn_amd import sampling, scan
+from hsn_amd import embedding, grad_clip, sampling, scan, scoring, unit_router
 from hsn_amd.kernels import ops
 from hsn_amd.unit_layer import unit_layer
 
@@ -53,19 +55,23 @@ class RecurrentLM(torch.nn.Module):
         self.out = weight(vocabulary, d, scale=d ** -0.5)
 
     def gates(self, tokens: Tensor) -> tuple[Tensor, Tensor]:
-        z = self.embed[tokens] @ self.Wz
+        z = embedding.embed(tokens, self.embed) @ self.Wz
         return z[..., :self.D], z[..., self.D:] - 1.0
 
     def forward(self, tokens: Tensor, reset: Tensor, h0: Tensor) -> tuple[Tensor, Tensor]:
         """``(logits [B, T, vocabulary], the state after the window)``, with a gradient."""
+        logits, _, h_T = self.window(tokens, reset, h0)
+        return logits, h_T
+
+    def window(self, tokens: Tensor, reset: Tensor, h0: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+        """The same with the units' balance loss (1 where all are chosen alike) between."""
         h, h_T = scan.gated_scan(*self.gates(tokens), reset, h0)
         flat = h.reshape(-1, self.D)
-        best, units = torch.topk(flat @ self.router.t(), self.k, dim=1)
-        share = torch.softmax(best, dim=1)
+        units, share, balance, _ = unit_router.choose_units(flat @ self.router.t(), self.k)
         pairs = flat.repeat_interleave(self.k, dim=0)
         o, _ = ops.mlp_op(pairs, units.reshape(-1), self.W1, self.b1, self.W2, self.b2)
         o = (o.view(-1, self.k, o.shape[1]) * share[..., None]).sum(1)
-        return (o @ self.out.t()).view(*tokens.shape, -1), h_T
+        return (o @ self.out.t()).view(*tokens.shape, -1), balance, h_T
 
     def units(self, h: Tensor) -> Tensor:
         """The logits of a few tokens' states, without a gradient."""
@@ -124,22 +130,25 @@ def phrases(rows: int, length: int, vocabulary: int, seed: int) -> tuple[Tensor,
 
 
 def train(model: RecurrentLM, steps: int, rows: int = 16, length: int = 256, windows: int = 2,
-          seed: int = 0) -> list[float]:
-    """Trains on fresh text, ``windows`` carried windows a step; returns the losses."""
+          seed: int = 0, balance_weight: float = 0.01, max_norm: float = 1.0) -> list[float]:
+    """Trains on fresh text, ``windows`` carried windows a step; returns the losses (without the
+    balance's)."""
     device = model.embed.device
     optimiser = torch.optim.AdamW(model.parameters(), lr=3e-3)
     losses = []
     for step in range(steps):
         tokens, start = (t.to(device) for t in phrases(rows, windows * length + 1, 32, seed + step))
         state = torch.zeros(rows, model.D, device=device)
-        total = 0.0
+        total = balance = 0.0
         for w in range(windows):
             at = slice(w * length, (w + 1) * length)
-            logits, state = model(tokens[:, at], start[:, at].contiguous(), state)
+            logits, load, state = model.window(tokens[:, at], start[:, at].contiguous(), state)
             target = tokens[:, at.start + 1:at.stop + 1]
-            total = total + torch.nn.functional.cross_entropy(logits.flatten(0, 1), target.flatten())
+            total = total - scoring.token_logprobs(logits, target)[0].mean()
+            balance = balance + load
         optimiser.zero_grad()
-        total.backward()
+        (total + balance_weight * balance).backward()
+        grad_clip.clip([p.grad for p in model.parameters()], max_norm)
         optimiser.step()
         losses.append(float(total.detach()) / windows)
     return losses

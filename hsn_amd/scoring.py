@@ -157,7 +157,7 @@ class TokenLogprobs(torch.autograd.Function):
 def token_logprobs(logits: Tensor, tokens: Tensor) -> tuple[Tensor, Tensor]:
     """``(logprob, entropy)`` of ``logits [..., V]`` and ``tokens [...]``, fp32 and of the tokens'
     shape, differentiable in ``logits``."""
-    if tokens.shape != logits.shape[:-1]:
+    if logits.dim() == 0 or tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens must be {tuple(logits.shape[:-1])}, got {tuple(tokens.shape)}")
     logprob, entropy = TokenLogprobs.apply(logits.reshape(-1, logits.shape[-1]), tokens.reshape(-1))
     return logprob.view(tokens.shape), entropy.view(tokens.shape)

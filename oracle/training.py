@@ -51,10 +51,10 @@ def score(logits, tokens, top=0):
             rest = torch.log(torch.exp(x).sum())
             logp = x - rest
             p = torch.exp(logp)
-            entropy[i] = -sum(float(q * l) for q, l in zip(p, logp) if q > 0)
+            entropy[i] = -torch.where(p > 0, p * logp, 0.0).sum()
             logprob[i] = logp[t] if given else 0.0
-        order = sorted((j for j, v in enumerate(row.tolist()) if v > -math.inf),
-                       key=lambda j: (-float(row[j]), j))[:top]
+        fine = torch.nonzero(row > -math.inf)[:, 0]  # (not NaN either)
+        order = fine[torch.sort(-row[fine], stable=True).indices][:top].tolist()
         for r, j in enumerate(order):
             best[i, r] = j
             best_logprob[i, r] = math.nan if math.isnan(float(entropy[i])) else logp[j]
