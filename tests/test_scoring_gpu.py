@@ -162,15 +162,19 @@ def test_strides(cuda_device, tokens):
         for start in (0, 1, 3, 1101):
             view, t = wide[:, start:start + 999], target[:, 1]
             out, ref = scoring.forward(view, t, top=4), scoring.forward(view.contiguous(), t.contiguous(), top=4)
-            for name in out:
-                assert torch.equal(out[name], ref[name]), name
+            # the sums' order goes by the rows' addresses, so either is within its bar of the formula's value
+            assert torch.equal(out["top_tokens"], ref["top_tokens"])
+            for name in ("logprob", "top_logprobs"):
+                _near(out[name], ref[name].cpu(), 2 * (60 + 2 * (ref[name].cpu().abs().double() + 1)) * U)
+            _near(out["entropy"], ref["entropy"].cpu(), 2 * 130 * U * ref["entropy"].cpu().double().clamp(min=1.0))
+            ref = out
             back = scoring.backward(view, t, out["stats"], d[:, 0], d[:1, 1].expand(6))
             same = scoring.backward(view.contiguous(), t.contiguous(), ref["stats"],
                                     d[:, 0].contiguous(), d[:1, 1].expand(6).contiguous())
             assert torch.equal(back, same)
         turned = wide[::2, :999]
-        assert torch.equal(scoring.forward(turned, target[::2, 0])["logprob"],
-                           scoring.forward(turned.contiguous(), target[::2, 0])["logprob"])
+        got, want = (scoring.forward(x, target[::2, 0])["logprob"].cpu() for x in (turned, turned.contiguous()))
+        _near(got, want, 2 * (60 + 2 * (want.abs().double() + 1)) * U)
 
 
 def test_the_gradient_against_differences(cuda_device):
@@ -214,7 +218,7 @@ def test_the_autograd_node(cuda_device):
     (scoring.token_logprobs(leaf, tokens.view(3, 4))[1].mean()).backward()
     assert torch.equal(leaf.grad.view(12, 250), scoring.backward(
         logits, tokens, out["stats"], None, torch.full((12,), 1 / 12, device=cuda_device)))
-    turned = logits.view(3, 4, 250).transpose(0, 1)
+    turned = logits.view(3, 4, 250).transpose(0, 1)  # (made contiguous by either)
     assert torch.equal(scoring.token_logprobs(turned, tokens.view(3, 4).t())[0],
                        scoring.token_logprobs(turned.contiguous(), tokens.view(3, 4).t())[0])
     one = scoring.token_logprobs(logits[0], tokens[0])[0]
