@@ -3,11 +3,14 @@
 //
 // Forward: one pass over the logits. A thread keeps the running largest logit m, S = sum e^(l - m) and
 // W = sum e^(l - m) (l - m) of what it has seen, raised to a new m once a batch of packs; lanes, waves and
-// a row's parts are joined in a fixed order. Where alternatives are wanted, each wave also keeps a list
-// of candidates in LDS: what is at least as large as the k-th largest of its lanes' own largest logits so
-// far (k of the wave's logits are, so nothing below it can be among the row's k largest), which few
-// batches after the first have. A list that is full is cut to its k largest. Sorted lists of waves and
-// parts are merged by one wave, a list a lane.
+// a row's parts are joined in a fixed order. Where alternatives are wanted, each thread also notes the
+// largest logit of each batch in LDS. After the pass the 64 columns' largest logits give a bound that k
+// logits reach and few more do; the batches with such a one, some k of them, are read once more, and
+// what reaches the bound goes to a list, where each finds its rank among the others. (Taken as the pass goes,
+// by a bound that rises, candidates cost 1000 x 131071 bf16 11 us for 5 alternatives and 27 for 20; so, 6
+// and 12.) A
+// list that is full, of equal logits, is cut to its k largest. The parts' sorted lists are merged by one
+// wave, a list a lane.
 //
 // Backward: d = g ([j = t] - p) - h p (log p + H), a pack at a time from the logits and four numbers a row.
 //
@@ -295,9 +298,12 @@ __device__ __forceinline__ void share_bound(Candidates& c, float (*columns)[kWav
 template <typename E, int WAVES, bool TOP>
 __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
     constexpr int kThreads = WAVES * kWave, kN = Pack<E>::kN;
+    // a thread's largest logit of each span of its batches (its order's upper half), to find the candidates again
+    constexpr int kSpans = WAVES == 16 ? 8 : 32;
     __shared__ float wave_sums[WAVES][3];
     __shared__ uint64_t lists[TOP ? WAVES : 1][TOP ? kList : 1], left[TOP ? kThreads : 1], sorted[kWave];
     __shared__ float columns[TOP ? WAVES : 1][kWave];
+    __shared__ uint16_t spans[TOP ? kSpans : 1][TOP ? kThreads : 1];
     __shared__ uint32_t filled;
     const int i = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     const int wave = uniform(threadIdx.x / kWave), lane = lane_id();
@@ -305,12 +311,17 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
     const RowPacks<E> in(row, a.V);
     const int begin = part * a.part_packs;
     const int end = part + 1 == a.parts ? in.packs : min(in.packs, begin + a.part_packs);
+    const bool last = part + 1 == a.parts;
+    constexpr int kPacks = kBatch * kThreads;  // of a batch
+    const int batches = (end - begin + kPacks - 1) / kPacks, span = (batches + kSpans - 1) / kSpans;
     Sums s;
     Candidates c(lists[TOP ? wave : 0], a.top);
-    bool first_batch = true;
-    const auto batch = [&](const auto& v, const auto& first) {
+    if constexpr (TOP) {
+        if (threadIdx.x == 0) filled = 0;
+        if (wave == 0) sorted[lane] = 0;
+    }
+    const auto largest = [](const auto& v, auto& most) {
         constexpr int N = sizeof(v) / sizeof(v[0]);
-        float most[N];
 #pragma unroll
         for (int b = 0; b < N; ++b) {
             most[b] = v[b][0];
@@ -320,6 +331,10 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
         float all = most[0];
 #pragma unroll
         for (int b = 1; b < N; ++b) all = fmaxf(all, most[b]);
+        return all;
+    };
+    const auto add = [&](const auto& v, float all) {
+        constexpr int N = sizeof(v) / sizeof(v[0]);
         s.raise(fmaxf(s.m, all));
 #pragma unroll
         for (int b = 0; b < N; ++b)
@@ -330,29 +345,14 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
                 s.S += e;
                 s.W = __builtin_fmaf(e, fmaxf(x, -200.0f), s.W);  // e is 0 there, and x may be -inf
             }
-        if constexpr (TOP) {
-            c.lane_most = fmaxf(c.lane_most, all);
-            if (first_batch) {  // (the same for all waves of the workgroup)
-                share_bound<WAVES>(c, columns);
-                c.take(v, most, first);
-            } else if (ballot(all >= c.from)) {
-                c.bound();
-                c.take(v, most, first);
-            }
-            first_batch = false;
-        }
     };
-    // (the loop is the same for all lanes: the candidates' lists are the wave's)
     Pack<E> next[kBatch];
     const auto load = [&](int p0) {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b)
             next[b] = load_pack(row + in.first(min(p0 + b * kThreads + int(threadIdx.x), end - 1)));
     };
-    if (begin < end) load(begin);
-    for (int p0 = begin; p0 < end; p0 += kBatch * kThreads) {
-        Pack<E> v[kBatch];
-        int first[kBatch];
+    const auto taken = [&](int p0, Pack<E> (&v)[kBatch], int (&first)[kBatch]) {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const int p = p0 + b * kThreads + int(threadIdx.x);
@@ -360,24 +360,65 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
             if (p >= end) v[b] = no_pack<E>();
             first[b] = in.first(p);
         }
-        if (p0 + kBatch * kThreads < end) load(p0 + kBatch * kThreads);
-        batch(v, first);
+    };
+    if (begin < end) load(begin);
+    float span_most = -__builtin_inff();
+    for (int batch = 0, p0 = begin; batch < batches; ++batch, p0 += kPacks) {
+        Pack<E> v[kBatch];
+        int first[kBatch];
+        float most[kBatch];
+        taken(p0, v, first);
+        if (p0 + kPacks < end) load(p0 + kPacks);
+        const float all = largest(v, most);
+        add(v, all);
+        if constexpr (TOP) {
+            c.lane_most = fmaxf(c.lane_most, all);
+            if (batches == 1) {  // the logits are here still
+                share_bound<WAVES>(c, columns);
+                c.take(v, most, first);
+            } else {
+                span_most = batch % span ? fmaxf(span_most, all) : all;
+                spans[batch / span][threadIdx.x] = static_cast<uint16_t>(score_key(span_most) >> 16);
+            }
+        }
     }
-    if (part + 1 == a.parts && in.has_rest()) {  // (fewer than 2 kN elements: the first threads')
-        Pack<E> v[1] = {no_pack<E>()};
-        const int first[1] = {in.rest(threadIdx.x)};
-        if (first[0] < a.V) v[0].e[0] = row[first[0]];
-        batch(v, first);
+    Pack<E> rest[1] = {no_pack<E>()};  // (fewer than 2 kN elements: the first threads')
+    const int rest_at[1] = {in.rest(threadIdx.x)};
+    float rest_most[1] = {-__builtin_inff()};
+    if (last && in.has_rest()) {
+        if (rest_at[0] < a.V) rest[0].e[0] = row[rest_at[0]];
+        largest(rest, rest_most);
+        add(rest, rest_most[0]);
+        if constexpr (TOP) c.lane_most = fmaxf(c.lane_most, rest_most[0]);
+    }
+    if constexpr (TOP) {
+        if (batches != 1) {
+            share_bound<WAVES>(c, columns);
+            // the spans with a logit that may be among the largest, once more
+            const uint32_t from = score_key(c.from) >> 16;
+            for (int t = 0; t * span < batches; ++t) {
+                const uint32_t key = spans[t][threadIdx.x];
+                const bool mine = key >= from && key > kKeyNegInf >> 16;
+                if (!ballot(mine)) continue;
+                for (int batch = t * span; batch < min(batches, (t + 1) * span); ++batch) {
+                    Pack<E> v[kBatch];
+                    int first[kBatch];
+                    float most[kBatch];
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b) next[b] = no_pack<E>();
+                    if (mine) load(begin + batch * kPacks);
+                    taken(begin + batch * kPacks, v, first);
+                    largest(v, most);
+                    c.take(v, most, first);
+                }
+            }
+        }
+        if (last && in.has_rest()) c.take(rest, rest_most, rest_at);
     }
     s = wave_join(s);
     if (lane == 0) wave_sums[wave][0] = s.m, wave_sums[wave][1] = s.S, wave_sums[wave][2] = s.W;
     uint64_t best = 0;
     if constexpr (TOP) {
-        if constexpr (WAVES > 1) __syncthreads();  // the columns are read
-        if (threadIdx.x == 0) filled = 0;
-        if (wave == 0) sorted[lane] = 0;
-        share_bound<WAVES>(c, columns);
-        if constexpr (WAVES == 1) wave_order();
         c.leave(left, &filled);
         if constexpr (WAVES > 1)
             __syncthreads();

@@ -12,7 +12,8 @@
  * the type's size as address. tokens[i * token_stride], int64 (token_bytes 8) or int32 (4).
  * Everything is computed in fp32: a log probability is right to about 2^-22 of max(1, |x|), a
  * probability to about 2^-20 of itself; a 16-bit gradient is rounded once. Sums are taken in an order
- * that depends on n, V, the type and the rows' addresses modulo 16 alone. 1 <= V <= 2^24, n V < 2^40, n < 2^24, top <= 32.
+ * that depends on n, V, the type and the rows' addresses modulo 16 alone. 1 <= V <= 2^24, n V < 2^40,
+ * n < 2^24, top <= 32.
  *
  * Nothing is allocated and nothing is kept between calls, so a call may be captured in a graph.
  * `stream` is a hipStream_t (NULL: the default stream). The call returns once the work is enqueued,
