@@ -165,10 +165,14 @@ __global__ __launch_bounds__(WAVES * kWave) void route_tokens(const Args a) {
     // the next tokens' logits are in flight while these are worked on (a token behind the last one: the last)
     Units<E, EACH> next;
     uint8_t next_valid = 1;
-    const auto load = [&](int64_t from) {
-        const int64_t i = from + lane / G, at = i < a.n ? i : a.n - 1;
-        next = load_units<E, EACH>(logits + at * a.row);
-        if (a.valid) next_valid = a.valid[at];
+    const E* from = logits + (t + lane / G) * a.row;  // (stepped, not multiplied, from turn to turn)
+    const E* const last = logits + int64_t(a.n - 1) * a.row;
+    const int64_t row_step = step * a.row;
+    const auto load = [&](int64_t first) {
+        const int64_t i = first + lane / G;
+        next = load_units<E, EACH>(i < a.n ? from : last);
+        from += row_step;
+        if (a.valid) next_valid = a.valid[i < a.n ? i : a.n - 1];
     };
     if (t < a.n) load(t);
     __syncthreads();
@@ -212,7 +216,7 @@ __global__ __launch_bounds__(WAVES * kWave) void route_tokens(const Args a) {
             e[j] = exp_of(x[j] - m);
             total += e[j];
         }
-        const float part = 1.0f / group_sum<G>(total);
+        const float part = __builtin_amdgcn_rcpf(group_sum<G>(total));  // (1 ulp)
 #pragma unroll
         for (int j = 0; j < EACH; ++j) sum[j] += live ? e[j] * part : 0.0f;
         float w[kSlots], chosen = 0.0f;
@@ -221,7 +225,7 @@ __global__ __launch_bounds__(WAVES * kWave) void route_tokens(const Args a) {
             w[q] = kept[q] ? exp_of(O::value(kept[q]) - m) : 0.0f;
             chosen += w[q];
         }
-        const float share = 1.0f / group_sum<G>(chosen);
+        const float share = __builtin_amdgcn_rcpf(group_sum<G>(chosen));
 #pragma unroll
         for (int q = 0; q < kSlots; ++q) {
             const int r = q * G + sub;
@@ -407,7 +411,7 @@ __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
             p[j] = exp_of(x[j] - m);
             total += p[j];
         }
-        const float part = 1.0f / group_sum<G>(total);
+        const float part = __builtin_amdgcn_rcpf(group_sum<G>(total));  // (1 ulp)
         float toward = 0.0f;
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
@@ -429,7 +433,7 @@ __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
             }
             mass = group_sum<G>(mass);
             mean = group_sum<G>(mean);
-            const float share = mass != 0.0f ? 1.0f / mass : 0.0f;  // (no unit chosen: 0)
+            const float share = mass != 0.0f ? __builtin_amdgcn_rcpf(mass) : 0.0f;  // (no unit chosen: 0)
             mean *= share;
 #pragma unroll
             for (int j = 0; j < EACH; ++j)
