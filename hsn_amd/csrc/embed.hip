@@ -534,12 +534,12 @@ void with_type(int dtype, F&& f) {
         f(bf16_t{});
 }
 
-// Chunks of the sorted list: as long as leaves some 4096 waves to fill the GPU, 8 entries (one
+// Chunks of the sorted list: as long as leaves some 2048 waves to fill the GPU, 8 entries (one
 // batch of loads) at least.
 int chunk_of(int64_t n, int D, int dtype) {
     const int lanes = lanes_of(D, dtype);
     const int64_t slices = (packs_of(D, dtype) + lanes - 1) / lanes;
-    const int64_t groups = 4096 * (kWave / lanes);
+    const int64_t groups = 2048 * (kWave / lanes);
     int chunk = kBatch;
     while (chunk < 1024 && n * slices > groups * chunk) chunk *= 2;
     return chunk;
