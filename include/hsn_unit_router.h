@@ -9,8 +9,8 @@
  *   load_e = c_e / sum c,  prob_e = (sum over live tokens of p_e) / R,  balance = M sum_e load_e prob_e
  * (1 where the units are chosen alike; 0 without a live token). An empty slot has unit -1 and share 0; a
  * token that is not live has k of them, and no gradient.
- * - A NaN logit is chosen first; a token with a NaN or +inf has NaN shares, and so is the balance, and
- *   so are its gradient and, through the balance, nothing of the other tokens'.
+ * - A NaN logit is chosen first. A token with a NaN or +inf has NaN shares and a NaN gradient, and makes
+ *   the probs and the balance NaN; the other tokens' gradients are not touched by it.
  * logits [n, M] in `dtype` (HSN_DTYPE_F32, _F16 or _BF16), rows `row` elements apart; valid is uint8.
  * Everything is computed in fp32; the sums over tokens are fp32 over at most a few hundred tokens and
  * float64 above, in an order that depends on n, M and the type alone.

@@ -110,13 +110,14 @@ def test_masked_units(cuda_device, M, k, io):
     _check(logits, k, cuda_device, torch.zeros(12, dtype=torch.bool))
 
 
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("M", [2, 8, 100])
-def test_nan_and_infinity(cuda_device, M, bad):
+def test_nan_and_infinity(cuda_device, M, bad, io):
     """Their own token's shares and gradient, and the means; not another token's."""
     from hsn_amd import unit_router
 
-    logits = _problem(6, M, "f32", 3)
+    logits = _problem(6, M, io, 3)
     logits[2, M - 1] = bad
     if math.isnan(bad):
         logits[4] = bad
