@@ -248,7 +248,7 @@ __device__ __forceinline__ void write_row(const Args& a, int i, const Sums& s, u
     if (lane < a.top) {
         const bool there = best != 0;
         const float l = key_value(static_cast<uint32_t>(best >> 32));
-        a.top_tokens[int64_t(i) * a.top + lane] = 
+        a.top_tokens[int64_t(i) * a.top + lane] =
             there ? int64_t(0xffffffffu - static_cast<uint32_t>(best)) : int64_t(-1);
         a.top_logprobs[int64_t(i) * a.top + lane] = there ? (l - s.m) - rest : -__builtin_inff();
     }
