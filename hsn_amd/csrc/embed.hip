@@ -535,7 +535,8 @@ void with_type(int dtype, F&& f) {
 }
 
 // Chunks of the sorted list: as long as leaves some 2048 waves to fill the GPU, 8 entries (one
-// batch of loads) at least.
+// batch of loads) at least (32768 x 2048 bf16 both ways with 4096 / 2048 / 1024 / 512 waves: 209 / 202 / 210 / 241
+// us; shorter lists do not care).
 int chunk_of(int64_t n, int D, int dtype) {
     const int lanes = lanes_of(D, dtype);
     const int64_t slices = (packs_of(D, dtype) + lanes - 1) / lanes;
@@ -545,8 +546,10 @@ int chunk_of(int64_t n, int D, int dtype) {
     return chunk;
 }
 
-// Entries a tile: the next launch reads all tiles' counts in every workgroup.
-int items_of(int64_t n) { return n <= 1 << 16 ? 4 : n <= 1 << 18 ? 8 : 32; }
+// Entries a tile, of 256 threads: small tiles leave more workgroups for a short list, but the next launch reads
+// all tiles' counts in every workgroup (gradients of n x 8 bf16 with 4 / 8 / 32 entries a thread: 20000 28 / 30 / 56
+// us, 65536 39 / 39 / 64, 200000 63 / 57 / 75, 400000 108 / 76 / 87, 1000000 343 / 148 / 114).
+int items_of(int64_t n) { return n <= 1 << 16 ? 4 : n <= 1 << 19 ? 8 : 32; }
 
 struct Workspace {
     Entry *a, *b;

@@ -26,7 +26,7 @@ __device__ __forceinline__ Pack<E> load_pack(const E* p) {
 
 // Outputs beyond half of the last-level cache are stored past it, which leaves it to what is read again (the
 // logits' second reading, say): see the kernels for what each gains. Smaller ones stay in it for whoever
-// reads them next.
+// reads them next (a gradient of 60 MB: 31.3 us, past the cache 32.2).
 constexpr int64_t kStream = int64_t(128) << 20;
 
 template <int BYTES>

@@ -570,6 +570,9 @@ Plan plan_forward(int n, int V, int dtype) {
     return split(4, packs, std::min<int64_t>(fill, (packs + batch - 1) / batch));
 }
 
+// The backward's, whose parts need no second launch: some 2048 workgroups, a batch at least (1 x 262144 bf16: 4.5 us,
+// by one workgroup 32; 301 x 50021: 11, one workgroup a row 15), of four waves, or one where a row is short (16384 x
+// 1000: 12 us, by four 18).
 Plan plan_backward(int n, int V, int dtype) {
     const int64_t packs = std::max<int64_t>(1, V / (16 / size_of(dtype)));
     const int waves = packs <= 2 * kBatch * kWave ? 1 : 4;

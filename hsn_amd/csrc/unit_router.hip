@@ -469,7 +469,7 @@ int lanes_of(int M) {
 }
 
 // Waves of a forward workgroup: 16 where the tokens keep a workgroup of them on each compute unit busy, else 4,
-// which leaves a SIMD to a wave.
+// which leaves a SIMD to a wave (8192 tokens of 8 units: the launch 4.9 us, by workgroups of 16 waves 7.4).
 int waves_of(int n, int M) { return n > int64_t(kMostGroups) * 4 * (kWave / lanes_of(M)) ? 16 : 4; }
 
 int groups_of(int n, int M) {
