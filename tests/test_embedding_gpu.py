@@ -99,6 +99,19 @@ def test_awkward_lists(cuda_device, n, kind):
     _check(tokens, V, 16, cuda_device, "bf16", "bf16")
 
 
+@pytest.mark.parametrize("n", [1, 31, 127, 128, 129, 1000, 5000])
+@pytest.mark.parametrize("V,D", [(2, 33), (40, 16), (40, 3), (700, 300)])
+def test_runs_across_groups(cuda_device, n, V, D):
+    """Short lists: runs within, across and over many of a workgroup's groups, and past its entries."""
+    _check(_tokens((n,), V, n + D), V, D, cuda_device, "bf16" if D == 16 else "f32", "bf16")
+    _check(_tokens((n,), V, n, padded=0.5, skew=False), V, D, cuda_device)
+
+
+def test_short_lists_of_wide_rows(cuda_device):
+    """More than 2^24 elements: chunks and joins after the short sort."""
+    _check(_tokens((4200,), 30, 0), 30, 4100, cuda_device, "bf16", "bf16")
+
+
 def test_a_long_list(cuda_device):
     """Large tiles and long chunks, wide rows; against sums in float64 on the GPU."""
     from hsn_amd import embedding

@@ -54,7 +54,7 @@ def test_embedding_refusals(lib, message):
     assert _embed_back(lib, d_out=None) == 1 and _embed_back(lib, d_table=None) == 1
     assert _embed_back(lib, d_out=65, code=1) == 1
     assert _embed_back(lib, ws=None) == 1 and _embed_back(lib, ws=72) == 1 and "16" in message()
-    assert _embed_back(lib, n=64) == 1 and "small" in message()
+    assert _embed_back(lib, n=48) == 1 and "small" in message()
 
 
 def test_embedding_workspace(lib):
@@ -64,8 +64,9 @@ def test_embedding_workspace(lib):
         assert lib.hsn_embed_workspace(1, n, V, D, code, ctypes.byref(size)) == 0
         return size.value
 
-    assert bytes_of(0) == 16
-    assert bytes_of(1) == 16 + 2 * 64 * 4  # an entry, a chunk's two sums
+    assert bytes_of(0) == 16 and bytes_of(1) == 16
+    assert bytes_of(8192) == 8 * 8192  # the entries alone
+    assert bytes_of(8192, D=4096) == 8 * 8192 + 8192 // 64 * 2 * 4096 * 4  # two sums of each chunk of 64
     # two lists of entries, the tiles' counts, two sums of each chunk of eight
     assert bytes_of(65536) == 2 * 8 * 65536 + 64 * 4096 + 65536 // 8 * 2 * 64 * 4
     assert lib.hsn_embed_workspace(1, 8, 8, 8, 0, None) == 1
