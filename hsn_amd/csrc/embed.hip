@@ -28,7 +28,9 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kDigit = 10, kBins = 1 << kDigit;
 constexpr int kSmall = 8192, kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
-constexpr int kEntries = 16;    // that a workgroup of the short sort places
+// Entries that a workgroup of the short sort places (gradients of 8192 x 512 with 8 / 16 / 32: 34.7 / 33.2 / 33.2 us,
+// 3063 x 100 17.0 / 16.5 / 17.2; the counts of half the registers, or of all, by vector instructions 34.6 and 35.1).
+constexpr int kEntries = 16;
 constexpr int kBatch = 8;       // entries of a chunk in flight
 constexpr int kCounts = 16;     // tiles' counts in flight
 constexpr int kRunThreads = 512, kRunChunk = 128;
