@@ -96,15 +96,25 @@ __device__ __forceinline__ Units<E, EACH> load_units(const E* p) {
     return v;
 }
 
-// A unit's key: the larger the logit, and among equal ones the lower the unit, the larger; NaN above all,
-// and 0 for -inf, which is never chosen.
+// A unit's key: the larger the logit, and among equal ones the lower the unit, the larger; NaN above all. Below
+// kLeast is -inf, which is never chosen (or nothing: 0).
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 is 0)
+    const uint32_t k = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+    return x == x ? k : 0xffffffffu;
+}
+__device__ __forceinline__ float of_order(uint32_t k) {
+    return __uint_as_float(k ^ (static_cast<int32_t>(k) < 0 ? 0x80000000u : 0xffffffffu));
+}
+constexpr uint32_t kLowest = 0x00800000u;  // that is larger than -inf's
+
 template <typename E>
 struct Order {  // a 16-bit logit in fp32 leaves at least 13 low bits free: 8 for the unit
     static_assert(HSN_ROUTER_MAX_UNITS <= 256, "8 bits hold a unit");
     using Key = uint32_t;
-    static __device__ __forceinline__ Key key(float x, int unit, uint32_t mask) {
-        const uint32_t k = (score_key(x) & 0xffffff00u) | (255u - unit);
-        return x == -__builtin_inff() ? 0 : k & mask;
+    static constexpr Key kLeast = kLowest;
+    static __device__ __forceinline__ Key key(float x, int unit) {
+        return (order_of(x) & 0xffffff00u) | (255u - unit);
     }
     static __device__ __forceinline__ float value(Key k) {
         return __uint_as_float(static_cast<int32_t>(k) < 0 ? (k & 0xffffff00u) ^ 0x80000000u : ~(k | 0xffu));
@@ -118,14 +128,11 @@ struct Order {  // a 16-bit logit in fp32 leaves at least 13 low bits free: 8 fo
 template <>
 struct Order<float> {
     using Key = uint64_t;
-    static __device__ __forceinline__ Key key(float x, int unit, uint32_t mask) {
-        const uint32_t k = x == -__builtin_inff() ? 0 : mask;
-        return uint64_t(score_key(x) & k) << 32 | ((0xffffffffu - unit) & k);
+    static constexpr Key kLeast = uint64_t(kLowest) << 32;
+    static __device__ __forceinline__ Key key(float x, int unit) {
+        return uint64_t(order_of(x)) << 32 | (0xffffffffu - unit);
     }
-    static __device__ __forceinline__ float value(Key key) {
-        const uint32_t k = static_cast<uint32_t>(key >> 32);
-        return __uint_as_float(k ^ (static_cast<int32_t>(k) < 0 ? 0x80000000u : 0xffffffffu));
-    }
+    static __device__ __forceinline__ float value(Key key) { return of_order(static_cast<uint32_t>(key >> 32)); }
     static __device__ __forceinline__ int unit(Key k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
     template <int G>
     static __device__ __forceinline__ Key largest(Key k) {
@@ -160,16 +167,19 @@ __global__ __launch_bounds__(WAVES * kWave) void route_tokens(const Args a) {
     float sum[EACH] = {};
     double whole[EACH] = {};
     uint32_t live_tokens = 0;
-    const int64_t step = int64_t(a.groups) * WAVES * kTokens;
-    int64_t t = (int64_t(blockIdx.x) * WAVES + wave) * kTokens;
+    // (n is below 2^30 and a step at most 2^18; addresses are stepped, not multiplied, from turn to turn)
+    const int step = a.groups * WAVES * kTokens;
+    int t = (static_cast<int>(blockIdx.x) * WAVES + wave) * kTokens;
     // the next tokens' logits are in flight while these are worked on (a token behind the last one: the last)
     Units<E, EACH> next;
     uint8_t next_valid = 1;
-    const E* from = logits + (t + lane / G) * a.row;  // (stepped, not multiplied, from turn to turn)
+    const E* from = logits + (t + lane / G) * a.row;
     const E* const last = logits + int64_t(a.n - 1) * a.row;
     const int64_t row_step = step * a.row;
-    const auto load = [&](int64_t first) {
-        const int64_t i = first + lane / G;
+    int64_t slot = int64_t(t + lane / G) * a.k + sub;
+    const int64_t slot_step = int64_t(step) * a.k;
+    const auto load = [&](int first) {
+        const int i = first + lane / G;
         next = load_units<E, EACH>(i < a.n ? from : last);
         from += row_step;
         if (a.valid) next_valid = a.valid[i < a.n ? i : a.n - 1];
@@ -177,16 +187,15 @@ __global__ __launch_bounds__(WAVES * kWave) void route_tokens(const Args a) {
     if (t < a.n) load(t);
     __syncthreads();
     int turn = 0;
-    for (; t < a.n; t += step) {
-        const int64_t i = t + lane / G;
-        const bool there = i < a.n;
+    for (; t < a.n; t += step, slot += slot_step) {
+        const bool there = t + lane / G < a.n;
         float x[EACH];
         Key key[EACH];
-        const uint32_t mask = there && next_valid ? 0xffffffffu : 0;
+        const bool wanted = there && next_valid;
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
             x[j] = place.mine(j) ? to_f32(next.e[j]) : -__builtin_inff();
-            key[j] = O::key(x[j], place.begin + j, mask);
+            key[j] = O::key(x[j], place.begin + j);
         }
         if (t + step < a.n) load(t + step);
         if constexpr (EACH == 4) {
@@ -203,12 +212,14 @@ __global__ __launch_bounds__(WAVES * kWave) void route_tokens(const Args a) {
                 if (q == 0 && s == 0) first = most;
                 const bool mine = key[0] == most;
 #pragma unroll
-                for (int j = 0; j + 1 < EACH; ++j) key[j] = mine ? key[j + 1] : key[j];
-                key[EACH - 1] = mine ? 0 : key[EACH - 1];
+                for (int j = 0; j < EACH; ++j) {  // (values: a choice between two places is made by number)
+                    const Key own = key[j], behind = j + 1 < EACH ? Key(key[j + 1 < EACH ? j + 1 : j]) : Key(0);
+                    key[j] = mine ? Key(behind) : Key(own);
+                }
                 kept[q] = sub == s ? most : kept[q];
             }
         }
-        const bool live = first != 0;
+        const bool live = wanted && first >= O::kLeast;
         const float m = O::value(first);
         float e[EACH], total = 0.0f;
 #pragma unroll
@@ -220,9 +231,11 @@ __global__ __launch_bounds__(WAVES * kWave) void route_tokens(const Args a) {
 #pragma unroll
         for (int j = 0; j < EACH; ++j) sum[j] += live ? e[j] * part : 0.0f;
         float w[kSlots], chosen = 0.0f;
+        bool is_one[kSlots];
 #pragma unroll
         for (int q = 0; q < kSlots; ++q) {
-            w[q] = kept[q] ? exp_of(O::value(kept[q]) - m) : 0.0f;
+            is_one[q] = wanted && kept[q] >= O::kLeast;
+            w[q] = is_one[q] ? exp_of(O::value(kept[q]) - m) : 0.0f;
             chosen += w[q];
         }
         const float share = __builtin_amdgcn_rcpf(group_sum<G>(chosen));
@@ -231,9 +244,9 @@ __global__ __launch_bounds__(WAVES * kWave) void route_tokens(const Args a) {
             const int r = q * G + sub;
             if (r >= a.k || !there) continue;
             const int u = O::unit(kept[q]);
-            a.units[i * a.k + r] = kept[q] ? u : -1;
-            a.shares[i * a.k + r] = kept[q] ? w[q] * share : 0.0f;
-            if (kept[q]) atomicAdd(&counts[u], 1u);
+            a.units[slot + q * G] = is_one[q] ? u : -1;
+            a.shares[slot + q * G] = is_one[q] ? w[q] * share : 0.0f;
+            if (is_one[q]) atomicAdd(&counts[u], 1u);
         }
         live_tokens += live && sub == 0;
         if (++turn % kFlush == 0) {
@@ -335,52 +348,63 @@ __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
     float2* const mine = slots[wave][lane / G];
     const E* logits = static_cast<const E*>(a.logits) + place.begin;
     E* to = static_cast<E*>(a.d_logits);
-    float load[EACH];
-    double all = 0.0;
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-        const double c = place.mine(j) ? static_cast<double>(a.tally[place.begin + j]) : 0.0;
-        load[j] = static_cast<float>(c);
-        all += c;
-    }
-#pragma unroll
-    for (int mask = 1; mask < G; mask *= 2) all += __shfl_xor(all, mask, kWave);
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) load[j] = all > 0.0 ? static_cast<float>(load[j] / all) : 0.0f;
-    const int64_t rows = a.tally[a.M];
-    const float pull = a.d_balance && rows > 0
-                           ? static_cast<float>(static_cast<double>(*a.d_balance) * a.M / static_cast<double>(rows))
-                           : 0.0f;
-    int token_of[kSlots], rank_of[kSlots];  // of the slots that the lane brings
+    // (n is below 2^30 and a step at most 2^18; addresses are stepped, not multiplied, from turn to turn)
+    const int step = static_cast<int>(gridDim.x) * kBackWaves * kTokens;
+    int t = (static_cast<int>(blockIdx.x) * kBackWaves + wave) * kTokens;
+    const int behind = a.n - 1;  // a token behind the last one reads the last
+    int token_of[kSlots];        // of the slots that the lane brings
+    int64_t slot[kSlots], last_slot[kSlots], cot[kSlots], last_cot[kSlots];
 #pragma unroll
     for (int q = 0; q < kSlots; ++q) {
-        const int s = q * kWave + lane;
+        const int s = q * kWave + lane, rank = s % a.k;
         token_of[q] = s / a.k;
-        rank_of[q] = s - token_of[q] * a.k;
+        slot[q] = int64_t(t + token_of[q]) * a.k + rank;
+        last_slot[q] = int64_t(behind) * a.k + rank;
+        cot[q] = (t + token_of[q]) * a.g_row + rank;
+        last_cot[q] = behind * a.g_row + rank;
     }
-    const int64_t step = int64_t(gridDim.x) * kBackWaves * kTokens;
-    int64_t t = (int64_t(blockIdx.x) * kBackWaves + wave) * kTokens;
+    const E *from = logits + (t + lane / G) * a.row, *const last = logits + behind * a.row;
+    int64_t at = int64_t(t + lane / G) * a.M + place.begin;
+    const int64_t row_step = step * a.row, slot_step = int64_t(step) * a.k, cot_step = step * a.g_row;
     Units<E, EACH> next;
     uint8_t next_valid = 1;
     int64_t next_unit[kSlots];
     float next_g[kSlots];
-    const auto bring = [&](int64_t from) {
-        const int64_t i = from + lane / G, at = i < a.n ? i : a.n - 1;
-        next = load_units<E, EACH>(logits + at * a.row);
-        if (a.valid) next_valid = a.valid[at];
+    const auto bring = [&](int first) {
+        const int i = first + lane / G;
+        next = load_units<E, EACH>(i < a.n ? from : last);
+        from += row_step;
+        if (a.valid) next_valid = a.valid[min(i, behind)];
         if (a.g) {
 #pragma unroll
             for (int q = 0; q < kSlots; ++q) {
-                const int64_t j = from + token_of[q] < a.n ? from + token_of[q] : a.n - 1;
-                next_unit[q] = a.units[j * a.k + rank_of[q]];
-                next_g[q] = a.g[j * a.g_row + rank_of[q]];
+                const bool there = first + token_of[q] < a.n;
+                next_unit[q] = a.units[there ? slot[q] : last_slot[q]];
+                next_g[q] = a.g[there ? cot[q] : last_cot[q]];
+                slot[q] += slot_step;
+                cot[q] += cot_step;
             }
         }
     };
     if (t < a.n) bring(t);
-    for (; t < a.n; t += step) {
-        const int64_t i = t + lane / G;
-        const bool there = i < a.n, wanted = there && next_valid;
+    double count[EACH], all = 0.0;
+    float load[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) count[j] = static_cast<double>(a.tally[place.begin + j]);
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) all += place.mine(j) ? count[j] : 0.0;
+#pragma unroll
+    for (int mask = 1; mask < G; mask *= 2) all += __shfl_xor(all, mask, kWave);
+    const double one = all > 0.0 ? 1.0 / all : 0.0;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) load[j] = place.mine(j) ? static_cast<float>(count[j] * one) : 0.0f;
+    const int64_t rows = a.tally[a.M];
+    const float pull = a.d_balance && rows > 0
+                           ? static_cast<float>(static_cast<double>(*a.d_balance) * a.M / static_cast<double>(rows))
+                           : 0.0f;
+    const int64_t at_step = int64_t(step) * a.M;
+    for (; t < a.n; t += step, at += at_step) {
+        const bool there = t + lane / G < a.n, wanted = there && next_valid;
         float x[EACH];
 #pragma unroll
         for (int j = 0; j < EACH; ++j) x[j] = place.mine(j) ? to_f32(next.e[j]) : -__builtin_inff();
@@ -443,13 +467,12 @@ __global__ __launch_bounds__(kBackThreads) void route_backward(const Args a) {
         E out[EACH];
 #pragma unroll
         for (int j = 0; j < EACH; ++j) out[j] = from_f32<E>(live ? d[j] : 0.0f);
-        E* at = to + i * a.M + place.begin;
         if (place.own == 0) {
-            __builtin_memcpy(at, out, sizeof(out));
+            __builtin_memcpy(to + at, out, sizeof(out));
         } else {
 #pragma unroll
             for (int j = 0; j < EACH; ++j)
-                if (place.mine(j)) at[j] = out[j];
+                if (place.mine(j)) to[at + j] = out[j];
         }
     }
 }
