@@ -69,6 +69,27 @@ def _check(logits, k, dev, valid=None, seed=0, parts=("shares", "balance")):
 
 
 @pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M,k", [(3, 2), (8, 3), (17, 16), (64, 8), (250, 16)])
+def test_the_smallest_and_largest_logits(cuda_device, M, k, io):
+    """Logits below the smallest normal one keep their order, of both signs and beside zeros; the type's
+    lowest value is chosen like any other, and -inf is not."""
+    info = torch.finfo(IO[io])
+    rows = 37
+    g = torch.Generator().manual_seed(M + k)
+    step = info.smallest_normal * info.eps  # the smallest step there is
+    small = (torch.randint(-100, 100, (rows, M), generator=g).double() * step).to(IO[io])
+    assert int(torch.unique(small).numel()) > 30 or rows * M < 200
+    small[::3, 0] = -0.0
+    edges = torch.tensor([info.min, -math.inf, info.min / 2, -1.0, 0.0]).to(IO[io])
+    edge = edges[torch.randint(0, 5, (rows, M), generator=g)]
+    edge[0] = info.min
+    edge[1] = -math.inf
+    edge[2] = -math.inf
+    edge[2, M // 2] = info.min
+    _check(torch.cat([small, edge]), k, cuda_device, seed=k)
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n,M,k", [(1, 1, 1), (1, 8, 2), (5, 3, 3), (33, 4, 4), (70, 8, 2), (130, 16, 5),
                                    (65, 17, 16), (40, 33, 7), (37, 64, 8), (21, 100, 3), (19, 129, 16),
                                    (9, 256, 8), (12, 255, 1)])
