@@ -1,14 +1,16 @@
 // Log probabilities of given tokens with the entropy, the most probable alternatives and the gradient
 // (include/hsn_score.h).
 //
-// Forward: one pass over the logits. A thread keeps the running largest logit m, S = sum e^(l - m) and
-// W = sum e^(l - m) (l - m) of what it has seen, raised to a new m once a batch of packs; lanes, waves and
-// a row's parts are joined in a fixed order. Where alternatives are wanted, each thread also notes the
-// largest logit of each batch in LDS. After the pass the 64 columns' largest logits give a bound that k
-// logits reach and few more do; the batches with such a one, some k of them, are read once more, and
-// what reaches the bound goes to a list, where each finds its rank among the others. (Taken as the pass goes,
-// by a bound that rises, candidates cost 1000 x 131071 bf16 11 us for 5 alternatives and 27 for 20; so, 6
-// and 12.) A
+// Forward: one pass over the logits. A thread keeps S = sum e^(l - m) and W = sum e^(l - m) (l - m) of what it
+// has seen, from a reference m that it raises to a batch's largest logit once that is well above; lanes, waves
+// and a row's parts are joined in a fixed order, from the largest logit. A batch's 16 or 32 numbers are added
+// in fp32, by pairs or fours, and a thread's batches in float64: they are up to 2^12 of a row, and sums in
+// one fp32 number round the same way where logits are alike (a background at -2.3 of 1048576: 3e-5 of S).
+// Where alternatives are wanted, each thread also notes the largest logit of each batch in LDS. After the pass
+// the 64 columns' largest logits give a bound that k logits reach and few more do; the batches with such a
+// one, some k of them, are read once more, and what reaches the bound goes to a list, where each finds its
+// rank among the others. (Taken as the pass goes, by a bound that rises, candidates cost 1000 x 131071 bf16 11 us
+// for 5 alternatives and 27 for 20; so, 6 and 12.) A
 // list that is full, of equal logits, is cut to its k largest. The parts' sorted lists are merged by one
 // wave, a list a lane.
 //
@@ -30,6 +32,7 @@ constexpr int kBatch = 4;      // packs a thread has in flight
 constexpr int kMostParts = 64;  // of a row: a lane each when they are joined
 constexpr int kList = 256;      // candidates of a wave
 constexpr float kLowest = -3.402823466e38f;
+constexpr float kAbove = 4.0f;  // a reference is raised by more than this, so a sum is scaled (and rounded) few times
 constexpr float kLog2 = 1.4426950408889634f;
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // score_key(-inf)
 constexpr uint64_t kNone = uint64_t(kKeyNegInf) << 32 | 0xffffffffu;  // no candidate is this small
@@ -58,39 +61,44 @@ struct Args {
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2); }
 
-// m, S and W of some logits. Of none: the lowest number, 0 and 0.
+// S and W of some logits from the reference m. Of none: 0, 0 and the lowest number.
+template <typename F>
 struct Sums {
-    float m = kLowest, S = 0.0f, W = 0.0f;
-    // The same sums from a reference `to` >= m. What is not finite in m and to enters S by the logits alone.
+    F S = 0, W = 0;
+    float m = kLowest;
+    // The same sums from another reference. What is not finite in m and to enters S by the logits alone.
     __device__ __forceinline__ void raise(float to) {
         const float d = fmaxf(m - to, -1e30f);  // the difference may leave fp32's range
-        const float f = exp_of(d);
-        W = f * __builtin_fmaf(d, S, W);
+        const F f = exp_of(d);
+        W = f * (d * S + W);
         S = f * S;
         m = to;
     }
-    __device__ __forceinline__ void add(const Sums& o) {
-        S += o.S;
-        W += o.W;
-    }
 };
 
-__device__ __forceinline__ float wave_largest(float v) {
+template <int G>
+__device__ __forceinline__ float group_largest(float v) {
     v = fmaxf(v, dpp_f32<dpp::kXor1>(v));
     v = fmaxf(v, dpp_f32<dpp::kXor2>(v));
-    v = fmaxf(v, dpp_f32<dpp::kHalfMirror>(v));
-    v = fmaxf(v, dpp_f32<dpp::kRor8>(v));
-    RowPair r = pair16(__float_as_uint(v));
-    v = fmaxf(__uint_as_float(r.lo), __uint_as_float(r.hi));
-    r = pair32(__float_as_uint(v));
-    return fmaxf(__uint_as_float(r.lo), __uint_as_float(r.hi));
+    if constexpr (G >= 8) v = fmaxf(v, dpp_f32<dpp::kHalfMirror>(v));
+    if constexpr (G >= 16) v = fmaxf(v, dpp_f32<dpp::kRor8>(v));
+    if constexpr (G >= 32) {
+        const RowPair r = pair16(__float_as_uint(v));
+        v = fmaxf(__uint_as_float(r.lo), __uint_as_float(r.hi));
+    }
+    if constexpr (G >= 64) {
+        const RowPair r = pair32(__float_as_uint(v));
+        v = fmaxf(__uint_as_float(r.lo), __uint_as_float(r.hi));
+    }
+    return v;
 }
 
-__device__ __forceinline__ Sums wave_join(Sums s) {
-    s.raise(wave_largest(s.m));
-    s.S = group_sum<kWave>(s.S);
-    s.W = group_sum<kWave>(s.W);
-    return s;
+// The sums of G lanes added, from the largest of `most`: each lane's largest logit, or below its m.
+template <int G>
+__device__ __forceinline__ void join_lanes(Sums<float>& s, float most) {
+    s.raise(group_largest<G>(fmaxf(s.m, most)));
+    s.S = group_sum<G>(s.S);
+    s.W = group_sum<G>(s.W);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -118,7 +126,7 @@ struct Candidates {
     int k, count = 0;
     uint64_t above = kNone;  // candidates are larger than this
     float from = -__builtin_inff();  // and their logits at least this
-    float lane_most = -__builtin_inff();
+    float lane_most = -__builtin_inff();  // the largest logit that the lane has seen
     __device__ Candidates(uint64_t* l, int top) : list(l), k(top) {}
 
     // Leaves the k largest, sorted.
@@ -146,9 +154,9 @@ struct Candidates {
         from = fmaxf(from, key_value(static_cast<uint32_t>(above >> 32)));
     }
 
-    // Raises the bound to the k-th largest of the lanes' largest (to 16 bits of its key, from below).
-    __device__ __forceinline__ void bound() {
-        const uint32_t key = score_key(lane_most);
+    // Raises the bound to the k-th largest of the lanes' numbers (to 16 bits of its key, from below).
+    __device__ __forceinline__ void bound(float most) {
+        const uint32_t key = score_key(most);
         uint32_t least = 0;
         for (int bit = 31; bit >= 16; --bit) {
             const uint32_t test = least | 1u << bit;
@@ -228,7 +236,7 @@ __device__ __forceinline__ uint64_t merge(const uint64_t* all, int lists, int ea
 
 // A row's values from its sums: one wave, lane 0 and the lanes of the alternatives.
 template <typename E>
-__device__ __forceinline__ void write_row(const Args& a, int i, const Sums& s, uint64_t best) {
+__device__ __forceinline__ void write_row(const Args& a, int i, const Sums<float>& s, uint64_t best) {
     const int lane = lane_id();
     const bool none = s.S == 0.0f;
     const float rest = none ? 0.0f : logf(s.S);
@@ -284,14 +292,15 @@ __device__ __forceinline__ Pack<E> no_pack() {
 // k)) where they lie anywhere), 24 for k = 20.
 template <int WAVES>
 __device__ __forceinline__ void share_bound(Candidates& c, float (*columns)[kWave]) {
+    float most = c.lane_most;
     if constexpr (WAVES > 1) {
         const int wave = threadIdx.x / kWave, lane = lane_id();
-        columns[wave][lane] = c.lane_most;
+        columns[wave][lane] = most;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) c.lane_most = fmaxf(c.lane_most, columns[w][lane]);
+        for (int w = 0; w < WAVES; ++w) most = fmaxf(most, columns[w][lane]);
     }
-    c.bound();
+    c.bound(most);
 }
 
 // A workgroup a part of a row.
@@ -314,7 +323,7 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
     const bool last = part + 1 == a.parts;
     constexpr int kPacks = kBatch * kThreads;  // of a batch
     const int batches = (end - begin + kPacks - 1) / kPacks, span = (batches + kSpans - 1) / kSpans;
-    Sums s;
+    Sums<double> sums;
     Candidates c(lists[TOP ? wave : 0], a.top);
     if constexpr (TOP) {
         if (threadIdx.x == 0) filled = 0;
@@ -335,16 +344,26 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
     };
     const auto add = [&](const auto& v, float all) {
         constexpr int N = sizeof(v) / sizeof(v[0]);
-        s.raise(fmaxf(s.m, all));
+        c.lane_most = fmaxf(c.lane_most, all);
+        if (all > sums.m + kAbove) sums.raise(all);
+        float S[N], W[N];
 #pragma unroll
-        for (int b = 0; b < N; ++b)
+        for (int b = 0; b < N; ++b) {
+            float e[kN], w[kN / 4];
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
-                const float x = v[b][j] - s.m;
-                const float e = exp_of(x);
-                s.S += e;
-                s.W = __builtin_fmaf(e, fmaxf(x, -200.0f), s.W);  // e is 0 there, and x may be -inf
+                float x = v[b][j] - sums.m;
+                e[j] = exp_of(x);
+                x = fmaxf(x, -200.0f);  // e is 0 there, and x may be -inf
+                w[j / 4] = j % 4 ? __builtin_fmaf(e[j], x, w[j / 4]) : e[j] * x;
             }
+#pragma unroll
+            for (int j = 0; j < kN; j += 4) e[j] = (e[j] + e[j + 1]) + (e[j + 2] + e[j + 3]);
+            S[b] = kN == 8 ? e[0] + e[4] : e[0];
+            W[b] = kN == 8 ? w[0] + w[kN / 8] : w[0];
+        }
+        sums.S += N == kBatch ? (S[0] + S[1 % N]) + (S[N / 2] + S[N - 1]) : S[0];
+        sums.W += N == kBatch ? (W[0] + W[1 % N]) + (W[N / 2] + W[N - 1]) : W[0];
     };
     Pack<E> next[kBatch];
     const auto load = [&](int p0) {
@@ -372,7 +391,6 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
         const float all = largest(v, most);
         add(v, all);
         if constexpr (TOP) {
-            c.lane_most = fmaxf(c.lane_most, all);
             if (batches == 1) {  // the logits are here still
                 share_bound<WAVES>(c, columns);
                 c.take(v, most, first);
@@ -389,7 +407,6 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
         if (rest_at[0] < a.V) rest[0].e[0] = row[rest_at[0]];
         largest(rest, rest_most);
         add(rest, rest_most[0]);
-        if constexpr (TOP) c.lane_most = fmaxf(c.lane_most, rest_most[0]);
     }
     if constexpr (TOP) {
         if (batches != 1) {
@@ -415,7 +432,8 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
         }
         if (last && in.has_rest()) c.take(rest, rest_most, rest_at);
     }
-    s = wave_join(s);
+    Sums<float> s{static_cast<float>(sums.S), static_cast<float>(sums.W), sums.m};
+    join_lanes<kWave>(s, c.lane_most);
     if (lane == 0) wave_sums[wave][0] = s.m, wave_sums[wave][1] = s.S, wave_sums[wave][2] = s.W;
     uint64_t best = 0;
     if constexpr (TOP) {
@@ -441,15 +459,9 @@ __global__ __launch_bounds__(WAVES * kWave) void score_rows(const Args a) {
     if constexpr (WAVES > 1) {
         if constexpr (!TOP) __syncthreads();
         if (wave) return;
-        float m = s.m;
-        for (int w = 1; w < WAVES; ++w) m = fmaxf(m, wave_sums[w][0]);
-        s.raise(m);  // wave 0's own
-        for (int w = 1; w < WAVES; ++w) {
-            Sums o;
-            o.m = wave_sums[w][0], o.S = wave_sums[w][1], o.W = wave_sums[w][2];
-            o.raise(m);
-            s.add(o);
-        }
+        const float* const mine = wave_sums[lane % WAVES];
+        s = {mine[1], mine[2], mine[0]};
+        join_lanes<WAVES>(s, s.m);
     }
     if (a.parts == 1) {
         write_row<E>(a, i, s, best);
@@ -464,17 +476,17 @@ template <typename E, bool TOP>
 __global__ __launch_bounds__(kWave) void score_join(const Args a) {
     __shared__ uint64_t lists[TOP ? kMostParts * HSN_SCORE_MAX_TOP : 1];
     const int i = blockIdx.x, lane = lane_id();
-    Sums s;
+    Sums<float> s;
     if (lane < a.parts) {
         const float4 v = a.part_sums[int64_t(i) * a.parts + lane];
-        s.m = v.x, s.S = v.y, s.W = v.z;
+        s = {v.y, v.z, v.x};
     }
     if constexpr (TOP) {
         const uint64_t* from = a.part_lists + int64_t(i) * a.parts * a.top;
         for (int j = lane; j < a.parts * a.top; j += kWave) lists[j] = from[j];
         wave_order();
     }
-    s = wave_join(s);
+    join_lanes<kWave>(s, s.m);
     uint64_t best = 0;
     if constexpr (TOP) best = merge(lists, a.parts, a.top, a.top);
     write_row<E>(a, i, s, best);

@@ -10,10 +10,12 @@
  *   equal ones by token; where there are fewer, the token is -1 and its log probability -inf.
  * logits [n, V] in `dtype` (HSN_DTYPE_F32, _F16 or _BF16), rows `row` elements apart, any multiple of
  * the type's size as address. tokens[i * token_stride], int64 (token_bytes 8) or int32 (4).
- * Everything is computed in fp32: a log probability is right to about 2^-22 of max(1, |x|), a
- * probability to about 2^-20 of itself; a 16-bit gradient is rounded once. Sums are taken in an order
- * that depends on n, V, the type and the rows' addresses modulo 16 alone. 1 <= V <= 2^24, n V < 2^40,
- * n < 2^24, top <= 32.
+ * Everything is computed in fp32, but for the sums over a thread's logits, which are float64 beyond 16
+ * or 32 of them: a log probability is right to about 2^-22 of max(1, |x|, log S) and the entropy to
+ * 2^-21 of max(1, log S), whatever the logits are. An exponential's argument is rounded, so a probability
+ * is right to about 2^-21 + 2^-23 |x| of itself (and to 2^-126); a 16-bit gradient is rounded once. Sums
+ * are taken in an order that depends on n, V, the type and the rows' addresses modulo 16 alone.
+ * 1 <= V <= 2^24, n V < 2^40, n < 2^24, top <= 32.
  *
  * Nothing is allocated and nothing is kept between calls, so a call may be captured in a graph.
  * `stream` is a hipStream_t (NULL: the default stream). The call returns once the work is enqueued,
