@@ -109,7 +109,8 @@ def backward(tokens: Tensor, d_out: Tensor, V: int, *, scale: float = 1.0,
     and ``d_out [..., D]`` (the last dimension contiguous, any other strides)."""
     dtype = d_out.dtype if dtype is None else dtype
     if tokens.dim() > 2 and d_out.shape[:-1] == tokens.shape:
-        return backward(tokens.reshape(-1), d_out.reshape(-1, d_out.shape[-1]), V, scale=scale, dtype=dtype)
+        return backward(tokens.reshape(-1), d_out.reshape(tokens.numel(), d_out.shape[-1]), V, scale=scale,
+                        dtype=dtype)
     native = native_calls("hsn_embed_workspace", "hsn_embed_backward")
     if native is not None and d_out.is_cuda:
         calls, size_at, call_at = native

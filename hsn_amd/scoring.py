@@ -159,7 +159,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor) -> tuple[Tensor, Tensor]:
     shape, differentiable in ``logits``."""
     if logits.dim() == 0 or tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens must be {tuple(logits.shape[:-1])}, got {tuple(tokens.shape)}")
-    logprob, entropy = TokenLogprobs.apply(logits.reshape(-1, logits.shape[-1]), tokens.reshape(-1))
+    logprob, entropy = TokenLogprobs.apply(logits.reshape(tokens.numel(), logits.shape[-1]),
+                                           tokens.reshape(-1))
     return logprob.view(tokens.shape), entropy.view(tokens.shape)
 
 
