@@ -6,8 +6,8 @@ l - max l - log(sum of exp(l - max l))``:
 
 :func:`forward` and :func:`backward` are the two passes, :func:`token_logprobs` the same as one
 autograd node: a language model's loss is ``-logprob.mean()``. The logits are fp32, bf16 or fp16 with
-rows any distance apart, and are read once each way; no ``[n, V]`` tensor but the gradient is made. A
-token outside the vocabulary is skipped: its log probability is 0 and it has no gradient. A logit of
+rows any distance apart, and are read once each way; the passes make no ``[n, V]`` tensor but the
+gradient. A token outside the vocabulary is skipped: its log probability is 0 and it has no gradient. A logit of
 ``-inf`` has no mass; a row of nothing else has the log probability ``-inf``, entropy 0 and no gradient. A
 row with a NaN or ``+inf`` has NaN for its values and its gradient. Every function requires ROCm tensors
 and the built HIP library; there is no CPU path here. Nothing is kept between calls.
@@ -156,7 +156,11 @@ class TokenLogprobs(torch.autograd.Function):
 
 def token_logprobs(logits: Tensor, tokens: Tensor) -> tuple[Tensor, Tensor]:
     """``(logprob, entropy)`` of ``logits [..., V]`` and ``tokens [...]``, fp32 and of the tokens'
-    shape, differentiable in ``logits``."""
+    shape, differentiable in ``logits``.
+
+    Leading dimensions that are not rows of one distance are copied, and so is their gradient: the
+    next-token slice ``logits[:, :-1]`` of several sequences is, where ``logits`` themselves with the
+    tokens moved up and -1 behind the last are not."""
     if logits.dim() == 0 or tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens must be {tuple(logits.shape[:-1])}, got {tuple(tokens.shape)}")
     logprob, entropy = TokenLogprobs.apply(logits.reshape(tokens.numel(), logits.shape[-1]),
