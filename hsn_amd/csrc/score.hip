@@ -10,7 +10,7 @@
 // the 64 columns' largest logits give a bound that k logits reach and few more do; the batches with such a
 // one, some k of them, are read once more, and what reaches the bound goes to a list, where each finds its
 // rank among the others. (Taken as the pass goes, by a bound that rises, candidates cost 1000 x 131071 bf16 11 us
-// for 5 alternatives and 27 for 20; so, 6 and 12.) A
+// for 5 alternatives and 27 for 20; so, 8 and 15.) A
 // list that is full, of equal logits, is cut to its k largest. The parts' sorted lists are merged by one
 // wave, a list a lane.
 //
@@ -564,14 +564,14 @@ Plan split(int waves, int64_t packs, int64_t parts) {
 
 // The forward's, with packs a row, from sweeps over n rows of V bf16 logits with five alternatives (us):
 // - a batch of a wave or two: a wave a row.
-// - a batch of four waves: those, whatever n is (64 x 8192: 8.0, by 16 waves 9.2).
+// - a batch of four waves: those, whatever n is (64 x 8192: 7.7, by 16 waves 8.3).
 // - a batch of 16 waves, of no more than 256 rows: those, without the second launch (1 x 32000 with 20
-//   alternatives: 8.9, by parts 13); and so all rows where n is above 128, as their waves fill the GPU (200 x
-//   262144: 33, four waves in four parts 39).
-// - up to 128 longer rows: parts of one batch of four waves, as far as 1024 workgroups go (1 x 131071: 10.7
-//   in 16 parts, 16.8 by 16 waves; 64 x 131071: 15 to 16 in 4 to 16 parts, 20 by 16 waves).
+//   alternatives: 8.0, by parts 12.5); and so all rows where n is above 128, as their waves fill the GPU (200 x
+//   262144: 31, four waves in four parts 35).
+// - up to 128 longer rows: parts of one batch of four waves, as far as 1024 workgroups go (1 x 131071: 11.0
+//   in 16 parts, 15.8 by 16 waves; 64 x 131071: 13.5 in 16 parts, 15 in 4, 16.7 by 16 waves).
 // - more rows: four waves each, in parts of at least eight batches while there are fewer than 1024 rows (300 x
-//   262144: 46 in 4 parts, 58 in one; but 301 x 50021 in fp32 31 in one and 34 in three).
+//   262144: 45 in 3 parts, 53 in one; but 301 x 50021 in fp32 18 in one and 21 in three).
 Plan plan_forward(int n, int V, int dtype) {
     const int64_t packs = std::max<int64_t>(1, V / (16 / size_of(dtype)));
     const int64_t batch = kBatch * 4 * kWave, fill = 1024 / std::max(n, 1);
