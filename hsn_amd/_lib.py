@@ -252,7 +252,12 @@ def ptr(t) -> int | None:
 
 def addr(t) -> int | None:
     """Device address of a tensor whose device the caller has checked (``None`` for an absent one)."""
-    return None if t is None else t.data_ptr()
+    if t is None:
+        return None
+    if t.is_neg():
+        raise ValueError(f"a view of negated values ({tuple(t.shape)} {t.dtype}) is not what its memory holds: "
+                         "call its resolve_neg()")
+    return t.data_ptr()
 
 
 def stream_of(device) -> int:

@@ -20,7 +20,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, call_on, called, native_calls, stream_of
+from ._lib import addr, call, call_on, called, native_calls, stream_of
 
 __all__ = ["MAX_TOKENS", "MAX_WIDTH", "forward", "backward", "embed", "Embed", "available"]
 
@@ -98,7 +98,7 @@ def forward(tokens: Tensor, table: Tensor, *, scale: float = 1.0,
     B, T, stride_b, stride_t = _rows_of(tokens, tokens.dim())
     out = torch.empty((*tokens.shape, D), dtype=dtype, device=dev)
     call_on(dev, "hsn_embed_forward", tokens.data_ptr(), stride_b, stride_t, _TOKEN_BYTES[tokens.dtype],
-            table.data_ptr(), table.stride(0), _DTYPE[table.dtype], float(scale), out.data_ptr(), code, B,
+            addr(table), table.stride(0), _DTYPE[table.dtype], float(scale), out.data_ptr(), code, B,
             T, V, D, stream_of(dev))
     return out
 
@@ -136,7 +136,7 @@ def backward(tokens: Tensor, d_out: Tensor, V: int, *, scale: float = 1.0,
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     d_table = torch.empty((V, D), dtype=dtype, device=dev)
     call_on(dev, "hsn_embed_backward", tokens.data_ptr(), stride_b, stride_t, _TOKEN_BYTES[tokens.dtype],
-            d_out.data_ptr(), row_b, row_t, _DTYPE[d_out.dtype], float(scale), d_table.data_ptr(), code, B,
+            addr(d_out), row_b, row_t, _DTYPE[d_out.dtype], float(scale), d_table.data_ptr(), code, B,
             T, V, D, ws.data_ptr(), size, stream_of(dev))
     return d_table
 
@@ -155,6 +155,7 @@ class Embed(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_out):
         tokens, = ctx.saved_tensors
+        d_out = d_out.resolve_neg()
         if d_out.stride(-1) != 1 and d_out.shape[-1] > 1:
             d_out = d_out.contiguous()  # an expanded cotangent (a sum's) has stride 0
         return None, backward(tokens, d_out, ctx.V, scale=ctx.scale, dtype=ctx.table_dtype), None, None

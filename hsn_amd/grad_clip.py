@@ -23,7 +23,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import call, call_on, called, native_calls, stream_of
+from ._lib import addr, call, call_on, called, native_calls, stream_of
 
 __all__ = ["norm", "clip", "available"]
 
@@ -93,8 +93,8 @@ def _run(grads: Sequence[Tensor], out: Optional[Sequence[Tensor]], max_norm: flo
     call("hsn_clip_workspace", numels, n, ctypes.byref(ws_bytes))
     result = torch.empty(2, dtype=torch.float64, device=dev)
     ws = torch.empty(ws_bytes.value, dtype=torch.uint8, device=dev)
-    call_on(dev, "hsn_clip", pointers(*[g.data_ptr() for g in grads]),
-            None if out is None else pointers(*[o.data_ptr() for o in out]), numels, codes, n,
+    call_on(dev, "hsn_clip", pointers(*[addr(g) for g in grads]),
+            None if out is None else pointers(*[addr(o) for o in out]), numels, codes, n,
             float(max_norm), result.data_ptr(), ws.data_ptr(), ws_bytes.value, stream_of(dev))
     for o in out or ():
         if not o.is_inference():

@@ -81,8 +81,8 @@ int dtype_code(at::ScalarType t) {
     return t == at::kFloat ? 0 : t == at::kHalf ? 1 : t == at::kBFloat16 ? 2 : -1;
 }
 
-// A tensor that the kernels can read at its address (no subclass with another storage).
-bool plain(const Tensor& t) { return t.has_storage() && t.layout() == at::kStrided; }
+// A tensor that the kernels can read at its address (no subclass with another storage, no negated view).
+bool plain(const Tensor& t) { return t.has_storage() && t.layout() == at::kStrided && !t.is_neg(); }
 
 // An absent tensor, or a contiguous one of this shape, type and device.
 bool dense(const Tensor* t, at::IntArrayRef shape, at::ScalarType type, at::Device device) {

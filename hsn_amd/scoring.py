@@ -92,7 +92,7 @@ def forward(logits: Tensor, tokens: Tensor, *, top: int = 0, save: bool = True) 
            "top_logprobs": new(n, top) if top else None, "stats": new(n, 4) if save else None}
     size = _workspace_bytes(n, V, code, top)
     ws = new(size, dtype=torch.uint8) if size else None
-    call_on(dev, "hsn_score_forward", logits.data_ptr(), row, code, tokens.data_ptr(), token_stride,
+    call_on(dev, "hsn_score_forward", addr(logits), row, code, tokens.data_ptr(), token_stride,
             _TOKEN_BYTES[tokens.dtype], out["logprob"].data_ptr(), out["entropy"].data_ptr(),
             addr(out["top_tokens"]), addr(out["top_logprobs"]), addr(out["stats"]), n, V, top,
             addr(ws), size, stream_of(dev))
@@ -105,7 +105,7 @@ def _cotangent(t: Optional[Tensor], name: str, n: int, device) -> tuple:
     if t.shape != (n,) or t.dtype != torch.float32 or t.device != device:
         raise ValueError(f"{name} must be ({n},) float32 on {device}, got {tuple(t.shape)} {t.dtype} "
                          f"on {t.device}")
-    return t.data_ptr(), t.stride(0)
+    return addr(t), t.stride(0)
 
 
 def backward(logits: Tensor, tokens: Tensor, stats: Tensor, d_logprob: Optional[Tensor],
@@ -128,8 +128,8 @@ def backward(logits: Tensor, tokens: Tensor, stats: Tensor, d_logprob: Optional[
     g, g_stride = _cotangent(d_logprob, "d_logprob", n, dev)
     h, h_stride = _cotangent(d_entropy, "d_entropy", n, dev)
     d_logits = torch.empty((n, V), dtype=logits.dtype, device=dev)
-    call_on(dev, "hsn_score_backward", logits.data_ptr(), row, _DTYPE[logits.dtype],
-            tokens.data_ptr(), token_stride, _TOKEN_BYTES[tokens.dtype], stats.data_ptr(), g, g_stride,
+    call_on(dev, "hsn_score_backward", addr(logits), row, _DTYPE[logits.dtype],
+            tokens.data_ptr(), token_stride, _TOKEN_BYTES[tokens.dtype], addr(stats), g, g_stride,
             h, h_stride, d_logits.data_ptr(), n, V, stream_of(dev))
     return d_logits
 
@@ -151,6 +151,7 @@ class TokenLogprobs(torch.autograd.Function):
         if d_logprob is None and d_entropy is None:
             return None, None
         logits, tokens, stats = ctx.saved_tensors
+        d_logprob, d_entropy = (None if d is None else d.resolve_neg() for d in (d_logprob, d_entropy))
         return backward(logits, tokens, stats, d_logprob, d_entropy), None
 
 

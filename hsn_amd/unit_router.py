@@ -95,7 +95,7 @@ def forward(logits: Tensor, k: int, *, valid: Optional[Tensor] = None) -> dict:
     balance = torch.empty((), dtype=torch.float32, device=dev)
     size = _workspace_bytes(n, M, code)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    call_on(dev, "hsn_unit_router_forward", logits.data_ptr(), row, code, valid_at, units.data_ptr(),
+    call_on(dev, "hsn_unit_router_forward", addr(logits), row, code, valid_at, units.data_ptr(),
             shares.data_ptr(), tally.data_ptr(), probs.data_ptr(), balance.data_ptr(), n, M, k,
             ws.data_ptr(), size, stream_of(dev))
     return {"units": units, "shares": shares, "balance": balance, "counts": tally[:M], "probs": probs,
@@ -133,7 +133,7 @@ def backward(logits: Tensor, units: Tensor, tally: Tensor, d_shares: Optional[Te
         raise ValueError(f"d_balance must be one float32 on {dev}, got {tuple(d_balance.shape)} "
                          f"{d_balance.dtype} on {d_balance.device}")
     d_logits = torch.empty((n, M), dtype=logits.dtype, device=dev)
-    call_on(dev, "hsn_unit_router_backward", logits.data_ptr(), row, _DTYPE[logits.dtype], valid_at,
+    call_on(dev, "hsn_unit_router_backward", addr(logits), row, _DTYPE[logits.dtype], valid_at,
             units_at, tally_at, addr(d_shares), g_row, addr(d_balance), d_logits.data_ptr(), n, M, k,
             stream_of(dev))
     return d_logits
@@ -157,6 +157,7 @@ class ChooseUnits(torch.autograd.Function):
         if d_shares is None and d_balance is None:
             return None, None, None
         logits, units, tally, valid = ctx.saved_tensors
+        d_shares, d_balance = (None if d is None else d.resolve_neg() for d in (d_shares, d_balance))
         if d_shares is not None and d_shares.stride(1) != 1 and d_shares.shape[1] > 1:
             d_shares = d_shares.contiguous()  # an expanded cotangent (a sum's) has stride 0
         return backward(logits, units, tally, d_shares, d_balance, valid=valid), None, None
