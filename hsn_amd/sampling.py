@@ -43,7 +43,7 @@ def _setting(v, name: str, dtype: torch.dtype, n: int, device):
                          f"{tuple(v.shape)} {v.dtype} on {v.device}")
     if not v.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return v.data_ptr(), 0
+    return addr(v), 0
 
 
 @lru_cache(maxsize=1024)
@@ -102,7 +102,7 @@ def sample(logits: Tensor, u: Tensor, *, temperature: Union[float, Tensor] = 1.0
     size = _workspace_bytes(n, V, code)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     tokens = torch.empty(n, dtype=torch.int64, device=dev)
-    call_on(dev, "hsn_sample", logits.data_ptr(), row, code, u.data_ptr(), t_at, k_at, p_at, m_at,
+    call_on(dev, "hsn_sample", addr(logits), row, code, addr(u), t_at, k_at, p_at, m_at,
          ctypes.byref(_Settings(t, k, p, m)), tokens.data_ptr(), n, V, addr(ws), size,
          stream_of(dev))
     return tokens

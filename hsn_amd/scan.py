@@ -81,7 +81,7 @@ def _dense(t: Optional[Tensor], name: str, shape: tuple, dtype: torch.dtype, dev
                          f"{t.dtype} on {t.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
+    return addr(t)
 
 
 @lru_cache(maxsize=1024)
@@ -120,7 +120,7 @@ def forward(y: Tensor, gate: Tensor, reset: Optional[Tensor] = None, h0: Optiona
     if save:
         marks = torch.empty((B, -(-T // SPAN), D), dtype=torch.float32, device=dev)
     ws, ws_bytes = _workspace(B, T, D, code, 0, dev)
-    call_on(dev, "hsn_scan_forward", y.data_ptr(), ys[0], ys[1], gate.data_ptr(), gs[0], gs[1], code,
+    call_on(dev, "hsn_scan_forward", addr(y), ys[0], ys[1], addr(gate), gs[0], gs[1], code,
          _candidate(candidate), reset_at, h0_at, h.data_ptr(), h_T.data_ptr(), addr(marks), B, T, D,
          addr(ws), ws_bytes, stream_of(dev))
     return {"h": h, "h_T": h_T, "marks": marks}
@@ -151,7 +151,7 @@ def backward(y: Tensor, gate: Tensor, marks: Tensor, reset: Optional[Tensor],
     d_gate = torch.empty(shape, dtype=io, device=dev)
     d_h0 = torch.empty((B, D), dtype=torch.float32, device=dev)
     ws, ws_bytes = _workspace(B, T, D, code, 1, dev)
-    call_on(dev, "hsn_scan_backward", y.data_ptr(), ys[0], ys[1], gate.data_ptr(), gs[0], gs[1], code,
+    call_on(dev, "hsn_scan_backward", addr(y), ys[0], ys[1], addr(gate), gs[0], gs[1], code,
          _candidate(candidate), reset_at, marks_at, addr(d_h), ds[0], ds[1], d_h_T_at,
          d_y.data_ptr(), d_gate.data_ptr(), d_h0.data_ptr(), B, T, D, addr(ws), ws_bytes,
          stream_of(dev))
@@ -178,6 +178,7 @@ class GatedScan(torch.autograd.Function):
         y, gate, reset, marks = ctx.saved_tensors
         if d_h is None and d_h_T is None:
             return None, None, None, None, None
+        d_h, d_h_T = (None if d is None else d.resolve_neg() for d in (d_h, d_h_T))
         if d_h is not None and d_h.stride(-1) != 1 and d_h.shape[-1] > 1:
             d_h = d_h.contiguous()  # an expanded cotangent (a sum's) has stride 0
         if d_h_T is not None:
@@ -218,7 +219,7 @@ def step(y: Tensor, gate: Tensor, state: Tensor, *, rows: Optional[Tensor] = Non
     if torch.is_grad_enabled() and (y.requires_grad or gate.requires_grad or state.requires_grad):
         raise ValueError("step has no gradient: call it under torch.no_grad()")
     h = torch.empty(shape, dtype=io, device=dev)
-    call_on(dev, "hsn_scan_step", y.data_ptr(), ys[0], gate.data_ptr(), gs[0], code, _candidate(candidate),
+    call_on(dev, "hsn_scan_step", addr(y), ys[0], addr(gate), gs[0], code, _candidate(candidate),
          rows_at, reset_at, state_at, h.data_ptr(), n, S, D, stream_of(dev))
     if n and not state.is_inference():
         torch.autograd.graph.increment_version(state)

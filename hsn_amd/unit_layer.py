@@ -98,8 +98,8 @@ def unit_layer(x: Tensor, router: Tensor, W1: Tensor, b1: Optional[Tensor], W2: 
     y = torch.empty((n, d_out), dtype=io, device=dev)
     size = _workspace_bytes(n, M, k, d_in, H, d_out, code, act)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    call_on(dev, "hsn_units_layer", x.data_ptr(), row, router.data_ptr(), W1.data_ptr(), addr(b1),
-         W2.data_ptr(), addr(b2), y.data_ptr(), n, M, k, d_in, H, d_out, code, act, ws.data_ptr(),
+    call_on(dev, "hsn_units_layer", addr(x), row, addr(router), addr(W1), addr(b1),
+         addr(W2), addr(b2), y.data_ptr(), n, M, k, d_in, H, d_out, code, act, ws.data_ptr(),
          size, stream_of(dev))
     return y
 
