@@ -5,14 +5,14 @@
 // has seen, from a reference m that it raises to a batch's largest logit once that is well above; lanes, waves
 // and a row's parts are joined in a fixed order, from the largest logit. A batch's 16 or 32 numbers are added
 // in fp32, by pairs or fours, and a thread's batches in float64: they are up to 2^12 of a row, and sums in
-// one fp32 number round the same way where logits are alike (a background at -2.3 of 1048576: 3e-5 of S).
+// one fp32 number round the same way where logits are alike (a background at -2.3 of 1048576: 3e-5 of S). The joins
+// are few steps, in fp32: in float64 too, 8192 x 32000 bf16 took 102 us instead of 93 and 1 x 32000 8.5 instead of 8.0.
 // Where alternatives are wanted, each thread also notes the largest logit of each batch in LDS. After the pass
 // the 64 columns' largest logits give a bound that k logits reach and few more do; the batches with such a
 // one, some k of them, are read once more, and what reaches the bound goes to a list, where each finds its
 // rank among the others. (Taken as the pass goes, by a bound that rises, candidates cost 1000 x 131071 bf16 11 us
-// for 5 alternatives and 27 for 20; so, 8 and 15.) A
-// list that is full, of equal logits, is cut to its k largest. The parts' sorted lists are merged by one
-// wave, a list a lane.
+// for 5 alternatives and 27 for 20; so, 8 and 15.) A list that is full, of equal logits, is cut to its k largest.
+// The parts' sorted lists are merged by one wave, a list a lane.
 //
 // Backward: d = g ([j = t] - p) - h p (log p + H), a pack at a time from the logits and four numbers a row.
 //
